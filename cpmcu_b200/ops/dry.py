@@ -62,6 +62,14 @@ class _NoLibrary:
     def cpm_listed_attention_tcgen05_max_pages():
         return 11808
 
+    @staticmethod
+    def cpm_kv4_attention_scratch_floats(d):
+        return 148 * 3 * 2 * 16 * (d + 2)
+
+    @staticmethod
+    def cpm_kv4_attention_most_tiles():
+        return 2048
+
     def __getattr__(self, name):
         return lambda *args: 0
 

@@ -1007,6 +1007,8 @@ class Ops:
         arena = self.workspace.persistent.arena if self.workspace is not None else None
         if arena is not None and arena.guards:
             arena.check_guards()
+        if int(self.lib.cpm_kv4_attention_error()):
+            raise RuntimeError("the attention over a 4-bit cache gave up waiting on a barrier; the results of this step are not valid")
         if int(self.lib.cpm_listed_tile_error()):
             raise RuntimeError("the block-list attention of a prompt chunk gave up waiting on a barrier; the results of "
                                "this step are not valid")
@@ -1660,6 +1662,193 @@ class Ops:
                                                  float(scale), _ptr(scratch), n_splits, 1 if tiles else 0, self._stream()),
               f"block-list attention (head_dim {d})")
         return out
+
+    # ---- a cache held in 4 bits ----
+    KV4_HEAD_DIMS = (32, 64, 96, 128)
+
+    @staticmethod
+    def kv4_page_bytes(d: int) -> int:
+        """Bytes of one page of one key-value head in 4 bits: 64 tokens' key and value codes, and a scale and a middle (bf16 each)
+        for both halves of every row."""
+        return 64 * d + 16 * PAGE_TOKENS
+
+    def _kv4(self, records: torch.Tensor, n_kv: int, d: int) -> torch.Tensor:
+        if d not in self.KV4_HEAD_DIMS:
+            raise ValueError(f"a 4-bit cache takes head sizes {self.KV4_HEAD_DIMS}, got {d}")
+        if records.dtype != torch.uint8 or records.device.type != self.device.type or not records.is_contiguous() \
+                or records.dim() != 3 or tuple(records.shape[1:]) != (n_kv, self.kv4_page_bytes(d)):
+            raise ValueError(f"4-bit cache: needs a contiguous uint8 tensor [pages, {n_kv}, {self.kv4_page_bytes(d)}] on the device, got "
+                             f"{records.dtype} {tuple(records.shape)}")
+        return records
+
+    def _table(self, page_table: torch.Tensor) -> torch.Tensor:
+        self._i32(page_table, "page table")
+        if page_table.dim() != 2:
+            raise ValueError("page table: needs [slots, pages]")
+        return page_table
+
+    def rope_store_kv4(self, qkv: torch.Tensor, n_heads: int, n_kv: int, d: int, positions: torch.Tensor, token_seq: torch.Tensor,
+                       slots: torch.Tensor, page_table: torch.Tensor, records: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor],
+                       magnitude: float, rot_dim: int) -> torch.Tensor:
+        """``rope_store`` for a cache in 4 bits: rotates q and k of qkv [tokens, (heads + 2 kv) * d] (all of a head, or with
+        ``rot_dim`` 0 nothing), quantises k and v into the records [pages, kv, bytes] of each token's sequence (None: stores nothing),
+        and returns the rotated q [tokens, heads, d].  Half a row of d/2 channels x from lo to hi is stored as s = bf16((hi - lo) / 15), m =
+        bf16(lo + 8 s) and codes c = round((x - m) / s) + 8 in 0..15, which stand for m + s (c - 8)."""
+        self._act(qkv, "qkv")
+        if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * d:
+            raise ValueError("qkv row size does not match the head counts")
+        n = qkv.shape[0]
+        if d not in self.KV4_HEAD_DIMS:
+            raise ValueError(f"a 4-bit cache takes head sizes {self.KV4_HEAD_DIMS}, got {d}")
+        if records is not None:
+            self._kv4(records, n_kv, d)
+        if rot_dim not in (0, d):
+            raise ValueError(f"rope_store_kv4 rotates all of a head or nothing, got {rot_dim} of {d} channels")
+        if rot_dim:
+            self._f32(inv_freq, "inv_freq")
+            if inv_freq.numel() != d // 2:
+                raise ValueError("inv_freq needs head_dim/2 entries")
+        for t, what in ((positions, "positions"), (token_seq, "token sequences")):
+            self._i32(t, what)
+            if t.numel() != n:
+                raise ValueError(f"{what}: needs one number a token")
+        self._i32(slots, "slots")
+        self._table(page_table)
+        q = self.empty(n, n_heads, d)
+        check(self.lib.cpm_rope_store_kv4(_ptr(qkv), _ptr(q), _ptr(records), _ptr(positions), _ptr(token_seq), _ptr(slots), _ptr(page_table),
+                                          page_table.shape[1], _ptr(inv_freq) if rot_dim else None, float(magnitude), n, n_heads, n_kv, d,
+                                          self.code, self._stream()), f"rope_store_kv4 (head_dim {d})")
+        return q
+
+    def kv4_values(self, records: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, slots: torch.Tensor,
+                   page_table: torch.Tensor, n_kv: int, d: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The keys and values (k, v), [tokens, kv, d] each in the compute dtype, that a 4-bit cache holds at the listed positions of the
+        listed sequences (``token_seq`` indexes ``slots``)."""
+        self._kv4(records, n_kv, d)
+        n = positions.numel()
+        self._i32(positions, "positions")
+        self._i32(token_seq, "token sequences")
+        if token_seq.numel() != n:
+            raise ValueError("token sequences: needs one number a token")
+        self._i32(slots, "slots")
+        self._table(page_table)
+        k, v = self.empty(n, n_kv, d), self.empty(n, n_kv, d)
+        check(self.lib.cpm_kv4_values(_ptr(records), _ptr(k), _ptr(v), _ptr(positions), _ptr(token_seq), _ptr(slots), _ptr(page_table),
+                                      page_table.shape[1], n, n_kv, d, self.code, self._stream()), f"kv4_values (head_dim {d})")
+        return k, v
+
+    def kv4_attention(self, q: torch.Tensor, records: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor,
+                      n_kv: int, scale: float, window: int = 0, cu_q: Optional[torch.Tensor] = None, tiles=None) -> torch.Tensor:
+        """Attention over a cache in 4 bits: q [tokens, heads, d] -> [tokens, heads * d].  Without ``cu_q`` every row of q is the last token
+        of a sequence of ``kv_len`` keys; with it sequence s brings the tokens cu_q[s] .. cu_q[s + 1], the last of its kv_len[s] keys, and
+        ``tiles`` = (sequence, first token, count) lists them in tiles of QUERY_TILE_TOKENS, as for ``prefill_attention``.  A token at
+        position p sees the keys p - window < j <= p (``window`` 0: all j <= p); a row that sees none gives zeros."""
+        self._act(q, "q")
+        if q.dim() != 3:
+            raise ValueError("q: needs [tokens, heads, d]")
+        n, n_heads, d = q.shape
+        self._kv4(records, n_kv, d)
+        if n_kv < 1 or n_heads % n_kv:
+            raise ValueError(f"{n_heads} heads cannot be grouped over {n_kv} key-value heads")
+        if window < 0:
+            raise ValueError("window: needs a number of keys, or 0 for all")
+        self._i32(kv_len, "key counts")
+        self._i32(slots, "slots")
+        self._table(page_table)
+        if slots.numel() != kv_len.numel():
+            raise ValueError("slots and key counts: need one number a sequence each")
+        tile_seq = tile_row = None
+        n_tiles, tile_tokens = n, 1
+        if cu_q is not None:
+            if tiles is None:
+                raise ValueError("several tokens a sequence need their query tiles")
+            self._i32(cu_q, "token offsets")
+            tile_seq, tile_row, n_tiles = tiles
+            self._i32(tile_seq, "tile sequences")
+            self._i32(tile_row, "tile rows")
+            if cu_q.numel() != kv_len.numel() + 1 or tile_seq.numel() < n_tiles or tile_row.numel() < n_tiles:
+                raise ValueError("token offsets need one entry more than sequences, and the tiles a sequence and a first token each")
+            tile_tokens = PREFILL_TILE_ROWS
+        elif kv_len.numel() != n:
+            raise ValueError(f"{n} rows of q and {kv_len.numel()} sequences: without token offsets each row is a sequence")
+        out = self.empty(n, n_heads * d)
+        if n == 0:
+            return out
+        scratch = self.empty(int(self.lib.cpm_kv4_attention_scratch_floats(d)), dtype=torch.float32)
+        # the kernel counts a launch's work in 32 bits: key-value heads x parts of a tile x pages of every tile
+        units = n_kv * (tile_tokens * (n_heads // n_kv) // 8 + 1) * max(1, page_table.shape[1])
+        step = max(1, min(self.lib.cpm_kv4_attention_most_tiles(), 0x7fffffff // units))
+        size = n_heads * d * self.element_size
+        for first in range(0, n_tiles, step):
+            count = min(step, n_tiles - first)
+            at = lambda t: _ptr(t) + 4 * first if _ptr(t) is not None else None     # noqa: E731
+            row = 0 if cu_q is not None else first
+            check(self.lib.cpm_kv4_attention(_ptr(q) + row * size, _ptr(records), _ptr(out) + row * size,
+                                             at(kv_len) if cu_q is None else _ptr(kv_len), at(slots) if cu_q is None else _ptr(slots),
+                                             _ptr(page_table), page_table.shape[1], _ptr(cu_q), at(tile_seq), at(tile_row), count,
+                                             _ptr(scratch), n_heads, n_kv, d, int(window), float(scale), self.code, self._stream()),
+                  f"attention over a 4-bit cache (head_dim {d}, {n_heads} heads, {n_kv} kv heads)")
+            LAUNCHES_EXTRA[0] += 1       # the shares, then their combination
+        return out
+
+    # ---- pages ----
+    COPY_TENSORS = 8                     # tensors of one launch
+
+    def copy_pages(self, tensors, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Copies the pages src[i] to the pages dst[i] (int32, on the device) in all layers of every tensor [layers, pages, ...], in one
+        launch.  A page may be the source of several; none may be written twice, or written and read.  A number that is no page of a
+        tensor leaves that copy out."""
+        self._i32(src, "source pages")
+        self._i32(dst, "destination pages")
+        if src.numel() != dst.numel():
+            raise ValueError(f"{src.numel()} source pages and {dst.numel()} destination pages")
+        words = []
+        for t in tensors:
+            if t.device.type != self.device.type or not t.is_contiguous() or t.dim() < 2:
+                raise ValueError(f"pages: needs contiguous tensors [layers, pages, ...] on the device, got {tuple(t.shape)} on {t.device}")
+            if t.numel() and src.numel():
+                page = t[0, 0].numel() * t.element_size()
+                words.append((t.data_ptr(), page * t.shape[1], page, t.shape[0], t.shape[1]))
+        for i in range(0, len(words), self.COPY_TENSORS):
+            part = words[i:i + self.COPY_TENSORS]
+            flat = (ctypes.c_int64 * (5 * len(part)))(*[w for five in part for w in five])
+            check(self.lib.cpm_copy_pages(flat, len(part), _ptr(src), _ptr(dst), src.numel(), self._stream()), "copy_pages")
+
+    # ---- drawing from a filtered distribution ----
+    def sample_filtered(self, logits: torch.Tensor, uniform: Optional[torch.Tensor], temperature: torch.Tensor,
+                        top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
+                        seed: int = 0, seq_key: Optional[torch.Tensor] = None, step_key: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """fp32 logits [rows, vocab] -> (token int32 [rows], its log-probability among the tokens that stayed, fp32 [rows]).  Per row:
+        ``temperature`` (0: the largest logit, lowest index among equals), then the ``top_k`` likeliest (0: all), of these the fewest whose
+        mass reaches ``top_p`` of theirs (1: all), of these the ones at least ``min_p`` times as likely as the likeliest (0: all); equal
+        ones stand by index.  The token is where ``uniform`` (in [0, 1)) falls in the kept masses in index order; without it the number
+        is the Philox value of (seed, seq_key, step_key), as in ``sample``.  Masses are whole multiples of 2^-40 of the likeliest, so a
+        row's token depends on nothing but the row.  A row without a number above -inf gives token 0 and -inf."""
+        self._f32(logits, "logits")
+        if logits.dim() != 2:
+            raise ValueError("logits: needs [rows, vocab]")
+        rows, vocab = logits.shape
+        given = ((uniform, "random numbers"), (temperature, "temperatures"), (top_p, "top-p"), (min_p, "min-p"))
+        for t, what in given:
+            if t is not None:
+                self._f32(t, what)
+        for t, what in ((top_k, "top-k"), (seq_key, "sequence keys"), (step_key, "step keys"), (out, "tokens")):
+            if t is not None:
+                self._i32(t, what)
+        for t, what in given + ((top_k, "top-k"), (seq_key, "sequence keys"), (step_key, "step keys"), (out, "tokens")):
+            if t is not None and t.numel() != rows:
+                raise ValueError(f"{what}: needs one number a row, got {t.numel()} for {rows} rows")
+        if temperature is None or (uniform is None and (seq_key is None or step_key is None)):
+            raise ValueError("sample_filtered needs temperatures, and random numbers or the keys to make them from")
+        if out is None:
+            out = self.result(rows, dtype=torch.int32)
+        logprob = self.result(rows, dtype=torch.float32)
+        check(self.lib.cpm_sample_filtered(_ptr(logits), logits.stride(0), rows, vocab, _ptr(out), _ptr(logprob), _ptr(uniform),
+                                           _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+                                           ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), self._stream()),
+              f"sample_filtered ({vocab} tokens)")
+        return out, logprob
 
 
 LAUNCHES_EXTRA = library.LAUNCHES

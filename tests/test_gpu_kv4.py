@@ -1,0 +1,506 @@
+"""The 4-bit cache's kernels, the copying of pages and the filtered sampling against the definitions (tests/plain/kv4_plain.py)."""
+import math
+
+import pytest
+import torch
+
+from tests.plain import kv4_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+DT = {"float32": torch.float32, "bfloat16": torch.bfloat16}
+PAGE = 64
+
+
+def _ops(dtype):
+    from cpmcu_b200.ops.ops import Ops
+    return Ops(DT[dtype], "cuda:0")
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32).cuda()
+
+
+def _tables(lengths, seed, spare=3):
+    """Page table [slots, pages], slots and the number of pages for sequences of the given lengths; pages and slots in no order."""
+    g = torch.Generator().manual_seed(seed)
+    pages = [(n + PAGE - 1) // PAGE for n in lengths]
+    total = sum(pages) + spare
+    order = torch.randperm(total, generator=g).tolist()
+    slots = torch.randperm(len(lengths) + 2, generator=g)[:len(lengths)].tolist()
+    table = torch.zeros(len(lengths) + 2, max(pages + [1]) + 1, dtype=torch.int32)
+    for s, n in zip(slots, pages):
+        table[s, :n] = torch.tensor([order.pop() for _ in range(n)], dtype=torch.int32)
+    return table.cuda(), slots, total
+
+
+def _every_position(lengths):
+    pos = [p for n in lengths for p in range(n)]
+    seq = [i for i, n in enumerate(lengths) for _ in range(n)]
+    return _i32(pos), _i32(seq)
+
+
+def _filled(ops, lengths, kv, d, seed, loud=1.0, v_scale=1.0):
+    """A cache that holds random keys and values; returns its parts and the values they stand for (fp32, on the host)."""
+    table, slots, total = _tables(lengths, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    records = torch.randint(0, 256, (total, kv, ops.kv4_page_bytes(d)), generator=g, dtype=torch.uint8).cuda()
+    records[..., 64 * d:] = 255                       # parameters that are no numbers wherever nothing is stored
+    n = sum(lengths)
+    pos, seq = _every_position(lengths)
+    k = torch.randn(n, kv, d, generator=g) * (1 + (loud - 1) * (torch.rand(1, kv, d, generator=g) > 0.9))
+    v = torch.randn(n, kv, d, generator=g) * v_scale + 0.2 * v_scale
+    f32 = _ops("float32")
+    if n:
+        qkv = torch.cat((torch.zeros(n, kv, d), k, v), 1).flatten(1).cuda()
+        f32.rope_store_kv4(qkv, kv, kv, d, pos, seq, _i32(slots), table, records, None, 1.0, 0)
+        kk, vv = f32.kv4_values(records, pos, seq, _i32(slots), table, kv, d)
+        kk, vv = kk.cpu(), vv.cpu()
+    else:
+        kk = vv = torch.zeros(0, kv, d)
+    at = [0]
+    for x in lengths:
+        at.append(at[-1] + x)
+    rows = [(kk[a:b], vv[a:b]) for a, b in zip(at, at[1:])]
+    return table, slots, records, rows
+
+
+# ---------------------------------------------------------------------------
+# store and read back
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("heads,kv", [(4, 1), (6, 2), (3, 3)])
+def test_store_and_read_without_rotation(dtype, d, heads, kv):
+    """Without a rotation every step of the definition is a rounding to 32 bits, so that the values are the same numbers."""
+    ops = _ops(dtype)
+    lengths = [1, 63, 64, 65, 200]
+    table, slots, total = _tables(lengths, 3)
+    pos, seq = _every_position(lengths)
+    g = torch.Generator().manual_seed(d + heads)
+    n = sum(lengths)
+    qkv = (torch.randn(n, heads + 2 * kv, d, generator=g) * torch.rand(n, heads + 2 * kv, 1, generator=g).mul(12).sub(6).exp()).to(DT[dtype])
+    qkv[5] = 0.75                                    # rows whose channels are all equal
+    qkv[6, :, :d // 2] = 0
+    qkv[7, :, 3] = 1e30 if dtype == "float32" else 1e20
+    records = torch.randint(0, 256, (total, kv, ops.kv4_page_bytes(d)), generator=g, dtype=torch.uint8).cuda()
+    before = records.clone()
+    q = ops.rope_store_kv4(qkv.flatten(1).cuda(), heads, kv, d, pos, seq, _i32(slots), table, records, None, 1.0, 0)
+    assert torch.equal(q.cpu(), qkv[:, :heads])
+    k, v = ops.kv4_values(records, pos, seq, _i32(slots), table, kv, d)
+    for got, x in ((k, qkv[:, heads:heads + kv]), (v, qkv[:, heads + kv:])):
+        want, s = plain.quantised(x)
+        assert torch.equal(got.cpu(), want.to(DT[dtype]))
+        # and the definition keeps what it says: half a step, and the roundings of s (15 steps of 2^-9) and of the middle
+        h = x.float().unflatten(-1, (2, -1))
+        off = (want.unflatten(-1, (2, -1)) - h).abs().amax(-1)
+        assert bool((off <= s * (0.5 + 16 / 512) + h.abs().amax(-1) * 2.0 ** -8).all())
+    # pages that nothing was stored into are as they were
+    used = torch.zeros(total, dtype=torch.bool)
+    for s, x in zip(slots, lengths):
+        used[table.cpu()[s, :(x + 63) // 64].long()] = True
+    assert torch.equal(records.cpu()[~used], before.cpu()[~used])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("tokens", [1, 5, 70])
+def test_store_rotates(dtype, d, tokens):
+    heads, kv, first = 5, 5, 1003
+    ops = _ops(dtype)
+    g = torch.Generator().manual_seed(d)
+    table, slots, total = _tables([first + tokens, first + tokens], 4)
+    pos = torch.arange(first, first + tokens).repeat(2)
+    qkv = torch.randn(2 * tokens, heads + 2 * kv, d, generator=g).to(DT[dtype])
+    inv_freq = 1.0 / 10000.0 ** (torch.arange(0, d, 2).float() / d)
+    records = torch.zeros(total, kv, ops.kv4_page_bytes(d), dtype=torch.uint8).cuda()
+    seq = torch.arange(2).repeat_interleave(tokens)
+    args = (_i32(pos.tolist()), _i32(seq.tolist()), _i32(slots), table)
+    q = ops.rope_store_kv4(qkv.flatten(1).cuda(), heads, kv, d, *args, records, inv_freq.cuda(), 1.19, d)
+    want = plain.rotated(qkv, pos, inv_freq, 1.19)
+    # an angle of about 1,000 is rounded to 2^-15, its sine moves by as much; bf16: half the spacing of its 8 bits besides
+    spacing = 2.0 ** (torch.log2(want[:, :heads].abs().clamp_min(1e-9)).floor() - 7) if dtype == "bfloat16" else 0.0
+    assert bool(((q.cpu().double() - want[:, :heads]).abs() <= 2e-3 + 0.5 * spacing).all())
+    k, v = _ops("float32").kv4_values(records, *args, kv, d)
+    _, s = plain.quantised(want[:, heads:heads + kv].float())
+    off = (k.cpu().double() - want[:, heads:heads + kv]).abs().unflatten(-1, (2, -1)).amax(-1)
+    assert bool((off <= s * (0.5 + 16 / 512) + 6 * 2.0 ** -8 + 2e-3).all())
+    assert torch.equal(v.cpu(), plain.quantised(qkv[:, heads + kv:])[0])
+
+
+def test_rows_that_are_no_numbers_stay_alone():
+    """A channel that is no number makes its half row one, and no other."""
+    ops, d, kv = _ops("float32"), 64, 2
+    table, slots, total = _tables([130], 5)
+    pos, seq = _every_position([130])
+    qkv = torch.randn(130, 3 * kv, d, generator=torch.Generator().manual_seed(1))
+    qkv[17, 2, 40] = math.nan
+    qkv[18, 5, 3] = math.inf
+    records = torch.zeros(total, kv, ops.kv4_page_bytes(d), dtype=torch.uint8).cuda()
+    ops.rope_store_kv4(qkv.flatten(1).cuda(), kv, kv, d, pos, seq, _i32(slots), table, records, None, 1.0, 0)
+    k, v = (t.cpu() for t in ops.kv4_values(records, pos, seq, _i32(slots), table, kv, d))
+    bad_k, bad_v = torch.zeros(130, kv, d, dtype=torch.bool), torch.zeros(130, kv, d, dtype=torch.bool)
+    bad_k[17, 0, 32:] = True
+    bad_v[18, 1, :32] = True
+    assert torch.equal(k.isnan(), bad_k) and torch.equal(v.isnan(), bad_v)
+    assert torch.equal(k[~bad_k], plain.quantised(qkv[:, 2:4])[0][~bad_k])
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+def _check(got, want, rows, dtype):
+    """bf16: one rounding of the output (2^-9, doubled for the sum's own) and weights of 11 bits (2^-11 of the largest value, doubled);
+    fp32: queries and weights of 22 bits and scores of up to about 100: 2^-22 * 100 of the largest value."""
+    assert got.shape == (want.shape[0], want.shape[1] * want.shape[2])
+    got = got.cpu().double().view(want.shape)
+    big = max([float(v.abs().nan_to_num(0).max()) for _, v in rows if v.numel()] + [0.0])
+    tol = want.abs() * 2.0 ** -8 + big * 2.0 ** -10 if dtype == "bfloat16" else torch.full_like(want, big * 100 * 2.0 ** -22)
+    assert bool(torch.isfinite(got).all())
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol.clamp_min(1e-30)).max())
+
+
+SHAPES = [(1, 1), (2, 1), (6, 2), (5, 1), (16, 2), (16, 1), (24, 1), (40, 2)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("heads,kv", SHAPES)
+def test_one_token_a_sequence(dtype, d, heads, kv):
+    ops = _ops(dtype)
+    lengths = [0, 1, 2, 15, 16, 17, 63, 64, 65, 130, 700]
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 11, loud=4.0)
+    q = torch.randn(len(lengths), heads, d, generator=torch.Generator().manual_seed(7)).to(DT[dtype])
+    for window in (0, 1, 16, 100):
+        got = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5, window=window)
+        want = torch.cat([plain.attention(q[i:i + 1], k, v, n - 1, d ** -0.5, window) for i, (n, (k, v)) in enumerate(zip(lengths, rows))])
+        _check(got, want, rows, dtype)
+        assert float(got[0].abs().max()) == 0.0           # no keys
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d,heads,kv", [(32, 3, 1), (64, 8, 1), (64, 6, 2), (96, 4, 2), (128, 16, 1), (128, 2, 2)])
+def test_several_tokens_a_sequence(dtype, d, heads, kv):
+    ops = _ops(dtype)
+    new = [1, 5, 0, 64, 65, 130, 30]
+    lengths = [1, 5, 40, 64, 200, 130, 161]
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 13)
+    q = torch.randn(sum(new), heads, d, generator=torch.Generator().manual_seed(7)).to(DT[dtype])
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    tiles = [(i, r) for i, n in enumerate(new) for r in range(0, n, 64)] + [(2, 0)]       # a tile of a sequence that brings nothing
+    args = dict(cu_q=_i32(cu), tiles=(_i32([t[0] for t in tiles]), _i32([t[1] for t in tiles]), len(tiles)))
+    for window in (0, 3, 90):
+        got = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5, window=window, **args)
+        want = torch.cat([plain.attention(q[cu[i]:cu[i + 1]], k, v, lengths[i] - new[i], d ** -0.5, window) for i, (k, v) in enumerate(rows)])
+        _check(got, want, rows, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("q_scale,v_scale", [(30.0, 1.0), (1e-6, 1e-6), (1.0, 1e6), (0.0, 1.0)])
+def test_magnitudes(dtype, q_scale, v_scale):
+    """Sharp and flat distributions, values of any size: what is kept in 16 bits is divided by powers of two first."""
+    ops, d, heads, kv = _ops(dtype), 64, 4, 2
+    lengths = [300, 77]
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 17, v_scale=v_scale)
+    q = (torch.randn(2, heads, d, generator=torch.Generator().manual_seed(7)) * q_scale).to(DT[dtype])
+    got = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5)
+    want = torch.cat([plain.attention(q[i:i + 1], k, v, n - 1, d ** -0.5, 0) for i, (n, (k, v)) in enumerate(zip(lengths, rows))])
+    _check(got, want, rows, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("poison", [math.nan, math.inf, 1e30])
+def test_tokens_that_are_not_seen_have_no_part(dtype, poison):
+    """Keys and values behind a prompt's token, or before its window, that are no numbers or very large, do not reach it."""
+    ops, d, heads, kv = _ops(dtype), 64, 4, 2
+    n, new = 150, 40
+    table, slots, total = _tables([n], 5)
+    pos, seq = _every_position([n])
+    g = torch.Generator().manual_seed(3)
+    kvs = torch.randn(n, 2 * kv, d, generator=g)
+    records = torch.zeros(total, kv, ops.kv4_page_bytes(d), dtype=torch.uint8).cuda()
+    f32 = _ops("float32")
+    store = lambda x: f32.rope_store_kv4(torch.cat((torch.zeros(n, kv, d), x), 1).flatten(1).cuda(), kv, kv, d, pos, seq, _i32(slots), table,  # noqa: E731
+                                         records, None, 1.0, 0)
+    q = torch.randn(new, heads, d, generator=g).to(DT[dtype]).cuda()
+    tiles = (_i32([0]), _i32([0]), 1)
+    run = lambda w: ops.kv4_attention(q, records, _i32([n]), _i32(slots), table, kv, d ** -0.5, window=w, cu_q=_i32([0, new]), tiles=tiles)  # noqa: E731
+    store(kvs)
+    clean = {w: run(w).cpu() for w in (0, 20)}
+    bad = kvs.clone()
+    bad[130] = poison                                  # position of the prompt's token 20
+    bad[60] = poison                                   # before every window
+    store(bad)
+    windowed = run(20).cpu()
+    assert torch.equal(windowed[:20], clean[20][:20])
+    bad[60] = kvs[60]
+    store(bad)
+    assert torch.equal(run(0).cpu()[:20], clean[0][:20])
+
+
+def test_shares_do_not_depend_on_neighbours():
+    """However a batch is cut among the blocks, a sequence's result stays within the tolerance, and one call gives the same bits twice."""
+    ops, d, heads, kv = _ops("bfloat16"), 128, 16, 1
+    lengths = [3000, 1, 64, 5000, 700, 0, 129] + [200] * 30
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 23)
+    q = torch.randn(len(lengths), heads, d, generator=torch.Generator().manual_seed(7)).bfloat16()
+    got = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5)
+    again = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5)
+    assert torch.equal(got, again)
+    want = torch.cat([plain.attention(q[i:i + 1], k, v, n - 1, d ** -0.5, 0) for i, (n, (k, v)) in enumerate(zip(lengths, rows))])
+    _check(got, want, rows, "bfloat16")
+    for i in (0, 3, 4):
+        alone = ops.kv4_attention(q[i:i + 1].cuda(), records, _i32(lengths[i:i + 1]), _i32(slots[i:i + 1]), table, kv, d ** -0.5)
+        _check(alone, want[i:i + 1], rows, "bfloat16")
+
+
+def test_more_tiles_than_a_launch_takes():
+    ops, d, heads, kv = _ops("bfloat16"), 32, 2, 1
+    lengths = [(i * 7) % 5 for i in range(4500)]
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 29)
+    q = torch.randn(len(lengths), heads, d, generator=torch.Generator().manual_seed(7)).bfloat16()
+    got = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5)
+    want = torch.cat([plain.attention(q[i:i + 1], k, v, n - 1, d ** -0.5, 0) for i, (n, (k, v)) in enumerate(zip(lengths, rows))])
+    _check(got, want, rows, "bfloat16")
+
+
+def test_offsets_beyond_32_bits():
+    """A page that begins behind 4 GB of records."""
+    ops, d, heads, kv = _ops("bfloat16"), 128, 16, 2
+    size = kv * ops.kv4_page_bytes(d)
+    total = (1 << 32) // size + 40
+    records = torch.empty(total, kv, size // kv, dtype=torch.uint8, device="cuda")
+    table = _i32([[total - 1, total - 7, 2, total - 3]])
+    n = 210
+    g = torch.Generator().manual_seed(2)
+    k, v = torch.randn(n, kv, d, generator=g), torch.randn(n, kv, d, generator=g)
+    pos, seq = _every_position([n])
+    f32 = _ops("float32")
+    f32.rope_store_kv4(torch.cat((torch.zeros(n, kv, d), k, v), 1).flatten(1).cuda(), kv, kv, d, pos, seq, _i32([0]), table, records, None, 1.0, 0)
+    got_k, got_v = f32.kv4_values(records, pos, seq, _i32([0]), table, kv, d)
+    assert torch.equal(got_k.cpu(), plain.quantised(k)[0]) and torch.equal(got_v.cpu(), plain.quantised(v)[0])
+    q = torch.randn(1, heads, d, generator=g).bfloat16()
+    got = ops.kv4_attention(q.cuda(), records, _i32([n]), _i32([0]), table, kv, d ** -0.5)
+    _check(got, plain.attention(q, got_k.cpu(), got_v.cpu(), n - 1, d ** -0.5, 0), [(got_k.cpu(), got_v.cpu())], "bfloat16")
+
+
+def test_another_stream_and_views():
+    """Calls on a stream of their own, of tensors that are parts of larger ones."""
+    ops, d, heads, kv = _ops("bfloat16"), 64, 8, 2
+    lengths = [100, 333]
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 31)
+    q = torch.randn(2, heads, d, generator=torch.Generator().manual_seed(7)).bfloat16()
+    want = torch.cat([plain.attention(q[i:i + 1], k, v, n - 1, d ** -0.5, 0) for i, (n, (k, v)) in enumerate(zip(lengths, rows))])
+    larger = torch.zeros(5, heads, d, dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        larger[1:3].copy_(q.cuda())
+        got = ops.kv4_attention(larger[1:3], records, _i32([7] + lengths)[1:], _i32([1] + slots)[1:], table, kv, d ** -0.5)
+    side.synchronize()
+    _check(got, want, rows, "bfloat16")
+
+
+def test_refusals_of_the_4_bit_cache():
+    ops, d, kv = _ops("bfloat16"), 64, 2
+    records = torch.zeros(4, kv, ops.kv4_page_bytes(d), dtype=torch.uint8).cuda()
+    table, one = torch.zeros(1, 4, dtype=torch.int32).cuda(), _i32([1])
+    zero = _i32([0])
+    q = torch.zeros(1, 4, d, dtype=torch.bfloat16).cuda()
+    call = lambda **k: ops.kv4_attention(**{**dict(q=q, records=records, kv_len=one, slots=zero, page_table=table, n_kv=kv, scale=1.0), **k})  # noqa: E731
+    call()
+    for bad in (dict(q=q.float()), dict(q=q[0]), dict(q=torch.zeros(1, 3, d, dtype=torch.bfloat16).cuda()), dict(records=records[:, :1]),
+                dict(records=records.float()), dict(n_kv=1), dict(kv_len=_i32([1, 1])), dict(slots=_i32([0, 0])), dict(kv_len=one.long()),
+                dict(window=-1), dict(cu_q=_i32([0, 1])), dict(cu_q=_i32([0]), tiles=(zero, zero, 1)), dict(cu_q=_i32([0, 1]), tiles=(zero, zero, 2)),
+                dict(page_table=table[0]), dict(q=torch.zeros(1, 4, 48, dtype=torch.bfloat16).cuda())):
+        with pytest.raises(ValueError):
+            call(**bad)
+    qkv = torch.zeros(1, 8 * d, dtype=torch.bfloat16).cuda()
+    inv = torch.ones(d // 2).cuda()
+    store = lambda **k: ops.rope_store_kv4(**{**dict(qkv=qkv, n_heads=4, n_kv=kv, d=d, positions=zero, token_seq=zero, slots=zero, page_table=table,  # noqa: E731
+                                                    records=records, inv_freq=inv, magnitude=1.0, rot_dim=d), **k})
+    store()
+    off = torch.zeros(8 * d + 1, dtype=torch.bfloat16).cuda()[1:].view(1, -1)
+    for bad in (dict(qkv=qkv[:, :-8]), dict(qkv=off), dict(rot_dim=d // 2), dict(inv_freq=inv[1:]), dict(positions=_i32([0, 1])), dict(token_seq=_i32([])),
+                dict(records=records[..., :-16]), dict(n_heads=5), dict(qkv=qkv.float())):
+        with pytest.raises(ValueError):
+            store(**bad)
+    with pytest.raises(ValueError):
+        ops.kv4_values(records, zero, _i32([0, 0]), zero, table, kv, d)
+    with pytest.raises(ValueError):
+        ops.kv4_values(records, zero, zero, zero, table, kv, 48)
+    assert ops.kv4_attention(q[:0], records, one[:0], zero[:0], table, kv, 1.0).shape == (0, 4 * d)
+
+
+# ---------------------------------------------------------------------------
+# pages
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shapes", [[(3, 20, 2, 64, 32)], [(2, 20, 5), (4, 20, 3), (1, 20, 7, 16)], [(1, 20, 1)] * 11, [(2, 20, 4096), (0, 20, 4), (5, 20, 9000)]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.uint8])
+def test_copy_pages(shapes, dtype):
+    ops = _ops("bfloat16")
+    g = torch.Generator().manual_seed(1)
+    tensors = [torch.randint(0, 200, s, generator=g).to(dtype) for s in shapes]
+    here = [t.cuda() for t in tensors]
+    src, dst = [3, 3, 19, 0, 25, 4, -1], [1, 2, 18, 5, 6, 40, 7]           # one page twice; numbers that are no page
+    ops.copy_pages(here, _i32(src), _i32(dst))
+    for t in tensors:
+        for a, b in zip(src[:4], dst[:4]):
+            t[:, b] = t[:, a]
+    for got, want in zip(here, tensors):
+        assert torch.equal(got.cpu(), want)
+
+
+def test_copy_pages_of_unaligned_tensors_and_refusals():
+    ops = _ops("bfloat16")
+    t = torch.arange(4 * 8 * 6 + 1, dtype=torch.int16).to(torch.uint8).cuda()[1:].view(4, 8, 6)
+    want = t.cpu().clone()
+    want[:, 7] = want[:, 2]
+    ops.copy_pages([t], _i32([2]), _i32([7]))
+    assert torch.equal(t.cpu(), want)
+    ops.copy_pages([], _i32([2]), _i32([7]))
+    ops.copy_pages([t], _i32([]), _i32([]))
+    for bad in (lambda: ops.copy_pages([t], _i32([2]), _i32([7, 1])), lambda: ops.copy_pages([t[:, :4]], _i32([2]), _i32([1])),
+                lambda: ops.copy_pages([t.cpu()], _i32([2]), _i32([1])), lambda: ops.copy_pages([t], _i32([2]).long(), _i32([1])),
+                lambda: ops.copy_pages([t.view(-1)], _i32([2]), _i32([1]))):
+        with pytest.raises(ValueError):
+            bad()
+    assert torch.equal(t.cpu(), want)
+
+
+# ---------------------------------------------------------------------------
+# filtered sampling
+# ---------------------------------------------------------------------------
+
+def _settings(rows, vocab, seed):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda: torch.rand(rows, generator=g)  # noqa: E731
+    t = torch.where(r() < 0.2, torch.zeros(rows), 0.3 + 1.5 * r())
+    k = torch.where(r() < 0.4, torch.zeros(rows), (vocab * r() ** 3).ceil()).int()
+    p = torch.where(r() < 0.4, torch.ones(rows), r())
+    m = torch.where(r() < 0.5, torch.zeros(rows), 0.2 * r())
+    return r(), t, k, p, m
+
+
+def _compare(ops, z, u, t, k, p, m):
+    tok, lp = ops.sample_filtered(z.cuda(), u.cuda(), t.cuda(), k.cuda(), p.cuda(), m.cuda())
+    for i in range(z.shape[0]):
+        want, logp = plain.sampled(z[i], float(u[i]), float(t[i]), int(k[i]), float(p[i]), float(m[i]))
+        assert int(tok[i]) == want, (i, int(tok[i]), want, float(t[i]), int(k[i]), float(p[i]), float(m[i]))
+        # two roundings of a difference of up to 100, and a logarithm of up to 30
+        assert float(lp[i]) == logp or abs(float(lp[i]) - logp) < 2e-5, (float(lp[i]), logp)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (7, 31), (5, 333), (40, 1000), (2, 5001), (150, 1030), (3, 20000)])
+def test_sample_filtered(rows, vocab):
+    z = torch.randn(rows, vocab, generator=torch.Generator().manual_seed(vocab)) * 3
+    _compare(_ops("bfloat16"), z, *_settings(rows, vocab, rows))
+
+
+@pytest.mark.parametrize("levels", [1, 2, 5])
+def test_sample_filtered_ties(levels):
+    """Rows of a few different logits: borders fall among equal ones, of which the first by index stay."""
+    rows, vocab = 60, 700
+    g = torch.Generator().manual_seed(levels)
+    z = torch.randint(0, levels, (rows, vocab), generator=g).float() * 0.5
+    _compare(_ops("bfloat16"), z, *_settings(rows, vocab, 5))
+
+
+def test_sample_filtered_edges():
+    vocab = 1500
+    z = torch.randn(16, vocab, generator=torch.Generator().manual_seed(3))
+    z[0] = -math.inf                                   # nothing to draw
+    z[1] = math.nan
+    z[2, :] = -math.inf
+    z[2, 700] = -5.0                                   # a single token
+    z[3, 10:] = -math.inf
+    z[4, ::2] = math.nan
+    z[5, [7, 900]] = math.inf
+    z[6] = torch.finfo(torch.float32).min              # masks of the type's lowest value
+    z[6, 1499] = 3.0
+    z[7] = torch.finfo(torch.float32).min
+    z[8] *= 1e4
+    u = torch.full((16,), 0.5)
+    u[9], u[10] = 0.0, 1.0 - 2.0 ** -24
+    t = torch.full((16,), 0.9)
+    t[11], t[12], t[13] = 1e-30, -1.0, math.nan
+    k = torch.zeros(16, dtype=torch.int32)
+    k[14], k[15] = vocab + 5, 1
+    p, m = torch.ones(16), torch.zeros(16)
+    p[3], p[4] = 0.0, 0.5
+    m[14] = 2.0
+    _compare(_ops("bfloat16"), z, u, t, k, p, m)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 73448), (64, 73448), (200, 40000), (1, 500000)])
+def test_sample_filtered_large_rows(rows, vocab):
+    """The largest vocabularies, against the definition in whole numbers on the device; the last does not fit in shared memory."""
+    ops = _ops("bfloat16")
+    z = (torch.randn(rows, vocab, generator=torch.Generator().manual_seed(1)) * 2).cuda()
+    u, t, k, p, m = (x.cuda() for x in _settings(rows, vocab, 9))
+    t = t.clamp_min(0.5)
+    tok, lp = ops.sample_filtered(z, u, t, k, p, m)
+    again, _ = ops.sample_filtered(z, u, t, k, p, m)
+    assert torch.equal(tok, again)
+    w = torch.exp((z - z.amax(1, keepdim=True)) / t[:, None])
+    units = (w.double() * plain.UNIT).long()
+    ranked, order = torch.sort(w, dim=1, descending=True, stable=True)
+    mass = units.gather(1, order).cumsum(1)
+    n = torch.where(k > 0, k, vocab).long()
+    within = mass.gather(1, n[:, None] - 1)
+    n = torch.where(p < 1, torch.minimum(n, (mass.double() < p.double()[:, None] * within.double()).sum(1) + 1), n)
+    n = torch.where(m > 0, torch.minimum(n, (ranked >= m[:, None]).sum(1)), n).clamp_min(1)
+    keep = torch.zeros_like(z, dtype=torch.bool).scatter(1, order, torch.arange(vocab, device="cuda") < n[:, None])
+    c = torch.where(keep, units, 0).cumsum(1)
+    target = (u.double() * c[:, -1].double()).long()
+    assert torch.equal(tok.long(), (c <= target[:, None]).sum(1))
+    want = (z.double().gather(1, tok.long()[:, None])[:, 0] - z.double().amax(1)) / t.double() - torch.log(c[:, -1].double() / plain.UNIT)
+    assert float((lp.double() - want).abs().max()) < 2e-5
+
+
+def test_sample_filtered_is_distributed_as_it_should():
+    """Frequencies over many given numbers against the kept probabilities: with 200,000 draws a share moves by 0.0011 (one sigma at one half)."""
+    ops, vocab, n = _ops("bfloat16"), 50, 200000
+    z = torch.randn(1, vocab, generator=torch.Generator().manual_seed(4)) * 1.5
+    u = torch.rand(n, generator=torch.Generator().manual_seed(5))
+    full = lambda x, dt=torch.float32: torch.full((n,), x, dtype=dt).cuda()  # noqa: E731
+    tok, lp = ops.sample_filtered(z.expand(n, vocab).contiguous().cuda(), u.cuda(), full(0.8), full(12, torch.int32), full(0.9), full(0.03))
+    share = torch.bincount(tok.long().cpu(), minlength=vocab).double() / n
+    prob = torch.softmax(z[0].double() / 0.8, 0)
+    ranked, order = torch.sort(prob, descending=True)
+    ranked = ranked[:12]
+    count = int((ranked.cumsum(0) < 0.9 * ranked.sum()).sum()) + 1
+    count = min(count, int((ranked >= 0.03 * ranked[0]).sum()))
+    want = torch.zeros(vocab, dtype=torch.float64)
+    want[order[:count]] = prob[order[:count]] / prob[order[:count]].sum()
+    assert float((share - want).abs().max()) < 6 * 0.0011
+    assert float((lp.cpu().double().exp() - want[tok.long().cpu()]).abs().max()) < 1e-5
+
+
+def test_sample_filtered_with_keys_draws_what_sample_draws():
+    """The numbers made from seed and keys are those of ``sample``: without filters both draw from the same distribution at the same place."""
+    ops = _ops("bfloat16")
+    rows, vocab = 300, 90
+    z = (torch.randn(rows, vocab, generator=torch.Generator().manual_seed(6))).cuda()
+    keys, steps = torch.arange(rows, dtype=torch.int32).cuda(), torch.full((rows,), 3, dtype=torch.int32).cuda()
+    t = torch.full((rows,), 1.1).cuda()
+    a = ops.sample(z, t, None, 77, keys, steps)
+    b, _ = ops.sample_filtered(z, None, t, seed=77, seq_key=keys, step_key=steps)
+    # masses are rounded differently: a draw within 1e-6 of a border may fall on its other side
+    assert int((a != b).sum()) <= 1
+
+
+def test_refusals_of_sample_filtered():
+    ops = _ops("bfloat16")
+    z, one = torch.zeros(2, 5).cuda(), torch.ones(2).cuda()
+    ops.sample_filtered(z, one * 0.5, one)
+    for bad in (dict(logits=z.bfloat16()), dict(logits=z[0]), dict(uniform=None), dict(temperature=None), dict(temperature=one[:1]),
+                dict(top_k=one), dict(top_p=one[:1]), dict(min_p=one.double()), dict(logits=torch.zeros(2, 10).cuda()[:, ::2])):
+        with pytest.raises(ValueError):
+            ops.sample_filtered(**{**dict(logits=z, uniform=one * 0.5, temperature=one), **bad})
+    assert ops.sample_filtered(z[:0], one[:0], one[:0])[0].numel() == 0
