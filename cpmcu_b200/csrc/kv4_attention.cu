@@ -9,25 +9,23 @@
 // 2^-14 and 2^15 in the same way.  bf16 queries: p s_v is rounded to fp16 (11 bits; the output has 8).  fp32 queries: q and p s_v are sums of
 // two fp16 numbers (22 bits), which costs a second product each.
 //
-// A block takes an equal share of all (tile, key-value head, page) units of the launch, in that order, so that a batch of unequal
-// sequences leaves no SM idle; a tile that is cut leaves its parts (maximum, sum, weighted values) to a second kernel.  One warp
-// brings whole records (a page of one head, 9,216 bytes at d = 128) into shared memory by bulk copies; four warps take 16 tokens of each
-// record and keep a softmax of their own, so that nothing synchronises them but the arrival of records.
+// One block an SM takes an equal share of all (tile, key-value head, page) units of the launch, in that order, so that a batch of unequal
+// sequences leaves no SM idle; a tile that is cut leaves its parts (weighted values, maximum, sum) to a second kernel.  Four warps take 16 tokens each
+// of a page, and the block's two to four groups of four warps every second to fourth page.  A warp brings its tokens into a ring of its own by
+// asynchronous 16-byte copies, of which a lane reads most of what it copied itself, and keeps a softmax of its own, so that nothing synchronises the
+// warps until a tile ends.  (Bulk copies of a slice's four pieces took longer than the arithmetic: each needs its addresses in uniform
+// registers.  Blocks of four warps, three an SM, leave three times as many parts to add up: 41 us instead of XX for one sequence of 131,071 keys.)
 #include "kv4.cuh"
-#include "tcgen05.cuh"
 
 CPM_BOUNDS_TU(kv4_attention)
 
 namespace {
 
-using namespace tc5;
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-constexpr int kWarps = 4;                              // warps that compute; one more brings the records
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kSlices = 4;                             // warps to a page
 constexpr int kTileTokens = 64;                        // tokens of a prompt's query tile
-constexpr int kMostTiles = 2048;                       // tiles of one launch (their prefix sums lie in shared memory)
-
-__device__ int g_kv4_error;                            // 1: a wait for a record gave up
+constexpr int kMostTiles = 512;                        // tiles of one launch (what they are lies in shared memory)
 
 struct AttendArgs {
     const void* q;
@@ -66,9 +64,8 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs& a, int i, int columns)
 // Units of a tile: pages (one where there is none, for the zeros that such a row gets) times parts and key-value heads.
 __device__ __forceinline__ int tile_units(const Tile& t, int n_kv) { return max(1, t.pages) * t.parts * n_kv; }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -85,12 +82,38 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Waits for a record, with a limit; where a wait has given up before, shortly (for what may still be under way into shared memory).
-__device__ __forceinline__ bool wait_record(uint32_t bar, uint32_t parity, bool alive) {
-    const uint32_t limit = alive ? kSpinLimit : 4096u;
-    for (uint32_t i = 0; i < limit; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    return false;
+// Two fp32 numbers in a register pair: one instruction for both.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 both(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x; below 2^-126 zero, which no sum of weights up to 2^8 notices.
+__device__ __forceinline__ float fast_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // The eight codes of a word as fp16 numbers c - 8: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.  A nibble put into the low bits of 1024
@@ -111,9 +134,9 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&r)[4]) {
 }
 // A lane's words of 16 tokens: word[pair][upper].
 template <int D>
-__device__ __forceinline__ void load_words(const uint8_t* codes, int slice, int lane, uint32_t (&w)[D / 32][2]) {
+__device__ __forceinline__ void load_words(const uint8_t* codes, int lane, uint32_t (&w)[D / 32][2]) {
     using L = Kv4<D>;
-    const uint8_t* p = codes + L::word(slice, 0, lane, 0);
+    const uint8_t* p = codes + L::word(0, 0, lane, 0);
     if constexpr (L::kRun == 2) {
 #pragma unroll
         for (int v = 0; v < D / 64; ++v) {
@@ -134,39 +157,58 @@ __device__ __forceinline__ int shift_of(float most) {
     const int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127 - 10;
     return most > 0.f && most < INFINITY ? max(-120, min(120, e)) : 0;
 }
-constexpr int kNoShift = -1000;                        // no value has been seen yet
+__device__ __forceinline__ float inverse_power2(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }      // of a power of two
 __device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Warps of a block, by what the registers allow: 16 with up to 128 registers a thread, 12 with 168, 8 with 255.
+constexpr int warps_of(int d, int nt, int terms) { return nt == 1 ? 16 : terms == 2 && d > 32 ? 8 : 12; }
 
 template <int D, int NT, int TERMS>
 struct Smem {
-    static constexpr int kStages = D >= 96 ? 5 : 8;
+    static constexpr int kWarps = warps_of(D, NT, TERMS);
+    static constexpr int kStages = D < 96 ? 6 : NT == 1 ? 3 : 4;
     static constexpr int kCols = 8 * NT;
     static constexpr int kQStride = D + 16;            // fp16 numbers a row: rows 32 bytes apart modulo 128
-    alignas(128) uint8_t records[kStages][Kv4<D>::kBytes];
+    // 16 tokens of a record: key codes, value codes, key parameters, value parameters
+    static constexpr int kStage = 2 * Kv4<D>::kSlice + 256;
+    static constexpr int kChunks = kStage / 16, kPieces = (kChunks + 31) / 32;
+    alignas(128) uint8_t ring[kWarps][kStages][kStage];
     alignas(16) __half q[TERMS][kCols][kQStride];
-    alignas(16) float merge[kWarps / 2][kCols][D + 4];
-    float merge_m[kWarps][kCols], merge_l[kWarps][kCols];
+    alignas(16) float merge[kWarps][8][D + 4];
+    alignas(16) float merge_m[kWarps][8], merge_l[kWarps][8];
     float q_sum[kCols][2], factor[kCols];
     int last[kCols];                                   // a column's last key, -1: no such column
-    alignas(8) uint64_t full[kStages], empty[kStages];
-    int scan[kThreads / 32 + 1];
+    int scan[kWarps];
     int prefix[kMostTiles + 1];
+    Tile tiles[kMostTiles];
 };
 
-// Blocks that take a share: each of them at least two units, since every further part costs the second kernel a read.
-__device__ __forceinline__ int sharing_blocks(int64_t units, int blocks) {
-    return (int)min((int64_t)blocks, max((int64_t)1, units / 2));
+// Blocks that take a share: each of them a page for every group of its warps, since every further part costs the second kernel a read; but
+// as many as there are whole rows of pages, for a block goes through these one after the other.
+struct Shares { int sharing, each, more; };            // the first ``more`` blocks have one unit more than ``each``
+__device__ __forceinline__ Shares shares_of(int units, int rows, int groups, int blocks) {
+    const int sharing = min(blocks, max(1, max(min(rows, units), (units + groups - 1) / groups)));
+    return Shares{sharing, units / sharing, units % sharing};
 }
-__device__ __forceinline__ int64_t share_begin(int64_t units, int sharing, int block) { return units * block / sharing; }
-__device__ __forceinline__ int block_of(int64_t unit, int64_t units, int sharing) { return (int)(((unit + 1) * sharing - 1) / units); }
+__device__ __forceinline__ int share_begin(const Shares& s, int block) { return block * s.each + min(block, s.more); }
+__device__ __forceinline__ int block_of(const Shares& s, int unit) {
+    const int longer = s.more * (s.each + 1);
+    return unit < longer ? unit / (s.each + 1) : s.more + (unit - longer) / s.each;
+}
 
-// Prefix sums of the tiles' units; every thread of the block takes part.
-__device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, int* prefix, int* scan) {
+// The tiles and the prefix sums of their units; every thread of the block takes part.
+__device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, Tile* tiles, int* prefix, int* scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int carry = 0;
+#pragma unroll 1
     for (int i0 = 0; i0 < a.n_tiles; i0 += blockDim.x) {
         const int i = i0 + threadIdx.x;
-        const int own = i < a.n_tiles ? tile_units(tile_of(a, i, columns), a.n_kv) : 0;
+        int own = 0;
+        if (i < a.n_tiles) {
+            const Tile t = tile_of(a, i, columns);
+            tiles[i] = t;
+            own = tile_units(t, a.n_kv);
+        }
         int v = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -176,6 +218,7 @@ __device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, int*
         if (lane == 31) scan[warp] = v;
         __syncthreads();
         int before = carry, all = carry;
+#pragma unroll 1
         for (int w = 0; w < warps; ++w) {
             if (w < warp) before += scan[w];
             all += scan[w];
@@ -189,6 +232,7 @@ __device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, int*
 }
 __device__ __forceinline__ int find_tile(const int* prefix, int n, int unit) {
     int lo = 0, hi = n;                                 // the last tile that begins at or before the unit (empty tiles begin where the next does)
+#pragma unroll 1
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (prefix[mid] <= unit) lo = mid; else hi = mid;
@@ -196,503 +240,513 @@ __device__ __forceinline__ int find_tile(const int* prefix, int n, int unit) {
     return lo;
 }
 
-// Blocks that an SM has room for: what the registers allow (207 of a thread at d = 128 and 16 columns, 255 for fp32).
-constexpr int blocks_per_sm(int d, int nt, int terms) { return nt == 1 ? 3 : terms == 2 && d > 32 ? 1 : 2; }
-constexpr int kMostBlocksPerSm = 3;
-
-template <int D> constexpr int64_t part_floats(int columns) { return (int64_t)columns * (D + 2); }
+// Scratch: a head of kHeadInts numbers for every block, then two parts a block.  A part holds for each column the weighted values, the
+// maximum and the sum.  A block whose last tile goes on in other blocks says so in its head, for the kernel that adds up.
+struct CutTile { int last_block, row, part, head, columns; };
+constexpr int kHeadInts = 8;
+template <int D> constexpr int kPartStride = D + 4;
+template <int D>
+__device__ __forceinline__ float* part_of(const AttendArgs& a, int blocks, int block, bool goes_on, int columns) {
+    return a.scratch + (int64_t)blocks * kHeadInts + ((int64_t)block * 2 + (goes_on ? 1 : 0)) * columns * kPartStride<D>;
+}
 
 template <typename T, int D, int NT, int TERMS>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, TERMS))
+__global__ void __launch_bounds__(32 * warps_of(D, NT, TERMS), 1)
 kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
     using L = Kv4<D>;
     using S = Smem<D, NT, TERMS>;
-    constexpr int COLS = S::kCols, STEPS = D / 16, E = D / 32;
-    extern __shared__ uint8_t raw[];
-    S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~(uintptr_t)127);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(smem_u32(&sm.full[i]), 1);
-            mbar_init(smem_u32(&sm.empty[i]), kWarps);
-        }
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
+    constexpr int COLS = S::kCols, STEPS = D / 16, E = D / 32, STAGES = S::kStages, WARPS = S::kWarps, GROUPS = WARPS / kSlices;
+    constexpr bool Q_IN_REGISTERS = NT == 1 && TERMS == 1;      // else they are read again for every 16 tokens: 32 registers more would leave room for a block less
+    extern __shared__ __align__(128) uint8_t raw[];
+    S& sm = *reinterpret_cast<S*>(raw);                  // (no arithmetic on the address: the compiler would lose that it is shared memory)
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slice = warp % kSlices, turn = warp / kSlices;      // its tokens of a page, and of how many pages the how-manieth
     pdl_launch_dependents();
     pdl_wait();
-    sum_tiles(a, COLS, sm.prefix, sm.scan);
-    const int64_t units = sm.prefix[a.n_tiles];
-    const int sharing = sharing_blocks(units, gridDim.x);
-    if ((int)blockIdx.x >= sharing || units == 0) return;
-    const int64_t begin = share_begin(units, sharing, blockIdx.x), end = share_begin(units, sharing, blockIdx.x + 1);
-    int64_t unit = begin;
-    int index = find_tile(sm.prefix, a.n_tiles, (int)unit);
+    sum_tiles(a, COLS, sm.tiles, sm.prefix, sm.scan);
+    const int units = sm.prefix[a.n_tiles];
+    const Shares shares = shares_of(units, a.cu_q ? 0 : a.n_tiles * a.n_kv * ((a.group + COLS - 1) / COLS), GROUPS, gridDim.x);
+    if (threadIdx.x == 0) reinterpret_cast<CutTile*>(a.scratch + (int64_t)blockIdx.x * kHeadInts)->last_block = -1;
+    if ((int)blockIdx.x >= shares.sharing || units == 0) return;
+    const int begin = share_begin(shares, blockIdx.x), end = share_begin(shares, blockIdx.x + 1);
+    const int start = find_tile(sm.prefix, a.n_tiles, begin);
 
-    if (warp == kWarps) {
-        // ---- the warp that brings records ----
-        bool alive = true;
-        int it = 0;
-        while (unit < end) {
-            while (sm.prefix[index + 1] <= unit) ++index;
-            const Tile t = tile_of(a, index, COLS);
-            const int pages = max(1, t.pages);
-            const int at = (int)unit - sm.prefix[index];
-            int page = at % pages;
-            const int head = (at / pages) % a.n_kv;
-            const int stop = (int)min((int64_t)pages, page + (end - unit));
-            unit += stop - page;
-            const int* table = a.page_table + (int64_t)t.slot * a.max_pages;
-            for (; page < stop; page += 32) {
-                const int n = min(32, stop - page);
-                const int mine = lane < n && t.pages > 0 ? CPM_PAGE(table, t.page0 + page + lane, a.max_pages) : 0;
-                for (int i = 0; i < n; ++i, ++it) {
-                    const int number = __shfl_sync(0xffffffffu, mine, i);
-                    const int stage = it % S::kStages;
-                    if (it >= S::kStages && alive)
-                        alive = mbar_wait_bounded(smem_u32(&sm.empty[stage]), ((it / S::kStages) & 1) ^ 1);
-                    if (lane == 0) {
-                        const uint32_t bar = smem_u32(&sm.full[stage]);
-                        if (t.pages > 0 && alive) {
-                            mbar_expect_tx(bar, L::kBytes);
-                            bulk_load(smem_u32(sm.records[stage]), a.records + ((int64_t)number * a.n_kv + head) * L::kBytes, L::kBytes, bar);
-                        } else {
-                            mbar_arrive(bar);            // a row without keys: nothing to bring
-                        }
-                    }
-                    __syncwarp();
-                }
+    // ---- what the warp has asked for: it runs ahead of what it works on by the ring's length, across the borders of tiles ----
+    // (units that are the warp's: every GROUPS-th of the block's, from ``turn`` on)
+    int ask_unit = begin + turn, ask_index = start, ask_end = begin, ask_page = 0, ask_ids = 0, ask_base = 0, ask_first = 0, asked = 0;
+    const int* ask_table = a.page_table;
+    const uint8_t* ask_records = a.records;
+    bool ask_any = false;
+    // where in a record the lane's i-th 16 bytes of a slice come from: key codes, value codes, key parameters, value parameters
+    const auto ask_from = [&](int i) {
+        const int c = 32 * i + lane;
+        return c < D / 2 ? slice * L::kSlice + 16 * c : c < D ? L::kValues + slice * L::kSlice + 16 * (c - D / 2)
+             : (c < D + 8 ? L::kKeyParams : L::kValueParams - 128) + slice * 128 + 16 * (c - D);
+    };
+    const auto ask = [&]() {
+        if (ask_unit < end) {
+            if (ask_unit >= ask_end) {                    // another row of pages: a tile's for one key-value head and part
+#pragma unroll 1
+                while (sm.prefix[ask_index + 1] <= ask_unit) ++ask_index;
+                const Tile t = sm.tiles[ask_index];
+                const uint32_t pages = max(1, t.pages), at = ask_unit - sm.prefix[ask_index], whole = at / pages;
+                ask_page = at - whole * pages;
+                ask_end = ask_unit - ask_page + (int)pages;
+                ask_any = t.pages > 0;
+                ask_first = t.page0;
+                ask_table = a.page_table + (int64_t)t.slot * a.max_pages;
+                ask_records = a.records + (int64_t)(whole % (uint32_t)a.n_kv) * L::kBytes;
+                ask_base = ask_page - 32 * GROUPS;
             }
+            if (ask_page - ask_base >= 32 * GROUPS) {      // the next 32 page numbers, one a lane
+                ask_base = ask_page;
+                const int i = ask_page + lane * GROUPS;
+                ask_ids = i - ask_page < min(ask_end, end) - ask_unit && ask_any ? CPM_PAGE(ask_table, ask_first + i, a.max_pages) : 0;
+            }
+            const int number = __shfl_sync(0xffffffffu, ask_ids, (ask_page - ask_base) / GROUPS);
+            if (ask_any) {                                 // (a row without keys: nothing to bring)
+                const uint8_t* from = ask_records + (int64_t)number * a.n_kv * L::kBytes;
+                const uint32_t to = smem_u32(sm.ring[warp][asked]) + lane * 16;
+#pragma unroll
+                for (int i = 0; i < S::kPieces; ++i)
+                    if (32 * i + 31 < S::kChunks || lane < S::kChunks - 32 * i) copy16(to + 512 * i, from + ask_from(i));
+            }
+            ask_page += GROUPS;
+            ask_unit += GROUPS;
+            if (++asked == STAGES) asked = 0;
         }
-        if (!alive && lane == 0) atomicExch(&g_kv4_error, 1);
-        return;
-    }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; ++i) ask();
 
-    // ---- the warps that compute ----
+    // ---- what it works on.  One loop over slices, with a tile's beginning and end inside: every part of the code is there once, since a
+    // block runs most of it a few times only and the first run of an instruction comes from L2 (80 KB of unrolled code took 25 us for one page) ----
     const int g = lane >> 2, j = lane & 3;
-    bool alive = true;
-    int it = 0;
-    while (unit < end) {
-        while (sm.prefix[index + 1] <= unit) ++index;
-        const Tile t = tile_of(a, index, COLS);
-        const int pages = max(1, t.pages);
-        const int at = (int)unit - sm.prefix[index];
-        const int first_page = at % pages, head = (at / pages) % a.n_kv, part = at / pages / a.n_kv;
-        const int stop = (int)min((int64_t)pages, first_page + (end - unit));
-        const int columns = min(COLS, t.tokens * a.group - part * COLS);
+    int unit = begin, index = start, stage = 0;
+    uint2 qf[Q_IN_REGISTERS ? STEPS : 1];
+    // of a lane's two columns of every eight: q's sums, the factor of the scores, minus the running maximum, the sum of weights, the
+    // power of two that p s_v is multiplied by, and the sums of p m_v
+    f32x2 q_sum[NT][2], factor[NT], minus[NT], sum[NT], down[NT], middle[NT][2];
+    float o[STEPS][NT][4];
+    float limit = 0.f;                                                                 // a value's scale above it makes ``down`` move
+    uint32_t blank = 0;                                                                // bit 2 n + c: the column has seen no key yet
+    const auto q_fragment = [&](int u, int k, int n) { return *reinterpret_cast<const uint2*>(&sm.q[u][8 * n + g][16 * k + 4 * j]); };
 
-        // queries of the tile: divided by a power of two, in fp16 (TERMS = 2: and what that leaves)
-        for (int c = warp; c < COLS; c += kWarps) {
-            float x[E];
-            const int n = part * COLS + c;
-            const int64_t row = ((int64_t)(t.row + n / a.group) * a.n_heads + head * a.group + n % a.group) * D;
-            float most = 0.f;
+#pragma unroll 1
+    while (unit < end) {
+        // ---- a tile begins ----
+#pragma unroll 1
+        while (sm.prefix[index + 1] <= unit) ++index;
+        const Tile t = sm.tiles[index];
+        const int pages = max(1, t.pages);
+        const uint32_t at = unit - sm.prefix[index], before = at / (uint32_t)pages;
+        const int first_page = at - before * pages, part = before / (uint32_t)a.n_kv, head = before - part * a.n_kv;
+        const int stop = min(pages, first_page + (end - unit));
+        const int columns = min(COLS, t.tokens * a.group - part * COLS), row = t.row;
+        const int key0 = t.page0 * kPageTokens + 16 * slice;
+        const int low = t.first_pos + part * COLS / a.group;                               // the last key that every column sees
+        const int top = t.pages > 0 ? t.first_pos + (part * COLS + columns - 1) / a.group : -1;      // the last that any column sees
+            // queries: divided by a power of two, in fp16 (TERMS = 2: and what that leaves).  All columns at once, some threads to each
+            if (threadIdx.x < 128) {
+                constexpr int PER = 128 / COLS, EP = D / PER;
+                const int c = threadIdx.x / PER, n = part * COLS + c, from = threadIdx.x % PER * EP;
+                const T* q = reinterpret_cast<const T*>(a.q) + ((int64_t)(row + n / a.group) * a.n_heads + head * a.group + n % a.group) * D + from;
+                float x[EP], most = 0.f;
+                if constexpr (EP % 4 == 0) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                x[i] = c < columns ? to_f32(reinterpret_cast<const T*>(a.q)[row + lane * E + i]) : 0.f;
-                most = fmaxf(most, fabsf(x[i]));
-            }
-            const int e = shift_of(warp_max(most));
-            const float down = power2(-e);
-            float sum = 0.f;
+                    for (int i = 0; i < EP; i += 4) {
+                        const float4 v = c < columns ? load4(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+                    }
+                } else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float y = x[i] * down;
-                sum += y;
-                const __half h = __float2half_rn(y);
-                sm.q[0][c][lane * E + i] = h;
-                if constexpr (TERMS == 2) sm.q[1][c][lane * E + i] = __float2half_rn(y - __half2float(h));
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if ((lane & 15) == 0) sm.q_sum[c][lane >> 4] = sum;
-            if (lane == 0) {
-                sm.factor[c] = power2(e) * a.scale * 1.4426950408889634f;
-                sm.last[c] = c < columns ? t.first_pos + n / a.group : -1;
-            }
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        uint32_t qf[TERMS][STEPS][NT][2];
-        float qs[NT][2][2], factor[NT][2];
-        int last[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                for (int u = 0; u < TERMS; ++u) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(&sm.q[u][8 * n + g][16 * k + 4 * j]);
-                    qf[u][k][n][0] = v.x;
-                    qf[u][k][n][1] = v.y;
+                    for (int i = 0; i < EP; ++i) x[i] = c < columns ? to_f32(q[i]) : 0.f;
                 }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int c = 8 * n + 2 * j + i;
-                qs[n][i][0] = sm.q_sum[c][0];
-                qs[n][i][1] = sm.q_sum[c][1];
-                factor[n][i] = sm.factor[c];
-                last[n][i] = sm.last[c];
+                for (int i = 0; i < EP; ++i) most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+                for (int d = 1; d < PER; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                const int e = shift_of(most);
+                const float by = power2(-e);
+                float total = 0.f;
+#pragma unroll
+                for (int i = 0; i < EP; i += 2) {
+                    const float y0 = x[i] * by, y1 = x[i + 1] * by;
+                    total += y0 + y1;
+                    const __half2 h = __floats2half2_rn(y0, y1);
+                    *reinterpret_cast<__half2*>(&sm.q[0][c][from + i]) = h;
+                    if constexpr (TERMS == 2) *reinterpret_cast<__half2*>(&sm.q[1][c][from + i]) = __floats2half2_rn(y0 - __low2float(h), y1 - __high2float(h));
+                }
+#pragma unroll
+                for (int d = 1; d < PER / 2; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+                if (threadIdx.x % (PER / 2) == 0) sm.q_sum[c][threadIdx.x % PER / (PER / 2)] = total;
+                if (from == 0) {
+                    sm.factor[c] = power2(e) * a.scale * 1.4426950408889634f;
+                    sm.last[c] = c < columns ? t.first_pos + n / a.group : -1;
+                }
             }
-        }
-        const int top = t.first_pos + (part * COLS + columns - 1) / a.group;           // the last key that any column sees
-        const int low = t.first_pos + part * COLS / a.group;                           // the last key that every column sees
+            __syncthreads();
+            if constexpr (Q_IN_REGISTERS)
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) qf[k] = q_fragment(0, k, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int c = 8 * n + 2 * j;
+                q_sum[n][0] = pair(sm.q_sum[c][0], sm.q_sum[c + 1][0]);
+                q_sum[n][1] = pair(sm.q_sum[c][1], sm.q_sum[c + 1][1]);
+                factor[n] = pair(sm.factor[c], sm.factor[c + 1]);
+                minus[n] = sum[n] = down[n] = middle[n][0] = middle[n][1] = pair(0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
+            }
+            limit = -1.f;
+            blank = 0xffffffffu;
 
-        float o[STEPS][NT][4], middle[NT][2][2], l[NT][2], m[NT][2];
+#pragma unroll 1
+        for (int page = first_page + (GROUPS + turn - (unit - begin) % GROUPS) % GROUPS; page < stop; page += GROUPS) {
+        ask();                                                                         // into the place that the last slice left
+        asm volatile("cp.async.wait_group %0;" :: "n"(STAGES - 1) : "memory");
+        __syncwarp();
+        const uint8_t* rec = sm.ring[warp][stage];
+        if (++stage == STAGES) stage = 0;
+        const int token0 = key0 + page * kPageTokens;
+        // a slice behind every column's last key, or before every window, has nothing to give
+        if (token0 <= top && (a.window == 0 || token0 + 15 > low - a.window)) {
+            uint2 kp[2], vp[2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                middle[n][i][0] = middle[n][i][1] = l[n][i] = 0.f;
-                m[n][i] = -INFINITY;
+            for (int r = 0; r < 2; ++r) {
+                kp[r] = *reinterpret_cast<const uint2*>(rec + 2 * L::kSlice + (g + 8 * r) * 8);
+                vp[r] = *reinterpret_cast<const uint2*>(rec + 2 * L::kSlice + 128 + (g + 8 * r) * 8);
             }
-        }
-        int shift[NT][2];                                                               // p s_v is kept divided by 2^shift
-#pragma unroll
-        for (int n = 0; n < NT; ++n) shift[n][0] = shift[n][1] = kNoShift;
-
-        for (int page = first_page; page < stop; ++page, ++it) {
-            const int stage = it % S::kStages;
-            if (!wait_record(smem_u32(&sm.full[stage]), (it / S::kStages) & 1, alive) && alive) {
-                alive = false;
-                atomicExch(&g_kv4_error, 1);
-            }
-            const uint8_t* rec = sm.records[stage];
-            const int token0 = (t.page0 + page) * kPageTokens + 16 * warp;
-            // a slice behind every column's last key, or before every window, has nothing to give
-            if (token0 <= top && (a.window == 0 || token0 + 15 > low - a.window) && t.pages > 0) {
-                const bool masked = token0 + 15 > low || (a.window && token0 <= top - a.window);
-                uint2 kp[2], vp[2];
+            uint32_t seen = 0xffffffffu;                                               // bit 4 n + 2 r + c: row g + 8 r is seen by the lane's column c
+            if (token0 + 15 > low || (a.window && token0 <= top - a.window)) {
+                seen = 0;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    kp[r] = *reinterpret_cast<const uint2*>(rec + L::kKeyParams + (16 * warp + g + 8 * r) * 8);
-                    vp[r] = *reinterpret_cast<const uint2*>(rec + L::kValueParams + (16 * warp + g + 8 * r) * 8);
-                    if (masked && token0 + g + 8 * r > top) kp[r] = vp[r] = make_uint2(0u, 0u);     // what lies there may be no number
-                }
-                // ---- scores ----
-                float s[2][NT][4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[h][n][i] = 0.f;
-                {
-                    uint32_t w[E][2];
-                    load_words<D>(rec, warp, lane, w);
-#pragma unroll
-                    for (int p = 0; p < E; ++p) {
-                        uint32_t lo[4], hi[4];
-                        unpack8(w[p][0], lo);
-                        unpack8(w[p][1], hi);
-#pragma unroll
-                        for (int odd = 0; odd < 2; ++odd) {
-                            const int k = 2 * p + odd;
-                            const uint32_t frag[4] = {lo[2 * odd], hi[2 * odd], lo[2 * odd + 1], hi[2 * odd + 1]};
-#pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int u = 0; u < TERMS; ++u) mma_f16(s[k * 2 / STEPS][n], frag, qf[u][k][n][0], qf[u][k][n][1]);
-                        }
-                    }
-                }
-                float x[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = i >> 1, c = i & 1;
-                        float v = s[0][n][i] * kv4_scale(kp[r].x) + s[1][n][i] * kv4_scale(kp[r].y);
-                        v += kv4_middle(kp[r].x) * qs[n][c][0] + kv4_middle(kp[r].y) * qs[n][c][1];
-                        x[n][i] = v * factor[n][c];
-                        if (masked) {
-                            const int token = token0 + g + 8 * r;
-                            if (token > last[n][c] || (a.window && token <= last[n][c] - a.window)) x[n][i] = -INFINITY;
-                        }
-                    }
-                // ---- the softmax's running maximum: it may lie up to 2^8 behind, so that it seldom moves ----
-                bool behind = false;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) behind |= x[n][i] > m[n][i & 1] + 8.f;
-                if (__any_sync(0xffffffffu, behind)) {
+                    const int token = token0 + g + 8 * r;
+                    if (token > top) kp[r] = vp[r] = make_uint2(0u, 0u);                // what lies there may be no number
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float v = fmaxf(x[n][c], x[n][2 + c]);
-#pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                            const float now = fmaxf(m[n][c], v);
-                            const float by = now > -INFINITY ? exp2f(m[n][c] - now) : 1.f;
-                            m[n][c] = now;
-                            l[n][c] *= by;
-                            middle[n][c][0] *= by;
-                            middle[n][c][1] *= by;
-#pragma unroll
-                            for (int k = 0; k < STEPS; ++k) { o[k][n][c] *= by; o[k][n][2 + c] *= by; }
+                            const int last = sm.last[8 * n + 2 * j + c];
+                            if (token <= last && (a.window == 0 || token > last - a.window)) seen |= 1u << (4 * n + 2 * r + c);
                         }
+                    // A row that only some columns see and that is no number would reach the others as 0 * NaN: it goes to
+                    // those that see it here, and is nobody's afterwards.
+                    const bool kbad = !(fabsf(kv4_scale(kp[r].x)) + fabsf(kv4_middle(kp[r].x)) + fabsf(kv4_scale(kp[r].y)) + fabsf(kv4_middle(kp[r].y)) < INFINITY);
+                    const bool bad0 = kbad || !(fabsf(kv4_scale(vp[r].x)) + fabsf(kv4_middle(vp[r].x)) < INFINITY);
+                    const bool bad1 = kbad || !(fabsf(kv4_scale(vp[r].y)) + fabsf(kv4_middle(vp[r].y)) < INFINITY);
+                    if (bad0 || bad1) {
+                        kp[r] = vp[r] = make_uint2(0u, 0u);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const f32x2 poison = pair(seen >> (4 * n + 2 * r) & 1 ? NAN : 0.f, seen >> (4 * n + 2 * r + 1) & 1 ? NAN : 0.f);
+                            if (bad0) middle[n][0] = add2(middle[n][0], poison);
+                            if (bad1) middle[n][1] = add2(middle[n][1], poison);
+                            seen &= ~(3u << (4 * n + 2 * r));
+                        }
+                    }
                 }
+            }
+            // ---- scores ----
+            float s[2][NT][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float by = m[n][i & 1];
-                        x[n][i] = masked && x[n][i] == -INFINITY ? 0.f : exp2f(x[n][i] - by);
-                        l[n][i & 1] += x[n][i];
+                    for (int i = 0; i < 4; ++i) s[h][n][i] = 0.f;
+            {
+                uint32_t w[E][2];
+                load_words<D>(rec, lane, w);
+#pragma unroll
+                for (int p = 0; p < E; ++p) {
+                    uint32_t lo[4], hi[4];
+                    unpack8(w[p][0], lo);
+                    unpack8(w[p][1], hi);
+#pragma unroll
+                    for (int odd = 0; odd < 2; ++odd) {
+                        const int k = 2 * p + odd;
+                        const uint32_t frag[4] = {lo[2 * odd], hi[2 * odd], lo[2 * odd + 1], hi[2 * odd + 1]};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int u = 0; u < TERMS; ++u) {
+                                const uint2 b = Q_IN_REGISTERS ? qf[Q_IN_REGISTERS ? k : 0] : q_fragment(u, k, n);
+                                mma_f16(s[k * 2 / STEPS][n], frag, b.x, b.y);
+                            }
                     }
-                // ---- the scale of p s_v: moves where a value's scale is more than 2^4 above it ----
-                const float sv[2][2] = {{kv4_scale(vp[0].x), kv4_scale(vp[0].y)}, {kv4_scale(vp[1].x), kv4_scale(vp[1].y)}};
-                const float most = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-                const int e = (int)(__float_as_uint(most) >> 23) - 127;
-                bool above = false;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) above |= e > min(shift[n][0], shift[n][1]) + 4;
-                if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            int now = kNoShift;                                        // of the values that the column sees and that are numbers
-#pragma unroll
-                            for (int r = 0; r < 2; ++r) {
-                                const float v = fmaxf(sv[r][0] < INFINITY ? sv[r][0] : 0.f, sv[r][1] < INFINITY ? sv[r][1] : 0.f);
-                                if (x[n][2 * r + c] > 0.f) now = max(now, (int)(__float_as_uint(v) >> 23) - 127);
-                            }
-#pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) now = max(now, __shfl_xor_sync(0xffffffffu, now, d));
-                            now = min(120, now);
-                            if (now > shift[n][c]) {
-                                now = max(-120, now);
-                                const float by = shift[n][c] > kNoShift ? exp2f((float)(shift[n][c] - now)) : 0.f;
-                                shift[n][c] = now;
-#pragma unroll
-                                for (int k = 0; k < STEPS; ++k) { o[k][n][c] *= by; o[k][n][2 + c] *= by; }
-                            }
-                        }
                 }
-                // ---- weights times scales, as the operand with tokens along K ----
-                uint32_t pf[TERMS][2][NT][2];
+            }
+            float x[NT][4], highest = -INFINITY;                                       // scores (of 2^x) less the running maximum
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const f32x2 s0 = pair(kv4_scale(kp[r].x), kv4_scale(kp[r].x)), s1 = pair(kv4_scale(kp[r].y), kv4_scale(kp[r].y));
+                const f32x2 m0 = pair(kv4_middle(kp[r].x), kv4_middle(kp[r].x)), m1 = pair(kv4_middle(kp[r].y), kv4_middle(kp[r].y));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float down[2] = {shift[n][0] > kNoShift ? power2(-shift[n][0]) : 0.f, shift[n][1] > kNoShift ? power2(-shift[n][1]) : 0.f};
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float x0 = x[n][2 * r], x1 = x[n][2 * r + 1], d0 = x0 * down[0], d1 = x1 * down[1];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float md = kv4_middle(h ? vp[r].y : vp[r].x);
-                            float y0 = d0 * sv[r][h], y1 = d1 * sv[r][h], z0 = x0 * md, z1 = x1 * md;
-                            if (masked) {                                              // a key that is not seen may have parameters that are no numbers
-                                if (x0 == 0.f) y0 = z0 = 0.f;
-                                if (x1 == 0.f) y1 = z1 = 0.f;
-                            }
-                            middle[n][0][h] += z0;
-                            middle[n][1][h] += z1;
-                            const uint32_t p = pack_half2(y0, y1);
-                            pf[0][h][n][r] = transpose8(p);
-                            if constexpr (TERMS == 2) {
-                                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&p));
-                                pf[TERMS - 1][h][n][r] = transpose8(pack_half2(y0 - back.x, y1 - back.y));
-                            }
-                        }
-                    }
+                    const f32x2 v = fma2(pair(s[0][n][2 * r], s[0][n][2 * r + 1]), s0, fma2(pair(s[1][n][2 * r], s[1][n][2 * r + 1]), s1, fma2(m0, q_sum[n][0], mul2(m1, q_sum[n][1]))));
+                    const float2 e = both(fma2(v, factor[n], minus[n]));
+                    x[n][2 * r] = seen & (1u << (4 * n + 2 * r)) ? e.x : -INFINITY;
+                    x[n][2 * r + 1] = seen & (2u << (4 * n + 2 * r)) ? e.y : -INFINITY;
+                    highest = fmaxf(highest, fmaxf(x[n][2 * r], x[n][2 * r + 1]));
                 }
-                // ---- weighted values ----
-                {
-                    uint32_t w[E][2];
-                    load_words<D>(rec + L::kValues, warp, lane, w);
+            }
+            const float sv[2][2] = {{kv4_scale(vp[0].x), kv4_scale(vp[0].y)}, {kv4_scale(vp[1].x), kv4_scale(vp[1].y)}};
+            const float largest = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+            // ---- the running maximum may lie up to 2^8 behind, and ``down`` fit scales up to 2^4 smaller, so that both seldom move ----
+            if (__any_sync(0xffffffffu, highest > 8.f || !(largest <= limit))) {
+                limit = INFINITY;
 #pragma unroll
-                    for (int p = 0; p < E; ++p) {
-                        uint32_t lo[4], hi[4];
-                        unpack8(w[p][0], lo);
-                        unpack8(w[p][1], hi);
+                for (int n = 0; n < NT; ++n) {
+                    const float2 old = both(minus[n]), was2 = both(down[n]);
+                    float now[2], next[2], by[2], shrink[2];
 #pragma unroll
-                        for (int odd = 0; odd < 2; ++odd) {
-                            const int k = 2 * p + odd;
-                            const uint32_t frag[4] = {lo[2 * odd], lo[2 * odd + 1], hi[2 * odd], hi[2 * odd + 1]};
+                    for (int c = 0; c < 2; ++c) {
+                        float high = -INFINITY, most = 0.f;
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
+                        for (int r = 0; r < 2; ++r) {
+                            const bool there = seen & ((1u << c) << (4 * n + 2 * r));
+                            x[n][2 * r + c] -= c ? old.y : old.x;
+                            high = fmaxf(high, x[n][2 * r + c]);
+                            if (there) most = fmaxf(most, fmaxf(sv[r][0] < INFINITY ? sv[r][0] : 0.f, sv[r][1] < INFINITY ? sv[r][1] : 0.f));
+                        }
 #pragma unroll
-                                for (int u = 0; u < TERMS; ++u) mma_f16(o[k][n], frag, pf[u][k * 2 / STEPS][n][0], pf[u][k * 2 / STEPS][n][1]);
+                        for (int d = 4; d < 32; d <<= 1) {
+                            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+                            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                        }
+                        const bool first = blank >> (2 * n + c) & 1;
+                        const float before = first ? -INFINITY : -(c ? old.y : old.x), was = c ? was2.y : was2.x;
+                        now[c] = fmaxf(before, high);
+                        by[c] = first ? 0.f : fast_exp2(before - now[c]);
+                        if (now[c] > -INFINITY) blank &= ~(1u << (2 * n + c));
+                        else now[c] = 0.f;
+                        // one over the power of two below the largest scale that the column has seen (0: none above 0)
+                        const float fit = most > 0.f ? power2(-max(-120, min(120, (int)(__float_as_uint(most) >> 23) - 127))) : 0.f;
+                        next[c] = was == 0.f ? fit : fit > 0.f ? fminf(was, fit) : was;
+                        shrink[c] = was > 0.f ? by[c] * (next[c] * inverse_power2(was)) : by[c];
+                        limit = fminf(limit, blank >> (2 * n + c) & 1 ? -1.f : next[c] > 0.f ? 16.f * inverse_power2(next[c]) : 0.f);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) x[n][2 * r + c] -= now[c];
+                    }
+                    const f32x2 b = pair(by[0], by[1]), z = pair(shrink[0], shrink[1]);
+                    minus[n] = pair(-now[0], -now[1]);
+                    down[n] = pair(next[0], next[1]);
+                    sum[n] = mul2(sum[n], b);
+                    middle[n][0] = mul2(middle[n][0], b);
+                    middle[n][1] = mul2(middle[n][1], b);
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float2 y = both(mul2(pair(o[k][n][2 * r], o[k][n][2 * r + 1]), z));
+                            o[k][n][2 * r] = y.x;
+                            o[k][n][2 * r + 1] = y.y;
+                        }
+                }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) limit = fminf(limit, __shfl_xor_sync(0xffffffffu, limit, d));
+            }
+            // ---- weights, and weights times scales as the operand with tokens along K ----
+            uint32_t pf[TERMS][2][NT][2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const f32x2 scale[2] = {pair(sv[r][0], sv[r][0]), pair(sv[r][1], sv[r][1])};
+                const f32x2 md[2] = {pair(kv4_middle(vp[r].x), kv4_middle(vp[r].x)), pair(kv4_middle(vp[r].y), kv4_middle(vp[r].y))};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const f32x2 p = pair(fast_exp2(x[n][2 * r]), fast_exp2(x[n][2 * r + 1])), d = mul2(p, down[n]);
+                    sum[n] = add2(sum[n], p);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 y = both(mul2(d, scale[h]));
+                        middle[n][h] = fma2(p, md[h], middle[n][h]);
+                        const uint32_t packed = pack_half2(y.x, y.y);
+                        pf[0][h][n][r] = transpose8(packed);
+                        if constexpr (TERMS == 2) {
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+                            pf[TERMS - 1][h][n][r] = transpose8(pack_half2(y.x - back.x, y.y - back.y));
                         }
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.empty[stage]));
+            // ---- weighted values ----
+            {
+                uint32_t w[E][2];
+                load_words<D>(rec + L::kSlice, lane, w);
+#pragma unroll
+                for (int p = 0; p < E; ++p) {
+                    uint32_t lo[4], hi[4];
+                    unpack8(w[p][0], lo);
+                    unpack8(w[p][1], hi);
+#pragma unroll
+                    for (int odd = 0; odd < 2; ++odd) {
+                        const int k = 2 * p + odd;
+                        const uint32_t frag[4] = {lo[2 * odd], lo[2 * odd + 1], hi[2 * odd], hi[2 * odd + 1]};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int u = 0; u < TERMS; ++u) mma_f16(o[k][n], frag, pf[u][k * 2 / STEPS][n][0], pf[u][k * 2 / STEPS][n][1]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
         }
 
-        // ---- the four warps' parts become one ----
+        // ---- a tile, or the block's part of it, ends: the warps' parts become one, eight columns at a time ----
+        const bool whole = first_page == 0 && stop == pages;
+        // a part of a tile that an earlier block began lies in the block's first place, one that goes on behind it in the second
+        float* mine = part_of<D>(a, gridDim.x, blockIdx.x, first_page == 0, COLS);
+        if (!whole && first_page == 0 && threadIdx.x == 0)
+            *reinterpret_cast<CutTile*>(a.scratch + (int64_t)blockIdx.x * kHeadInts) =
+                CutTile{block_of(shares, unit - first_page + pages - 1), row, part, head, columns};
+        const auto leave = [&](int n) {
+            const float2 m = both(minus[n]), d = both(down[n]);
+            if (g == 0) *reinterpret_cast<float2*>(&sm.merge_m[warp][2 * j]) = make_float2(blank >> (2 * n) & 1 ? -INFINITY : -m.x, blank >> (2 * n + 1) & 1 ? -INFINITY : -m.y);
+            const f32x2 up = pair(d.x > 0.f ? inverse_power2(d.x) : 0.f, d.y > 0.f ? inverse_power2(d.y) : 0.f);
+            f32x2 l = sum[n], mid[2] = {middle[n][0], middle[n][1]};
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) {
-                    l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], d);
-                    middle[n][c][0] += __shfl_xor_sync(0xffffffffu, middle[n][c][0], d);
-                    middle[n][c][1] += __shfl_xor_sync(0xffffffffu, middle[n][c][1], d);
-                }
-        if (g == 0)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    sm.merge_m[warp][8 * n + 2 * j + c] = m[n][c];
-                    sm.merge_l[warp][8 * n + 2 * j + c] = l[n][c];
-                }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        float all_m[NT][2], all_l[NT][2], by[NT][2], up[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = 8 * n + 2 * j + c;
-                float v = sm.merge_m[0][col];
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) v = fmaxf(v, sm.merge_m[w][col]);
-                float sum = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w)
-                    if (sm.merge_m[w][col] > -INFINITY) sum += sm.merge_l[w][col] * exp2f(sm.merge_m[w][col] - v);
-                all_m[n][c] = v;
-                all_l[n][c] = sum;
-                up[n][c] = shift[n][c] > kNoShift ? power2(shift[n][c]) : 0.f;
-                by[n][c] = m[n][c] > -INFINITY ? exp2f(m[n][c] - v) : 0.f;
+            for (int i = 4; i < 32; i <<= 1) {
+                l = add2(l, __shfl_xor_sync(0xffffffffu, l, i));
+                mid[0] = add2(mid[0], __shfl_xor_sync(0xffffffffu, mid[0], i));
+                mid[1] = add2(mid[1], __shfl_xor_sync(0xffffffffu, mid[1], i));
             }
-        // channel of a lane's sums: block k, channels 2 g (i < 2) and 2 g + 1
+            if (g == 0) *reinterpret_cast<float2*>(&sm.merge_l[warp][2 * j]) = both(l);
+            // channel of a lane's sums: block k, channels 2 g (the first two) and 2 g + 1
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = i & 1;
-                    o[k][n][i] = by[n][c] > 0.f ? (o[k][n][i] * up[n][c] + middle[n][c][k * 2 / STEPS]) * by[n][c] : 0.f;
-                }
-#pragma unroll
-        for (int round = kWarps / 2; round > 0; round >>= 1) {
-            if (warp >= round && warp < 2 * round) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-                            *reinterpret_cast<float2*>(&sm.merge[warp - round][8 * n + 2 * j + c][16 * k + 2 * g]) = make_float2(o[k][n][c], o[k][n][2 + c]);
+            for (int k = 0; k < STEPS; ++k) {
+                const float2 even = both(fma2(pair(o[k][n][0], o[k][n][1]), up, mid[k * 2 / STEPS])), odd = both(fma2(pair(o[k][n][2], o[k][n][3]), up, mid[k * 2 / STEPS]));
+                *reinterpret_cast<float2*>(&sm.merge[warp][2 * j][16 * k + 2 * g]) = make_float2(even.x, odd.x);
+                *reinterpret_cast<float2*>(&sm.merge[warp][2 * j + 1][16 * k + 2 * g]) = make_float2(even.y, odd.y);
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (warp < round) {
+        };
+#pragma unroll 1
+        for (int n = 0; n < NT; ++n) {
+            if (NT == 1 || n == 0) leave(0);
+            else leave(NT - 1);
+            __syncthreads();
+            constexpr int EP = D / 16;                                                  // 16 threads to a column
+            const int col = threadIdx.x / 16, from = threadIdx.x % 16 * EP;
+            if (col < min(8, columns - 8 * n)) {
+                float high = -INFINITY, total = 0.f, y[EP];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int w = 0; w < WARPS; ++w) high = fmaxf(high, sm.merge_m[w][col]);
 #pragma unroll
-                    for (int k = 0; k < STEPS; ++k)
+                for (int i = 0; i < EP; ++i) y[i] = 0.f;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const float2 v = *reinterpret_cast<const float2*>(&sm.merge[warp][8 * n + 2 * j + c][16 * k + 2 * g]);
-                            o[k][n][c] += v.x;
-                            o[k][n][2 + c] += v.y;
-                        }
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-        }
-        if (warp == 0) {
-            const bool whole = first_page == 0 && stop == pages;
-            // a part of a tile that an earlier block began lies in the block's first place, one that goes on behind it in the second
-            float* mine = a.scratch + ((int64_t)blockIdx.x * 2 + (first_page == 0 ? 1 : 0)) * part_floats<D>(COLS);
+                for (int w = 0; w < WARPS; ++w) {
+                    const float m = sm.merge_m[w][col], by = m > -INFINITY ? fast_exp2(m - high) : 0.f;
+                    total += sm.merge_l[w][col] * by;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int col = 8 * n + 2 * j + c;
-                    if (col >= columns) continue;
-                    if (whole) {
-                        const int q = part * COLS + col;
-                        T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(t.row + q / a.group) * a.n_heads + head * a.group + q % a.group) * D;
-                        const float inv = all_l[n][c] > 0.f ? 1.f / all_l[n][c] : 0.f;
-#pragma unroll
-                        for (int k = 0; k < STEPS; ++k) {
-                            out[16 * k + 2 * g] = from_f32<T>(o[k][n][c] * inv);
-                            out[16 * k + 2 * g + 1] = from_f32<T>(o[k][n][2 + c] * inv);
-                        }
-                    } else {
-                        float* p = mine + (int64_t)col * (D + 2);
-#pragma unroll
-                        for (int k = 0; k < STEPS; ++k) *reinterpret_cast<float2*>(p + 2 + 16 * k + 2 * g) = make_float2(o[k][n][c], o[k][n][2 + c]);
-                        if (g == 0) {
-                            p[0] = all_m[n][c];
-                            p[1] = all_l[n][c];
-                        }
+                    for (int i = 0; i < EP; i += 2) {
+                        const float2 z = *reinterpret_cast<const float2*>(&sm.merge[w][col][from + i]);
+                        y[i] += z.x * by;
+                        y[i + 1] += z.y * by;
                     }
                 }
+                if (whole) {
+                    const int q = part * COLS + 8 * n + col;
+                    const float inv = total == 0.f ? 0.f : 1.f / total;
+                    T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(row + q / a.group) * a.n_heads + head * a.group + q % a.group) * D + from;
+                    if constexpr (EP % 4 == 0) {
+#pragma unroll
+                        for (int i = 0; i < EP; i += 4) store4(out + i, make_float4(y[i] * inv, y[i + 1] * inv, y[i + 2] * inv, y[i + 3] * inv));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < EP; ++i) out[i] = from_f32<T>(y[i] * inv);
+                    }
+                } else {
+                    float* p = mine + (int64_t)(8 * n + col) * kPartStride<D>;
+#pragma unroll
+                    for (int i = 0; i < EP; i += 2) *reinterpret_cast<float2*>(p + from + i) = make_float2(y[i], y[i + 1]);
+                    if (from == 0) *reinterpret_cast<float2*>(p + D) = make_float2(high, total);
+                }
+            }
+            __syncthreads();
         }
         unit += stop - first_page;
     }
 }
 
-// Adds up the parts of the tiles that were cut: one block per tile, part and key-value head, a warp per column.
+// Adds up the parts of the tiles that were cut, one block per tile and column: a tile belongs to the block that began it (blockIdx.y), whose
+// head says which block had its end.  A warp has four of its parts under way at a time.
+constexpr int kCombineWarps = 16, kCombineParts = 4;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256)
-kv4_combine_kernel(const __grid_constant__ AttendArgs a, int blocks) {
-    constexpr int COLS = 8 * NT;
-    __shared__ int scan[9];
-    __shared__ int prefix[kMostTiles + 1];
+__global__ void __launch_bounds__(kCombineWarps * 32)
+kv4_combine_kernel(const __grid_constant__ AttendArgs a) {
+    constexpr int COLS = 8 * NT, E = D / 32;
+    __shared__ float tops[kCombineWarps], sums[kCombineWarps], values[kCombineWarps][D];
     pdl_launch_dependents();
     pdl_wait();
-    const int index = blockIdx.x;
-    const Tile t = tile_of(a, index, COLS);
-    if ((int)blockIdx.y >= t.parts * a.n_kv) return;
-    sum_tiles(a, COLS, prefix, scan);
-    const int64_t units = prefix[a.n_tiles];
-    const int sharing = sharing_blocks(units, blocks);
-    const int pages = max(1, t.pages);
-    const int64_t begin = prefix[index] + (int64_t)blockIdx.y * pages, last = begin + pages - 1;
-    const int b0 = block_of(begin, units, sharing), b1 = block_of(last, units, sharing);
-    if (b0 == b1) return;                                                                // the block that had it all wrote the output
-    const int head = blockIdx.y % a.n_kv, part = blockIdx.y / a.n_kv;
-    const int columns = min(COLS, t.tokens * a.group - part * COLS);
-    const int lane = threadIdx.x & 31;
-    for (int c = threadIdx.x >> 5; c < columns; c += 8) {
-        const auto place = [&](int b) { return a.scratch + ((int64_t)b * 2 + (b == b0 ? 1 : 0)) * part_floats<D>(COLS) + (int64_t)c * (D + 2); };
-        float top = -INFINITY;
-        for (int b = b0 + lane; b <= b1; b += 32) top = fmaxf(top, place(b)[0]);
-        top = warp_max(top);
-        float l = 0.f, o[D / 32];
+    const int c = blockIdx.x, b0 = blockIdx.y, blocks = gridDim.y;
+    const CutTile cut = *reinterpret_cast<const CutTile*>(a.scratch + (int64_t)b0 * kHeadInts);
+    if (cut.last_block < 0 || c >= cut.columns) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const auto place = [&](int b) { return part_of<D>(a, blocks, b, b == b0, COLS) + (int64_t)c * kPartStride<D>; };
+    float top = -INFINITY;
+    for (int b = b0 + threadIdx.x; b <= cut.last_block; b += kCombineWarps * 32) top = fmaxf(top, place(b)[D]);
+    top = warp_max(top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-        for (int b = b0; b <= b1; ++b) {
-            const float* p = place(b);
-            const float by = p[0] > -INFINITY ? exp2f(p[0] - top) : 0.f;
-            l += p[1] * by;
+    for (int w = 0; w < kCombineWarps; ++w) top = fmaxf(top, tops[w]);
+    float l = 0.f, o[E];
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) o[i] += by > 0.f ? p[2 + lane + 32 * i] * by : 0.f;
+    for (int i = 0; i < E; ++i) o[i] = 0.f;
+#pragma unroll 1
+    for (int b = b0 + warp; b <= cut.last_block; b += kCombineWarps * kCombineParts) {
+        float v[kCombineParts][E];
+        float2 ml[kCombineParts];
+#pragma unroll
+        for (int u = 0; u < kCombineParts; ++u) {
+            const float* p = place(min(b + u * kCombineWarps, cut.last_block));
+            ml[u] = *reinterpret_cast<const float2*>(p + D);
+            if (b + u * kCombineWarps > cut.last_block) ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[u][i] = p[lane + 32 * i];
         }
-        const int q = part * COLS + c;
-        T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(t.row + q / a.group) * a.n_heads + head * a.group + q % a.group) * D;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) out[lane + 32 * i] = from_f32<T>(o[i] * inv);
+        for (int u = 0; u < kCombineParts; ++u) {
+            const float by = ml[u].x > -INFINITY ? exp2f(ml[u].x - top) : 0.f;
+            l += ml[u].y * by;
+#pragma unroll
+            for (int i = 0; i < E; ++i) o[i] += v[u][i] * by;
+        }
+    }
+    if (lane == 0) sums[warp] = l;
+#pragma unroll
+    for (int i = 0; i < E; ++i) values[warp][lane + 32 * i] = o[i];
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kCombineWarps; ++w) l += sums[w];
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int q = cut.part * COLS + c;
+    T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(cut.row + q / a.group) * a.n_heads + cut.head * a.group + q % a.group) * D;
+    for (int i = threadIdx.x; i < D; i += kCombineWarps * 32) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kCombineWarps; ++w) v += values[w][i];
+        out[i] = from_f32<T>(v * inv);
     }
 }
 
 template <typename T, int D, int NT, int TERMS>
 int attend(const AttendArgs& a, cudaStream_t stream) {
     static bool done[kMaxDevices];
-    constexpr int bytes = (int)sizeof(Smem<D, NT, TERMS>) + 128;
+    constexpr int bytes = (int)sizeof(Smem<D, NT, TERMS>);
     const int status = ensure_dynamic_smem(kv4_attention_kernel<T, D, NT, TERMS>, bytes, done);
     if (status != CPM_OK) return status;
     const int sms = device_sms();
     if (sms <= 0) return CPM_BAD_ARGUMENT;
-    const int blocks = sms * blocks_per_sm(D, NT, TERMS);
-    cpm_launch(kLaunchAttention, kv4_attention_kernel<T, D, NT, TERMS>, dim3(blocks), kThreads, bytes, stream, a);
-    const int most_tokens = a.cu_q ? kTileTokens : 1;
-    const int64_t rows = (int64_t)((most_tokens * a.group + 8 * NT - 1) / (8 * NT)) * a.n_kv;
-    if (rows > 65535) return CPM_BAD_ARGUMENT;
-    cpm_launch(kLaunchAttention, kv4_combine_kernel<T, D, NT>, dim3(a.n_tiles, (unsigned)rows), 256, 0, stream, a, blocks);
+    const int blocks = sms;
+    cpm_launch(kLaunchAttention, kv4_attention_kernel<T, D, NT, TERMS>, dim3(blocks), 32 * warps_of(D, NT, TERMS), bytes, stream, a);
+    cpm_launch(kLaunchAttention, kv4_combine_kernel<T, D, NT>, dim3(8 * NT, blocks), kCombineWarps * 32, 0, stream, a);
     return launch_status();
 }
 
@@ -718,24 +772,16 @@ int by_head_size(const AttendArgs& a, int d, cudaStream_t stream) {
 
 // 32-bit floats that a launch needs for the parts of tiles that are cut.
 CPM_API int64_t cpm_kv4_attention_scratch_floats(int d) {
-    return (int64_t)device_sms() * kMostBlocksPerSm * 2 * 16 * (d + 2);
+    return (int64_t)device_sms() * (kHeadInts + 2 * 16 * (d + 4));
 }
 CPM_API int cpm_kv4_attention_most_tiles() { return kMostTiles; }
-// Reads and clears the error that a kernel recorded (0: none).
-CPM_API int cpm_kv4_attention_error() {
-    int code = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&code, g_kv4_error, sizeof(int)) != cudaSuccess) return -1;
-    if (code) cudaMemcpyToSymbol(g_kv4_error, &zero, sizeof(int));
-    return code;
-}
-
 CPM_API int cpm_kv4_attention(const void* q, const void* records, void* out, const int* kv_len, const int* slots, const int* page_table,
                               int max_pages, const int* cu_q, const int* tile_seq, const int* tile_row, int n_tiles, float* scratch, int n_heads,
                               int n_kv, int d, int window, float scale, int dtype, cudaStream_t stream) {
     if (n_tiles <= 0) return CPM_OK;
     if (n_tiles > kMostTiles || n_heads < 1 || n_kv < 1 || n_heads % n_kv || window < 0) return CPM_BAD_ARGUMENT;
     if ((cu_q == nullptr) != (tile_seq == nullptr) || (cu_q == nullptr) != (tile_row == nullptr)) return CPM_BAD_ARGUMENT;
-    if ((uintptr_t)records & 15) return CPM_BAD_ARGUMENT;
+    if (((uintptr_t)records | (uintptr_t)q | (uintptr_t)out) & 15) return CPM_BAD_ARGUMENT;
     const AttendArgs a{q, out, (const uint8_t*)records, kv_len, slots, page_table, cu_q, tile_seq, tile_row, scratch, max_pages, n_tiles, n_heads, n_kv,
                        n_heads / n_kv, window, scale};
     return dtype == CPM_BF16 ? by_head_size<bf16, 1>(a, d, stream) : by_head_size<float, 2>(a, d, stream);

@@ -64,11 +64,11 @@ class _NoLibrary:
 
     @staticmethod
     def cpm_kv4_attention_scratch_floats(d):
-        return 148 * 3 * 2 * 16 * (d + 2)
+        return 148 * (8 + 2 * 16 * (d + 4))
 
     @staticmethod
     def cpm_kv4_attention_most_tiles():
-        return 2048
+        return 512
 
     def __getattr__(self, name):
         return lambda *args: 0

@@ -202,9 +202,8 @@ def load() -> ctypes.CDLL:
         lib.cpm_retention_tiles_scratch_floats.restype = c_int64
         lib.cpm_kv4_attention_scratch_floats.argtypes = [c_int]
         lib.cpm_kv4_attention_scratch_floats.restype = c_int64
-        for name in ("cpm_kv4_attention_most_tiles", "cpm_kv4_attention_error"):
-            getattr(lib, name).argtypes = []
-            getattr(lib, name).restype = c_int
+        lib.cpm_kv4_attention_most_tiles.argtypes = []
+        lib.cpm_kv4_attention_most_tiles.restype = c_int
         lib.cpm_mingru_summary_floats.argtypes = [c_int, c_int]
         lib.cpm_mingru_summary_floats.restype = c_int64
         for name, argtypes in _SIGNATURES.items():

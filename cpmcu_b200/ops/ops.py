@@ -1007,8 +1007,6 @@ class Ops:
         arena = self.workspace.persistent.arena if self.workspace is not None else None
         if arena is not None and arena.guards:
             arena.check_guards()
-        if int(self.lib.cpm_kv4_attention_error()):
-            raise RuntimeError("the attention over a 4-bit cache gave up waiting on a barrier; the results of this step are not valid")
         if int(self.lib.cpm_listed_tile_error()):
             raise RuntimeError("the block-list attention of a prompt chunk gave up waiting on a barrier; the results of "
                                "this step are not valid")
