@@ -11,17 +11,27 @@
 // Sums are whole numbers, so they do not depend on the order in which thousands of threads form them: the same row and number give the same
 // token whatever the launch.  (With fp32 sums the border between two of 70,000 tokens moves by more than their distance.)
 //
-// A row is read once.  Its weights lie in the shared memory of a cluster of blocks (one to eight; the fewer rows, the more blocks a row), and every
-// step runs there: the k-th weight and the weight at which the mass is reached are found by radix selection on the weight's bits (11 + 10 + 10, of
-// which only the first looks at every weight's histogram), counts and masses of the blocks being added over distributed shared memory.
+// A row is read once.  Its weights lie in the shared memory of a cluster of blocks (one to eight; the fewer rows, the more blocks a row).  One
+// histogram of the weights' upper bits (32 bins to an octave) says in which bin the k-th weight lies, and, since a bin's weights differ by 1/32 at
+// most, in which few bins the mass is reached.  The tokens in these bins, a few hundred, go to the cluster's first block, which finds the border by
+// radix selection with exact masses; where no more than kAlone tokens are above the border of top-k, all of them go there and it draws as well.
+// (A cluster's barrier takes about 2 us, and a look into a neighbour's shared memory half of that: a selection over the whole row with
+// all blocks' histograms added up at every step took 41 us for one row of 73,448.)
 // What a row cannot do without is its logits, 4 bytes a token.
 #include "common.cuh"
 #include "philox.cuh"
 
 namespace {
 
-constexpr int kFilterThreads = 1024;
-constexpr int kBins = 1024;                            // a weight's bits 30..20 end at 1016, the largest weight being 1
+constexpr int kFilterThreads = 512;
+constexpr int kFilterWarps = kFilterThreads / 32;
+constexpr int kMostBlocks = 8;                         // of a cluster
+constexpr int kOctaveBits = 18;                        // bits of a weight below those that number its bin
+constexpr int kCoarseBins = 4096;                      // bins 0 .. 4064, the largest weight being 1
+constexpr int kOwnBins = kCoarseBins / kFilterThreads;
+constexpr int kFineBins = 1024;                        // of a step of the selection
+constexpr int kListed = 2048;                          // tokens that are set apart for the selection
+constexpr int kAlone = 512;                            // up to so many the first block goes on without the others
 constexpr int kLimbBits = 14;                          // a mass is added in three limbs: 32-bit adds in shared memory are one instruction
 constexpr int kMostVocab = 1 << 21;                    // so that a limb's sum over a block's tokens stays within 32 bits
 
@@ -36,16 +46,29 @@ struct FilterArgs {
     float* logprob;
 };
 
+// What the first block has found and the others read: the weights to set apart, or the border.
+struct Plan {
+    uint32_t low, high;                                // bits of the weights to set apart
+    int complete;                                      // all from ``low`` up are
+    int apart;                                         // whether they are few enough, else their masses go into bins
+    uint32_t border;                                   // tokens above it stay, and the first ``ties`` of the ``equal`` ones at it
+    uint64_t ties, equal;
+};
+
 struct FilterShared {
-    uint32_t bins[3][kBins];
-    uint64_t warp_sum[33];
+    alignas(16) uint32_t coarse[kCoarseBins];
+    alignas(16) uint32_t fine[3][kFineBins];
+    uint32_t list[kListed];                            // bits of the weights that are set apart, in the first block
+    int place[kListed];                                // and their tokens
+    int listed;
+    uint64_t warp_sum[kFilterWarps + 1];
     uint64_t found_before, found_here;                 // what lies above the bin that was found, and in it
-    int found_bin;
-    ArgMax best;                                       // of this block; read by the others
-    uint64_t mass;                                     // likewise
-    int count;
+    int found_bin, low_bin, high_bin, cut;
+    alignas(8) ArgMax best[kMostBlocks];                          // of the cluster's blocks, which write here
+    uint64_t mass[kMostBlocks];
+    int count[kMostBlocks];
+    Plan plan;
     ArgMax scratch[33];
-    int cut;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -58,6 +81,7 @@ __device__ __forceinline__ uint32_t cluster_blocks() {
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
+// Reads, writes and additions in the shared memory of the cluster's block ``rank``, at the place that ``own`` is in this block's.
 __device__ __forceinline__ uint32_t peer32(const void* own, uint32_t rank) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_address(own, rank)) : "memory");
@@ -68,16 +92,25 @@ __device__ __forceinline__ uint64_t peer64(const void* own, uint32_t rank) {
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_address(own, rank)) : "memory");
     return v;
 }
-
-__device__ __forceinline__ uint64_t units_of(float w) { return (uint64_t)((double)w * 1099511627776.0); }
-
-__device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+__device__ __forceinline__ void put32(const void* own, uint32_t rank, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" :: "r"(cluster_address(own, rank)), "r"(v) : "memory");
 }
-// Inclusive sums over the block's threads in order; the block's total is left in sums[32].
-__device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t* sums) {
+__device__ __forceinline__ void put64(const void* own, uint32_t rank, uint64_t v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(cluster_address(own, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t add32(const void* own, uint32_t rank, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(cluster_address(own, rank)), "r"(v) : "memory");
+    return old;
+}
+
+// floor(w 2^40) of a weight (0 to 1) by its bits: 24 bits of significand, shifted.
+__device__ __forceinline__ uint64_t units_of(uint32_t bits) {
+    return ((uint64_t)((bits & 0x7fffffu) | 0x800000u) << 17) >> min(63u, 127u - (bits >> 23));
+}
+
+// Inclusive sums over the block's threads in order; the block's total is left in the last of ``sums``.
+__device__ __noinline__ uint64_t block_scan64(uint64_t v, uint64_t* sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -88,18 +121,23 @@ __device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t* sums) {
     if (lane == 31) sums[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        const uint64_t own = sums[lane];
+        const uint64_t own = lane < kFilterWarps ? sums[lane] : 0;
         uint64_t x = own;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
+        for (int o = 1; o < kFilterWarps; o <<= 1) {
             const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        sums[lane] = x - own;
-        if (lane == 31) sums[32] = x;
+        __syncwarp();
+        if (lane < kFilterWarps) sums[lane] = x - own;
+        if (lane == kFilterWarps - 1) sums[kFilterWarps] = x;
     }
     __syncthreads();
     return v + sums[warp];
+}
+__device__ __forceinline__ uint64_t block_sum64(uint64_t v, FilterShared& sm) {
+    block_scan64(v, sm.warp_sum);
+    return sm.warp_sum[kFilterWarps];
 }
 
 // STAGED: the block's weights lie in shared memory; else (a vocabulary that eight blocks' do not hold) they are formed again from the logits.
@@ -109,9 +147,17 @@ struct Row {
     float* w;
     int n;                                             // tokens of the block
     float top, t;
+    float inverse;                                     // 1 / t where the quotient by it is exact, else 0
+    // (x - top) / t correctly rounded.  For t within 2^60 of 1 by Markstein's method (IBM J. Res. Dev. 34, 1990): with r = 1 / t rounded, q = x r, and
+    // the remainder x - q t, which a fused multiply-add gives exactly, q + r (x - q t) rounds to the quotient.  Where it overflows the weight is 0.
+    __device__ __forceinline__ float over_t(float x) const {
+        if (inverse == 0.f) return __fdiv_rn(x, t);
+        const float q = __fmul_rn(x, inverse);
+        return __fmaf_rn(__fmaf_rn(-q, t, x), inverse, q);
+    }
     __device__ __forceinline__ float form(float x) const {
         if (top == INFINITY) return x == INFINITY ? 1.f : 0.f;
-        const float v = expf(__fdiv_rn(__fsub_rn(x, top), t));
+        const float v = expf(over_t(__fsub_rn(x, top)));
         return v >= 0.f ? v : 0.f;                     // a logit that is no number is never drawn
     }
     __device__ __forceinline__ float at(int i) const {
@@ -122,113 +168,163 @@ struct Row {
 
 struct Border { uint32_t bits; uint64_t above, here; };      // a weight, and the count or mass of the tokens above it and at it
 
-// The weight at which the running count (MASS false) or mass of the tokens, from the largest weight down, first reaches ``need``; only weights from
-// ``least`` up are looked at, and the caller knows that these suffice.
-template <bool MASS, bool STAGED>
-__device__ Border select(const Row<STAGED>& row, FilterShared& sm, double need, uint32_t least) {
-    const uint32_t blocks = cluster_blocks();
-    uint32_t prefix = 0;
-    uint64_t above = 0, here = 0;
-#pragma unroll 1
-    for (int level = 0; level < 3; ++level) {
-        const int low = level == 0 ? 20 : level == 1 ? 10 : 0;
-        for (int i = threadIdx.x; i < kBins; i += kFilterThreads)
+// The bin of sm.fine, counts or masses in limbs, at which the running sum from the last bin down, starting with ``above``, first reaches ``need``: left in
+// sm.found_bin, with what lies above it and in it.
+__device__ __noinline__ void find_fine(FilterShared& sm, double need, uint64_t above) {
+    const int bin = kFineBins - 2 - 2 * threadIdx.x;    // two bins a thread
+    uint64_t v[2] = {0, 0};
 #pragma unroll
-            for (int u = 0; u < (MASS ? 3 : 1); ++u) sm.bins[u][i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < row.n; i += kFilterThreads) {
-            const float w = row.at(i);
-            const uint32_t bits = __float_as_uint(w);
-            if (bits < least || (level > 0 && (bits >> (low + 10)) != prefix)) continue;
-            const int bin = level == 0 ? bits >> 20 : (bits >> low) & (kBins - 1);
-            if constexpr (MASS) {
-                const uint64_t v = units_of(w);
-                atomicAdd(&sm.bins[0][bin], (uint32_t)v & ((1u << kLimbBits) - 1));
-                atomicAdd(&sm.bins[1][bin], (uint32_t)(v >> kLimbBits) & ((1u << kLimbBits) - 1));
-                atomicAdd(&sm.bins[2][bin], (uint32_t)(v >> (2 * kLimbBits)));
-            } else {
-                atomicAdd(&sm.bins[0][bin], 1u);
-            }
-        }
-        cluster_sync();
-        const int bin = kBins - 1 - threadIdx.x;        // one bin a thread, from the largest weights down
-        uint64_t v = 0;
-        for (uint32_t b = 0; b < blocks; ++b)
-#pragma unroll
-            for (int u = 0; u < (MASS ? 3 : 1); ++u) v += (uint64_t)peer32(&sm.bins[u][bin], b) << (u * kLimbBits);
-        const uint64_t upto = above + block_scan64(v, sm.warp_sum);
-        if ((double)(upto - v) < need && (double)upto >= need) {
-            sm.found_bin = bin;
-            sm.found_before = upto - v;
-            sm.found_here = v;
-        }
-        cluster_sync();                                 // the bins have been read
-        prefix = level == 0 ? sm.found_bin : (prefix << 10) | sm.found_bin;
-        above = sm.found_before;
-        here = sm.found_here;
+    for (int u = 0; u < 3; ++u) {
+        v[0] += (uint64_t)sm.fine[u][bin + 1] << (u * kLimbBits);
+        v[1] += (uint64_t)sm.fine[u][bin] << (u * kLimbBits);
     }
-    return Border{prefix, above, here};
+    uint64_t upto = above + block_scan64(v[0] + v[1], sm.warp_sum) - v[0] - v[1];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if ((double)upto < need && (double)(upto + v[i]) >= need) {
+            sm.found_bin = bin + 1 - i;
+            sm.found_before = upto;
+            sm.found_here = v[i];
+        }
+        upto += v[i];
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void clear_fine(FilterShared& sm) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 3 * kFineBins; i += kFilterThreads) sm.fine[0][i] = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ void add_fine(FilterShared& sm, bool mass, int bin, uint32_t bits) {
+    if (!mass) {
+        atomicAdd(&sm.fine[0][bin], 1u);
+        return;
+    }
+    const uint64_t v = units_of(bits);
+    atomicAdd(&sm.fine[0][bin], (uint32_t)v & ((1u << kLimbBits) - 1));
+    atomicAdd(&sm.fine[1][bin], (uint32_t)(v >> kLimbBits) & ((1u << kLimbBits) - 1));
+    atomicAdd(&sm.fine[2][bin], (uint32_t)(v >> (2 * kLimbBits)));
+}
+__device__ __forceinline__ int bits_of_range(uint32_t low, uint32_t high) { return max(1, 32 - __clz(high - low - 1)); }
+
+// The weight at which the running count (``mass`` false) or mass of the listed tokens, from the largest weight down, first reaches ``need``.  Looked at are
+// the weights of [low, high), which are known to hold it; ``above``: what lies above them.  By the first block alone.
+__device__ __noinline__ Border select(FilterShared& sm, bool mass, int listed, double need, uint64_t above, uint32_t low, uint32_t high) {
+    uint32_t prefix = 0;
+    int done = bits_of_range(low, high);                // key bits from here up are the prefix
+#pragma unroll 1
+    while (done > 0) {
+        const int shift = max(0, done - 10);
+        clear_fine(sm);
+#pragma unroll 1
+        for (int i = threadIdx.x; i < listed; i += kFilterThreads) {
+            const uint32_t bits = sm.list[i], key = bits - low;
+            if (bits >= low && bits < high && (key >> done) == prefix) add_fine(sm, mass, (key >> shift) & ((1u << (done - shift)) - 1), bits);
+        }
+        __syncthreads();
+        find_fine(sm, need, above);
+        prefix = (prefix << (done - shift)) | sm.found_bin;
+        above = sm.found_before;
+        done = shift;
+    }
+    return Border{low + prefix, above, sm.found_here};
 }
 
-// Sum over the cluster of a number of each block.
-__device__ __forceinline__ uint64_t cluster_total(uint64_t own_of_thread, FilterShared& sm) {
-    block_scan64(own_of_thread, sm.warp_sum);
-    if (threadIdx.x == 0) sm.mass = sm.warp_sum[32];
-    cluster_sync();
-    uint64_t all = 0;
-    for (uint32_t b = 0; b < cluster_blocks(); ++b) all += peer64(&sm.mass, b);
-    cluster_sync();
-    return all;
+// The first bin, from the largest weights down, at whose end the running sum of count times ``each(bin)`` reaches ``need``; ``otherwise`` where none does.
+template <typename Each>
+__device__ __forceinline__ void find_bin(FilterShared& sm, Each each, double need, int* bin, uint64_t* before) {
+    const int top_bin = kCoarseBins - 1 - kOwnBins * threadIdx.x;
+    uint64_t sum = 0;
+#pragma unroll 1
+    for (int q = 0; q < kOwnBins; ++q) sum += (uint64_t)sm.coarse[top_bin - q] * each(top_bin - q);
+    uint64_t upto = block_scan64(sum, sm.warp_sum) - sum;
+    if ((double)upto < need && (double)(upto + sum) >= need)
+#pragma unroll 1
+        for (int q = 0; q < kOwnBins; ++q) {
+            const uint64_t here = (uint64_t)sm.coarse[top_bin - q] * each(top_bin - q);
+            if ((double)upto < need && (double)(upto + here) >= need) {
+                *bin = top_bin - q;
+                *before = upto;
+            }
+            upto += here;
+        }
+    __syncthreads();
+}
+
+// Of the tokens at a border that mass decides, how many it takes.
+__device__ __forceinline__ uint64_t ties_of(const Border& b, double need, uint64_t* equal) {
+    const uint64_t each = units_of(b.bits), there = b.here / each;
+    uint64_t n = (uint64_t)ceil((need - (double)b.above) / (double)each);
+    n = min(max(n, (uint64_t)1), there);
+    while (n > 1 && (double)(b.above + (n - 1) * each) >= need) --n;
+    while (n < there && (double)(b.above + n * each) < need) ++n;
+    *equal = there;
+    return n;
 }
 
 template <bool STAGED>
-__global__ void __launch_bounds__(kFilterThreads)
+__global__ void __launch_bounds__(kFilterThreads, 2)
 sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     extern __shared__ float weights[];
     __shared__ FilterShared sm;
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t blocks = cluster_blocks(), rank = cluster_rank();
-    const int r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31;
     const int first = min(a.vocab, (int)rank * a.per_block);
     Row<STAGED> row;
     row.n = min(a.vocab, first + a.per_block) - first;
     row.z = a.logits + (int64_t)r * a.ld + first;
     row.w = weights;
+    const float t = a.temperature ? a.temperature[r] : 0.f, p = a.top_p ? a.top_p[r] : 1.f;
+    int k = a.top_k ? a.top_k[r] : 0;
+    float ratio = a.min_p ? a.min_p[r] : 0.f;
+    if (p <= 0.f || ratio > 1.f) k = 1;
+    if (!(ratio <= 1.f)) ratio = 0.f;                          // above one: the first token alone, which it would leave out as well
+    const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
+    const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[r], (uint32_t)a.step_key[r]);
+
+    asm volatile("barrier.cluster.arrive;" ::: "memory");       // (nothing is put into a block that has not begun)
 
     // the largest logit, lowest index among equals
     ArgMax best{-INFINITY, 0x7fffffff};
     const int whole = ((uintptr_t)row.z & 15) == 0 ? row.n & ~3 : 0;
+#pragma unroll 1
     for (int i0 = 4 * tid; i0 < whole; i0 += 16 * kFilterThreads) {
         float4 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + 4 * u * kFilterThreads;
-            v[u] = i < whole ? *reinterpret_cast<const float4*>(row.z + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (int q = 0; q < 4; ++q) {
+            const int i = i0 + 4 * q * kFilterThreads;
+            v[q] = i < whole ? *reinterpret_cast<const float4*>(row.z + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + 4 * u * kFilterThreads;
+        for (int q = 0; q < 4; ++q) {
+            const int i = i0 + 4 * q * kFilterThreads;
             if (i >= whole) break;
-            if constexpr (STAGED) *reinterpret_cast<float4*>(weights + i) = v[u];
-            best = better(best, ArgMax{v[u].x, first + i});
-            best = better(best, ArgMax{v[u].y, first + i + 1});
-            best = better(best, ArgMax{v[u].z, first + i + 2});
-            best = better(best, ArgMax{v[u].w, first + i + 3});
+            if constexpr (STAGED) *reinterpret_cast<float4*>(weights + i) = v[q];
+            best = better(best, ArgMax{v[q].x, first + i});
+            best = better(best, ArgMax{v[q].y, first + i + 1});
+            best = better(best, ArgMax{v[q].z, first + i + 2});
+            best = better(best, ArgMax{v[q].w, first + i + 3});
         }
     }
+#pragma unroll 1
     for (int i = whole + tid; i < row.n; i += kFilterThreads) {
         const float v = row.z[i];
         if constexpr (STAGED) weights[i] = v;
         best = better(best, ArgMax{v, first + i});
     }
+    if (by_count || by_mass)
+#pragma unroll 1
+        for (int i = tid; i < kCoarseBins; i += kFilterThreads) sm.coarse[i] = 0;
+    if (tid == 0) sm.listed = 0;
     best = block_argmax(best, sm.scratch);
-    if (tid == 0) sm.best = best;
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+    if (tid < (int)blocks) put64(&sm.best[rank], tid, (uint64_t)__float_as_uint(best.v) | (uint64_t)(uint32_t)best.i << 32);
     cluster_sync();
     best = ArgMax{-INFINITY, 0x7fffffff};
-    for (uint32_t b = 0; b < blocks; ++b) best = better(best, ArgMax{__uint_as_float(peer32(&sm.best.v, b)), (int)peer32(&sm.best.i, b)});
-    cluster_sync();
-    const float t = a.temperature ? a.temperature[r] : 0.f;
+#pragma unroll 1
+    for (uint32_t b = 0; b < blocks; ++b) best = better(best, sm.best[b]);
     if (best.v == -INFINITY || !(t > 0.f)) {                   // nothing that can be drawn: token 0; a greedy row: the largest
         if (rank == 0 && tid == 0) {
             a.token[r] = best.v == -INFINITY ? 0 : best.i;
@@ -238,128 +334,313 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     }
     row.top = best.v;
     row.t = t;
-    if constexpr (STAGED) {
-        for (int i = tid; i < row.n; i += kFilterThreads) weights[i] = row.form(weights[i]);
-        __syncthreads();
-    }
+    row.inverse = t > 0x1p-60f && t < 0x1p60f ? __frcp_rn(t) : 0.f;
 
-    // which tokens stay: those above the border, of those at it the first ``ties``, and of all only from ``ratio`` up
-    int k = a.top_k ? a.top_k[r] : 0;
-    const float p = a.top_p ? a.top_p[r] : 1.f;
-    float ratio = a.min_p ? a.min_p[r] : 0.f;
-    if (p <= 0.f || ratio > 1.f) k = 1;
-    if (!(ratio <= 1.f)) ratio = 0.f;                          // above one: the first token alone, which it would leave out as well
+    // weights, their histogram, and (where mass alone decides) their mass.  A thread's tokens are neighbours, an odd number of them, so that sums by
+    // thread go by index and a warp's accesses to shared memory are in different banks
+    const int strip = (row.n + kFilterThreads - 1) / kFilterThreads | 1, i0 = min(row.n, tid * strip), i1 = min(row.n, i0 + strip);
+    uint64_t own_mass = 0;
+    if (by_count || by_mass) {
+#pragma unroll 2
+        for (int i = i0; i < i1; ++i) {
+            const float w = STAGED ? row.form(weights[i]) : row.at(i);
+            if constexpr (STAGED) weights[i] = w;
+            atomicAdd(&sm.coarse[__float_as_uint(w) >> kOctaveBits], 1u);
+            if (!by_count) own_mass += units_of(__float_as_uint(w));
+        }
+    } else if constexpr (STAGED) {
+#pragma unroll 2
+        for (int i = i0; i < i1; ++i) weights[i] = row.form(weights[i]);
+    }
+    __syncthreads();
+    const auto put_mass = [&](uint64_t own) {                  // the block's sum into the first block's (or every block's) list of sums
+        const uint64_t all = block_sum64(own, sm);
+        if (tid < (int)blocks) put64(&sm.mass[rank], tid, all);
+    };
+    const auto all_mass = [&]() {
+        uint64_t all = 0;
+#pragma unroll 1
+        for (uint32_t b = 0; b < blocks; ++b) all += sm.mass[b];
+        return all;
+    };
+
     uint32_t border = 0;
-    uint64_t ties = ~0ull, equal = 0;                          // tokens to keep at the border, and tokens there
-    if (k > 0 && k < a.vocab) {
-        const Border b = select<false>(row, sm, (double)k, 0u);
-        border = b.bits;
-        ties = (uint64_t)k - b.above;
-        equal = b.here;
-    }
-    if (p < 1.f && p > 0.f && k != 1) {
-        uint64_t own = 0;                                      // mass of the tokens that top-k leaves
-        for (int i = tid; i < row.n; i += kFilterThreads) {
-            const float w = row.at(i);
-            if (__float_as_uint(w) > border || border == 0) own += units_of(w);
-        }
-        uint64_t within = cluster_total(own, sm);
-        if (border) within += ties * units_of(__uint_as_float(border));
-        const double need = (double)p * (double)within;
-        const Border b = select<true>(row, sm, need, border);
-        const uint64_t each = units_of(__uint_as_float(b.bits));
-        const uint64_t there = b.here / each;
-        uint64_t n = (uint64_t)ceil((need - (double)b.above) / (double)each);
-        n = min(max(n, (uint64_t)1), there);
-        while (n > 1 && (double)(b.above + (n - 1) * each) >= need) --n;
-        while (n < there && (double)(b.above + n * each) < need) ++n;
-        if (b.bits == border) n = min(n, ties);
-        border = b.bits;
-        ties = n;
-        equal = there;
-    }
-    // a warp's tokens are neighbours, so that sums by warp go by index
-    const int per_warp = ((row.n + 31) / 32 + 31) & ~31;
-    const int w0 = min(row.n, warp * per_warp), w1 = min(row.n, w0 + per_warp);
-    int cut = 0x7fffffff;                                      // the last token of the block that may stay at the border
-    if (ties < equal) {
-        int mine = 0;
-        for (int i = w0 + lane; i < w1; i += 32) mine += __float_as_uint(row.at(i)) == border;
-        const int of_warp = __reduce_add_sync(0xffffffffu, mine);
-        const uint64_t upto = block_scan64(lane == 0 ? of_warp : 0, sm.warp_sum);
-        if (tid == 0) {
-            sm.count = (int)sm.warp_sum[32];
-            sm.cut = 0x7fffffff;
-        }
+    uint64_t ties = ~0ull, equal = 0;
+    if (by_count || by_mass) {
+        if (by_mass && !by_count) put_mass(own_mass);
+        if (rank > 0)
+#pragma unroll 1
+            for (int i = tid; i < kCoarseBins; i += kFilterThreads)
+                if (sm.coarse[i]) add32(&sm.coarse[i], 0, sm.coarse[i]);
         cluster_sync();
-        int64_t left = (int64_t)ties;                          // to keep in this block and behind it
-        for (uint32_t b = 0; b < rank; ++b) left -= (int)peer32(&sm.count, b);
-        if (left <= 0) {
-            cut = -1;
-        } else {
-            const int64_t before = (int64_t)__shfl_sync(0xffffffffu, upto, 0) - of_warp;
-            if (before < left && left < before + of_warp + 1 && of_warp > 0) {
-                int64_t seen = before;
-                for (int i0 = w0; i0 < w1; i0 += 32) {
-                    const int i = i0 + lane;
-                    const uint32_t hit = __ballot_sync(0xffffffffu, i < w1 && __float_as_uint(row.at(i)) == border);
-                    if (seen + __popc(hit) >= left) {
-                        if (lane == 0) sm.cut = i0 + __fns(hit, 0, (int)(left - seen));
-                        break;
+        uint64_t within = by_mass && !by_count ? all_mass() : 0;      // mass of the tokens that top-k leaves
+#pragma unroll 1
+        for (int round = by_count ? 0 : 1; round < (by_mass ? 2 : 1); ++round) {
+            // ---- which weights the border may be among ----
+            const double need = round == 0 ? (double)k : (double)p * (double)within;
+            uint64_t above = 0;                                // what lies above them (known to the first block alone)
+            uint64_t some = 0;                                 // no fewer tokens than they are (likewise)
+            uint32_t low = 0, high = 0, complete = 0;
+            if (rank == 0) {
+                if (round == 0) {
+                    find_bin(sm, [](int) { return (uint64_t)1; }, need, &sm.found_bin, &sm.found_before);
+                    above = sm.found_before;
+                    low = (uint32_t)sm.found_bin << kOctaveBits;
+                    some = sm.coarse[sm.found_bin];
+                    complete = above + some <= kListed;
+                    high = complete ? 0x3f800001u : low + (1u << kOctaveBits);
+                } else {
+                    // from where the masses reach ``need`` if every weight were its bin's upper end, to where they do with the lower ends
+                    const int last = border >> kOctaveBits;
+                    if (tid == 0) {
+                        sm.high_bin = kCoarseBins - 1;
+                        sm.low_bin = last;
                     }
-                    seen += __popc(hit);
+                    __syncthreads();
+                    find_bin(sm, [](int bin) { return units_of((uint32_t)(bin + 1) << kOctaveBits); }, need, &sm.high_bin, &sm.found_before);
+                    find_bin(sm, [](int bin) { return units_of((uint32_t)bin << kOctaveBits); }, need, &sm.low_bin, &sm.found_before);
+                    const uint32_t low_bin = max(sm.low_bin, last), high_bin = max((uint32_t)sm.high_bin, low_bin);
+                    low = max(border, low_bin << kOctaveBits);
+                    high = (high_bin + 1) << kOctaveBits;
+                    uint64_t count = 0;
+                    for (uint32_t bin = low_bin + tid; bin <= high_bin; bin += kFilterThreads) count += sm.coarse[bin];
+                    some = block_sum64(count, sm);
                 }
             }
-            __syncthreads();
-            cut = sm.cut;
+            Border b{};
+            int listed = 0;
+            bool known = round == 0;                           // whether ``above`` is
+#pragma unroll 1
+            while (true) {
+                if (rank == 0) {
+                    clear_fine(sm);
+                    if (tid == 0) {
+                        sm.plan.low = low;
+                        sm.plan.high = high;
+                        sm.plan.complete = complete;
+                        sm.plan.apart = some <= kListed;
+                        sm.listed = 0;
+                    }
+                }
+                cluster_sync();
+                low = peer32(&sm.plan.low, 0);
+                high = peer32(&sm.plan.high, 0);
+                complete = peer32(&sm.plan.complete, 0);
+                const bool apart = peer32(&sm.plan.apart, 0);
+                const int range = bits_of_range(low, high), shift = max(0, range - 10);
+                uint64_t over = 0;
+                int hits = 0;
+                if (!apart && rank > 0) clear_fine(sm);
+#pragma unroll 2
+                for (int i = i0; i < i1; ++i) {
+                    const uint32_t bits = __float_as_uint(row.at(i));
+                    if (bits >= high) over += units_of(bits);
+                    else if (bits >= low) {
+                        ++hits;
+                        if (!apart) add_fine(sm, round > 0, (bits - low) >> shift, bits);
+                    }
+                }
+                if (!known) put_mass(over);
+                if (apart) {
+                    // ---- the tokens themselves to the first block: a warp asks for room once, and then goes through its tokens again ----
+                    const int all = __reduce_add_sync(0xffffffffu, hits);
+                    if (all) {
+                        uint32_t at = lane == 0 ? add32(&sm.listed, 0, all) : 0;
+                        at = __shfl_sync(0xffffffffu, at, 0);
+                        int before = hits;
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const int x = __shfl_up_sync(0xffffffffu, before, o);
+                            if (lane >= o) before += x;
+                        }
+                        at += before - hits;
+#pragma unroll 1
+                        for (int i = i0; i < i1 && hits > 0; ++i) {
+                            const uint32_t bits = __float_as_uint(row.at(i));
+                            if (bits >= low && bits < high) {
+                                if (at < kListed) {
+                                    put32(&sm.list[at], 0, bits);
+                                    put32(&sm.place[at], 0, first + i);
+                                }
+                                ++at;
+                                --hits;
+                            }
+                        }
+                    }
+                } else if (rank > 0) {
+                    __syncthreads();
+#pragma unroll 1
+                    for (int i = tid; i < 3 * kFineBins; i += kFilterThreads)
+                        if (sm.fine[0][i]) add32(&sm.fine[0][i], 0, sm.fine[0][i]);
+                }
+                cluster_sync();
+                if (!known) above = all_mass();
+                known = true;
+                if (apart) {
+                    listed = (int)peer32(&sm.listed, 0);
+                    if (rank == 0) b = select(sm, round > 0, listed, need, complete ? 0 : above, low, high);
+                    break;
+                }
+                // ---- too many for the list (equal weights, or a mass that flat tails make up): their masses in 1,024 bins, and on with one of these ----
+                if (rank == 0) {
+                    find_fine(sm, need, above);
+                    low += (uint32_t)sm.found_bin << shift;
+                    high = min(high, low + (1u << shift));
+                    above = sm.found_before;
+                    some = round > 0 ? sm.found_here / max((uint64_t)1, units_of(low)) : sm.found_here;
+                    if (tid == 0) sm.plan.apart = shift > 0;
+                    b = Border{low, above, sm.found_here};
+                }
+                cluster_sync();
+                if (peer32(&sm.plan.apart, 0) == 0) break;      // a single weight is left
+                cluster_sync();                                // (read before the next plan is made)
+            }
+            if (complete) {
+                // ---- all that top-k leaves is here: the first block goes on alone ----
+                if (rank == 0) {
+                    border = b.bits;
+                    ties = (uint64_t)k - b.above;
+                    equal = b.here;
+                    if (by_mass) {
+                        uint64_t sum = 0;
+#pragma unroll 1
+                        for (int i = tid; i < listed; i += kFilterThreads)
+                            if (sm.list[i] > border) sum += units_of(sm.list[i]);
+                        within = block_sum64(sum, sm) + ties * units_of(border);
+                        const double mass_need = (double)p * (double)within;
+                        const Border m = select(sm, true, listed, mass_need, 0, border, high);
+                        uint64_t there;
+                        uint64_t n = ties_of(m, mass_need, &there);
+                        if (m.bits == border) n = min(n, ties);
+                        border = m.bits;
+                        ties = n;
+                        equal = there;
+                    }
+                }
+                if (listed <= kAlone) {
+                    if (rank > 0) return;
+                    // a thread's token: does it stay, and what is kept in front of it?
+                    const uint32_t bits = tid < listed ? sm.list[tid] : 0;
+                    const int place = tid < listed ? sm.place[tid] : 0;
+                    bool stays = tid < listed && bits >= border && __uint_as_float(bits) >= ratio;
+                    if (stays && bits == border && ties < equal) {
+                        uint64_t before = 0;
+#pragma unroll 1
+                        for (int i = 0; i < listed; ++i) before += sm.list[i] == border && sm.place[i] < place;
+                        stays = before < ties;
+                    }
+                    const uint64_t mine = stays ? units_of(bits) : 0;
+                    const uint64_t total = block_sum64(mine, sm);
+                    __syncthreads();
+                    uint64_t* kept = reinterpret_cast<uint64_t*>(sm.fine[0]);
+                    if (tid < listed) kept[tid] = mine;
+                    __syncthreads();
+                    if (!stays) return;
+                    uint64_t before = 0;
+#pragma unroll 4
+                    for (int i = 0; i < listed; ++i) before += sm.place[i] < place ? kept[i] : 0;
+                    const uint64_t target = min((uint64_t)((double)u * (double)total), total - 1);
+                    if (target >= before && target < before + mine) {
+                        a.token[r] = place;
+                        a.logprob[r] = (row.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(a.logits[(int64_t)r * a.ld + place], row.top), t))
+                                     - logf((float)((double)total * (1.0 / 1099511627776.0)));
+                    }
+                    return;
+                }
+                round = 2;
+            } else if (rank == 0) {
+                if (round == 0) {
+                    border = b.bits;
+                    ties = (uint64_t)k - b.above;
+                    equal = b.here;
+                } else {
+                    uint64_t there;
+                    uint64_t n = ties_of(b, need, &there);
+                    if (b.bits == border) n = min(n, ties);
+                    border = b.bits;
+                    ties = n;
+                    equal = there;
+                }
+            }
+            // ---- known to all ----
+            if (rank == 0 && tid == 0) {
+                sm.plan.border = border;
+                sm.plan.ties = ties;
+                sm.plan.equal = equal;
+            }
+            cluster_sync();
+            border = peer32(&sm.plan.border, 0);
+            ties = peer64(&sm.plan.ties, 0);
+            equal = peer64(&sm.plan.equal, 0);
+            if (round == 0 && by_mass) {
+                uint64_t sum = 0;                              // (the second round looks at the row's masses anyway)
+#pragma unroll 1
+                for (int i = i0; i < i1; ++i)
+                    if (__float_as_uint(row.at(i)) > border) sum += units_of(__float_as_uint(row.at(i)));
+                put_mass(sum);
+                cluster_sync();
+                within = all_mass() + ties * units_of(border);
+                cluster_sync();                                // read before the next sums are put there
+            }
         }
+    }
+
+    // ---- the draw, by index ----
+    if (__float_as_uint(ratio) > border) {                     // min-p leaves fewer
+        border = __float_as_uint(ratio);
+        ties = equal = 0;
+    }
+    int cut = 0x7fffffff;                                      // the last token of the thread that may stay at the border
+    if (ties < equal) {
+        int mine = 0;
+#pragma unroll 1
+        for (int i = i0; i < i1; ++i) mine += __float_as_uint(row.at(i)) == border;
+        const uint64_t upto = block_scan64(mine, sm.warp_sum);
+        if (tid < (int)blocks) put32(&sm.count[rank], tid, (uint32_t)sm.warp_sum[kFilterWarps]);
         cluster_sync();
+        int64_t left = (int64_t)ties - ((int64_t)upto - mine);     // to keep of the thread's and those behind them
+#pragma unroll 1
+        for (uint32_t b = 0; b < rank; ++b) left -= sm.count[b];
+        if (left < mine) {
+            cut = -1;
+#pragma unroll 1
+            for (int i = i0; i < i1 && left > 0; ++i)
+                if (__float_as_uint(row.at(i)) == border) {
+                    cut = i;
+                    --left;
+                }
+        }
     }
     const auto kept = [&](int i) -> uint64_t {
-        const float w = row.at(i);
-        const uint32_t bits = __float_as_uint(w);
-        const bool stays = (bits > border || (bits == border && i <= cut)) && w >= ratio;
-        return stays ? units_of(w) : 0;
+        const uint32_t bits = __float_as_uint(row.at(i));
+        return bits > border || (bits == border && i <= cut) ? units_of(bits) : 0;
     };
     uint64_t mine = 0;
-    for (int i = w0 + lane; i < w1; i += 32) mine += kept(i);
-    const uint64_t of_warp = warp_sum64(mine);
-    const uint64_t upto = __shfl_sync(0xffffffffu, block_scan64(lane == 0 ? of_warp : 0, sm.warp_sum), 0);
-    if (tid == 0) sm.mass = sm.warp_sum[32];
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) mine += kept(i);
+    const uint64_t upto = block_scan64(mine, sm.warp_sum);
+    if (tid < (int)blocks) put64(&sm.mass[rank], tid, sm.warp_sum[kFilterWarps]);
     cluster_sync();
-    uint64_t total = 0, before = 0;
+    uint64_t total = 0, run = upto - mine;
+#pragma unroll 1
     for (uint32_t b = 0; b < blocks; ++b) {
-        const uint64_t m = peer64(&sm.mass, b);
-        if (b < rank) before += m;
-        total += m;
+        if (b < rank) run += sm.mass[b];
+        total += sm.mass[b];
     }
-    cluster_sync();                                            // no block leaves while another may read from it
-    const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[r], (uint32_t)a.step_key[r]);
     const uint64_t target = min((uint64_t)((double)u * (double)total), total - 1);
-    uint64_t run = before + upto - of_warp;
-    if (of_warp == 0 || target < run || target >= run + of_warp) return;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const int i = i0 + lane;
-        uint64_t v = i < w1 ? kept(i) : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t x = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += x;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, run + v > target);
-        if (past) {
-            if (lane == __ffs(past) - 1) {
-                const float z = row.z[i];
-                a.token[r] = first + i;
-                a.logprob[r] = (row.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(z, row.top), t)) - logf((float)((double)total * (1.0 / 1099511627776.0)));
-            }
+    if (target < run || target >= run + mine) return;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+        run += kept(i);
+        if (run > target) {
+            a.token[r] = first + i;
+            a.logprob[r] = (row.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(row.z[i], row.top), t)) - logf((float)((double)total * (1.0 / 1099511627776.0)));
             return;
         }
-        run += __shfl_sync(0xffffffffu, v, 31);
     }
 }
 
-constexpr int kMostStaged = (227 * 1024 - (int)sizeof(FilterShared) - 1024) / 4;      // weights that a block's shared memory holds
+constexpr int kMostStaged = (113 * 1024 - (int)sizeof(FilterShared) - 1024) / 4;      // weights that a block's half of the shared memory holds
 
 }  // namespace
 
@@ -372,7 +653,7 @@ CPM_API int cpm_sample_filtered(const float* logits, int64_t ld, int n_rows, int
     const int sms = device_sms();
     // as many blocks a row as run at the same time, and as the weights need; a block of few tokens is not worth its barriers
     int blocks = 8;
-    while (blocks > 1 && ((int64_t)n_rows * blocks > sms || vocab < 1024 * blocks) && (vocab + blocks / 2 - 1) / (blocks / 2) <= kMostStaged - 4) blocks /= 2;
+    while (blocks > 1 && ((int64_t)n_rows * blocks > 2 * sms || vocab < 1024 * blocks) && (vocab + blocks / 2 - 1) / (blocks / 2) <= kMostStaged - 4) blocks /= 2;
     const int per_block = ((vocab + blocks - 1) / blocks + 3) & ~3;
     const FilterArgs a{logits, ld, vocab, per_block, uniform, temperature, top_p, min_p, top_k, seq_key, step_key, seed, token, logprob};
     if (per_block <= kMostStaged) {
