@@ -122,13 +122,14 @@ _SIGNATURES = {
     "cpm_rope_store_kv4": [_P, _P, _P, _P, _P, _P, _P, c_int, _P, c_float, c_int, c_int, c_int, c_int, c_int, _P],
     "cpm_kv4_values": [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P],
     "cpm_kv4_attention": [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_float, c_int, _P],
+    "cpm_kv4_prompt": [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, _P],
     "cpm_copy_pages": [_P, c_int, _P, _P, c_int, _P],
     "cpm_sample_filtered": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P],
     "cpm_latent_attention_mma": [_P, _P, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, _P],
 }
 
 # source files whose kernels follow page tables; the checked build (CPMCU_CHECK_BOUNDS=1) keeps a record per file
-BOUNDS_FILES = ("attention_bf16", "attention_generic", "attention_tcgen05", "elementwise", "kv4_attention", "kv4_store",
+BOUNDS_FILES = ("attention_bf16", "attention_generic", "attention_tcgen05", "elementwise", "kv4_attention", "kv4_prompt", "kv4_store",
                 "latent_attention", "sink_attention", "sparse", "talking_attention")
 
 _lock = threading.Lock()
@@ -202,8 +203,9 @@ def load() -> ctypes.CDLL:
         lib.cpm_retention_tiles_scratch_floats.restype = c_int64
         lib.cpm_kv4_attention_scratch_floats.argtypes = [c_int]
         lib.cpm_kv4_attention_scratch_floats.restype = c_int64
-        lib.cpm_kv4_attention_most_tiles.argtypes = []
-        lib.cpm_kv4_attention_most_tiles.restype = c_int
+        for name in ("cpm_kv4_attention_most_tiles", "cpm_kv4_prompt_error"):
+            getattr(lib, name).argtypes = []
+            getattr(lib, name).restype = c_int
         lib.cpm_mingru_summary_floats.argtypes = [c_int, c_int]
         lib.cpm_mingru_summary_floats.restype = c_int64
         for name, argtypes in _SIGNATURES.items():

@@ -1007,6 +1007,8 @@ class Ops:
         arena = self.workspace.persistent.arena if self.workspace is not None else None
         if arena is not None and arena.guards:
             arena.check_guards()
+        if int(self.lib.cpm_kv4_prompt_error()):
+            raise RuntimeError("the prompts' attention over a 4-bit cache gave up waiting on a barrier; the results of this step are not valid")
         if int(self.lib.cpm_listed_tile_error()):
             raise RuntimeError("the block-list attention of a prompt chunk gave up waiting on a barrier; the results of "
                                "this step are not valid")
@@ -1718,6 +1720,14 @@ class Ops:
                                           self.code, self._stream()), f"rope_store_kv4 (head_dim {d})")
         return q
 
+    KV4_PROMPT_SHARE = 3                 # from a third of the SMs on
+
+    def kv4_prompt_ok(self, n_tokens: int, n_heads: int, n_kv: int, d: int, scale: float) -> bool:
+        """Whether prompt tokens go to the tcgen05 kernel: 256 query rows a block and a block an SM, so that it needs some of them."""
+        blocks = (n_tokens * (n_heads // n_kv) + 255) // 256 * n_kv
+        return (self.use_tcgen05_attention and self.code == BF16 and d in (64, 128) and scale > 0
+                and blocks * self.KV4_PROMPT_SHARE >= self.sm_count)
+
     def kv4_values(self, records: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, slots: torch.Tensor,
                    page_table: torch.Tensor, n_kv: int, d: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """The keys and values (k, v), [tokens, kv, d] each in the compute dtype, that a 4-bit cache holds at the listed positions of the
@@ -1771,6 +1781,11 @@ class Ops:
             raise ValueError(f"{n} rows of q and {kv_len.numel()} sequences: without token offsets each row is a sequence")
         out = self.empty(n, n_heads * d)
         if n == 0:
+            return out
+        if self.kv4_prompt_ok(n, n_heads, n_kv, d, scale) if cu_q is not None else False:
+            check(self.lib.cpm_kv4_prompt(_ptr(q), _ptr(records), _ptr(out), _ptr(kv_len), _ptr(slots), _ptr(page_table), page_table.shape[1],
+                                          _ptr(cu_q), _ptr(tile_seq), _ptr(tile_row), n_tiles, n_heads, n_kv, d, int(window), float(scale),
+                                          self._stream()), f"prompt attention over a 4-bit cache (head_dim {d})")
             return out
         scratch = self.empty(int(self.lib.cpm_kv4_attention_scratch_floats(d)), dtype=torch.float32)
         # the kernel counts a launch's work in 32 bits: key-value heads x parts of a tile x pages of every tile

@@ -180,10 +180,13 @@ def test_one_token_a_sequence(dtype, d, heads, kv):
         assert float(got[0].abs().max()) == 0.0           # no keys
 
 
+@pytest.mark.parametrize("tcgen05", [False, True])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("d,heads,kv", [(32, 3, 1), (64, 8, 1), (64, 6, 2), (96, 4, 2), (128, 16, 1), (128, 2, 2)])
-def test_several_tokens_a_sequence(dtype, d, heads, kv):
+@pytest.mark.parametrize("d,heads,kv", [(32, 3, 1), (64, 8, 1), (64, 6, 2), (96, 4, 2), (128, 16, 1), (128, 2, 2), (64, 4, 2), (128, 5, 1), (64, 40, 2)])
+def test_several_tokens_a_sequence(dtype, d, heads, kv, tcgen05):
     ops = _ops(dtype)
+    ops.KV4_PROMPT_SHARE = 1000 if tcgen05 else 0             # either kernel, whatever the number of tokens
+    assert ops.kv4_prompt_ok(295, heads, kv, d, 1.0) == (tcgen05 and dtype == "bfloat16" and d in (64, 128))
     new = [1, 5, 0, 64, 65, 130, 30]
     lengths = [1, 5, 40, 64, 200, 130, 161]
     table, slots, records, rows = _filled(ops, lengths, kv, d, 13)
@@ -199,6 +202,23 @@ def test_several_tokens_a_sequence(dtype, d, heads, kv):
         _check(got, want, rows, dtype)
 
 
+@pytest.mark.parametrize("q_scale,v_scale", [(30.0, 1.0), (1e-6, 1e-6), (1.0, 1e6), (0.0, 1.0)])
+def test_magnitudes_of_a_prompt(q_scale, v_scale):
+    """The same for prompt tokens on the tcgen05 kernel, with pages of very different values."""
+    ops, d, heads, kv, n, new = _ops("bfloat16"), 128, 4, 2, 400, 100
+    ops.KV4_PROMPT_SHARE = 1000
+    table, slots, records, rows = _filled(ops, [n], kv, d, 17, v_scale=v_scale)
+    f32 = _ops("float32")
+    pos, seq = _every_position([n])
+    k, v = rows[0]
+    v = v * torch.where(torch.arange(n) % 130 < 64, 1.0, 1e-3)[:, None, None]
+    f32.rope_store_kv4(torch.cat((torch.zeros(n, kv, d), k, v), 1).flatten(1).cuda(), kv, kv, d, pos, seq, _i32(slots), table, records, None, 1.0, 0)
+    rows = [tuple(t.cpu() for t in f32.kv4_values(records, pos, seq, _i32(slots), table, kv, d))]
+    q = (torch.randn(new, heads, d, generator=torch.Generator().manual_seed(7)) * q_scale).bfloat16()
+    got = ops.kv4_attention(q.cuda(), records, _i32([n]), _i32(slots), table, kv, d ** -0.5, cu_q=_i32([0, new]), tiles=(_i32([0, 0]), _i32([0, 64]), 2))
+    _check(got, plain.attention(q, *rows[0], n - new, d ** -0.5, 0), rows, "bfloat16")
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("q_scale,v_scale", [(30.0, 1.0), (1e-6, 1e-6), (1.0, 1e6), (0.0, 1.0)])
 def test_magnitudes(dtype, q_scale, v_scale):
@@ -212,11 +232,13 @@ def test_magnitudes(dtype, q_scale, v_scale):
     _check(got, want, rows, dtype)
 
 
+@pytest.mark.parametrize("tcgen05", [False, True])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("poison", [math.nan, math.inf, 1e30])
-def test_tokens_that_are_not_seen_have_no_part(dtype, poison):
+def test_tokens_that_are_not_seen_have_no_part(dtype, poison, tcgen05):
     """Keys and values behind a prompt's token, or before its window, that are no numbers or very large, do not reach it."""
     ops, d, heads, kv = _ops(dtype), 64, 4, 2
+    ops.KV4_PROMPT_SHARE = 1000 if tcgen05 else 0
     n, new = 150, 40
     table, slots, total = _tables([n], 5)
     pos, seq = _every_position([n])
