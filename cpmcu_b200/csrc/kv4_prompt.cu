@@ -3,7 +3,7 @@
 // A block takes 256 rows of queries, the query heads of one key-value head for some consecutive tokens (16 tokens at 16 heads), so that all of them share
 // every key and value.  Four warps unpack the codes, a page of 64 keys a step, into fp16 tiles in shared memory: K [keys][d] and V
 // [d][keys], 128-byte swizzle, the K-major operands of S = Q K^T and O += P V (tcgen05.mma, accumulators in tensor memory); four tiles of each.  Eight
-// warps are the softmax, a thread to a row, which writes P as fp16 over the S it read; one warp issues the products of both halves of 128
+// warps are the softmax, a thread to a row, which writes P as fp16 over the S it read; a warp each issues the two kinds of products of both halves of 128
 // rows.  A half has two S: the next page's scores are formed while this one's are in the softmax, so that only the softmax itself is in a
 // row's way.  (With one S of 128 keys a half waited 5,600 of 8,500 cycles for its products: 347 us instead of XX.)
 //
@@ -32,7 +32,7 @@ constexpr int kRows = 256;
 constexpr int kStages = 4;                              // tiles of keys, and of values
 constexpr int kInfos = 8;                               // steps that unpacking may be ahead of the softmax, and one
 constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4;
-constexpr int kThreads = (kSoftmaxWarps + 1 + kUnpackWarps) * 32;      // 128 registers each
+constexpr int kThreads = (kSoftmaxWarps + 2 + kUnpackWarps) * 32;      // 128 registers each
 constexpr float kBehind = 8.0f;                         // the running maximum may lie 2^8 behind
 constexpr int kQHalf = 128 * 128, kKHalf = 64 * 128;    // 128 rows of Q, 64 keys: runs of 128 bytes
 constexpr int kQExtra = 128 * 32, kKExtra = 64 * 32;    // 16 more columns, two runs of 16 bytes a row
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 kv4_prompt_kernel(const __grid_constant__ Args a) {
     using Z = Sizes<D>;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages], s_full[2][2], p_full[2][2], o_done[2];      // (of two S the softmax may be two steps ahead of the products: each has its own barriers)
+    __shared__ __align__(8) uint64_t q_full[2], k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages], s_full[2][2], p_full[2][2], o_done[2][2];      // (of two S the softmax may be two steps ahead of the products: each has its own barriers)
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ StepInfo info[kInfos];
@@ -208,7 +208,8 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             mbar_init(smem_u32(&s_full[i][1]), 1);
             mbar_init(smem_u32(&p_full[i][0]), 4);
             mbar_init(smem_u32(&p_full[i][1]), 4);
-            mbar_init(smem_u32(&o_done[i]), 1);
+            mbar_init(smem_u32(&o_done[i][0]), 1);
+            mbar_init(smem_u32(&o_done[i][1]), 1);
         }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -235,9 +236,9 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     };
     auto aborted = [&]() { return *(volatile int*)&abort_flag != 0; };
 
-    if (warp > kSoftmaxWarps) {
+    if (warp >= kSoftmaxWarps + 2) {
         // ---- unpacking: a warp takes 16 tokens of every page, whose codes were asked for a page ahead ----
-        const int slice = warp - kSoftmaxWarps - 1, g = lane >> 2, j4 = lane & 3;
+        const int slice = warp - kSoftmaxWarps - 2, g = lane >> 2, j4 = lane & 3;
         const int* table = a.page_table + (int64_t)a.slots[seq] * a.max_pages;
         const uint8_t* records = a.records + (int64_t)head_kv * Kv4<D>::kBytes;
         const int64_t page_stride = (int64_t)a.n_kv * Kv4<D>::kBytes;
@@ -374,47 +375,48 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             if (lane == 0) mbar_arrive(smem_u32(&v_full[s]));
         }
     } else if (warp == kSoftmaxWarps) {
-        // ---- the products, issued by one thread: the next page's scores before this page's values ----
+        // ---- scores, issued by one thread as soon as a page's keys are there and an S is free ----
         if (lane == 0 && n_steps > 0) {
-            const auto issue_qk = [&](int i, int st) {
+            if (!mbar_wait_bounded(smem_u32(&q_full[0]), 0) || !mbar_wait_bounded(smem_u32(&q_full[1]), 0)) fail(ERR_Q);
+#pragma unroll 1
+            for (int st = 0; st < n_steps && !aborted(); ++st) {
                 const int s = st % kStages;
-                const uint32_t to = tmem + i * 128 + (st & 1) * 64;
-#pragma unroll
-                for (int half = 0; half < Z::kHalves; ++half) {
-                    const uint64_t da = smem_desc_sw128(q_smem + i * Z::kQ + half * kQHalf), db = smem_desc_sw128(k_smem + s * Z::kKv + half * kKHalf);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) tcgen05_mma_f16(to, da + 2 * k, db + 2 * k, Z::idesc(64), (half | k) != 0);
-                }
-                tcgen05_mma_f16(to, smem_desc_plain(qx_smem + i * kQExtra, 128), smem_desc_plain(kx_smem + s * kKExtra, 64), Z::idesc(64), 1);
-                tcgen05_commit(smem_u32(&s_full[i][st & 1]));
-            };
-            const auto issue_pv = [&](int i, int st) {
-                const uint64_t db = smem_desc_sw128(v_smem + (st % kStages) * Z::kKv);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    tcgen05_mma_f16_ts(tmem + Z::kO + i * D, tmem + i * 128 + (st & 1) * 64 + k * 8, db + 2 * k, Z::idesc(D), st > 0 || k != 0);
-                tcgen05_commit(smem_u32(&o_done[i]));
-            };
-            bool ok = true;
-            if (!mbar_wait_bounded(smem_u32(&q_full[0]), 0) || !mbar_wait_bounded(smem_u32(&q_full[1]), 0)) { fail(ERR_Q); ok = false; }
+                if (!mbar_wait_bounded(smem_u32(&k_full[s]), (st / kStages) & 1)) { fail(ERR_K_FULL); break; }
 #pragma unroll 1
-            for (int st = -1; ok && st < n_steps && !aborted(); ++st) {
-                if (st + 1 < n_steps) {
-                    const int s1 = (st + 1) % kStages;
-                    if (!mbar_wait_bounded(smem_u32(&k_full[s1]), ((st + 1) / kStages) & 1)) { fail(ERR_K_FULL); break; }
+                for (int i = 0; i < 2; ++i) {
+                    if (st >= 2 && !mbar_wait_bounded(smem_u32(&o_done[i][st & 1]), ((st - 2) >> 1) & 1)) { fail(ERR_O_FULL); break; }
                     tcgen05_fence_after();
-#pragma unroll 1
-                    for (int i = 0; i < 2; ++i) issue_qk(i, st + 1);
-                    tcgen05_commit(smem_u32(&k_empty[s1]));
+                    const uint32_t to = tmem + i * 128 + (st & 1) * 64;
+#pragma unroll
+                    for (int half = 0; half < Z::kHalves; ++half) {
+                        const uint64_t da = smem_desc_sw128(q_smem + i * Z::kQ + half * kQHalf), db = smem_desc_sw128(k_smem + s * Z::kKv + half * kKHalf);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) tcgen05_mma_f16(to, da + 2 * k, db + 2 * k, Z::idesc(64), (half | k) != 0);
+                    }
+                    tcgen05_mma_f16(to, smem_desc_plain(qx_smem + i * kQExtra, 128), smem_desc_plain(kx_smem + s * kKExtra, 64), Z::idesc(64), 1);
+                    tcgen05_commit(smem_u32(&s_full[i][st & 1]));
                 }
-                if (st < 0) continue;
+                tcgen05_commit(smem_u32(&k_empty[s]));
+            }
+        }
+        __syncwarp();
+    } else if (warp == kSoftmaxWarps + 1) {
+        // ---- weighted values, issued by one thread ----
+        if (lane == 0) {
+            bool ok = true;
+#pragma unroll 1
+            for (int st = 0; ok && st < n_steps && !aborted(); ++st) {
                 const int s = st % kStages;
                 if (!mbar_wait_bounded(smem_u32(&v_full[s]), (st / kStages) & 1)) { fail(ERR_V_FULL); break; }
+                const uint64_t db = smem_desc_sw128(v_smem + s * Z::kKv);
 #pragma unroll 1
                 for (int i = 0; i < 2; ++i) {
                     if (!mbar_wait_bounded(smem_u32(&p_full[i][st & 1]), (st >> 1) & 1)) { fail(ERR_P_FULL); ok = false; break; }
                     tcgen05_fence_after();
-                    issue_pv(i, st);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tcgen05_mma_f16_ts(tmem + Z::kO + i * D, tmem + i * 128 + (st & 1) * 64 + k * 8, db + 2 * k, Z::idesc(D), st > 0 || k != 0);
+                    tcgen05_commit(smem_u32(&o_done[i][st & 1]));
                 }
                 if (ok) tcgen05_commit(smem_u32(&v_empty[s]));
             }
@@ -521,7 +523,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                     l *= alpha;
                     if (st > 0) {
                         // the products of the page before have to be in O
-                        if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i]), (st - 1) & 1)) && lane == 0) fail(ERR_O_FULL);
+                        if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i][(st - 1) & 1]), ((st - 1) >> 1) & 1)) && lane == 0) fail(ERR_O_FULL);
                         tcgen05_fence_after();
                         const float by = alpha * power2(power - power_new);
 #pragma unroll 1
@@ -572,7 +574,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             if (lane == 0) mbar_arrive(smem_u32(&p_full[i][st & 1]));
         }
         if (ok && n_steps > 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i]), (n_steps - 1) & 1))) {
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i][(n_steps - 1) & 1]), ((n_steps - 1) >> 1) & 1))) {
                 if (lane == 0) fail(ERR_O_FULL);
                 ok = false;
             }
