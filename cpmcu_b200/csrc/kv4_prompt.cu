@@ -5,7 +5,8 @@
 // [d][keys], 128-byte swizzle, the K-major operands of S = Q K^T and O += P V (tcgen05.mma, accumulators in tensor memory); four tiles of each.  Eight
 // warps are the softmax, a thread to a row, which writes P as fp16 over the S it read; a warp each issues the two kinds of products of both halves of 128
 // rows.  A half has two S: the next page's scores are formed while this one's are in the softmax, so that only the softmax itself is in a
-// row's way.  (With one S of 128 keys a half waited 5,600 of 8,500 cycles for its products: 347 us instead of XX.)
+// row's way.  (2,048 tokens of 32 heads on 2 behind 4,101 keys, 172 GFLOP: one S of
+// 128 keys, whose softmax waits for its products, 347 us; two and one warp for all products, 333; as it is, 269, 640 TFLOP/s.)
 //
 // fp16 and not bf16: its 11 bits hold s (c - 8) exactly, 8 bits times 3, so that scores are as exact as their fp32 sums.  The rest of a
 // key's product, m times the sum of the query's half row, is 16 more columns of the operands: m three times and the sum as three fp16 numbers,
@@ -15,7 +16,7 @@
 // values so far.
 //
 // Unpacking a key and a value costs about two instructions a number, 256 rows of softmax four to five; a block of 128 rows would pay it twice.
-// Bound by the exponentials and the issue slots of the softmax; see the launcher for where the other kernel is faster.
+// Bound by the unpacking warps, about 3,000 cycles a page with their barriers, where the softmax takes 1,800 and the products 1,400.
 //
 // Every wait is bounded: a block that gives up records an error, stops, frees its tensor memory and returns (nothing is in flight then: tiles are
 // written by ordinary stores).
@@ -55,7 +56,8 @@ struct Args {
     bf16* out;
     const uint8_t* records;
     const int *kv_len, *slots, *page_table, *cu_q, *tile_seq, *tile_row;
-    int max_pages, n_heads, n_kv, group, window, tile_tokens;
+    float* parts;                                       // with shares of the keys: [share][row of q][d + 2]: values, maximum, sum
+    int max_pages, n_heads, n_kv, group, window, tile_tokens, n_tokens;
     float scale;
 };
 
@@ -182,8 +184,10 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     if (n_rows <= 0) return;
     const int pos_low = history + row0 + first / a.group, pos_high = history + row0 + (first + n_rows - 1) / a.group;
     const int n_keys = min(kv_len, pos_high + 1);
-    const int page0 = a.window ? max(0, pos_low - a.window + 1) / kPageTokens : 0;
-    const int n_steps = max(0, (n_keys + kPageTokens - 1) / kPageTokens - page0);
+    // few rows and many keys: a tile's pages are shared out over gridDim.z blocks
+    const int first_page = a.window ? max(0, pos_low - a.window + 1) / kPageTokens : 0;
+    const int all_steps = max(0, (n_keys + kPageTokens - 1) / kPageTokens - first_page), share = (all_steps + gridDim.z - 1) / gridDim.z;
+    const int page0 = first_page + blockIdx.z * share, n_steps = max(0, min(share, all_steps - (int)blockIdx.z * share));
     // whether some row sees some key of a step and not another
     const auto in_part = [&](int st) {
         const int key0 = (page0 + st) * kPageTokens;
@@ -581,7 +585,9 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             tcgen05_fence_after();
         }
         if (ok) {
-            const float inv = l == 0.f ? 0.f : power2(power) / l;
+            const bool shared = gridDim.z > 1;
+            float* mine = a.parts + ((int64_t)blockIdx.z * a.n_tokens * a.n_heads + at / D) * (D + 4);
+            const float by = shared ? (n_steps > 0 ? power2(power) : 0.f) : l == 0.f ? 0.f : power2(power) / l;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t o[16];
@@ -594,10 +600,13 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                 }
                 if (valid)
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        store4(a.out + at + c * 16 + e, make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                                                    __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv));
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 y = make_float4(__uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by, __uint_as_float(o[e + 2]) * by, __uint_as_float(o[e + 3]) * by);
+                        if (shared) store4(mine + c * 16 + e, y);
+                        else store4(a.out + at + c * 16 + e, y);
+                    }
             }
+            if (valid && shared) *reinterpret_cast<float2*>(mine + D) = make_float2(m, l);
         }
     }
     tcgen05_fence_before();
@@ -608,14 +617,44 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     }
 }
 
+// Adds up the shares of a row of q: a warp a row.
 template <int D>
-int prompt(const Args& a, int n_tiles, cudaStream_t stream) {
+__global__ void __launch_bounds__(256)
+kv4_prompt_join_kernel(const float* __restrict__ parts, bf16* __restrict__ out, int64_t rows, int shares) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const auto place = [&](int z) { return parts + ((int64_t)z * rows + row) * (D + 4); };
+    float top = -INFINITY, l = 0.f, o[D / 32];
+    for (int z = 0; z < shares; ++z) top = fmaxf(top, place(z)[D]);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int z = 0; z < shares; ++z) {
+        const float* p = place(z);
+        const float2 ml = *reinterpret_cast<const float2*>(p + D);
+        const float by = ml.x > -INFINITY ? ex2(ml.x - top) : 0.f;
+        l += ml.y * by;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] += p[lane + 32 * i] * by;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) out[row * D + lane + 32 * i] = from_f32<bf16>(o[i] * inv);
+}
+
+template <int D>
+int prompt(const Args& a, int n_tiles, int shares, cudaStream_t stream) {
     static bool done[kMaxDevices];
     const int status = ensure_dynamic_smem(kv4_prompt_kernel<D>, Sizes<D>::kSmem, done);
     if (status != CPM_OK) return status;
-    const int64_t parts = (int64_t)((a.tile_tokens * a.group + kRows - 1) / kRows) * a.n_kv;
-    if (n_tiles > 65535 || parts > 0x7fffffff) return CPM_BAD_ARGUMENT;
-    cpm_launch(kLaunchAttention, kv4_prompt_kernel<D>, dim3((unsigned)parts, n_tiles), kThreads, Sizes<D>::kSmem, stream, a);
+    const int64_t blocks = (int64_t)((a.tile_tokens * a.group + kRows - 1) / kRows) * a.n_kv, rows = (int64_t)a.n_tokens * a.n_heads;
+    if (n_tiles > 65535 || blocks > 0x7fffffff || rows / 8 >= 0x7fffffff) return CPM_BAD_ARGUMENT;
+    cpm_launch(kLaunchAttention, kv4_prompt_kernel<D>, dim3((unsigned)blocks, n_tiles, shares), kThreads, Sizes<D>::kSmem, stream, a);
+    if (shares > 1)
+        cpm_launch(kLaunchAttention, kv4_prompt_join_kernel<D>, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, (const float*)a.parts, a.out, rows, shares);
     return launch_status();
 }
 
@@ -629,20 +668,21 @@ CPM_API int cpm_kv4_prompt_error() {
     return code;
 }
 
-// q, out bf16 [tokens, heads, d]; the tiles are of 64 tokens, taken together up to 256 rows of a key-value head.
+// q, out bf16 [tokens, heads, d]; the tiles are of 64 tokens, taken together up to 256 rows of a key-value head.  ``shares`` > 1: a tile's keys are shared out
+// over so many blocks, whose parts (shares x tokens x heads x (d + 4) floats in ``parts``) a second kernel adds up; every token has to be in a tile then.
 CPM_API int cpm_kv4_prompt(const void* q, const void* records, void* out, const int* kv_len, const int* slots, const int* page_table, int max_pages,
-                           const int* cu_q, const int* tile_seq, const int* tile_row, int n_tiles, int n_heads, int n_kv, int d, int window, float scale,
-                           cudaStream_t stream) {
+                           const int* cu_q, const int* tile_seq, const int* tile_row, int n_tiles, float* parts, int shares, int n_tokens, int n_heads, int n_kv,
+                           int d, int window, float scale, cudaStream_t stream) {
     if (n_tiles <= 0) return CPM_OK;
-    if (n_heads < 1 || n_kv < 1 || n_heads % n_kv || window < 0 || !(scale > 0.f)) return CPM_BAD_ARGUMENT;
+    if (n_heads < 1 || n_kv < 1 || n_heads % n_kv || window < 0 || !(scale > 0.f) || shares < 1 || shares > 64 || (shares > 1 && !parts)) return CPM_BAD_ARGUMENT;
     if (((uintptr_t)records | (uintptr_t)q | (uintptr_t)out) & 15) return CPM_BAD_ARGUMENT;
     const int group = n_heads / n_kv;
     const int tile_tokens = group == 1 ? 256 : group == 2 ? 128 : 64;
-    const kv4p::Args a{(const bf16*)q, (bf16*)out, (const uint8_t*)records, kv_len, slots, page_table, cu_q, tile_seq, tile_row, max_pages, n_heads, n_kv,
-                       group, window, tile_tokens, scale};
+    const kv4p::Args a{(const bf16*)q, (bf16*)out, (const uint8_t*)records, kv_len, slots, page_table, cu_q, tile_seq, tile_row, parts, max_pages,
+                       n_heads, n_kv, group, window, tile_tokens, n_tokens, scale};
     switch (d) {
-        case 64: return kv4p::prompt<64>(a, n_tiles, stream);
-        case 128: return kv4p::prompt<128>(a, n_tiles, stream);
+        case 64: return kv4p::prompt<64>(a, n_tiles, shares, stream);
+        case 128: return kv4p::prompt<128>(a, n_tiles, shares, stream);
         default: return CPM_BAD_ARGUMENT;
     }
 }

@@ -1720,13 +1720,20 @@ class Ops:
                                           self.code, self._stream()), f"rope_store_kv4 (head_dim {d})")
         return q
 
-    KV4_PROMPT_SHARE = 3                 # from a third of the SMs on
+    KV4_PROMPT_BLOCKS = 5                # query rows that fill so many blocks go to the tcgen05 kernel
 
     def kv4_prompt_ok(self, n_tokens: int, n_heads: int, n_kv: int, d: int, scale: float) -> bool:
-        """Whether prompt tokens go to the tcgen05 kernel: 256 query rows a block and a block an SM, so that it needs some of them."""
-        blocks = (n_tokens * (n_heads // n_kv) + 255) // 256 * n_kv
+        """Whether prompt tokens go to the tcgen05 kernel, which takes 256 query rows of a key-value head a block and shares few blocks' keys out.
+        us, token by token's kernel and this one: 32 heads on 2 of 128, 32 tokens behind 8,000 keys (4 blocks) 45 and 46, 64 tokens 73 and 41, 64
+        behind 500 27 and 24; 16 on 2 of 64, 64 behind 8,000 (4 blocks) 36 and 27, behind 500 18 and 18; 8 on 4 of 128, 128 behind 8,000 (4
+        blocks) 45 and 48, 256 72 and 45."""
         return (self.use_tcgen05_attention and self.code == BF16 and d in (64, 128) and scale > 0
-                and blocks * self.KV4_PROMPT_SHARE >= self.sm_count)
+                and (n_tokens * (n_heads // n_kv) + 255) // 256 * n_kv >= self.KV4_PROMPT_BLOCKS)
+
+    def kv4_prompt_shares(self, n_tokens: int, n_heads: int, n_kv: int, longest: int) -> int:
+        """Blocks that share the keys of a tile of query rows: a wave of blocks, with four pages or more each."""
+        blocks = (n_tokens * (n_heads // n_kv) + 255) // 256 * n_kv
+        return max(1, min(self.sm_count // blocks, (longest + 4 * PAGE_TOKENS - 1) // (4 * PAGE_TOKENS), 32))
 
     def kv4_values(self, records: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, slots: torch.Tensor,
                    page_table: torch.Tensor, n_kv: int, d: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -1746,11 +1753,13 @@ class Ops:
         return k, v
 
     def kv4_attention(self, q: torch.Tensor, records: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor,
-                      n_kv: int, scale: float, window: int = 0, cu_q: Optional[torch.Tensor] = None, tiles=None) -> torch.Tensor:
+                      n_kv: int, scale: float, window: int = 0, cu_q: Optional[torch.Tensor] = None, tiles=None,
+                      longest: int = 0) -> torch.Tensor:
         """Attention over a cache in 4 bits: q [tokens, heads, d] -> [tokens, heads * d].  Without ``cu_q`` every row of q is the last token
         of a sequence of ``kv_len`` keys; with it sequence s brings the tokens cu_q[s] .. cu_q[s + 1], the last of its kv_len[s] keys, and
         ``tiles`` = (sequence, first token, count) lists them in tiles of QUERY_TILE_TOKENS, as for ``prefill_attention``.  A token at
-        position p sees the keys p - window < j <= p (``window`` 0: all j <= p); a row that sees none gives zeros."""
+        position p sees the keys p - window < j <= p (``window`` 0: all j <= p); a row that sees none gives zeros.  ``longest``: a bound on the
+        sequences' keys where the caller knows one (0: the page table's width); it only decides how a prompt's keys are shared out."""
         self._act(q, "q")
         if q.dim() != 3:
             raise ValueError("q: needs [tokens, heads, d]")
@@ -1782,10 +1791,14 @@ class Ops:
         out = self.empty(n, n_heads * d)
         if n == 0:
             return out
-        if self.kv4_prompt_ok(n, n_heads, n_kv, d, scale) if cu_q is not None else False:
+        if cu_q is not None and self.kv4_prompt_ok(n, n_heads, n_kv, d, scale):
+            shares = self.kv4_prompt_shares(n, n_heads, n_kv, longest or page_table.shape[1] * PAGE_TOKENS)
+            parts = self.empty(shares * n * n_heads * (d + 4), dtype=torch.float32) if shares > 1 else None
             check(self.lib.cpm_kv4_prompt(_ptr(q), _ptr(records), _ptr(out), _ptr(kv_len), _ptr(slots), _ptr(page_table), page_table.shape[1],
-                                          _ptr(cu_q), _ptr(tile_seq), _ptr(tile_row), n_tiles, n_heads, n_kv, d, int(window), float(scale),
-                                          self._stream()), f"prompt attention over a 4-bit cache (head_dim {d})")
+                                          _ptr(cu_q), _ptr(tile_seq), _ptr(tile_row), n_tiles, _ptr(parts), shares, n, n_heads, n_kv, d,
+                                          int(window), float(scale), self._stream()), f"prompt attention over a 4-bit cache (head_dim {d})")
+            if shares > 1:
+                LAUNCHES_EXTRA[0] += 1
             return out
         scratch = self.empty(int(self.lib.cpm_kv4_attention_scratch_floats(d)), dtype=torch.float32)
         # the kernel counts a launch's work in 32 bits: key-value heads x parts of a tile x pages of every tile

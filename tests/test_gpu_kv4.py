@@ -180,12 +180,14 @@ def test_one_token_a_sequence(dtype, d, heads, kv):
         assert float(got[0].abs().max()) == 0.0           # no keys
 
 
-@pytest.mark.parametrize("tcgen05", [False, True])
+@pytest.mark.parametrize("tcgen05,shares", [(False, 0), (True, 1), (True, 3), (True, 0)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("d,heads,kv", [(32, 3, 1), (64, 8, 1), (64, 6, 2), (96, 4, 2), (128, 16, 1), (128, 2, 2), (64, 4, 2), (128, 5, 1), (64, 40, 2)])
-def test_several_tokens_a_sequence(dtype, d, heads, kv, tcgen05):
+def test_several_tokens_a_sequence(dtype, d, heads, kv, tcgen05, shares):
     ops = _ops(dtype)
-    ops.KV4_PROMPT_SHARE = 1000 if tcgen05 else 0             # either kernel, whatever the number of tokens
+    ops.KV4_PROMPT_BLOCKS = 0 if tcgen05 else 1 << 30         # either kernel, whatever the number of tokens
+    if shares:
+        ops.kv4_prompt_shares = lambda *a: shares
     assert ops.kv4_prompt_ok(295, heads, kv, d, 1.0) == (tcgen05 and dtype == "bfloat16" and d in (64, 128))
     new = [1, 5, 0, 64, 65, 130, 30]
     lengths = [1, 5, 40, 64, 200, 130, 161]
@@ -206,7 +208,7 @@ def test_several_tokens_a_sequence(dtype, d, heads, kv, tcgen05):
 def test_magnitudes_of_a_prompt(q_scale, v_scale):
     """The same for prompt tokens on the tcgen05 kernel, with pages of very different values."""
     ops, d, heads, kv, n, new = _ops("bfloat16"), 128, 4, 2, 400, 100
-    ops.KV4_PROMPT_SHARE = 1000
+    ops.KV4_PROMPT_BLOCKS = 0
     table, slots, records, rows = _filled(ops, [n], kv, d, 17, v_scale=v_scale)
     f32 = _ops("float32")
     pos, seq = _every_position([n])
@@ -238,7 +240,7 @@ def test_magnitudes(dtype, q_scale, v_scale):
 def test_tokens_that_are_not_seen_have_no_part(dtype, poison, tcgen05):
     """Keys and values behind a prompt's token, or before its window, that are no numbers or very large, do not reach it."""
     ops, d, heads, kv = _ops(dtype), 64, 4, 2
-    ops.KV4_PROMPT_SHARE = 1000 if tcgen05 else 0
+    ops.KV4_PROMPT_BLOCKS = 0 if tcgen05 else 1 << 30
     n, new = 150, 40
     table, slots, total = _tables([n], 5)
     pos, seq = _every_position([n])
