@@ -13,6 +13,9 @@ back as soon as every key in them has fallen out of the window of all later quer
 so what such a group holds per sequence is bounded by the window and the step size;
 the pages of the first tokens that such a window keeps (``CacheNeeds.keep_first``) stay.
 
+A sequence can be forked: its copies share its full pages, each of which goes back to the free list with its last holder, and have a copy
+of the last, partial one and of its state.  A lane whose needs ask for 4 bits has one tensor of records instead of keys and values.
+
 The reference keeps one sequence in one contiguous buffer per layer
 (src/model/kvcache.cuh:7-26) and its per-sequence counters in host-side fields of each
 layer object (src/model/minicpm4/minicpm4_kvcache.cuh:211-213).
@@ -20,12 +23,12 @@ layer object (src/model/minicpm4/minicpm4_kvcache.cuh:211-213).
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from ..memory import Staging
-from ..parts.base import PAGE_TOKENS, CacheNeeds
+from ..parts.base import PAGE_TOKENS, CacheNeeds, kv4_page_bytes
 from .allocator import CacheFull, FreeList, HandleError
 
 RELEASED = -1          # entry of a sequence's page list whose page went back to the pool
@@ -56,8 +59,10 @@ class CacheGroup:
         self.page_table = make("state", (n_slots, max_pages_per_seq), torch.int32, True)
         self._dirty: Dict[int, int] = {}      # slot -> first table column not yet on the device
         n = len(lanes)
-        self.k = self.v = self.pooled = None
-        if needs.kv_heads > 0:
+        self.k = self.v = self.pooled = self.records = None
+        if needs.kv_heads > 0 and needs.bits == 4:
+            self.records = make("pages", (n, n_pages, needs.kv_heads, kv4_page_bytes(needs.head_dim)), torch.uint8, True)
+        elif needs.kv_heads > 0:
             # zeros, not empty: a kernel may multiply a masked weight of 0 with whatever a page
             # holds beyond the sequence's end, and that has to be a finite number
             self.k = make("pages", (n, n_pages, needs.kv_heads, PAGE_TOKENS, needs.head_dim), dtype, True)
@@ -72,6 +77,8 @@ class CacheGroup:
                 self.pooled = make("pages", (n, n_pages, needs.kv_heads, per_page, needs.head_dim), torch.float32, False)
 
     def bytes_per_token(self) -> int:
+        if self.records is not None:
+            return self.needs.kv_heads * kv4_page_bytes(self.needs.head_dim) // PAGE_TOKENS * len(self.lanes)
         if self.k is None:
             return 0
         row = self.needs.head_dim + ((self.needs.value_dim or self.needs.head_dim) if self.needs.values else 0)
@@ -137,6 +144,58 @@ class CacheGroup:
         self._dirty.clear()
 
 
+    def tensors(self) -> List[torch.Tensor]:
+        """What the group's pages hold: [lanes, pages, ...] each."""
+        return [t for t in (self.k, self.v, self.pooled, self.records) if t is not None]
+
+    def fork(self, slot: int, children: Sequence[int], length: int) -> List[Tuple[int, int]]:
+        """The children hold the sequence's pages with it; from the first page on that a later token still changes each takes
+        pages of its own.  Returns the pages to copy, (from, to).  All or nothing."""
+        pages = self.pages_of_slot.get(slot, [])[:pages_for(length)]
+        # a full page is never written again, but for the pooled keys whose windows reach into the next one
+        own = max(0, length - self.needs.pooled_kernel + 1 if self.needs.pooled_stride else length) // PAGE_TOKENS
+        own = min(own, len(pages))
+        shared = [p for p in pages[:own] if p != RELEASED]
+        fresh = self.pages.take((len(pages) - own) * len(children))
+        moves: List[Tuple[int, int]] = []
+        for child in children:
+            mine, fresh = fresh[:len(pages) - own], fresh[len(pages) - own:]
+            self.pages.share(shared)
+            moves.extend((a, b) for a, b in zip(pages[own:], mine) if a != RELEASED)
+            self.pages_of_slot[child] = pages[:own] + mine
+            if slot in self.first_live:
+                self.first_live[child] = self.first_live[slot]
+            self._dirty[child] = 0
+        return moves
+
+    def fork_needs(self, slot: int, n: int, length: int) -> int:
+        """Pages that ``fork`` takes for ``n`` children."""
+        pages = pages_for(length)
+        own = max(0, length - self.needs.pooled_kernel + 1 if self.needs.pooled_stride else length) // PAGE_TOKENS
+        return max(0, pages - own) * n
+
+    def compact(self) -> List[Tuple[int, int]]:
+        """Gives the held pages the lowest numbers; returns the pages to copy, (from, to)."""
+        held = self.pages.n_held
+        high = [p for p in range(held, self.n_pages) if self.pages.is_held(p)]
+        moves = list(zip(high, [p for p in range(held) if not self.pages.is_held(p)]))
+        if moves:
+            self.pages.move(moves)
+            to = dict(moves)
+            for slot, pages in self.pages_of_slot.items():
+                changed = [i for i, p in enumerate(pages) if p in to]
+                if changed:
+                    self.pages_of_slot[slot] = [to.get(p, p) for p in pages]
+                    self._dirty[slot] = min(self._dirty.get(slot, changed[0]), changed[0])
+        return moves
+
+
+def copy_pages(tensors: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copies pages in tensors [layers, pages, ...] by torch; an engine on the device puts its kernel in the place of it."""
+    for t in tensors:
+        t[:, dst.long()] = t[:, src.long()]
+
+
 @dataclass
 class Lane:
     """What one run of a layer sees of the cache."""
@@ -157,6 +216,14 @@ class Lane:
     @property
     def pooled(self) -> Optional[torch.Tensor]:
         return None if self.group.pooled is None else self.group.pooled[self.index_in_group]
+
+    @property
+    def records(self) -> Optional[torch.Tensor]:
+        return None if self.group.records is None else self.group.records[self.index_in_group]
+
+    @property
+    def n_pages(self) -> int:
+        return 0 if self.group.k is None and self.group.records is None else self.group.n_pages
 
     @property
     def page_table(self) -> torch.Tensor:
@@ -192,6 +259,7 @@ class Cache:
         per_seq = pages_for(max_seq_tokens) if max_seq_tokens else n_pages
         self.max_pages_per_seq = max(1, min(per_seq, n_pages))
         self.slots = FreeList(self.n_slots, "slot")
+        self.copy_pages = copy_pages                  # (tensors, from, to): see ``fork_sequence`` and ``compact``
         self.lengths: Dict[int, int] = {}
 
         self.groups: List[CacheGroup] = []
@@ -303,6 +371,46 @@ class Cache:
             for g in windowed:
                 g.trim(s, n)
 
+    def fork_sequence(self, slot: int, n: int) -> List[int]:
+        """``n`` further sequences that hold what this one does, in slots of their own: full pages are shared, the last, partial
+        one and the per-sequence state are copied, behind what is queued on the current stream.  All or nothing."""
+        if not self.slots.is_held(slot):
+            raise HandleError(f"slot {slot} is not open")
+        length = self.lengths[slot]
+        if n > self.slots.n_free:
+            raise CacheFull(f"{n} sequences wanted, {self.slots.n_free} of {self.n_slots} slots free")
+        for g in self.groups:
+            if g.fork_needs(slot, n, length) > g.pages.n_free:
+                raise CacheFull(f"forking a sequence of {length} tokens {n} times needs {g.fork_needs(slot, n, length)} pages, "
+                                f"{g.pages.n_free} of {g.n_pages} are free")
+        if n <= 0:
+            return []
+        children = self.slots.take(n)
+        for child in children:
+            self.lengths[child] = length
+        for g in self.groups:
+            self._copy(g.tensors(), g.fork(slot, children, length))
+        states = [t.unsqueeze(0) for lane in self.lanes for t in lane.state.values()]
+        self._copy(states, [(slot, child) for child in children])
+        return children
+
+    def compact(self) -> int:
+        """Moves pages so that every group's held ones have the lowest numbers, behind what is queued on the current stream; the next
+        ``sync`` brings the page tables up to date and has to come before the next step.  Returns the number of pages moved."""
+        moved = 0
+        for g in self.groups:
+            moves = g.compact()
+            self._copy(g.tensors(), moves)
+            moved += len(moves)
+        return moved
+
+    def _copy(self, tensors: List[torch.Tensor], moves: List[Tuple[int, int]]) -> None:
+        if not tensors or not moves:
+            return
+        both = torch.empty(2, len(moves), dtype=torch.int32, device=self.device)
+        self.staging.copy(torch.tensor([a for a, _ in moves] + [b for _, b in moves], dtype=torch.int32), [both.view(-1)])
+        self.copy_pages(tensors, both[0], both[1])
+
     def close_sequence(self, slot: int) -> None:
         if not self.slots.is_held(slot):
             raise HandleError(f"slot {slot} is not open (closed twice?)")
@@ -326,19 +434,20 @@ class Cache:
         return sum(g.bytes_per_token() for g in self.groups)
 
     def check_consistent(self) -> None:
-        """Every page is free or held by exactly one open sequence; raises otherwise."""
+        """Every page is free, or held as often as open sequences name it; raises otherwise."""
         for g in self.groups:
-            seen = set()
+            seen: Dict[int, int] = {}
             for slot, pages in g.pages_of_slot.items():
                 if not self.slots.is_held(slot):
                     raise HandleError(f"pages held by closed slot {slot}")
                 for p in pages:
                     if p == RELEASED:
                         continue
-                    if p in seen:
-                        raise HandleError(f"page {p} is held twice")
-                    seen.add(p)
+                    seen[p] = seen.get(p, 0) + 1
                     if not g.pages.is_held(p):
                         raise HandleError(f"page {p} is in use but marked free")
+            for p, times in seen.items():
+                if times != g.pages.times_held(p):
+                    raise HandleError(f"page {p} is held {g.pages.times_held(p)} times and named by {times} sequences")
             if len(seen) != g.pages.n_held:
                 raise HandleError(f"{g.pages.n_held - len(seen)} pages are lost (held by no sequence)")

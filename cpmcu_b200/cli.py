@@ -8,7 +8,7 @@ has them; every flag has a ``--kebab-case`` and a ``--snake_case`` spelling.
 Options the reference has and this library leaves out belong to parts that are not
 built (draft models, quantized weights, the per-flag sparse-attention knobs: those come
 from the folder's config.json here).  Added: ``--prompt-ids`` (token ids, no tokenizer
-needed), ``--top-p``, ``--max-batch``, ``--max-tokens``, ``--plugin`` (a module that registers
+needed), ``--top-p``, ``--top-k``, ``--min-p``, ``--samples``, ``--cache-bits``, ``--max-batch``, ``--max-tokens``, ``--plugin`` (a module that registers
 parts or an architecture of its own).
 """
 from __future__ import annotations
@@ -48,6 +48,10 @@ def create_cli_parser() -> argparse.ArgumentParser:
                    help="Number of tokens to generate (default: 1024)")
     g.add_argument("--temperature", "--temp", type=float, default=0.0, help="Temperature (default: 0.0)")
     g.add_argument("--top-p", "--top_p", type=float, default=1.0, help="Nucleus mass kept when sampling (default: 1.0)")
+    g.add_argument("--top-k", "--top_k", type=int, default=0, help="Likeliest tokens kept when sampling (default: 0 = all)")
+    g.add_argument("--min-p", "--min_p", type=float, default=0.0,
+                   help="Least probability kept when sampling, relative to the likeliest token's (default: 0)")
+    g.add_argument("--samples", type=int, default=1, help="Answers to every prompt; the prompt runs once (default: 1)")
     g.add_argument("--random-seed", "--random_seed", type=int, default=None, help="Random seed")
     g.add_argument("--ignore-eos", "--ignore_eos", default=False, **flag,
                    help="Ignore EOS tokens during generation (default: False)")
@@ -76,6 +80,8 @@ def create_cli_parser() -> argparse.ArgumentParser:
     g.add_argument("--chunk-length", "--chunk_length", type=int, default=2048, help="Chunked prefill size (default: 2048)")
     g.add_argument("--plain-output", "--plain_output", default=False, **flag,
                    help="Use plain text output (default: False; output is always plain here)")
+    g.add_argument("--cache-bits", "--cache_bits", type=int, default=None, choices=[4, 16],
+                   help="Bits of a key or value in the cache (default: the configuration's, 16)")
     g.add_argument("--max-batch", "--max_batch", type=int, default=64, help="Most sequences in one batch (default: 64)")
     g.add_argument("--max-tokens", "--max_tokens", type=int, default=None,
                    help="Tokens the cache holds (default: from --memory-limit)")
@@ -141,7 +147,8 @@ def run_generation(args) -> int:
     tokenizer = None if args.prompt_ids else _load_tokenizer(args.model_path)
     llm = LLM(args.model_path, apply_sparse=not args.dense, memory_limit=args.memory_limit, chunk_length=args.chunk_length, dtype=args.dtype,
               cuda_graph=args.cuda_graph, temperature=args.temperature, random_seed=args.random_seed,
-              top_p=args.top_p, max_batch=args.max_batch, max_tokens=args.max_tokens)
+              top_p=args.top_p, max_batch=args.max_batch, max_tokens=args.max_tokens, top_k=args.top_k, min_p=args.min_p,
+              cache_bits=args.cache_bits)
     llm.tokenizer = tokenizer
     prompts = make_prompts(args, tokenizer)
     terminators = [] if args.ignore_eos else list(llm.model.spec.stop_token_ids)
@@ -151,7 +158,7 @@ def run_generation(args) -> int:
     print(f"[cpmcu_b200] cache holds {llm.cache.max_tokens} tokens, longest sequence {max_len}", file=sys.stderr)
     llm.load_from_hf()
 
-    if args.use_stream and len(prompts) == 1:
+    if args.use_stream and len(prompts) == 1 and args.samples == 1:
         tokens = []
         for item in llm.generate(prompts[0], args.num_generate, terminators, use_stream=True):
             tokens.append(item["token"])
@@ -159,7 +166,7 @@ def run_generation(args) -> int:
         print()
         results = [tokens]
     else:
-        results = [r.tokens for r in llm.generate_batch(prompts, args.num_generate, terminators)]
+        results = [r.tokens for r in llm.generate_batch(prompts, args.num_generate, terminators, samples=args.samples)]
         for i, toks in enumerate(results):
             shown = tokenizer.decode(toks, skip_special_tokens=True) if tokenizer else " ".join(map(str, toks))
             print(f"[{i}] {shown}")

@@ -81,6 +81,7 @@ class MiniCPMConfig:
     torch_dtype: str
     eos_token_ids: List[int] = field(default_factory=list)
     bos_token_id: Optional[int] = None
+    cache_bits: int = 16          # 4: keys and values are held in 4 bits (cpmcu_b200.ops: rope_store_kv4, kv4_attention)
 
     architecture = "MiniCPMForCausalLM"
 
@@ -121,6 +122,9 @@ class MiniCPMConfig:
         dtype = r.string("torch_dtype", default="bfloat16")
         eos = r.int_or_ints("eos_token_id", default=[])
         bos = r.integer("bos_token_id", default=None)
+        bits = r.integer("cache_bits", default=16, minimum=1)
+        if bits is not None:
+            r.check(bits in (4, 16), f"'cache_bits' is 4 or 16, got {bits}")
 
         if head_dim is None and hidden is not None and heads is not None:
             r.check(hidden % heads == 0,
@@ -190,7 +194,7 @@ class MiniCPMConfig:
             intermediate_size=inter, rms_norm_eps=eps, hidden_act=act, scale_emb=scale_emb,
             dim_model_base=dim_model_base, scale_depth=scale_depth, tie_word_embeddings=tie,
             rope_theta=theta, max_position_embeddings=max_pos, rope_scaling=rope,
-            sparse_config=sparse, torch_dtype=dtype, eos_token_ids=eos, bos_token_id=bos,
+            sparse_config=sparse, torch_dtype=dtype, eos_token_ids=eos, bos_token_id=bos, cache_bits=bits,
         )
 
     @classmethod
@@ -224,6 +228,8 @@ class MiniCPMConfig:
             d["scale_depth"] = self.scale_depth
         if self.eos_token_ids:
             d["eos_token_id"] = self.eos_token_ids[0] if len(self.eos_token_ids) == 1 else list(self.eos_token_ids)
+        if self.cache_bits != 16:
+            d["cache_bits"] = self.cache_bits
         if self.bos_token_id is not None:
             d["bos_token_id"] = self.bos_token_id
         return d

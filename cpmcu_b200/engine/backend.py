@@ -16,6 +16,7 @@ class EngineBackend:
         self.stepper = stepper
         self.ops = stepper.ops
         self.seed = int(seed)
+        stepper.cache.copy_pages = self.ops.copy_pages
         self.runner = DecodeRunner(stepper, use_graph=use_graph, seed=seed)
         self._max_batch = int(max_batch)
         self.slots: List[int] = []
@@ -34,6 +35,11 @@ class EngineBackend:
         n = len(keys)
         if all(p.greedy for p in sampling):
             out = self.ops.sample(logits)
+        elif any(p.filtered for p in sampling):
+            i = torch.tensor(list(keys) + list(steps) + [p.top_k for p in sampling], dtype=torch.int32).view(3, n).to(self.ops.device)
+            f = torch.tensor([p.temperature for p in sampling] + [p.top_p for p in sampling] + [p.min_p for p in sampling],
+                             dtype=torch.float32).view(3, n).to(self.ops.device)
+            out, _ = self.ops.sample_filtered(logits, None, f[0], i[2], f[1], f[2], self.seed, i[0], i[1])
         else:
             i = torch.tensor(list(keys) + list(steps), dtype=torch.int32).view(2, n).to(self.ops.device)
             f = torch.tensor([p.temperature for p in sampling] + [p.top_p for p in sampling],
@@ -58,6 +64,31 @@ class EngineBackend:
             logits = self.stepper.step(batch)
             tokens = self._sample(logits, keys, [0] * len(prompts), sampling)
             self.ops.raise_on_kernel_error()            # the host has just waited for the tokens anyway
+        except BaseException:
+            self.abort()
+            raise
+        return tokens
+
+    def prefill_forked(self, prompts, which, keys, sampling) -> List[int]:
+        """As ``prefill`` for sequences that begin alike: sequence j has the prompt ``prompts[which[j]]``.  Every prompt runs once
+        and is forked for its further sequences, each of which draws its own first token from the prompt's logits."""
+        firsts = self.stepper.open(len(prompts))
+        self.open = set(firsts)
+        try:
+            batch = [SequenceStep(s, list(p), [len(p) - 1]) for s, p in zip(firsts, prompts)]
+            self.h2d_bytes += 4 * sum(len(p) for p in prompts)
+            logits = self.stepper.step(batch)
+            cache = self.stepper.cache
+            slots_of = []
+            for i, s in enumerate(firsts):
+                more = cache.fork_sequence(s, sum(1 for w in which if w == i) - 1)
+                self.open.update(more)
+                slots_of.append([s] + more)
+            cache.sync()
+            self.slots = [slots_of[w].pop(0) for w in which]
+            rows = logits[torch.tensor(list(which), dtype=torch.int64).to(logits.device)].contiguous()
+            tokens = self._sample(rows, keys, [0] * len(which), sampling)
+            self.ops.raise_on_kernel_error()
         except BaseException:
             self.abort()
             raise

@@ -30,13 +30,17 @@ def bucket_size(n: int) -> int:
 
 
 class _Bucket:
-    def __init__(self, size: int, device: torch.device):
+    def __init__(self, size: int, device: torch.device, filtered: bool = False):
+        """``filtered``: its sequences are drawn under top-k and min-p too (a kernel of its own, so a recording of its own)."""
         i32 = dict(dtype=torch.int32, device=device)
         self.size = size
         # what a batch begins with lies in the rows of one tensor (each on a 16-byte boundary), so that one copy brings it
-        self.block = torch.zeros(9, (size + 3) // 4 * 4, **i32)
+        self.filtered = bool(filtered)
+        self.block = torch.zeros(11 if filtered else 9, (size + 3) // 4 * 4, **i32)
         self.ids, self.positions, self.kv_len, self.slot, self.live, self.seq_key, self.step_key = (row[:size] for row in self.block[:7])
-        self.temperature, self.top_p = (row[:size] for row in self.block[7:].view(torch.float32))
+        self.temperature, self.top_p = (row[:size] for row in self.block[7:9].view(torch.float32))
+        if filtered:
+            self.min_p, self.top_k = self.block[9].view(torch.float32)[:size], self.block[10][:size]
         self.kv_len.fill_(1)
         self.top_p.fill_(1.0)
         self.token_seq = torch.arange(size, **i32)
@@ -57,7 +61,7 @@ class DecodeRunner:
         self.ops = stepper.ops
         self.use_graph = bool(use_graph)
         self.seed = int(seed)
-        self.buckets: Dict[int, _Bucket] = {}
+        self.buckets: Dict[object, _Bucket] = {}           # by size; with filters by (size, True)
         self.pad_slot = self.cache.open_sequence()       # scratch sequence the padding entries use
         self.cache.reserve(self.pad_slot, 1)
         self.cache.set_length(self.pad_slot, 1)
@@ -95,16 +99,20 @@ class DecodeRunner:
         self.ops.begin_step()
         ctx.extras["step_begun"] = True
         b.logits = self.model.forward(ctx, b.want_rows)
-        self.ops.sample(b.logits, b.temperature, b.top_p, self.seed, b.seq_key, b.step_key, out=b.sampled)
+        if b.filtered:
+            self.ops.sample_filtered(b.logits, None, b.temperature, b.top_k, b.top_p, b.min_p, self.seed, b.seq_key, b.step_key, out=b.sampled)
+        else:
+            self.ops.sample(b.logits, b.temperature, b.top_p, self.seed, b.seq_key, b.step_key, out=b.sampled)
         self.ops.advance_decode(b.ids, b.positions, b.kv_len, b.step_key, b.sampled, b.live)
 
-    def _bucket(self, n: int) -> _Bucket:
+    def _bucket(self, n: int, filtered: bool = False) -> _Bucket:
         size = bucket_size(n)
-        b = self.buckets.get(size)
+        key = (size, True) if filtered else size
+        b = self.buckets.get(key)
         if b is None:
-            b = _Bucket(size, self.ops.device)
+            b = _Bucket(size, self.ops.device, filtered)
             b.slot.fill_(self.pad_slot)
-            self.buckets[size] = b
+            self.buckets[key] = b
         return b
 
     def _prepare(self, b: _Bucket) -> None:
@@ -140,7 +148,7 @@ class DecodeRunner:
         """Sets the batch: ``last_tokens`` are the tokens to feed next; every sequence's
         position is its current length in the cache."""
         n = len(slots)
-        b = self._bucket(n)
+        b = self._bucket(n, any(p.filtered for p in sampling))
         self._prepare(b)
         lengths = [self.cache.length(s) for s in slots]
         last_tokens, seq_keys, step_keys = list(last_tokens), list(seq_keys), list(step_keys)
@@ -151,7 +159,11 @@ class DecodeRunner:
             last_tokens + [0] * pad + lengths + [0] * pad + [length + 1 for length in lengths] + [1] * pad
             + list(slots) + [self.pad_slot] * pad + [1] * n + [0] * pad + seq_keys + [0] * pad + step_keys + [0] * pad, dtype=torch.int32)
         reals = torch.tensor([p.temperature for p in sampling] + [0.0] * pad + [p.top_p for p in sampling] + [1.0] * pad, dtype=torch.float32)
-        self.cache.staging.copy(torch.cat((ints, reals.view(torch.int32))), [b.block.view(-1)])
+        parts = [ints, reals.view(torch.int32)]
+        if b.filtered:
+            parts.append(torch.tensor([p.min_p for p in sampling] + [0.0] * pad, dtype=torch.float32).view(torch.int32))
+            parts.append(torch.tensor([p.top_k for p in sampling] + [0] * pad, dtype=torch.int32))
+        self.cache.staging.copy(torch.cat(parts), [b.block.view(-1)])
         self.current = b
         self.slots = list(slots)
 

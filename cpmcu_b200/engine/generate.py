@@ -17,7 +17,7 @@ import time
 from dataclasses import dataclass, field
 from typing import Callable, List, Optional, Protocol, Sequence
 
-from ..cache import CacheFull, pages_for
+from ..cache import PAGE_TOKENS, CacheFull, pages_for
 from ..sampling import SamplingParams
 
 
@@ -41,6 +41,8 @@ class Backend(Protocol):
     def abort(self) -> None:
         """Something failed in the middle of a batch: every sequence of it that is still open is closed."""
 
+    # Optional: ``prefill_forked(prompts, which, keys, sampling)``, as ``prefill`` for sequences that begin alike (needed for requests
+    # with a ``group``).
     # Optional: ``max_sequence_pages()`` (the most pages one sequence may hold) and ``vocab_size()``; with them
     # a request that cannot run is refused before anything is opened.
 
@@ -52,6 +54,7 @@ class Request:
     sampling: SamplingParams = SamplingParams()
     stop_token_ids: Sequence[int] = ()
     key: int = 0                       # random key of the request (its index, by default)
+    group: Optional[int] = None        # requests of one group have the same prompt: it runs once, and they are forked from it
 
 
 @dataclass
@@ -91,11 +94,13 @@ def plan_batches(requests: Sequence[Request], max_batch: int, capacity_pages: in
             bad = next((t for t in r.prompt if not 0 <= int(t) < vocab_size), None)
             if bad is not None:
                 raise ValueError(f"request {i}: token id {bad} is outside the vocabulary [0, {vocab_size})")
-        if cur and (len(cur) >= max_batch or pages + need > capacity_pages):
+        # one more of a group holds the prompt's full pages with the first
+        shared = len(r.prompt) // PAGE_TOKENS if r.group is not None and any(requests[j].group == r.group for j in cur) else 0
+        if cur and (len(cur) >= max_batch or pages + need - shared > capacity_pages):
             batches.append(cur)
-            cur, pages = [], 0
+            cur, pages, shared = [], 0, 0
         cur.append(i)
-        pages += need
+        pages += need - shared
     if cur:
         batches.append(cur)
     return batches
@@ -109,6 +114,10 @@ def run_requests(backend: Backend, requests: Sequence[Request],
     for i, r in enumerate(requests):
         if len(r.prompt) == 0:
             raise ValueError(f"request {i} has an empty prompt")
+    heads = {}
+    for i, r in enumerate(requests):
+        if r.group is not None and list(heads.setdefault(r.group, r).prompt) != list(r.prompt):
+            raise ValueError(f"request {i} has another prompt than the first of its group {r.group}")
     results = [Finished() for _ in requests]
     stats = GenerationStats()
     sync = sync or (lambda: None)
@@ -142,11 +151,18 @@ def _run_batches(backend, requests, plan, results, stats, on_token, sync) -> Non
             continue
         sync()
         t0 = time.perf_counter()
-        first = backend.prefill([reqs[j].prompt for j in runnable], [keys[j] for j in runnable],
-                                [sampling[j] for j in runnable])
+        groups = [reqs[j].group for j in runnable]
+        if any(g is not None and groups.index(g) < n for n, g in enumerate(groups)):
+            heads = [n for n, g in enumerate(groups) if g is None or groups.index(g) == n]       # the first of every group
+            which = [heads.index(n if g is None else groups.index(g)) for n, g in enumerate(groups)]
+            first = backend.prefill_forked([reqs[runnable[n]].prompt for n in heads], which, [keys[j] for j in runnable],
+                                           [sampling[j] for j in runnable])
+        else:
+            first = backend.prefill([reqs[j].prompt for j in runnable], [keys[j] for j in runnable],
+                                    [sampling[j] for j in runnable])
         sync()
         stats.prefill_time += time.perf_counter() - t0
-        stats.prompt_tokens += sum(len(reqs[j].prompt) for j in runnable)
+        stats.prompt_tokens += sum(len(reqs[j].prompt) for n, j in enumerate(runnable) if groups[n] is None or groups.index(groups[n]) == n)
 
         def take(j: int, pos: int, token: int) -> bool:
             """Records a token; True if the sequence goes on."""

@@ -37,10 +37,12 @@ class LLM:
                  cuda_graph: bool = False, temperature: float = 0.0, random_seed: Optional[int] = None,
                  top_p: float = 1.0, max_batch: int = 64, max_tokens: Optional[int] = None,
                  max_seq_tokens: Optional[int] = None, device: str = "cuda:0", apply_sparse: bool = True,
-                 use_arena: bool = True):
+                 use_arena: bool = True, top_k: int = 0, min_p: float = 0.0, cache_bits: Optional[int] = None):
         """``apply_sparse`` False runs a model whose configuration has a ``sparse_config`` with dense attention
         (the reference's switch of the same name, cpmcu/llm.py:32, chooses the other way round).  ``use_arena``
-        False leaves every tensor to torch's allocator (``max_tokens`` must then be given)."""
+        False leaves every tensor to torch's allocator (``max_tokens`` must then be given).  ``cache_bits`` 4 holds keys and
+        values in 4 bits (None: what the configuration says, 16 without a word): the cache then takes 0.28 to 0.31 of the bytes, so
+        that more or longer sequences fit."""
         self.use_arena = bool(use_arena)
         self.storage = None
         self.path = path
@@ -48,6 +50,13 @@ class LLM:
         if not apply_sparse and getattr(self.config, "sparse_config", None) is not None:
             import dataclasses
             self.config = dataclasses.replace(self.config, sparse_config=None)
+        if cache_bits is not None:
+            import dataclasses
+            if not hasattr(self.config, "cache_bits"):
+                raise ValueError(f"{self.arch.name} has no cache in 4 bits")
+            if cache_bits not in (4, 16):
+                raise ValueError(f"cache_bits is 4 or 16, got {cache_bits}")
+            self.config = dataclasses.replace(self.config, cache_bits=int(cache_bits))
         self.dtype = parse_dtype(dtype if dtype is not None else getattr(self.config, "torch_dtype", "bfloat16"))
         self.device = device
         self.memory_limit = float(memory_limit)
@@ -55,6 +64,7 @@ class LLM:
         self.cuda_graph = bool(cuda_graph)
         self.temperature = float(temperature)
         self.top_p = float(top_p)
+        self.top_k, self.min_p = int(top_k), float(min_p)
         self.seed = 0 if random_seed is None else int(random_seed)
         self.max_batch = int(max_batch)
         self.max_tokens = max_tokens
@@ -129,13 +139,20 @@ class LLM:
     def generate_batch(self, prompts: Sequence[Prompt], generation_length: int = 100,
                        terminators: Sequence[int] = (), temperature: Optional[float] = None,
                        top_p: Optional[float] = None,
-                       on_token: Optional[Callable[[int, int, bool], None]] = None) -> List[Finished]:
-        """Generates for a batch of prompts of unequal lengths; results in the prompts' order."""
+                       on_token: Optional[Callable[[int, int, bool], None]] = None, top_k: Optional[int] = None,
+                       min_p: Optional[float] = None, samples: int = 1) -> List[Finished]:
+        """Generates for a batch of prompts of unequal lengths; results in the prompts' order.  ``samples`` > 1: so many answers to
+        every prompt, one after the other in the results; the prompt runs once, and the answers share its pages in the cache."""
+        if samples < 1:
+            raise ValueError(f"samples must be >= 1, got {samples}")
         backend = self._ready()
         sp = SamplingParams(self.temperature if temperature is None else float(temperature),
-                            self.top_p if top_p is None else float(top_p))
-        reqs = [Request(_as_list(p), int(generation_length), sp, tuple(int(t) for t in terminators), key=i)
-                for i, p in enumerate(prompts)]
+                            self.top_p if top_p is None else float(top_p),
+                            self.top_k if top_k is None else int(top_k),
+                            self.min_p if min_p is None else float(min_p))
+        reqs = [Request(tokens, int(generation_length), sp, tuple(int(t) for t in terminators), key=i * samples + j,
+                        group=i if samples > 1 else None)
+                for i, tokens in enumerate(_as_list(p) for p in prompts) for j in range(samples)]
         results, stats = run_requests(backend, reqs, on_token, sync=torch.cuda.synchronize)
         self.last_stats = stats
         return results

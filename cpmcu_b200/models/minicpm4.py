@@ -45,6 +45,7 @@ def model_spec(cfg: MiniCPMConfig) -> ModelSpec:
         "n_kv_heads": cfg.num_key_value_heads, "head_dim": cfg.head_dim,
         "position": position_spec(cfg),
         "sparse": cfg.sparse_config.to_json() if cfg.sparse_config else None,
+        "cache_bits": cfg.cache_bits,
     })
     ffn = PartSpec("gated_ffn", {"hidden_size": cfg.hidden_size, "intermediate_size": cfg.intermediate_size,
                                  "activation": cfg.hidden_act})

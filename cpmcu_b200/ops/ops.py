@@ -21,7 +21,7 @@ import torch
 from . import library
 from .library import check
 
-from ..parts.base import PAGE_TOKENS, QUERY_TILE_TOKENS
+from ..parts.base import KV4_HEAD_DIMS, PAGE_TOKENS, QUERY_TILE_TOKENS, kv4_page_bytes
 
 F32, BF16 = 0, 1
 FAST_HEAD_DIMS = (32, 64, 96, 128)       # head sizes the tensor-core attention kernels are built for
@@ -1664,13 +1664,8 @@ class Ops:
         return out
 
     # ---- a cache held in 4 bits ----
-    KV4_HEAD_DIMS = (32, 64, 96, 128)
-
-    @staticmethod
-    def kv4_page_bytes(d: int) -> int:
-        """Bytes of one page of one key-value head in 4 bits: 64 tokens' key and value codes, and a scale and a middle (bf16 each)
-        for both halves of every row."""
-        return 64 * d + 16 * PAGE_TOKENS
+    KV4_HEAD_DIMS = KV4_HEAD_DIMS
+    kv4_page_bytes = staticmethod(kv4_page_bytes)
 
     def _kv4(self, records: torch.Tensor, n_kv: int, d: int) -> torch.Tensor:
         if d not in self.KV4_HEAD_DIMS:

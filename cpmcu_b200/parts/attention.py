@@ -16,7 +16,7 @@ from typing import Any, Dict, Mapping, Optional
 
 import torch
 
-from .base import MIXERS, POSITIONS, CacheNeeds, Mixer, PartSpec, WeightSpec, build_part
+from .base import KV4_HEAD_DIMS, MIXERS, POSITIONS, CacheNeeds, Mixer, PartSpec, WeightSpec, build_part
 
 
 @MIXERS.register("gqa_attention")
@@ -27,8 +27,8 @@ class GroupedQueryAttention(Mixer):
 
     def __init__(self, ops, hidden_size: int, n_heads: int, n_kv_heads: int, head_dim: int,
                  position: PartSpec, window: Optional[int] = None, sparse: Optional[Mapping[str, int]] = None,
-                 softmax_scale: Optional[float] = None, position_name: str = ""):
-        """``position_name``: infix of the position part's own tensors below this part's prefix (an encoding with
+                 softmax_scale: Optional[float] = None, position_name: str = "", cache_bits: int = 16):
+        """``cache_bits`` 4: keys and values are held in 4 bits (``Ops.rope_store_kv4``).  ``position_name``: infix of the position part's own tensors below this part's prefix (an encoding with
         learned tables declares them in its ``weight_specs``; the rotary encodings have none)."""
         super().__init__(ops)
         if window and sparse:
@@ -39,6 +39,12 @@ class GroupedQueryAttention(Mixer):
             raise ValueError(f"{n_heads} heads cannot be grouped over {n_kv_heads} key-value heads")
         if head_dim % 16 or head_dim > 256:
             raise ValueError(f"head_dim {head_dim}: the attention kernels take multiples of 16 up to 256")
+        if cache_bits not in (4, 16):
+            raise ValueError(f"cache_bits is 4 or 16, got {cache_bits}")
+        if cache_bits == 4 and (sparse or head_dim not in KV4_HEAD_DIMS):
+            raise ValueError(f"a cache in 4 bits takes dense attention with head sizes {KV4_HEAD_DIMS}"
+                             + (", not a sparse configuration" if sparse else f", not {head_dim}"))
+        self.four_bits = cache_bits == 4
         self.hidden_size, self.n_heads, self.n_kv, self.d = int(hidden_size), int(n_heads), int(n_kv_heads), int(head_dim)
         self.window = int(window) if window else 0
         self.sparse = dict(sparse) if sparse else None
@@ -77,7 +83,7 @@ class GroupedQueryAttention(Mixer):
         stride = self.sparse["kernel_stride"] if self.sparse else 0
         kernel = self.sparse["kernel_size"] if self.sparse else 0
         return CacheNeeds(kv_heads=self.n_kv, head_dim=self.d, window=self.window or None,
-                          pooled_stride=stride, pooled_kernel=kernel)
+                          pooled_stride=stride, pooled_kernel=kernel, bits=4 if self.four_bits else 0)
 
     def cache_bytes_read(self, kv_len: int) -> int:
         keys = min(kv_len, self.window) if self.window else kv_len
@@ -88,13 +94,15 @@ class GroupedQueryAttention(Mixer):
             blocks = sp["topk"] + sp["window_size"] // sp["block_size"]
             keys = min(kv_len, blocks * sp["block_size"])
             pooled = max(0, (kv_len - sp["kernel_size"]) // sp["kernel_stride"] + 1) * self.n_kv * self.d * 4
+        if self.four_bits:
+            return keys * self.n_kv * (self.d + 16)
         return 2 * keys * self.n_kv * self.d * self.ops.element_size + pooled
 
     # ---- forward ----
     def forward(self, ctx, y: torch.Tensor, lane, writes_cache: bool) -> torch.Tensor:
         ops = self.ops
-        if lane.k is not None:
-            ops.set_page_limit(lane.k.shape[0])          # the checked build's kernels compare page numbers with it
+        if lane.n_pages:
+            ops.set_page_limit(lane.n_pages)             # the checked build's kernels compare page numbers with it
         qkv = ops.linear(y, self.w_qkv)
         inv_freq, magnitude, rot_dim = self.position.rotary() or (None, 1.0, -1)
         k_cache, v_cache = lane.k, lane.v
@@ -103,6 +111,12 @@ class GroupedQueryAttention(Mixer):
             row = qkv.view(ctx.n_tokens, self.n_heads + 2 * self.n_kv, self.d)
             self.position.apply(ctx, row[:, :self.n_heads], row[:, self.n_heads:self.n_heads + self.n_kv])
             inv_freq, magnitude, rot_dim = None, 1.0, 0
+        if self.four_bits:
+            q = ops.rope_store_kv4(qkv, self.n_heads, self.n_kv, self.d, ctx.positions, ctx.token_seq, ctx.slot_dev, lane.page_table,
+                                   lane.records if writes_cache else None, inv_freq, magnitude, rot_dim)
+            prompt = {} if ctx.is_decode else dict(cu_q=ctx.cu_q, tiles=ctx.q_tiles, longest=ctx.max_kv_len)
+            out = ops.kv4_attention(q, lane.records, ctx.kv_len_dev, ctx.slot_dev, lane.page_table, self.n_kv, self.scale, self.window, **prompt)
+            return ops.linear(out, self.w_o)
         if rot_dim >= 0 and ops.fused_decode_ok(ctx, self.d, rot_dim, self.window, self.sparse):
             # one token per sequence: the attention kernel rotates, stores the new key and value, and attends
             out = ops.decode_attention_rope(qkv, lane, ctx.kv_len_dev, ctx.slot_dev, self.n_heads, self.n_kv, self.d,

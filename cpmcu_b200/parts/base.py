@@ -25,6 +25,13 @@ T = TypeVar("T")
 PAGE_TOKENS = 64
 # Query tokens per tile of the tiled prompt attention kernels (StepContext.q_tiles is made for this size).
 QUERY_TILE_TOKENS = 64
+# Head sizes of a cache in 4 bits, and the bytes of one page of one key-value head in it: 64 tokens' key and value codes, and a scale and a
+# middle (bf16 each) for both halves of every row.
+KV4_HEAD_DIMS = (32, 64, 96, 128)
+
+
+def kv4_page_bytes(d: int) -> int:
+    return 64 * d + 16 * PAGE_TOKENS
 
 
 class Registry(Generic[T]):
@@ -157,7 +164,8 @@ class CacheNeeds:
     ``pooled_stride`` tokens (mean-pooled keys); 0 = none.  values: False when the
     lane keeps key rows only (a shared latent that keys and values are both made
     from).  value_dim: the size of a value row where it differs from a key row's (0: the same).  keep_first: with a
-    window, the number of a sequence's first tokens that stay needed whatever the window.  state: tensors of fixed size per sequence, name -> (shape, dtype); they
+    window, the number of a sequence's first tokens that stay needed whatever the window.  bits: 4 when keys and values are held in 4 bits, one
+    record of both per page and key-value head (0: in the cache's type).  state: tensors of fixed size per sequence, name -> (shape, dtype); they
     are zero when a sequence starts.
     """
 
@@ -170,10 +178,11 @@ class CacheNeeds:
     values: bool = True
     value_dim: int = 0
     keep_first: int = 0
+    bits: int = 0
 
     def group_key(self) -> Tuple:
         return (self.kv_heads, self.head_dim, self.window, self.pooled_stride, self.pooled_kernel, self.values, self.value_dim,
-                self.keep_first if self.window else 0)
+                self.keep_first if self.window else 0, self.bits)
 
     def seen_through(self, window: Optional[int]) -> "CacheNeeds":
         """The same needs when a further reader looks at the lane through ``window`` (None: at every key): the lane keeps
@@ -181,7 +190,7 @@ class CacheNeeds:
         if self.window is None or (window is not None and window <= self.window):
             return self
         return CacheNeeds(self.kv_heads, self.head_dim, window, self.pooled_stride, self.pooled_kernel, self.state, self.values,
-                          self.value_dim, self.keep_first)
+                          self.value_dim, self.keep_first, self.bits)
 
     def with_state(self, more: Mapping[str, Tuple[Tuple[int, ...], torch.dtype]]) -> "CacheNeeds":
         """The same needs with further per-sequence tensors (a block adds its own to its mixer's)."""
@@ -191,7 +200,7 @@ class CacheNeeds:
                 raise ValueError(f"per-sequence state '{name}' is declared twice for one lane")
             both[name] = what
         return CacheNeeds(self.kv_heads, self.head_dim, self.window, self.pooled_stride, self.pooled_kernel, both, self.values,
-                          self.value_dim, self.keep_first)
+                          self.value_dim, self.keep_first, self.bits)
 
 
 # ---------------------------------------------------------------------------
