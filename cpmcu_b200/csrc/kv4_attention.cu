@@ -14,7 +14,7 @@
 // of a page, and the block's two to four groups of four warps every second to fourth page.  A warp brings its tokens into a ring of its own by
 // asynchronous 16-byte copies, of which a lane reads most of what it copied itself, and keeps a softmax of its own, so that nothing synchronises the
 // warps until a tile ends.  (Bulk copies of a slice's four pieces took longer than the arithmetic: each needs its addresses in uniform
-// registers.  Blocks of four warps, three an SM, leave three times as many parts to add up: 41 us instead of XX for one sequence of 131,071 keys.)
+// registers.  Blocks of four warps, three an SM, leave three times as many parts to add up: 41 us where blocks of twelve took 30, for one sequence of 131,071 keys.)
 #include "kv4.cuh"
 
 CPM_BOUNDS_TU(kv4_attention)
@@ -61,9 +61,6 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs& a, int i, int columns)
     t.parts = (t.tokens * a.group + columns - 1) / columns;
     return t;
 }
-// Units of a tile: pages (one where there is none, for the zeros that such a row gets) times parts and key-value heads.
-__device__ __forceinline__ int tile_units(const Tile& t, int n_kv) { return max(1, t.pages) * t.parts * n_kv; }
-
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
 }
@@ -174,30 +171,40 @@ struct Smem {
     static constexpr int kChunks = kStage / 16, kPieces = (kChunks + 31) / 32;
     alignas(128) uint8_t ring[kWarps][kStages][kStage];
     alignas(16) __half q[TERMS][kCols][kQStride];
-    alignas(16) float merge[kWarps][8][D + 4];
+    alignas(16) float merge[kWarps][8][D + 8];         // rows 32 bytes apart modulo 128
     alignas(16) float merge_m[kWarps][8], merge_l[kWarps][8];
     float q_sum[kCols][2], factor[kCols];
     int last[kCols];                                   // a column's last key, -1: no such column
     int scan[kWarps];
+    int place, last_block;                             // of the head that the block writes (-1: none); of its row, where it has one only
     int prefix[kMostTiles + 1];
     Tile tiles[kMostTiles];
 };
 
-// Blocks that take a share: each of them a page for every group of its warps, since every further part costs the second kernel a read; but
-// as many as there are whole rows of pages, for a block goes through these one after the other.
-struct Shares { int sharing, each, more; };            // the first ``more`` blocks have one unit more than ``each``
-__device__ __forceinline__ Shares shares_of(int units, int rows, int groups, int blocks) {
-    const int sharing = min(blocks, max(1, max(min(rows, units), (units + groups - 1) / groups)));
-    return Shares{sharing, units / sharing, units % sharing};
+// A row of pages (a tile's, of one key-value head and part) costs a block its pages and some more, for the queries that it prepares and the parts
+// that it adds up.  All rows lie one behind the other in a line of such costs, a row's extra cost first.
+constexpr int extra_cost(int groups) { return 4 * groups; }
+// Sharing by cost: each of the blocks takes a piece of the line, wherever rows begin or end; fewer blocks where there is little.
+struct Shares { int sharing, each, more; };            // the first ``more`` blocks have one more than ``each``
+__device__ __forceinline__ Shares shares_of(int cost, int groups, int blocks) {
+    const int least = groups + extra_cost(groups) / 4, sharing = min(blocks, max(1, (cost + least - 1) / least));
+    return Shares{sharing, cost / sharing, cost % sharing};
 }
 __device__ __forceinline__ int share_begin(const Shares& s, int block) { return block * s.each + min(block, s.more); }
-__device__ __forceinline__ int block_of(const Shares& s, int unit) {
+__device__ __forceinline__ int block_of(const Shares& s, int at) {
     const int longer = s.more * (s.each + 1);
-    return unit < longer ? unit / (s.each + 1) : s.more + (unit - longer) / s.each;
+    return at < longer ? at / (s.each + 1) : s.more + (at - longer) / s.each;
+}
+// Sharing by rows: a block works on one row alone, a row has a block or more by its number of pages.  Taken where there are four blocks or more
+// to a row of single tokens: a block that another row begins in takes as long again for its queries and sums as for 15 pages.
+__host__ __device__ __forceinline__ int rows_of_tile(const AttendArgs& a, int columns) { return a.n_kv * ((a.group + columns - 1) / columns); }
+__host__ __device__ __forceinline__ bool shares_by_rows(const AttendArgs& a, int columns, int blocks) {
+    return !a.cu_q && (int64_t)4 * a.n_tiles * rows_of_tile(a, columns) <= blocks;
 }
 
-// The tiles and the prefix sums of their units; every thread of the block takes part.
-__device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, Tile* tiles, int* prefix, int* scan) {
+// The tiles and the prefix sums of their rows' costs; every thread of the block takes part.  (A row without keys counts as one page, for the
+// zeros that it gets.)
+__device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, int extra, Tile* tiles, int* prefix, int* scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int carry = 0;
 #pragma unroll 1
@@ -207,7 +214,7 @@ __device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, Tile
         if (i < a.n_tiles) {
             const Tile t = tile_of(a, i, columns);
             tiles[i] = t;
-            own = tile_units(t, a.n_kv);
+            own = (extra + max(1, t.pages)) * t.parts * a.n_kv;
         }
         int v = own;
 #pragma unroll
@@ -230,19 +237,20 @@ __device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, Tile
     if (threadIdx.x == 0) prefix[a.n_tiles] = carry;
     __syncthreads();
 }
-__device__ __forceinline__ int find_tile(const int* prefix, int n, int unit) {
-    int lo = 0, hi = n;                                 // the last tile that begins at or before the unit (empty tiles begin where the next does)
+__device__ __forceinline__ int find_tile(const int* prefix, int n, int at) {
+    int lo = 0, hi = n;                                 // the last tile that begins there or before (empty tiles begin where the next does)
 #pragma unroll 1
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= unit) lo = mid; else hi = mid;
+        if (prefix[mid] <= at) lo = mid; else hi = mid;
     }
     return lo;
 }
 
 // Scratch: a head of kHeadInts numbers for every block, then two parts a block.  A part holds for each column the weighted values, the
-// maximum and the sum.  A block whose last tile goes on in other blocks says so in its head, for the kernel that adds up.
-struct CutTile { int last_block, row, part, head, columns; };
+// maximum and the sum.  A row that several blocks share has its head, for the kernel that adds up, from the block that begins it: in that block's place,
+// or, where blocks have one row each, in the row's.
+struct CutRow { int first_block, last_block, row, part, head, columns; };
 constexpr int kHeadInts = 8;
 template <int D> constexpr int kPartStride = D + 4;
 template <int D>
@@ -262,17 +270,70 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slice = warp % kSlices, turn = warp / kSlices;      // its tokens of a page, and of how many pages the how-manieth
     pdl_launch_dependents();
     pdl_wait();
-    sum_tiles(a, COLS, sm.tiles, sm.prefix, sm.scan);
-    const int units = sm.prefix[a.n_tiles];
-    const Shares shares = shares_of(units, a.cu_q ? 0 : a.n_tiles * a.n_kv * ((a.group + COLS - 1) / COLS), GROUPS, gridDim.x);
-    if (threadIdx.x == 0) reinterpret_cast<CutTile*>(a.scratch + (int64_t)blockIdx.x * kHeadInts)->last_block = -1;
-    if ((int)blockIdx.x >= shares.sharing || units == 0) return;
-    const int begin = share_begin(shares, blockIdx.x), end = share_begin(shares, blockIdx.x + 1);
-    const int start = find_tile(sm.prefix, a.n_tiles, begin);
+    constexpr int EXTRA = extra_cost(GROUPS);
+    sum_tiles(a, COLS, EXTRA, sm.tiles, sm.prefix, sm.scan);
+    const int cost = sm.prefix[a.n_tiles];
+    int begin = 0, end = 0, start = 0;                                                    // the block's piece of the line, and its first tile
+    if (shares_by_rows(a, COLS, gridDim.x)) {
+        // a row of n pages has 1 + n / each blocks, but no more than have a page for each of their groups
+        const int per_tile = rows_of_tile(a, COLS), rows = a.n_tiles * per_tile, spare = (int)gridDim.x - rows;
+        const int each = (cost - rows * EXTRA + spare - 1) / spare;
+        int block = blockIdx.x;
+#pragma unroll 1
+        for (int i0 = 0; i0 < a.n_tiles; i0 += 32) {
+            const int pages = i0 + lane < a.n_tiles ? max(1, sm.tiles[i0 + lane].pages) : 0;
+            const int blocks = pages ? min(1 + pages / each, (pages + GROUPS - 1) / GROUPS) : 0;
+            int v = blocks * per_tile;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += x;
+            }
+            const uint32_t behind = __ballot_sync(0xffffffffu, v > block);
+            if (behind) {
+                const int from = __ffs(behind) - 1, n = __shfl_sync(0xffffffffu, blocks, from), m = __shfl_sync(0xffffffffu, pages, from);
+                block -= __shfl_sync(0xffffffffu, v, from) - n * per_tile;
+                start = i0 + from;
+                const int row = block / n, k = block - row * n, first = sm.prefix[start] + row * (EXTRA + m);
+                begin = first + (k ? EXTRA + k * (m / n) + min(k, m % n) : 0);
+                end = first + EXTRA + (k + 1) * (m / n) + min(k + 1, m % n);
+                if (threadIdx.x == 0) {
+                    sm.last_block = (int)blockIdx.x - k + n - 1;
+                    sm.place = k ? -1 : start * per_tile + row;
+                }
+                break;
+            }
+            block -= __shfl_sync(0xffffffffu, v, 31);
+        }
+    } else {
+        const Shares shares = shares_of(cost, GROUPS, gridDim.x);
+        if ((int)blockIdx.x < shares.sharing) {
+            begin = share_begin(shares, blockIdx.x);
+            end = share_begin(shares, blockIdx.x + 1);
+            start = find_tile(sm.prefix, a.n_tiles, begin);
+        }
+        if (threadIdx.x == 0) {
+            sm.last_block = -1;
+            sm.place = blockIdx.x;
+            reinterpret_cast<CutRow*>(a.scratch + (int64_t)blockIdx.x * kHeadInts)->last_block = -1;
+        }
+    }
+    if (begin >= end) return;
+    // The row of pages at a place of the line: its tile, its number among the tile's, and which of its pages are the block's.
+    const auto walk = [&](int& at, int& index, uint32_t& row, int& first, int& stop) {
+#pragma unroll 1
+        while (sm.prefix[index + 1] <= at) ++index;
+        const int pages = max(1, sm.tiles[index].pages), in = at - sm.prefix[index];
+        row = (uint32_t)in / (uint32_t)(EXTRA + pages);
+        const int within = in - row * (EXTRA + pages);
+        first = max(0, within - EXTRA);
+        stop = min(pages, within + end - at - EXTRA);
+        at += min(EXTRA + pages - within, end - at);
+    };
 
-    // ---- what the warp has asked for: it runs ahead of what it works on by the ring's length, across the borders of tiles ----
-    // (units that are the warp's: every GROUPS-th of the block's, from ``turn`` on)
-    int ask_unit = begin + turn, ask_index = start, ask_end = begin, ask_page = 0, ask_ids = 0, ask_base = 0, ask_first = 0, asked = 0;
+    // ---- what the warp has asked for: it runs ahead of what it works on by the ring's length, across the borders of rows ----
+    // (of the block's pages of a row, every GROUPS-th from ``turn`` on)
+    int ask_at = begin, ask_index = start, ask_page = 0, ask_stop = 0, ask_ids = 0, ask_base = 0, ask_first = 0, asked = 0;
     const int* ask_table = a.page_table;
     const uint8_t* ask_records = a.records;
     bool ask_any = false;
@@ -283,24 +344,24 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
              : (c < D + 8 ? L::kKeyParams : L::kValueParams - 128) + slice * 128 + 16 * (c - D);
     };
     const auto ask = [&]() {
-        if (ask_unit < end) {
-            if (ask_unit >= ask_end) {                    // another row of pages: a tile's for one key-value head and part
+        if (ask_page >= ask_stop && ask_at < end) {        // the next row that has a page for the warp
+            uint32_t row = 0;
 #pragma unroll 1
-                while (sm.prefix[ask_index + 1] <= ask_unit) ++ask_index;
-                const Tile t = sm.tiles[ask_index];
-                const uint32_t pages = max(1, t.pages), at = ask_unit - sm.prefix[ask_index], whole = at / pages;
-                ask_page = at - whole * pages;
-                ask_end = ask_unit - ask_page + (int)pages;
-                ask_any = t.pages > 0;
-                ask_first = t.page0;
-                ask_table = a.page_table + (int64_t)t.slot * a.max_pages;
-                ask_records = a.records + (int64_t)(whole % (uint32_t)a.n_kv) * L::kBytes;
-                ask_base = ask_page - 32 * GROUPS;
+            while (ask_page >= ask_stop && ask_at < end) {
+                walk(ask_at, ask_index, row, ask_page, ask_stop);
+                ask_page += turn;
             }
+            ask_any = sm.tiles[ask_index].pages > 0;
+            ask_first = sm.tiles[ask_index].page0;
+            ask_table = a.page_table + (int64_t)sm.tiles[ask_index].slot * a.max_pages;
+            ask_records = a.records + (int64_t)(row % (uint32_t)a.n_kv) * L::kBytes;
+            ask_base = ask_page - 32 * GROUPS;
+        }
+        if (ask_page < ask_stop) {
             if (ask_page - ask_base >= 32 * GROUPS) {      // the next 32 page numbers, one a lane
                 ask_base = ask_page;
                 const int i = ask_page + lane * GROUPS;
-                ask_ids = i - ask_page < min(ask_end, end) - ask_unit && ask_any ? CPM_PAGE(ask_table, ask_first + i, a.max_pages) : 0;
+                ask_ids = i < ask_stop && ask_any ? CPM_PAGE(ask_table, ask_first + i, a.max_pages) : 0;
             }
             const int number = __shfl_sync(0xffffffffu, ask_ids, (ask_page - ask_base) / GROUPS);
             if (ask_any) {                                 // (a row without keys: nothing to bring)
@@ -311,7 +372,6 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
                     if (32 * i + 31 < S::kChunks || lane < S::kChunks - 32 * i) copy16(to + 512 * i, from + ask_from(i));
             }
             ask_page += GROUPS;
-            ask_unit += GROUPS;
             if (++asked == STAGES) asked = 0;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -322,7 +382,7 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
     // ---- what it works on.  One loop over slices, with a tile's beginning and end inside: every part of the code is there once, since a
     // block runs most of it a few times only and the first run of an instruction comes from L2 (80 KB of unrolled code took 25 us for one page) ----
     const int g = lane >> 2, j = lane & 3;
-    int unit = begin, index = start, stage = 0;
+    int at = begin, index = start, stage = 0;
     uint2 qf[Q_IN_REGISTERS ? STEPS : 1];
     // of a lane's two columns of every eight: q's sums, the factor of the scores, minus the running maximum, the sum of weights, the
     // power of two that p s_v is multiplied by, and the sums of p m_v
@@ -333,278 +393,280 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
     const auto q_fragment = [&](int u, int k, int n) { return *reinterpret_cast<const uint2*>(&sm.q[u][8 * n + g][16 * k + 4 * j]); };
 
 #pragma unroll 1
-    while (unit < end) {
-        // ---- a tile begins ----
-#pragma unroll 1
-        while (sm.prefix[index + 1] <= unit) ++index;
+    while (at < end) {
+        // ---- a row of pages begins ----
+        uint32_t in_tile;
+        int first_page, stop;
+        walk(at, index, in_tile, first_page, stop);
+        if (stop <= first_page) break;                                                  // only a part of a row's extra cost is left
         const Tile t = sm.tiles[index];
-        const int pages = max(1, t.pages);
-        const uint32_t at = unit - sm.prefix[index], before = at / (uint32_t)pages;
-        const int first_page = at - before * pages, part = before / (uint32_t)a.n_kv, head = before - part * a.n_kv;
-        const int stop = min(pages, first_page + (end - unit));
+        const int pages = max(1, t.pages), part = in_tile / (uint32_t)a.n_kv, head = in_tile - part * a.n_kv;
         const int columns = min(COLS, t.tokens * a.group - part * COLS), row = t.row;
         const int key0 = t.page0 * kPageTokens + 16 * slice;
         const int low = t.first_pos + part * COLS / a.group;                               // the last key that every column sees
         const int top = t.pages > 0 ? t.first_pos + (part * COLS + columns - 1) / a.group : -1;      // the last that any column sees
-            // queries: divided by a power of two, in fp16 (TERMS = 2: and what that leaves).  All columns at once, some threads to each
-            if (threadIdx.x < 128) {
-                constexpr int PER = 128 / COLS, EP = D / PER;
-                const int c = threadIdx.x / PER, n = part * COLS + c, from = threadIdx.x % PER * EP;
-                const T* q = reinterpret_cast<const T*>(a.q) + ((int64_t)(row + n / a.group) * a.n_heads + head * a.group + n % a.group) * D + from;
-                float x[EP], most = 0.f;
-                if constexpr (EP % 4 == 0) {
+        // queries: divided by a power of two, in fp16 (TERMS = 2: and what that leaves).  All columns at once, some threads to each
+        if (threadIdx.x < 128) {
+            constexpr int PER = 128 / COLS, EP = D / PER;
+            const int c = threadIdx.x / PER, n = part * COLS + c, from = threadIdx.x % PER * EP;
+            const T* q = reinterpret_cast<const T*>(a.q) + ((int64_t)(row + n / a.group) * a.n_heads + head * a.group + n % a.group) * D + from;
+            float x[EP], most = 0.f;
+            if constexpr (EP % 4 == 0) {
 #pragma unroll
-                    for (int i = 0; i < EP; i += 4) {
-                        const float4 v = c < columns ? load4(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < EP; ++i) x[i] = c < columns ? to_f32(q[i]) : 0.f;
+                for (int i = 0; i < EP; i += 4) {
+                    const float4 v = c < columns ? load4(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
                 }
+            } else {
 #pragma unroll
-                for (int i = 0; i < EP; ++i) most = fmaxf(most, fabsf(x[i]));
-#pragma unroll
-                for (int d = 1; d < PER; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                const int e = shift_of(most);
-                const float by = power2(-e);
-                float total = 0.f;
-#pragma unroll
-                for (int i = 0; i < EP; i += 2) {
-                    const float y0 = x[i] * by, y1 = x[i + 1] * by;
-                    total += y0 + y1;
-                    const __half2 h = __floats2half2_rn(y0, y1);
-                    *reinterpret_cast<__half2*>(&sm.q[0][c][from + i]) = h;
-                    if constexpr (TERMS == 2) *reinterpret_cast<__half2*>(&sm.q[1][c][from + i]) = __floats2half2_rn(y0 - __low2float(h), y1 - __high2float(h));
-                }
-#pragma unroll
-                for (int d = 1; d < PER / 2; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-                if (threadIdx.x % (PER / 2) == 0) sm.q_sum[c][threadIdx.x % PER / (PER / 2)] = total;
-                if (from == 0) {
-                    sm.factor[c] = power2(e) * a.scale * 1.4426950408889634f;
-                    sm.last[c] = c < columns ? t.first_pos + n / a.group : -1;
-                }
+                for (int i = 0; i < EP; ++i) x[i] = c < columns ? to_f32(q[i]) : 0.f;
             }
-            __syncthreads();
-            if constexpr (Q_IN_REGISTERS)
 #pragma unroll
-                for (int k = 0; k < STEPS; ++k) qf[k] = q_fragment(0, k, 0);
+            for (int i = 0; i < EP; ++i) most = fmaxf(most, fabsf(x[i]));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int c = 8 * n + 2 * j;
-                q_sum[n][0] = pair(sm.q_sum[c][0], sm.q_sum[c + 1][0]);
-                q_sum[n][1] = pair(sm.q_sum[c][1], sm.q_sum[c + 1][1]);
-                factor[n] = pair(sm.factor[c], sm.factor[c + 1]);
-                minus[n] = sum[n] = down[n] = middle[n][0] = middle[n][1] = pair(0.f, 0.f);
+            for (int d = 1; d < PER; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            const int e = shift_of(most);
+            const float by = power2(-e);
+            float total = 0.f;
 #pragma unroll
-                for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
+            for (int i = 0; i < EP; i += 2) {
+                const float y0 = x[i] * by, y1 = x[i + 1] * by;
+                total += y0 + y1;
+                const __half2 h = __floats2half2_rn(y0, y1);
+                *reinterpret_cast<__half2*>(&sm.q[0][c][from + i]) = h;
+                if constexpr (TERMS == 2) *reinterpret_cast<__half2*>(&sm.q[1][c][from + i]) = __floats2half2_rn(y0 - __low2float(h), y1 - __high2float(h));
             }
-            limit = -1.f;
-            blank = 0xffffffffu;
+#pragma unroll
+            for (int d = 1; d < PER / 2; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            if (threadIdx.x % (PER / 2) == 0) sm.q_sum[c][threadIdx.x % PER / (PER / 2)] = total;
+            if (from == 0) {
+                sm.factor[c] = power2(e) * a.scale * 1.4426950408889634f;
+                sm.last[c] = c < columns ? t.first_pos + n / a.group : -1;
+            }
+        }
+        __syncthreads();
+        if constexpr (Q_IN_REGISTERS)
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) qf[k] = q_fragment(0, k, 0);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int c = 8 * n + 2 * j;
+            q_sum[n][0] = pair(sm.q_sum[c][0], sm.q_sum[c + 1][0]);
+            q_sum[n][1] = pair(sm.q_sum[c][1], sm.q_sum[c + 1][1]);
+            factor[n] = pair(sm.factor[c], sm.factor[c + 1]);
+            minus[n] = sum[n] = down[n] = middle[n][0] = middle[n][1] = pair(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
+        }
+        limit = -1.f;
+        blank = 0xffffffffu;
 
 #pragma unroll 1
-        for (int page = first_page + (GROUPS + turn - (unit - begin) % GROUPS) % GROUPS; page < stop; page += GROUPS) {
-        ask();                                                                         // into the place that the last slice left
-        asm volatile("cp.async.wait_group %0;" :: "n"(STAGES - 1) : "memory");
-        __syncwarp();
-        const uint8_t* rec = sm.ring[warp][stage];
-        if (++stage == STAGES) stage = 0;
-        const int token0 = key0 + page * kPageTokens;
-        // a slice behind every column's last key, or before every window, has nothing to give
-        if (token0 <= top && (a.window == 0 || token0 + 15 > low - a.window)) {
-            uint2 kp[2], vp[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                kp[r] = *reinterpret_cast<const uint2*>(rec + 2 * L::kSlice + (g + 8 * r) * 8);
-                vp[r] = *reinterpret_cast<const uint2*>(rec + 2 * L::kSlice + 128 + (g + 8 * r) * 8);
-            }
-            uint32_t seen = 0xffffffffu;                                               // bit 4 n + 2 r + c: row g + 8 r is seen by the lane's column c
-            if (token0 + 15 > low || (a.window && token0 <= top - a.window)) {
-                seen = 0;
+        for (int page = first_page + turn; page < stop; page += GROUPS) {
+            ask();                                                                         // into the place that the last slice left
+            asm volatile("cp.async.wait_group %0;" :: "n"(STAGES - 1) : "memory");
+            __syncwarp();
+            const uint8_t* rec = sm.ring[warp][stage];
+            if (++stage == STAGES) stage = 0;
+            const int token0 = key0 + page * kPageTokens;
+            // a slice behind every column's last key, or before every window, has nothing to give
+            if (token0 <= top && (a.window == 0 || token0 + 15 > low - a.window)) {
+                uint2 kp[2], vp[2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int token = token0 + g + 8 * r;
-                    if (token > top) kp[r] = vp[r] = make_uint2(0u, 0u);                // what lies there may be no number
+                    kp[r] = *reinterpret_cast<const uint2*>(rec + 2 * L::kSlice + (g + 8 * r) * 8);
+                    vp[r] = *reinterpret_cast<const uint2*>(rec + 2 * L::kSlice + 128 + (g + 8 * r) * 8);
+                }
+                uint32_t seen = 0xffffffffu;                                               // bit 4 n + 2 r + c: row g + 8 r is seen by the lane's column c
+                if (token0 + 15 > low || (a.window && token0 <= top - a.window)) {
+                    seen = 0;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int token = token0 + g + 8 * r;
+                        if (token > top) kp[r] = vp[r] = make_uint2(0u, 0u);                // what lies there may be no number
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const int last = sm.last[8 * n + 2 * j + c];
+                                if (token <= last && (a.window == 0 || token > last - a.window)) seen |= 1u << (4 * n + 2 * r + c);
+                            }
+                        // A row that only some columns see and that is no number would reach the others as 0 * NaN: it goes to
+                        // those that see it here, and is nobody's afterwards.
+                        const bool kbad = !(fabsf(kv4_scale(kp[r].x)) + fabsf(kv4_middle(kp[r].x)) + fabsf(kv4_scale(kp[r].y)) + fabsf(kv4_middle(kp[r].y)) < INFINITY);
+                        const bool bad0 = kbad || !(fabsf(kv4_scale(vp[r].x)) + fabsf(kv4_middle(vp[r].x)) < INFINITY);
+                        const bool bad1 = kbad || !(fabsf(kv4_scale(vp[r].y)) + fabsf(kv4_middle(vp[r].y)) < INFINITY);
+                        if (bad0 || bad1) {
+                            kp[r] = vp[r] = make_uint2(0u, 0u);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const f32x2 poison = pair(seen >> (4 * n + 2 * r) & 1 ? NAN : 0.f, seen >> (4 * n + 2 * r + 1) & 1 ? NAN : 0.f);
+                                if (bad0) middle[n][0] = add2(middle[n][0], poison);
+                                if (bad1) middle[n][1] = add2(middle[n][1], poison);
+                                seen &= ~(3u << (4 * n + 2 * r));
+                            }
+                        }
+                    }
+                }
+                // ---- scores ----
+                float s[2][NT][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int last = sm.last[8 * n + 2 * j + c];
-                            if (token <= last && (a.window == 0 || token > last - a.window)) seen |= 1u << (4 * n + 2 * r + c);
-                        }
-                    // A row that only some columns see and that is no number would reach the others as 0 * NaN: it goes to
-                    // those that see it here, and is nobody's afterwards.
-                    const bool kbad = !(fabsf(kv4_scale(kp[r].x)) + fabsf(kv4_middle(kp[r].x)) + fabsf(kv4_scale(kp[r].y)) + fabsf(kv4_middle(kp[r].y)) < INFINITY);
-                    const bool bad0 = kbad || !(fabsf(kv4_scale(vp[r].x)) + fabsf(kv4_middle(vp[r].x)) < INFINITY);
-                    const bool bad1 = kbad || !(fabsf(kv4_scale(vp[r].y)) + fabsf(kv4_middle(vp[r].y)) < INFINITY);
-                    if (bad0 || bad1) {
-                        kp[r] = vp[r] = make_uint2(0u, 0u);
+                        for (int i = 0; i < 4; ++i) s[h][n][i] = 0.f;
+                {
+                    uint32_t w[E][2];
+                    load_words<D>(rec, lane, w);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const f32x2 poison = pair(seen >> (4 * n + 2 * r) & 1 ? NAN : 0.f, seen >> (4 * n + 2 * r + 1) & 1 ? NAN : 0.f);
-                            if (bad0) middle[n][0] = add2(middle[n][0], poison);
-                            if (bad1) middle[n][1] = add2(middle[n][1], poison);
-                            seen &= ~(3u << (4 * n + 2 * r));
+                    for (int p = 0; p < E; ++p) {
+                        uint32_t lo[4], hi[4];
+                        unpack8(w[p][0], lo);
+                        unpack8(w[p][1], hi);
+#pragma unroll
+                        for (int odd = 0; odd < 2; ++odd) {
+                            const int k = 2 * p + odd;
+                            const uint32_t frag[4] = {lo[2 * odd], hi[2 * odd], lo[2 * odd + 1], hi[2 * odd + 1]};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int u = 0; u < TERMS; ++u) {
+                                    const uint2 b = Q_IN_REGISTERS ? qf[Q_IN_REGISTERS ? k : 0] : q_fragment(u, k, n);
+                                    mma_f16(s[k * 2 / STEPS][n], frag, b.x, b.y);
+                                }
                         }
                     }
                 }
-            }
-            // ---- scores ----
-            float s[2][NT][4];
+                float x[NT][4], highest = -INFINITY;                                       // scores (of 2^x) less the running maximum
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int r = 0; r < 2; ++r) {
+                    const f32x2 s0 = pair(kv4_scale(kp[r].x), kv4_scale(kp[r].x)), s1 = pair(kv4_scale(kp[r].y), kv4_scale(kp[r].y));
+                    const f32x2 m0 = pair(kv4_middle(kp[r].x), kv4_middle(kp[r].x)), m1 = pair(kv4_middle(kp[r].y), kv4_middle(kp[r].y));
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < NT; ++n) {
+                        const f32x2 v = fma2(pair(s[0][n][2 * r], s[0][n][2 * r + 1]), s0, fma2(pair(s[1][n][2 * r], s[1][n][2 * r + 1]), s1, fma2(m0, q_sum[n][0], mul2(m1, q_sum[n][1]))));
+                        const float2 e = both(fma2(v, factor[n], minus[n]));
+                        x[n][2 * r] = seen & (1u << (4 * n + 2 * r)) ? e.x : -INFINITY;
+                        x[n][2 * r + 1] = seen & (2u << (4 * n + 2 * r)) ? e.y : -INFINITY;
+                        highest = fmaxf(highest, fmaxf(x[n][2 * r], x[n][2 * r + 1]));
+                    }
+                }
+                const float sv[2][2] = {{kv4_scale(vp[0].x), kv4_scale(vp[0].y)}, {kv4_scale(vp[1].x), kv4_scale(vp[1].y)}};
+                const float largest = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+                // ---- the running maximum may lie up to 2^8 behind, and ``down`` fit scales up to 2^4 smaller, so that both seldom move ----
+                if (__any_sync(0xffffffffu, highest > 8.f || !(largest <= limit))) {
+                    limit = INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[h][n][i] = 0.f;
-            {
-                uint32_t w[E][2];
-                load_words<D>(rec, lane, w);
+                    for (int n = 0; n < NT; ++n) {
+                        const float2 old = both(minus[n]), was2 = both(down[n]);
+                        float now[2], next[2], by[2], shrink[2];
 #pragma unroll
-                for (int p = 0; p < E; ++p) {
-                    uint32_t lo[4], hi[4];
-                    unpack8(w[p][0], lo);
-                    unpack8(w[p][1], hi);
+                        for (int c = 0; c < 2; ++c) {
+                            float high = -INFINITY, most = 0.f;
 #pragma unroll
-                    for (int odd = 0; odd < 2; ++odd) {
-                        const int k = 2 * p + odd;
-                        const uint32_t frag[4] = {lo[2 * odd], hi[2 * odd], lo[2 * odd + 1], hi[2 * odd + 1]};
+                            for (int r = 0; r < 2; ++r) {
+                                const bool there = seen & ((1u << c) << (4 * n + 2 * r));
+                                high = fmaxf(high, x[n][2 * r + c]);
+                                if (there) most = fmaxf(most, fmaxf(sv[r][0] < INFINITY ? sv[r][0] : 0.f, sv[r][1] < INFINITY ? sv[r][1] : 0.f));
+                            }
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                            for (int d = 4; d < 32; d <<= 1) {
+                                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                            }
+                            // a column moves by its own keys alone, so that its neighbours' have no part in its rounding
+                            const bool first = blank >> (2 * n + c) & 1, move = first || high > 8.f;
+                            const float less = c ? old.y : old.x, was = c ? was2.y : was2.x;
+                            now[c] = move ? high - less : -less;
+                            by[c] = first ? 0.f : move ? fast_exp2(-less - now[c]) : 1.f;
+                            if (now[c] > -INFINITY) blank &= ~(1u << (2 * n + c));
+                            else now[c] = 0.f;
+                            // one over the power of two below the largest scale that the column has seen (0: none above 0)
+                            const float fit = most > 0.f ? power2(-max(-120, min(120, (int)(__float_as_uint(most) >> 23) - 127))) : 0.f;
+                            next[c] = was == 0.f || most > 16.f * inverse_power2(was) ? fit : was;
+                            shrink[c] = was > 0.f ? by[c] * (next[c] * inverse_power2(was)) : by[c];
+                            limit = fminf(limit, blank >> (2 * n + c) & 1 ? -1.f : next[c] > 0.f ? 16.f * inverse_power2(next[c]) : 0.f);
 #pragma unroll
-                            for (int u = 0; u < TERMS; ++u) {
-                                const uint2 b = Q_IN_REGISTERS ? qf[Q_IN_REGISTERS ? k : 0] : q_fragment(u, k, n);
-                                mma_f16(s[k * 2 / STEPS][n], frag, b.x, b.y);
+                            for (int r = 0; r < 2; ++r)
+                                if (move) x[n][2 * r + c] = x[n][2 * r + c] - less - now[c];
+                        }
+                        const f32x2 b = pair(by[0], by[1]), z = pair(shrink[0], shrink[1]);
+                        minus[n] = pair(-now[0], -now[1]);
+                        down[n] = pair(next[0], next[1]);
+                        sum[n] = mul2(sum[n], b);
+                        middle[n][0] = mul2(middle[n][0], b);
+                        middle[n][1] = mul2(middle[n][1], b);
+#pragma unroll
+                        for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float2 y = both(mul2(pair(o[k][n][2 * r], o[k][n][2 * r + 1]), z));
+                                o[k][n][2 * r] = y.x;
+                                o[k][n][2 * r + 1] = y.y;
                             }
                     }
+#pragma unroll
+                    for (int d = 1; d < 4; d <<= 1) limit = fminf(limit, __shfl_xor_sync(0xffffffffu, limit, d));
                 }
-            }
-            float x[NT][4], highest = -INFINITY;                                       // scores (of 2^x) less the running maximum
+                // ---- weights, and weights times scales as the operand with tokens along K ----
+                uint32_t pf[TERMS][2][NT][2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const f32x2 s0 = pair(kv4_scale(kp[r].x), kv4_scale(kp[r].x)), s1 = pair(kv4_scale(kp[r].y), kv4_scale(kp[r].y));
-                const f32x2 m0 = pair(kv4_middle(kp[r].x), kv4_middle(kp[r].x)), m1 = pair(kv4_middle(kp[r].y), kv4_middle(kp[r].y));
+                for (int r = 0; r < 2; ++r) {
+                    const f32x2 scale[2] = {pair(sv[r][0], sv[r][0]), pair(sv[r][1], sv[r][1])};
+                    const f32x2 md[2] = {pair(kv4_middle(vp[r].x), kv4_middle(vp[r].x)), pair(kv4_middle(vp[r].y), kv4_middle(vp[r].y))};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const f32x2 v = fma2(pair(s[0][n][2 * r], s[0][n][2 * r + 1]), s0, fma2(pair(s[1][n][2 * r], s[1][n][2 * r + 1]), s1, fma2(m0, q_sum[n][0], mul2(m1, q_sum[n][1]))));
-                    const float2 e = both(fma2(v, factor[n], minus[n]));
-                    x[n][2 * r] = seen & (1u << (4 * n + 2 * r)) ? e.x : -INFINITY;
-                    x[n][2 * r + 1] = seen & (2u << (4 * n + 2 * r)) ? e.y : -INFINITY;
-                    highest = fmaxf(highest, fmaxf(x[n][2 * r], x[n][2 * r + 1]));
-                }
-            }
-            const float sv[2][2] = {{kv4_scale(vp[0].x), kv4_scale(vp[0].y)}, {kv4_scale(vp[1].x), kv4_scale(vp[1].y)}};
-            const float largest = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-            // ---- the running maximum may lie up to 2^8 behind, and ``down`` fit scales up to 2^4 smaller, so that both seldom move ----
-            if (__any_sync(0xffffffffu, highest > 8.f || !(largest <= limit))) {
-                limit = INFINITY;
+                    for (int n = 0; n < NT; ++n) {
+                        const f32x2 p = pair(fast_exp2(x[n][2 * r]), fast_exp2(x[n][2 * r + 1])), d = mul2(p, down[n]);
+                        sum[n] = add2(sum[n], p);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float2 old = both(minus[n]), was2 = both(down[n]);
-                    float now[2], next[2], by[2], shrink[2];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float high = -INFINITY, most = 0.f;
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const bool there = seen & ((1u << c) << (4 * n + 2 * r));
-                            x[n][2 * r + c] -= c ? old.y : old.x;
-                            high = fmaxf(high, x[n][2 * r + c]);
-                            if (there) most = fmaxf(most, fmaxf(sv[r][0] < INFINITY ? sv[r][0] : 0.f, sv[r][1] < INFINITY ? sv[r][1] : 0.f));
+                        for (int h = 0; h < 2; ++h) {
+                            const float2 y = both(mul2(d, scale[h]));
+                            middle[n][h] = fma2(p, md[h], middle[n][h]);
+                            const uint32_t packed = pack_half2(y.x, y.y);
+                            pf[0][h][n][r] = transpose8(packed);
+                            if constexpr (TERMS == 2) {
+                                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+                                pf[TERMS - 1][h][n][r] = transpose8(pack_half2(y.x - back.x, y.y - back.y));
+                            }
                         }
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) {
-                            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
-                            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                        }
-                        const bool first = blank >> (2 * n + c) & 1;
-                        const float before = first ? -INFINITY : -(c ? old.y : old.x), was = c ? was2.y : was2.x;
-                        now[c] = fmaxf(before, high);
-                        by[c] = first ? 0.f : fast_exp2(before - now[c]);
-                        if (now[c] > -INFINITY) blank &= ~(1u << (2 * n + c));
-                        else now[c] = 0.f;
-                        // one over the power of two below the largest scale that the column has seen (0: none above 0)
-                        const float fit = most > 0.f ? power2(-max(-120, min(120, (int)(__float_as_uint(most) >> 23) - 127))) : 0.f;
-                        next[c] = was == 0.f ? fit : fit > 0.f ? fminf(was, fit) : was;
-                        shrink[c] = was > 0.f ? by[c] * (next[c] * inverse_power2(was)) : by[c];
-                        limit = fminf(limit, blank >> (2 * n + c) & 1 ? -1.f : next[c] > 0.f ? 16.f * inverse_power2(next[c]) : 0.f);
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) x[n][2 * r + c] -= now[c];
                     }
-                    const f32x2 b = pair(by[0], by[1]), z = pair(shrink[0], shrink[1]);
-                    minus[n] = pair(-now[0], -now[1]);
-                    down[n] = pair(next[0], next[1]);
-                    sum[n] = mul2(sum[n], b);
-                    middle[n][0] = mul2(middle[n][0], b);
-                    middle[n][1] = mul2(middle[n][1], b);
-#pragma unroll
-                    for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const float2 y = both(mul2(pair(o[k][n][2 * r], o[k][n][2 * r + 1]), z));
-                            o[k][n][2 * r] = y.x;
-                            o[k][n][2 * r + 1] = y.y;
-                        }
                 }
+                // ---- weighted values ----
+                {
+                    uint32_t w[E][2];
+                    load_words<D>(rec + L::kSlice, lane, w);
 #pragma unroll
-                for (int d = 1; d < 4; d <<= 1) limit = fminf(limit, __shfl_xor_sync(0xffffffffu, limit, d));
-            }
-            // ---- weights, and weights times scales as the operand with tokens along K ----
-            uint32_t pf[TERMS][2][NT][2];
+                    for (int p = 0; p < E; ++p) {
+                        uint32_t lo[4], hi[4];
+                        unpack8(w[p][0], lo);
+                        unpack8(w[p][1], hi);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const f32x2 scale[2] = {pair(sv[r][0], sv[r][0]), pair(sv[r][1], sv[r][1])};
-                const f32x2 md[2] = {pair(kv4_middle(vp[r].x), kv4_middle(vp[r].x)), pair(kv4_middle(vp[r].y), kv4_middle(vp[r].y))};
+                        for (int odd = 0; odd < 2; ++odd) {
+                            const int k = 2 * p + odd;
+                            const uint32_t frag[4] = {lo[2 * odd], lo[2 * odd + 1], hi[2 * odd], hi[2 * odd + 1]};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const f32x2 p = pair(fast_exp2(x[n][2 * r]), fast_exp2(x[n][2 * r + 1])), d = mul2(p, down[n]);
-                    sum[n] = add2(sum[n], p);
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float2 y = both(mul2(d, scale[h]));
-                        middle[n][h] = fma2(p, md[h], middle[n][h]);
-                        const uint32_t packed = pack_half2(y.x, y.y);
-                        pf[0][h][n][r] = transpose8(packed);
-                        if constexpr (TERMS == 2) {
-                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&packed));
-                            pf[TERMS - 1][h][n][r] = transpose8(pack_half2(y.x - back.x, y.y - back.y));
+                                for (int u = 0; u < TERMS; ++u) mma_f16(o[k][n], frag, pf[u][k * 2 / STEPS][n][0], pf[u][k * 2 / STEPS][n][1]);
                         }
                     }
                 }
             }
-            // ---- weighted values ----
-            {
-                uint32_t w[E][2];
-                load_words<D>(rec + L::kSlice, lane, w);
-#pragma unroll
-                for (int p = 0; p < E; ++p) {
-                    uint32_t lo[4], hi[4];
-                    unpack8(w[p][0], lo);
-                    unpack8(w[p][1], hi);
-#pragma unroll
-                    for (int odd = 0; odd < 2; ++odd) {
-                        const int k = 2 * p + odd;
-                        const uint32_t frag[4] = {lo[2 * odd], lo[2 * odd + 1], hi[2 * odd], hi[2 * odd + 1]};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int u = 0; u < TERMS; ++u) mma_f16(o[k][n], frag, pf[u][k * 2 / STEPS][n][0], pf[u][k * 2 / STEPS][n][1]);
-                    }
-                }
-            }
-        }
-        __syncwarp();
+            __syncwarp();
         }
 
-        // ---- a tile, or the block's part of it, ends: the warps' parts become one, eight columns at a time ----
+        // ---- a row, or the block's part of it, ends: the warps' parts become one, eight columns at a time ----
         const bool whole = first_page == 0 && stop == pages;
-        // a part of a tile that an earlier block began lies in the block's first place, one that goes on behind it in the second
+        // a part of a row that an earlier block began lies in the block's first place, one that goes on behind it in the second
         float* mine = part_of<D>(a, gridDim.x, blockIdx.x, first_page == 0, COLS);
-        if (!whole && first_page == 0 && threadIdx.x == 0)
-            *reinterpret_cast<CutTile*>(a.scratch + (int64_t)blockIdx.x * kHeadInts) =
-                CutTile{block_of(shares, unit - first_page + pages - 1), row, part, head, columns};
+        if (first_page == 0 && threadIdx.x == 0 && (!whole || sm.last_block >= 0)) {
+            const int last = sm.prefix[index] + ((int)in_tile + 1) * (EXTRA + pages) - 1;
+            const int last_block = whole ? -1 : sm.last_block >= 0 ? sm.last_block : block_of(shares_of(sm.prefix[a.n_tiles], GROUPS, gridDim.x), last);
+            *reinterpret_cast<CutRow*>(a.scratch + (int64_t)sm.place * kHeadInts) = CutRow{(int)blockIdx.x, last_block, row, part, head, columns};
+        }
         const auto leave = [&](int n) {
             const float2 m = both(minus[n]), d = both(down[n]);
             if (g == 0) *reinterpret_cast<float2*>(&sm.merge_m[warp][2 * j]) = make_float2(blank >> (2 * n) & 1 ? -INFINITY : -m.x, blank >> (2 * n + 1) & 1 ? -INFINITY : -m.y);
@@ -630,61 +692,50 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
             if (NT == 1 || n == 0) leave(0);
             else leave(NT - 1);
             __syncthreads();
-            constexpr int EP = D / 16;                                                  // 16 threads to a column
-            const int col = threadIdx.x / 16, from = threadIdx.x % 16 * EP;
+            const int col = warp;                                                       // a warp to a column
             if (col < min(8, columns - 8 * n)) {
-                float high = -INFINITY, total = 0.f, y[EP];
+                const float m = lane < WARPS ? sm.merge_m[lane % WARPS][col] : -INFINITY, high = warp_max(m);
+                const float by = m > -INFINITY ? fast_exp2(m - high) : 0.f;
+                const float total = warp_sum(lane < WARPS ? sm.merge_l[lane % WARPS][col] * by : 0.f);
+                float y[D / 32];
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) high = fmaxf(high, sm.merge_m[w][col]);
-#pragma unroll
-                for (int i = 0; i < EP; ++i) y[i] = 0.f;
+                for (int i = 0; i < D / 32; ++i) y[i] = 0.f;
 #pragma unroll
                 for (int w = 0; w < WARPS; ++w) {
-                    const float m = sm.merge_m[w][col], by = m > -INFINITY ? fast_exp2(m - high) : 0.f;
-                    total += sm.merge_l[w][col] * by;
+                    const float b = __shfl_sync(0xffffffffu, by, w);
 #pragma unroll
-                    for (int i = 0; i < EP; i += 2) {
-                        const float2 z = *reinterpret_cast<const float2*>(&sm.merge[w][col][from + i]);
-                        y[i] += z.x * by;
-                        y[i + 1] += z.y * by;
-                    }
+                    for (int i = 0; i < D / 32; ++i) y[i] += sm.merge[w][col][lane + 32 * i] * b;
                 }
                 if (whole) {
                     const int q = part * COLS + 8 * n + col;
                     const float inv = total == 0.f ? 0.f : 1.f / total;
-                    T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(row + q / a.group) * a.n_heads + head * a.group + q % a.group) * D + from;
-                    if constexpr (EP % 4 == 0) {
+                    T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(row + q / a.group) * a.n_heads + head * a.group + q % a.group) * D;
 #pragma unroll
-                        for (int i = 0; i < EP; i += 4) store4(out + i, make_float4(y[i] * inv, y[i + 1] * inv, y[i + 2] * inv, y[i + 3] * inv));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < EP; ++i) out[i] = from_f32<T>(y[i] * inv);
-                    }
+                    for (int i = 0; i < D / 32; ++i) out[lane + 32 * i] = from_f32<T>(y[i] * inv);
                 } else {
                     float* p = mine + (int64_t)(8 * n + col) * kPartStride<D>;
 #pragma unroll
-                    for (int i = 0; i < EP; i += 2) *reinterpret_cast<float2*>(p + from + i) = make_float2(y[i], y[i + 1]);
-                    if (from == 0) *reinterpret_cast<float2*>(p + D) = make_float2(high, total);
+                    for (int i = 0; i < D / 32; ++i) p[lane + 32 * i] = y[i];
+                    if (lane == 0) *reinterpret_cast<float2*>(p + D) = make_float2(high, total);
                 }
             }
             __syncthreads();
         }
-        unit += stop - first_page;
     }
 }
 
-// Adds up the parts of the tiles that were cut, one block per tile and column: a tile belongs to the block that began it (blockIdx.y), whose
-// head says which block had its end.  A warp has four of its parts under way at a time.
+// Adds up the parts of the rows that were cut, one block per row and column; blockIdx.y is the place of the row's head.  A warp has four of its
+// parts under way at a time.
 constexpr int kCombineWarps = 16, kCombineParts = 4;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kCombineWarps * 32)
-kv4_combine_kernel(const __grid_constant__ AttendArgs a) {
+kv4_combine_kernel(const __grid_constant__ AttendArgs a, int blocks) {
     constexpr int COLS = 8 * NT, E = D / 32;
     __shared__ float tops[kCombineWarps], sums[kCombineWarps], values[kCombineWarps][D];
     pdl_launch_dependents();
     pdl_wait();
-    const int c = blockIdx.x, b0 = blockIdx.y, blocks = gridDim.y;
-    const CutTile cut = *reinterpret_cast<const CutTile*>(a.scratch + (int64_t)b0 * kHeadInts);
+    const CutRow cut = *reinterpret_cast<const CutRow*>(a.scratch + (int64_t)blockIdx.y * kHeadInts);
+    const int c = blockIdx.x, b0 = cut.first_block;
     if (cut.last_block < 0 || c >= cut.columns) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const auto place = [&](int b) { return part_of<D>(a, blocks, b, b == b0, COLS) + (int64_t)c * kPartStride<D>; };
@@ -746,7 +797,8 @@ int attend(const AttendArgs& a, cudaStream_t stream) {
     if (sms <= 0) return CPM_BAD_ARGUMENT;
     const int blocks = sms;
     cpm_launch(kLaunchAttention, kv4_attention_kernel<T, D, NT, TERMS>, dim3(blocks), 32 * warps_of(D, NT, TERMS), bytes, stream, a);
-    cpm_launch(kLaunchAttention, kv4_combine_kernel<T, D, NT>, dim3(8 * NT, blocks), kCombineWarps * 32, 0, stream, a);
+    const int heads = shares_by_rows(a, 8 * NT, blocks) ? a.n_tiles * rows_of_tile(a, 8 * NT) : blocks;
+    cpm_launch(kLaunchAttention, kv4_combine_kernel<T, D, NT>, dim3(8 * NT, heads), kCombineWarps * 32, 0, stream, a, blocks);
     return launch_status();
 }
 

@@ -1670,9 +1670,10 @@ class Ops:
     def _kv4(self, records: torch.Tensor, n_kv: int, d: int) -> torch.Tensor:
         if d not in self.KV4_HEAD_DIMS:
             raise ValueError(f"a 4-bit cache takes head sizes {self.KV4_HEAD_DIMS}, got {d}")
-        if records.dtype != torch.uint8 or records.device.type != self.device.type or not records.is_contiguous() \
-                or records.dim() != 3 or tuple(records.shape[1:]) != (n_kv, self.kv4_page_bytes(d)):
-            raise ValueError(f"4-bit cache: needs a contiguous uint8 tensor [pages, {n_kv}, {self.kv4_page_bytes(d)}] on the device, got "
+        shape = records.shape
+        if records.dtype != torch.uint8 or not records.is_cuda or not records.is_contiguous() or len(shape) != 3 or shape[1] != n_kv \
+                or shape[2] != kv4_page_bytes(d):
+            raise ValueError(f"4-bit cache: needs a contiguous uint8 tensor [pages, {n_kv}, {kv4_page_bytes(d)}] on the device, got "
                              f"{records.dtype} {tuple(records.shape)}")
         return records
 
@@ -1712,7 +1713,7 @@ class Ops:
         q = self.empty(n, n_heads, d)
         check(self.lib.cpm_rope_store_kv4(_ptr(qkv), _ptr(q), _ptr(records), _ptr(positions), _ptr(token_seq), _ptr(slots), _ptr(page_table),
                                           page_table.shape[1], _ptr(inv_freq) if rot_dim else None, float(magnitude), n, n_heads, n_kv, d,
-                                          self.code, self._stream()), f"rope_store_kv4 (head_dim {d})")
+                                          self.code, self._stream()), "rope_store_kv4")
         return q
 
     KV4_PROMPT_BLOCKS = 5                # query rows that fill so many blocks go to the tcgen05 kernel
@@ -1744,7 +1745,7 @@ class Ops:
         self._table(page_table)
         k, v = self.empty(n, n_kv, d), self.empty(n, n_kv, d)
         check(self.lib.cpm_kv4_values(_ptr(records), _ptr(k), _ptr(v), _ptr(positions), _ptr(token_seq), _ptr(slots), _ptr(page_table),
-                                      page_table.shape[1], n, n_kv, d, self.code, self._stream()), f"kv4_values (head_dim {d})")
+                                      page_table.shape[1], n, n_kv, d, self.code, self._stream()), "kv4_values")
         return k, v
 
     def kv4_attention(self, q: torch.Tensor, records: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor,
@@ -1791,24 +1792,25 @@ class Ops:
             parts = self.empty(shares * n * n_heads * (d + 4), dtype=torch.float32) if shares > 1 else None
             check(self.lib.cpm_kv4_prompt(_ptr(q), _ptr(records), _ptr(out), _ptr(kv_len), _ptr(slots), _ptr(page_table), page_table.shape[1],
                                           _ptr(cu_q), _ptr(tile_seq), _ptr(tile_row), n_tiles, _ptr(parts), shares, n, n_heads, n_kv, d,
-                                          int(window), float(scale), self._stream()), f"prompt attention over a 4-bit cache (head_dim {d})")
+                                          int(window), float(scale), self._stream()), "prompt attention over a 4-bit cache")
             if shares > 1:
                 LAUNCHES_EXTRA[0] += 1
             return out
-        scratch = self.empty(int(self.lib.cpm_kv4_attention_scratch_floats(d)), dtype=torch.float32)
-        # the kernel counts a launch's work in 32 bits: key-value heads x parts of a tile x pages of every tile
-        units = n_kv * (tile_tokens * (n_heads // n_kv) // 8 + 1) * max(1, page_table.shape[1])
+        scratch = self.empty(self.lib.cpm_kv4_attention_scratch_floats(d), dtype=torch.float32)
+        # the kernel counts a launch's work in 32 bits: key-value heads x parts of a tile x pages and 16 more of every tile
+        units = n_kv * (tile_tokens * (n_heads // n_kv) // 8 + 1) * (page_table.shape[1] + 17)
         step = max(1, min(self.lib.cpm_kv4_attention_most_tiles(), 0x7fffffff // units))
         size = n_heads * d * self.element_size
+        at_q, at_out, at_len, at_slot = _ptr(q), _ptr(out), _ptr(kv_len), _ptr(slots)
+        at_seq, at_row = _ptr(tile_seq), _ptr(tile_row)
         for first in range(0, n_tiles, step):
-            count = min(step, n_tiles - first)
-            at = lambda t: _ptr(t) + 4 * first if _ptr(t) is not None else None     # noqa: E731
-            row = 0 if cu_q is not None else first
-            check(self.lib.cpm_kv4_attention(_ptr(q) + row * size, _ptr(records), _ptr(out) + row * size,
-                                             at(kv_len) if cu_q is None else _ptr(kv_len), at(slots) if cu_q is None else _ptr(slots),
-                                             _ptr(page_table), page_table.shape[1], _ptr(cu_q), at(tile_seq), at(tile_row), count,
-                                             _ptr(scratch), n_heads, n_kv, d, int(window), float(scale), self.code, self._stream()),
-                  f"attention over a 4-bit cache (head_dim {d}, {n_heads} heads, {n_kv} kv heads)")
+            check(self.lib.cpm_kv4_attention(at_q, _ptr(records), at_out, at_len, at_slot, _ptr(page_table), page_table.shape[1], _ptr(cu_q), at_seq,
+                                             at_row, min(step, n_tiles - first), _ptr(scratch), n_heads, n_kv, d, int(window), float(scale), self.code,
+                                             self._stream()), "attention over a 4-bit cache")
+            if cu_q is not None:         # the next tiles of the same rows, or the next rows and their sequences
+                at_seq, at_row = at_seq + 4 * step, at_row + 4 * step
+            else:
+                at_q, at_out, at_len, at_slot = at_q + step * size, at_out + step * size, at_len + 4 * step, at_slot + 4 * step
             LAUNCHES_EXTRA[0] += 1       # the shares, then their combination
         return out
 
@@ -1825,15 +1827,16 @@ class Ops:
             raise ValueError(f"{src.numel()} source pages and {dst.numel()} destination pages")
         words = []
         for t in tensors:
-            if t.device.type != self.device.type or not t.is_contiguous() or t.dim() < 2:
+            shape = t.shape
+            if not t.is_cuda or not t.is_contiguous() or len(shape) < 2:
                 raise ValueError(f"pages: needs contiguous tensors [layers, pages, ...] on the device, got {tuple(t.shape)} on {t.device}")
             if t.numel() and src.numel():
-                page = t[0, 0].numel() * t.element_size()
-                words.append((t.data_ptr(), page * t.shape[1], page, t.shape[0], t.shape[1]))
-        for i in range(0, len(words), self.COPY_TENSORS):
-            part = words[i:i + self.COPY_TENSORS]
-            flat = (ctypes.c_int64 * (5 * len(part)))(*[w for five in part for w in five])
-            check(self.lib.cpm_copy_pages(flat, len(part), _ptr(src), _ptr(dst), src.numel(), self._stream()), "copy_pages")
+                layer = t.numel() // shape[0] * t.element_size()
+                words += (t.data_ptr(), layer, layer // shape[1], shape[0], shape[1])
+        for i in range(0, len(words), 5 * self.COPY_TENSORS):
+            part = words[i:i + 5 * self.COPY_TENSORS]
+            check(self.lib.cpm_copy_pages((ctypes.c_int64 * len(part))(*part), len(part) // 5, _ptr(src), _ptr(dst), src.numel(), self._stream()),
+                  "copy_pages")
 
     # ---- drawing from a filtered distribution ----
     def sample_filtered(self, logits: torch.Tensor, uniform: Optional[torch.Tensor], temperature: torch.Tensor,
