@@ -35,8 +35,12 @@ struct AttendArgs {
     const int *cu_q, *tile_seq, *tile_row;             // null: one token per sequence
     float* scratch;
     int max_pages, n_tiles, n_heads, n_kv, group, window;
-    float scale;
+    float scale, per_group, per_kv;                    // 1 / group, 1 / n_kv
 };
+
+// n / m for 0 <= n < 2^20 and 1 / m: the quotient's error, below 2^-3 / m, stays away from the next whole number, which is 1 / (2 m) off.  (A division
+// of whole numbers is some twenty instructions, all of which a block of a few pages fetches from L2.)
+__device__ __forceinline__ int quotient(int n, float per) { return (int)(((float)n + 0.5f) * per); }
 
 // One query tile: its sequence's first query row, tokens, keys, and the pages that any of its queries sees.
 struct Tile { int row, tokens, first_pos, kv_len, page0, pages, slot, parts; };
@@ -106,6 +110,8 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ void store2(float* p, float lo, float hi) { *reinterpret_cast<float2*>(p) = make_float2(lo, hi); }
+__device__ __forceinline__ void store2(bf16* p, float lo, float hi) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(lo, hi); }
 // 2^x; below 2^-126 zero, which no sum of weights up to 2^8 notices.
 __device__ __forceinline__ float fast_exp2(float x) {
     float r;
@@ -163,7 +169,7 @@ constexpr int warps_of(int d, int nt, int terms) { return nt == 1 ? 16 : terms =
 template <int D, int NT, int TERMS>
 struct Smem {
     static constexpr int kWarps = warps_of(D, NT, TERMS);
-    static constexpr int kStages = D < 96 ? 6 : NT == 1 ? 3 : 4;
+    static constexpr int kStages = D < 96 ? 6 : 3;
     static constexpr int kCols = 8 * NT;
     static constexpr int kQStride = D + 16;            // fp16 numbers a row: rows 32 bytes apart modulo 128
     // 16 tokens of a record: key codes, value codes, key parameters, value parameters
@@ -171,8 +177,11 @@ struct Smem {
     static constexpr int kChunks = kStage / 16, kPieces = (kChunks + 31) / 32;
     alignas(128) uint8_t ring[kWarps][kStages][kStage];
     alignas(16) __half q[TERMS][kCols][kQStride];
-    alignas(16) float merge[kWarps][8][D + 8];         // rows 32 bytes apart modulo 128
-    alignas(16) float merge_m[kWarps][8], merge_l[kWarps][8];
+    // what the warps leave at a row's end: their sums as they lie in the registers (16 channels of 8 columns after the other, a lane's four
+    // numbers together), and of each column the maximum, the sum of weights, both halves' middles, and the factor of the sums
+    alignas(16) float merge[kWarps][NT][D / 16][32][4];
+    alignas(16) float merge_m[kWarps][kCols], merge_l[kWarps][kCols], merge_mid[2][kWarps][kCols], merge_up[kWarps][kCols];
+    float end_m[kCols], end_l[kCols], end_mid[2][kCols];
     float q_sum[kCols][2], factor[kCols];
     int last[kCols];                                   // a column's last key, -1: no such column
     int scan[kWarps];
@@ -182,7 +191,8 @@ struct Smem {
 };
 
 // A row of pages (a tile's, of one key-value head and part) costs a block its pages and some more, for the queries that it prepares and the parts
-// that it adds up.  All rows lie one behind the other in a line of such costs, a row's extra cost first.
+// that it adds up.  All rows lie one behind the other in a line of such costs, a row's extra cost first.  (Extra cost of 2, 4 and 8 pages for each group
+// of warps: 64 sequences of up to 8,192 keys, 14 heads on 2 of 64, 31.0, 27.6 and 29.5 us; 200 of up to 4,000, 32 on 8 of 128, 172, 163 and 177.)
 constexpr int extra_cost(int groups) { return 4 * groups; }
 // Sharing by cost: each of the blocks takes a piece of the line, wherever rows begin or end; fewer blocks where there is little.
 struct Shares { int sharing, each, more; };            // the first ``more`` blocks have one more than ``each``
@@ -221,6 +231,12 @@ __device__ __forceinline__ void sum_tiles(const AttendArgs& a, int columns, int 
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += x;
+        }
+        if (a.n_tiles <= 32) {                              // one warp has them all
+            if (i < a.n_tiles) prefix[i] = v - own;
+            if (threadIdx.x == 31) prefix[a.n_tiles] = v;
+            __syncthreads();
+            return;
         }
         if (lane == 31) scan[warp] = v;
         __syncthreads();
@@ -354,7 +370,7 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
             ask_any = sm.tiles[ask_index].pages > 0;
             ask_first = sm.tiles[ask_index].page0;
             ask_table = a.page_table + (int64_t)sm.tiles[ask_index].slot * a.max_pages;
-            ask_records = a.records + (int64_t)(row % (uint32_t)a.n_kv) * L::kBytes;
+            ask_records = a.records + (int64_t)((int)row - quotient(row, a.per_kv) * a.n_kv) * L::kBytes;
             ask_base = ask_page - 32 * GROUPS;
         }
         if (ask_page < ask_stop) {
@@ -400,16 +416,16 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
         walk(at, index, in_tile, first_page, stop);
         if (stop <= first_page) break;                                                  // only a part of a row's extra cost is left
         const Tile t = sm.tiles[index];
-        const int pages = max(1, t.pages), part = in_tile / (uint32_t)a.n_kv, head = in_tile - part * a.n_kv;
+        const int pages = max(1, t.pages), part = quotient(in_tile, a.per_kv), head = (int)in_tile - part * a.n_kv;
         const int columns = min(COLS, t.tokens * a.group - part * COLS), row = t.row;
         const int key0 = t.page0 * kPageTokens + 16 * slice;
-        const int low = t.first_pos + part * COLS / a.group;                               // the last key that every column sees
-        const int top = t.pages > 0 ? t.first_pos + (part * COLS + columns - 1) / a.group : -1;      // the last that any column sees
+        const int low = t.first_pos + quotient(part * COLS, a.per_group);                               // the last key that every column sees
+        const int top = t.pages > 0 ? t.first_pos + quotient(part * COLS + columns - 1, a.per_group) : -1;      // the last that any column sees
         // queries: divided by a power of two, in fp16 (TERMS = 2: and what that leaves).  All columns at once, some threads to each
-        if (threadIdx.x < 128) {
-            constexpr int PER = 128 / COLS, EP = D / PER;
-            const int c = threadIdx.x / PER, n = part * COLS + c, from = threadIdx.x % PER * EP;
-            const T* q = reinterpret_cast<const T*>(a.q) + ((int64_t)(row + n / a.group) * a.n_heads + head * a.group + n % a.group) * D + from;
+        if (threadIdx.x < 16 * COLS) {
+            constexpr int PER = 16, EP = D / PER;
+            const int c = threadIdx.x / PER, n = part * COLS + c, token = quotient(n, a.per_group), from = threadIdx.x % PER * EP;
+            const T* q = reinterpret_cast<const T*>(a.q) + ((int64_t)(row + token) * a.n_heads + head * a.group + n - token * a.group) * D + from;
             float x[EP], most = 0.f;
             if constexpr (EP % 4 == 0) {
 #pragma unroll
@@ -441,7 +457,7 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
             if (threadIdx.x % (PER / 2) == 0) sm.q_sum[c][threadIdx.x % PER / (PER / 2)] = total;
             if (from == 0) {
                 sm.factor[c] = power2(e) * a.scale * 1.4426950408889634f;
-                sm.last[c] = c < columns ? t.first_pos + n / a.group : -1;
+                sm.last[c] = c < columns ? t.first_pos + token : -1;
             }
         }
         __syncthreads();
@@ -667,10 +683,9 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
             const int last_block = whole ? -1 : sm.last_block >= 0 ? sm.last_block : block_of(shares_of(sm.prefix[a.n_tiles], GROUPS, gridDim.x), last);
             *reinterpret_cast<CutRow*>(a.scratch + (int64_t)sm.place * kHeadInts) = CutRow{(int)blockIdx.x, last_block, row, part, head, columns};
         }
-        const auto leave = [&](int n) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
             const float2 m = both(minus[n]), d = both(down[n]);
-            if (g == 0) *reinterpret_cast<float2*>(&sm.merge_m[warp][2 * j]) = make_float2(blank >> (2 * n) & 1 ? -INFINITY : -m.x, blank >> (2 * n + 1) & 1 ? -INFINITY : -m.y);
-            const f32x2 up = pair(d.x > 0.f ? inverse_power2(d.x) : 0.f, d.y > 0.f ? inverse_power2(d.y) : 0.f);
             f32x2 l = sum[n], mid[2] = {middle[n][0], middle[n][1]};
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) {
@@ -678,49 +693,63 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
                 mid[0] = add2(mid[0], __shfl_xor_sync(0xffffffffu, mid[0], i));
                 mid[1] = add2(mid[1], __shfl_xor_sync(0xffffffffu, mid[1], i));
             }
-            if (g == 0) *reinterpret_cast<float2*>(&sm.merge_l[warp][2 * j]) = both(l);
-            // channel of a lane's sums: block k, channels 2 g (the first two) and 2 g + 1
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-                const float2 even = both(fma2(pair(o[k][n][0], o[k][n][1]), up, mid[k * 2 / STEPS])), odd = both(fma2(pair(o[k][n][2], o[k][n][3]), up, mid[k * 2 / STEPS]));
-                *reinterpret_cast<float2*>(&sm.merge[warp][2 * j][16 * k + 2 * g]) = make_float2(even.x, odd.x);
-                *reinterpret_cast<float2*>(&sm.merge[warp][2 * j + 1][16 * k + 2 * g]) = make_float2(even.y, odd.y);
+            if (g == 0) {
+                const int c = 8 * n + 2 * j;
+                *reinterpret_cast<float2*>(&sm.merge_m[warp][c]) = make_float2(blank >> (2 * n) & 1 ? -INFINITY : -m.x, blank >> (2 * n + 1) & 1 ? -INFINITY : -m.y);
+                *reinterpret_cast<float2*>(&sm.merge_up[warp][c]) = make_float2(d.x > 0.f ? inverse_power2(d.x) : 0.f, d.y > 0.f ? inverse_power2(d.y) : 0.f);
+                *reinterpret_cast<float2*>(&sm.merge_l[warp][c]) = both(l);
+                *reinterpret_cast<float2*>(&sm.merge_mid[0][warp][c]) = both(mid[0]);
+                *reinterpret_cast<float2*>(&sm.merge_mid[1][warp][c]) = both(mid[1]);
             }
-        };
-#pragma unroll 1
-        for (int n = 0; n < NT; ++n) {
-            if (NT == 1 || n == 0) leave(0);
-            else leave(NT - 1);
-            __syncthreads();
-            const int col = warp;                                                       // a warp to a column
-            if (col < min(8, columns - 8 * n)) {
-                const float m = lane < WARPS ? sm.merge_m[lane % WARPS][col] : -INFINITY, high = warp_max(m);
-                const float by = m > -INFINITY ? fast_exp2(m - high) : 0.f;
-                const float total = warp_sum(lane < WARPS ? sm.merge_l[lane % WARPS][col] * by : 0.f);
-                float y[D / 32];
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) y[i] = 0.f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float b = __shfl_sync(0xffffffffu, by, w);
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) y[i] += sm.merge[w][col][lane + 32 * i] * b;
-                }
-                if (whole) {
-                    const int q = part * COLS + 8 * n + col;
-                    const float inv = total == 0.f ? 0.f : 1.f / total;
-                    T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(row + q / a.group) * a.n_heads + head * a.group + q % a.group) * D;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) out[lane + 32 * i] = from_f32<T>(y[i] * inv);
-                } else {
-                    float* p = mine + (int64_t)(8 * n + col) * kPartStride<D>;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) p[lane + 32 * i] = y[i];
-                    if (lane == 0) *reinterpret_cast<float2*>(p + D) = make_float2(high, total);
-                }
-            }
-            __syncthreads();
+            for (int k = 0; k < STEPS; ++k)
+                *reinterpret_cast<float4*>(sm.merge[warp][n][k][lane]) = make_float4(o[k][n][0], o[k][n][1], o[k][n][2], o[k][n][3]);
         }
+        __syncthreads();
+#pragma unroll 1
+        for (int c = warp; c < columns; c += WARPS) {                                   // a warp to a column, a lane to a warp's part of it
+            const bool there = lane < WARPS;
+            const int w = lane % WARPS;
+            const float m = there ? sm.merge_m[w][c] : -INFINITY, high = warp_max(m), by = m > -INFINITY ? fast_exp2(m - high) : 0.f;
+            const float l = warp_sum(there ? sm.merge_l[w][c] * by : 0.f);
+            const float mid0 = warp_sum(there ? sm.merge_mid[0][w][c] * by : 0.f), mid1 = warp_sum(there ? sm.merge_mid[1][w][c] * by : 0.f);
+            if (there) sm.merge_up[w][c] *= by;
+            if (lane == 0) {
+                sm.end_m[c] = high;
+                sm.end_l[c] = l;
+                sm.end_mid[0][c] = mid0;
+                sm.end_mid[1][c] = mid1;
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = threadIdx.x; i < NT * D * 2; i += 32 * WARPS) {                     // two channels of two columns
+            const int n = i / (2 * D), k = i / 32 % STEPS, c = 8 * n + 2 * (i & 3), channel = 16 * k + 2 * (i >> 2 & 7);
+            f32x2 y0 = *reinterpret_cast<const f32x2*>(&sm.end_mid[k * 2 / STEPS][c]), y1 = y0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(sm.merge[w][n][k][i & 31]);
+                const f32x2 up = *reinterpret_cast<const f32x2*>(&sm.merge_up[w][c]);
+                y0 = fma2(x.x, up, y0);
+                y1 = fma2(x.y, up, y1);
+            }
+            const float2 even = both(y0), odd = both(y1);                                // (channel, columns c and c + 1; channel + 1)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (c + e >= columns) break;
+                const float lo = e ? even.y : even.x, hi = e ? odd.y : odd.x, l = sm.end_l[c + e];
+                if (whole) {
+                    const int q = part * COLS + c + e, token = sm.last[c + e] - t.first_pos;
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    store2(reinterpret_cast<T*>(a.out) + ((int64_t)(row + token) * a.n_heads + head * a.group + q - token * a.group) * D + channel, lo * inv, hi * inv);
+                } else {
+                    float* p = mine + (int64_t)(c + e) * kPartStride<D>;
+                    *reinterpret_cast<float2*>(p + channel) = make_float2(lo, hi);
+                    if (channel == 0) *reinterpret_cast<float2*>(p + D) = make_float2(sm.end_m[c + e], l);
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -730,67 +759,70 @@ constexpr int kCombineWarps = 16, kCombineParts = 4;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kCombineWarps * 32)
 kv4_combine_kernel(const __grid_constant__ AttendArgs a, int blocks) {
-    constexpr int COLS = 8 * NT, E = D / 32;
+    constexpr int COLS = 8 * NT, E = D / 32, STRIDE = COLS * kPartStride<D>;
     __shared__ float tops[kCombineWarps], sums[kCombineWarps], values[kCombineWarps][D];
     pdl_launch_dependents();
     pdl_wait();
     const CutRow cut = *reinterpret_cast<const CutRow*>(a.scratch + (int64_t)blockIdx.y * kHeadInts);
-    const int c = blockIdx.x, b0 = cut.first_block;
-    if (cut.last_block < 0 || c >= cut.columns) return;
+    const int c = blockIdx.x, b0 = cut.first_block, last = cut.last_block;
+    if (last < 0 || c >= cut.columns) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const auto place = [&](int b) { return part_of<D>(a, blocks, b, b == b0, COLS) + (int64_t)c * kPartStride<D>; };
-    float top = -INFINITY;
-    for (int b = b0 + threadIdx.x; b <= cut.last_block; b += kCombineWarps * 32) top = fmaxf(top, place(b)[D]);
-    top = warp_max(top);
-    if (lane == 0) tops[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kCombineWarps; ++w) top = fmaxf(top, tops[w]);
-    float l = 0.f, o[E];
+    const float* parts = part_of<D>(a, blocks, 0, false, COLS) + c * kPartStride<D>;
+    float top = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.f;
 #pragma unroll 1
-    for (int b = b0 + warp; b <= cut.last_block; b += kCombineWarps * kCombineParts) {
+    for (int b = b0 + warp; b <= last; b += kCombineWarps * kCombineParts) {
         float v[kCombineParts][E];
         float2 ml[kCombineParts];
 #pragma unroll
         for (int u = 0; u < kCombineParts; ++u) {
-            const float* p = place(min(b + u * kCombineWarps, cut.last_block));
+            const int x = b + u * kCombineWarps, y = min(x, last);
+            const float* p = parts + (2 * y + (y == b0)) * STRIDE;
             ml[u] = *reinterpret_cast<const float2*>(p + D);
-            if (b + u * kCombineWarps > cut.last_block) ml[u] = make_float2(-INFINITY, 0.f);
+            if (x > last) ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[u][i] = p[lane + 32 * i];
         }
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < kCombineParts; ++u) now = fmaxf(now, ml[u].x);
+        const float back = top > -INFINITY ? exp2f(top - now) : 0.f;
+        top = now;
+        l *= back;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] *= back;
 #pragma unroll
         for (int u = 0; u < kCombineParts; ++u) {
-            const float by = ml[u].x > -INFINITY ? exp2f(ml[u].x - top) : 0.f;
+            const float by = ml[u].x > -INFINITY ? exp2f(ml[u].x - now) : 0.f;
             l += ml[u].y * by;
 #pragma unroll
-            for (int i = 0; i < E; ++i) o[i] += v[u][i] * by;
+            for (int i = 0; i < E; ++i) o[i] += b + u * kCombineWarps <= last ? v[u][i] * by : 0.f;
         }
     }
-    if (lane == 0) sums[warp] = l;
+    if (lane == 0) {
+        tops[warp] = top;
+        sums[warp] = l;
+    }
 #pragma unroll
     for (int i = 0; i < E; ++i) values[warp][lane + 32 * i] = o[i];
     __syncthreads();
-    l = 0.f;
+    if (warp >= E) return;
+    const bool there = lane < kCombineWarps;
+    const float m = there ? tops[lane % kCombineWarps] : -INFINITY, high = warp_max(m), by = m > -INFINITY ? exp2f(m - high) : 0.f;
+    const float total = warp_sum(there ? sums[lane % kCombineWarps] * by : 0.f), inv = total > 0.f ? 1.f / total : 0.f;
+    float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kCombineWarps; ++w) l += sums[w];
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int q = cut.part * COLS + c;
-    T* out = reinterpret_cast<T*>(a.out) + ((int64_t)(cut.row + q / a.group) * a.n_heads + cut.head * a.group + q % a.group) * D;
-    for (int i = threadIdx.x; i < D; i += kCombineWarps * 32) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kCombineWarps; ++w) v += values[w][i];
-        out[i] = from_f32<T>(v * inv);
-    }
+    for (int w = 0; w < kCombineWarps; ++w) v += values[w][32 * warp + lane] * __shfl_sync(0xffffffffu, by, w);
+    const int q = cut.part * COLS + c, token = quotient(q, a.per_group);
+    reinterpret_cast<T*>(a.out)[((int64_t)(cut.row + token) * a.n_heads + cut.head * a.group + q - token * a.group) * D + 32 * warp + lane] = from_f32<T>(v * inv);
 }
 
 template <typename T, int D, int NT, int TERMS>
 int attend(const AttendArgs& a, cudaStream_t stream) {
     static bool done[kMaxDevices];
     constexpr int bytes = (int)sizeof(Smem<D, NT, TERMS>);
+    static_assert(bytes <= 227 * 1024, "a block's shared memory");
     const int status = ensure_dynamic_smem(kv4_attention_kernel<T, D, NT, TERMS>, bytes, done);
     if (status != CPM_OK) return status;
     const int sms = device_sms();
@@ -831,10 +863,10 @@ CPM_API int cpm_kv4_attention(const void* q, const void* records, void* out, con
                               int max_pages, const int* cu_q, const int* tile_seq, const int* tile_row, int n_tiles, float* scratch, int n_heads,
                               int n_kv, int d, int window, float scale, int dtype, cudaStream_t stream) {
     if (n_tiles <= 0) return CPM_OK;
-    if (n_tiles > kMostTiles || n_heads < 1 || n_kv < 1 || n_heads % n_kv || window < 0) return CPM_BAD_ARGUMENT;
+    if (n_tiles > kMostTiles || n_heads < 1 || n_heads > 8192 || n_kv < 1 || n_heads % n_kv || window < 0) return CPM_BAD_ARGUMENT;
     if ((cu_q == nullptr) != (tile_seq == nullptr) || (cu_q == nullptr) != (tile_row == nullptr)) return CPM_BAD_ARGUMENT;
     if (((uintptr_t)records | (uintptr_t)q | (uintptr_t)out) & 15) return CPM_BAD_ARGUMENT;
     const AttendArgs a{q, out, (const uint8_t*)records, kv_len, slots, page_table, cu_q, tile_seq, tile_row, scratch, max_pages, n_tiles, n_heads, n_kv,
-                       n_heads / n_kv, window, scale};
+                       n_heads / n_kv, window, scale, (float)n_kv / (float)n_heads, 1.f / (float)n_kv};
     return dtype == CPM_BF16 ? by_head_size<bf16, 1>(a, d, stream) : by_head_size<float, 2>(a, d, stream);
 }
