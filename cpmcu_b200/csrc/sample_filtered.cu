@@ -27,8 +27,10 @@ constexpr int kFilterThreads = 512;
 constexpr int kFilterWarps = kFilterThreads / 32;
 constexpr int kMostBlocks = 8;                         // of a cluster
 constexpr int kOctaveBits = 18;                        // bits of a weight below those that number its bin
-constexpr int kCoarseBins = 4096;                      // bins 0 .. 4064, the largest weight being 1
+constexpr int kCoarseBins = 1536;                      // 48 octaves down from 1; what is smaller (less than 2^-40 has no mass) lies in bin 0
+constexpr int kFirstBin = (0x3f800000 >> kOctaveBits) + 1 - kCoarseBins;
 constexpr int kOwnBins = kCoarseBins / kFilterThreads;
+constexpr uint32_t kWhole = 110u << 23;                // bits of 2^-17: from here up a weight times 2^40 is a whole number as it is
 constexpr int kFineBins = 1024;                        // of a step of the selection
 constexpr int kListed = 2048;                          // tokens that are set apart for the selection
 constexpr int kAlone = 512;                            // up to so many the first block goes on without the others
@@ -50,16 +52,25 @@ struct FilterArgs {
 struct Plan {
     uint32_t low, high;                                // bits of the weights to set apart
     int complete;                                      // all from ``low`` up are
+    int known;                                         // whether the mass above ``high`` is
     int apart;                                         // whether they are few enough, else their masses go into bins
     uint32_t border;                                   // tokens above it stay, and the first ``ties`` of the ``equal`` ones at it
     uint64_t ties, equal;
 };
 
 struct FilterShared {
-    alignas(16) uint32_t coarse[kCoarseBins];
-    alignas(16) uint32_t fine[3][kFineBins];
-    uint32_t list[kListed];                            // bits of the weights that are set apart, in the first block
-    int place[kListed];                                // and their tokens
+    alignas(16) uint32_t coarse[kCoarseBins];          // tokens of the row in each bin (in the first block)
+    union {
+        alignas(16) uint32_t fine[3][kFineBins];
+        uint32_t low[2][kCoarseBins];                  // before that: the sums of their weights' bits below the bin's number, by 16 bits
+    };
+    union {
+        struct {
+            uint32_t list[kListed];                    // bits of the weights that are set apart, in the first block
+            int place[kListed];                        // and their tokens
+        };
+        uint32_t own[2][kCoarseBins];                  // before that: the block's bins, see count_own
+    };
     int listed;
     uint64_t warp_sum[kFilterWarps + 1];
     uint64_t found_before, found_here;                 // what lies above the bin that was found, and in it
@@ -107,6 +118,51 @@ __device__ __forceinline__ uint32_t add32(const void* own, uint32_t rank, uint32
 // floor(w 2^40) of a weight (0 to 1) by its bits: 24 bits of significand, shifted.
 __device__ __forceinline__ uint64_t units_of(uint32_t bits) {
     return ((uint64_t)((bits & 0x7fffffu) | 0x800000u) << 17) >> min(63u, 127u - (bits >> 23));
+}
+
+// Of a weight below 2^-17.
+__device__ __forceinline__ uint32_t small_units_of(uint32_t bits) {
+    return bits < kWhole ? ((bits & 0x7fffffu) | 0x800000u) >> min(31u, 110u - (bits >> 23)) : 0u;
+}
+__device__ __forceinline__ int bin_of(uint32_t bits) { return max(0, (int)(bits >> kOctaveBits) - kFirstBin); }
+__device__ __forceinline__ uint32_t bin_begin(int bin) { return bin > 0 ? (uint32_t)(bin + kFirstBin) << kOctaveBits : 0u; }
+
+// A block's bins: own[1] holds the number of tokens, 15 bits, above the sum of the upper 2 of the 18 bits below a bin's number, own[0] the sum of all 18
+// modulo 2^32; with less than 2^15 tokens the one tells how often the other has run over.  Without staged weights: the number alone.
+constexpr int kCountBits = 17;
+template <bool STAGED>
+__device__ __forceinline__ void count_own(FilterShared& sm, uint32_t bits, bool masses) {
+    const int bin = bin_of(bits);
+    if constexpr (STAGED) {
+        atomicAdd(&sm.own[1][bin], 1u << kCountBits | (bits >> (kOctaveBits - 2) & 3u));
+        if (masses) atomicAdd(&sm.own[0][bin], bits & ((1u << kOctaveBits) - 1));
+    } else {
+        atomicAdd(&sm.own[1][bin], 1u);
+    }
+}
+// Adds them to the row's, in the first block.
+template <bool STAGED>
+__device__ __forceinline__ void add_own(FilterShared& sm, bool masses) {
+#pragma unroll 1
+    for (int bin = threadIdx.x; bin < kCoarseBins; bin += kFilterThreads) {
+        const uint32_t packed = sm.own[1][bin];
+        if (!packed) continue;
+        add32(&sm.coarse[bin], 0, STAGED ? packed >> kCountBits : packed);
+        if (STAGED && masses) {
+            const uint64_t least = (uint64_t)(packed & ((1u << kCountBits) - 1)) << (kOctaveBits - 2);
+            const uint64_t sum = least + (uint32_t)(sm.own[0][bin] - (uint32_t)least);
+            add32(&sm.low[0][bin], 0, (uint32_t)sum & 0xffffu);
+            add32(&sm.low[1][bin], 0, (uint32_t)(sum >> 16));
+        }
+    }
+}
+// The mass of a bin: exact where its weights' bits have been summed and it lies above 2^-17, else a bound from above or below.
+__device__ __forceinline__ uint64_t bin_mass(const FilterShared& sm, int bin, bool summed, bool upper) {
+    if (bin == 0) return 0;
+    const uint64_t n = sm.coarse[bin], low = summed ? sm.low[0][bin] + ((uint64_t)sm.low[1][bin] << 16) : upper ? n * ((1u << kOctaveBits) - 1) : 0;
+    const uint32_t begin = bin_begin(bin);
+    const uint64_t v = (n * ((begin & 0x7fffffu) | 0x800000u) + low) << 17 >> (127u - (begin >> 23));
+    return upper || begin >= kWhole ? v : v - min(v, n);
 }
 
 // Inclusive sums over the block's threads in order; the block's total is left in the last of ``sums``.
@@ -230,18 +286,18 @@ __device__ __noinline__ Border select(FilterShared& sm, bool mass, int listed, d
     return Border{low + prefix, above, sm.found_here};
 }
 
-// The first bin, from the largest weights down, at whose end the running sum of count times ``each(bin)`` reaches ``need``; ``otherwise`` where none does.
+// The first bin, from the largest weights down, at whose end the running sum of ``each(bin)`` reaches ``need``, and the sum before it; left alone where none does.
 template <typename Each>
 __device__ __forceinline__ void find_bin(FilterShared& sm, Each each, double need, int* bin, uint64_t* before) {
     const int top_bin = kCoarseBins - 1 - kOwnBins * threadIdx.x;
     uint64_t sum = 0;
 #pragma unroll 1
-    for (int q = 0; q < kOwnBins; ++q) sum += (uint64_t)sm.coarse[top_bin - q] * each(top_bin - q);
+    for (int q = 0; q < kOwnBins; ++q) sum += each(top_bin - q);
     uint64_t upto = block_scan64(sum, sm.warp_sum) - sum;
     if ((double)upto < need && (double)(upto + sum) >= need)
 #pragma unroll 1
         for (int q = 0; q < kOwnBins; ++q) {
-            const uint64_t here = (uint64_t)sm.coarse[top_bin - q] * each(top_bin - q);
+            const uint64_t here = each(top_bin - q);
             if ((double)upto < need && (double)(upto + here) >= need) {
                 *bin = top_bin - q;
                 *before = upto;
@@ -302,21 +358,21 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
             const int i = i0 + 4 * q * kFilterThreads;
             if (i >= whole) break;
             if constexpr (STAGED) *reinterpret_cast<float4*>(weights + i) = v[q];
-            best = better(best, ArgMax{v[q].x, first + i});
-            best = better(best, ArgMax{v[q].y, first + i + 1});
-            best = better(best, ArgMax{v[q].z, first + i + 2});
-            best = better(best, ArgMax{v[q].w, first + i + 3});
+            if (v[q].x > best.v) best = ArgMax{v[q].x, first + i};       // (a thread's tokens come by index)
+            if (v[q].y > best.v) best = ArgMax{v[q].y, first + i + 1};
+            if (v[q].z > best.v) best = ArgMax{v[q].z, first + i + 2};
+            if (v[q].w > best.v) best = ArgMax{v[q].w, first + i + 3};
         }
     }
 #pragma unroll 1
     for (int i = whole + tid; i < row.n; i += kFilterThreads) {
         const float v = row.z[i];
         if constexpr (STAGED) weights[i] = v;
-        best = better(best, ArgMax{v, first + i});
+        if (v > best.v) best = ArgMax{v, first + i};
     }
     if (by_count || by_mass)
 #pragma unroll 1
-        for (int i = tid; i < kCoarseBins; i += kFilterThreads) sm.coarse[i] = 0;
+        for (int i = tid; i < kCoarseBins; i += kFilterThreads) sm.coarse[i] = sm.low[0][i] = sm.low[1][i] = sm.own[0][i] = sm.own[1][i] = 0;
     if (tid == 0) sm.listed = 0;
     best = block_argmax(best, sm.scratch);
     asm volatile("barrier.cluster.wait;" ::: "memory");
@@ -339,15 +395,19 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     // weights, their histogram, and (where mass alone decides) their mass.  A thread's tokens are neighbours, an odd number of them, so that sums by
     // thread go by index and a warp's accesses to shared memory are in different banks
     const int strip = (row.n + kFilterThreads - 1) / kFilterThreads | 1, i0 = min(row.n, tid * strip), i1 = min(row.n, i0 + strip);
-    uint64_t own_mass = 0;
+    const bool summed = STAGED && by_mass && !by_count;        // whether the bins' masses are
+    uint64_t own_mass = 0;                                     // of the thread's tokens that bins do not tell exactly
     if (by_count || by_mass) {
-#pragma unroll 2
+        uint32_t small = 0;
+#pragma unroll 4
         for (int i = i0; i < i1; ++i) {
             const float w = STAGED ? row.form(weights[i]) : row.at(i);
             if constexpr (STAGED) weights[i] = w;
-            atomicAdd(&sm.coarse[__float_as_uint(w) >> kOctaveBits], 1u);
-            if (!by_count) own_mass += units_of(__float_as_uint(w));
+            count_own<STAGED>(sm, __float_as_uint(w), summed);
+            if (summed) small += small_units_of(__float_as_uint(w));
+            else if (!STAGED && !by_count) own_mass += units_of(__float_as_uint(w));
         }
+        own_mass += small;
     } else if constexpr (STAGED) {
 #pragma unroll 2
         for (int i = i0; i < i1; ++i) weights[i] = row.form(weights[i]);
@@ -368,12 +428,16 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     uint64_t ties = ~0ull, equal = 0;
     if (by_count || by_mass) {
         if (by_mass && !by_count) put_mass(own_mass);
-        if (rank > 0)
-#pragma unroll 1
-            for (int i = tid; i < kCoarseBins; i += kFilterThreads)
-                if (sm.coarse[i]) add32(&sm.coarse[i], 0, sm.coarse[i]);
+        add_own<STAGED>(sm, summed);
         cluster_sync();
-        uint64_t within = by_mass && !by_count ? all_mass() : 0;      // mass of the tokens that top-k leaves
+        uint64_t within = by_mass && !by_count ? all_mass() : 0;      // mass of the tokens that top-k leaves (known to the first block alone, unless by_count)
+        if (summed && rank == 0) {
+            uint64_t sum = 0;
+#pragma unroll 1
+            for (int bin = tid; bin < kCoarseBins; bin += kFilterThreads)
+                if (bin_begin(bin) >= kWhole) sum += bin_mass(sm, bin, true, true);
+            within += block_sum64(sum, sm);
+        }
 #pragma unroll 1
         for (int round = by_count ? 0 : 1; round < (by_mass ? 2 : 1); ++round) {
             // ---- which weights the border may be among ----
@@ -381,35 +445,39 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
             uint64_t above = 0;                                // what lies above them (known to the first block alone)
             uint64_t some = 0;                                 // no fewer tokens than they are (likewise)
             uint32_t low = 0, high = 0, complete = 0;
+            bool known = round == 0;                           // whether ``above`` is
             if (rank == 0) {
                 if (round == 0) {
-                    find_bin(sm, [](int) { return (uint64_t)1; }, need, &sm.found_bin, &sm.found_before);
+                    find_bin(sm, [&](int bin) { return (uint64_t)sm.coarse[bin]; }, need, &sm.found_bin, &sm.found_before);
                     above = sm.found_before;
-                    low = (uint32_t)sm.found_bin << kOctaveBits;
+                    low = bin_begin(sm.found_bin);
                     some = sm.coarse[sm.found_bin];
                     complete = above + some <= kListed;
-                    high = complete ? 0x3f800001u : low + (1u << kOctaveBits);
+                    high = complete ? 0x3f800001u : bin_begin(sm.found_bin + 1);
                 } else {
-                    // from where the masses reach ``need`` if every weight were its bin's upper end, to where they do with the lower ends
-                    const int last = border >> kOctaveBits;
+                    // from where the masses reach ``need`` by their bounds from above, to where they do by those from below
+                    const int last = bin_of(border);
                     if (tid == 0) {
                         sm.high_bin = kCoarseBins - 1;
                         sm.low_bin = last;
                     }
                     __syncthreads();
-                    find_bin(sm, [](int bin) { return units_of((uint32_t)(bin + 1) << kOctaveBits); }, need, &sm.high_bin, &sm.found_before);
-                    find_bin(sm, [](int bin) { return units_of((uint32_t)bin << kOctaveBits); }, need, &sm.low_bin, &sm.found_before);
-                    const uint32_t low_bin = max(sm.low_bin, last), high_bin = max((uint32_t)sm.high_bin, low_bin);
-                    low = max(border, low_bin << kOctaveBits);
-                    high = (high_bin + 1) << kOctaveBits;
+                    find_bin(sm, [&](int bin) { return bin_mass(sm, bin, summed, true); }, need, &sm.high_bin, &sm.found_before);
+                    find_bin(sm, [&](int bin) { return bin_mass(sm, bin, summed, false); }, need, &sm.low_bin, &sm.found_before);
+                    const int low_bin = max(sm.low_bin, last), high_bin = max(sm.high_bin, low_bin);
+                    low = max(border, bin_begin(low_bin));
+                    high = bin_begin(high_bin + 1);
+                    if (summed && bin_begin(low_bin) >= kWhole) {      // exact so far
+                        above = sm.found_before;
+                        known = true;
+                    }
                     uint64_t count = 0;
-                    for (uint32_t bin = low_bin + tid; bin <= high_bin; bin += kFilterThreads) count += sm.coarse[bin];
+                    for (int bin = low_bin + tid; bin <= high_bin; bin += kFilterThreads) count += sm.coarse[bin];
                     some = block_sum64(count, sm);
                 }
             }
             Border b{};
             int listed = 0;
-            bool known = round == 0;                           // whether ``above`` is
 #pragma unroll 1
             while (true) {
                 if (rank == 0) {
@@ -418,6 +486,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                         sm.plan.low = low;
                         sm.plan.high = high;
                         sm.plan.complete = complete;
+                        sm.plan.known = known;
                         sm.plan.apart = some <= kListed;
                         sm.listed = 0;
                     }
@@ -426,6 +495,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 low = peer32(&sm.plan.low, 0);
                 high = peer32(&sm.plan.high, 0);
                 complete = peer32(&sm.plan.complete, 0);
+                known = peer32(&sm.plan.known, 0);
                 const bool apart = peer32(&sm.plan.apart, 0);
                 const int range = bits_of_range(low, high), shift = max(0, range - 10);
                 uint64_t over = 0;
@@ -434,8 +504,9 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
 #pragma unroll 2
                 for (int i = i0; i < i1; ++i) {
                     const uint32_t bits = __float_as_uint(row.at(i));
-                    if (bits >= high) over += units_of(bits);
-                    else if (bits >= low) {
+                    if (bits >= high) {
+                        if (!known) over += units_of(bits);
+                    } else if (bits >= low) {
                         ++hits;
                         if (!apart) add_fine(sm, round > 0, (bits - low) >> shift, bits);
                     }
@@ -641,6 +712,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
 }
 
 constexpr int kMostStaged = (113 * 1024 - (int)sizeof(FilterShared) - 1024) / 4;      // weights that a block's half of the shared memory holds
+static_assert(kMostStaged < 1 << (32 - kCountBits), "a block's tokens in a packed count");
 
 }  // namespace
 
