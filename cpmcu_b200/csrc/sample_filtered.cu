@@ -12,12 +12,14 @@
 // token whatever the launch.  (With fp32 sums the border between two of 70,000 tokens moves by more than their distance.)
 //
 // A row is read once.  Its weights lie in the shared memory of a cluster of blocks (one to eight; the fewer rows, the more blocks a row).  One
-// histogram of the weights' upper bits (32 bins to an octave) says in which bin the k-th weight lies, and, since a bin's weights differ by 1/32 at
-// most, in which few bins the mass is reached.  The tokens in these bins, a few hundred, go to the cluster's first block, which finds the border by
-// radix selection with exact masses; where no more than kAlone tokens are above the border of top-k, all of them go there and it draws as well.
+// histogram of the weights' upper bits (32 bins to an octave) holds each bin's number of tokens and, where mass decides, the sum of their lower bits: so the
+// bin in which the k-th token lies, or at which the mass is reached, is known exactly.  The tokens in that bin, a few hundred, go to the cluster's first
+// block, which finds the border by radix selection; where no more than kRanked tokens are in or above the bin of top-k, all of them go there, each is
+// compared with each, and it draws as well.  In the same pass a thread sums what it keeps above the bin, so that the draw looks at few tokens again.
 // (A cluster's barrier takes about 2 us, and a look into a neighbour's shared memory half of that: a selection over the whole row with
-// all blocks' histograms added up at every step took 41 us for one row of 73,448.)
-// What a row cannot do without is its logits, 4 bytes a token.
+// all blocks' histograms added up at every step took 41 us for one row of 73,448, bins of counts alone 25, and this 15.)
+// 64 rows of 73,448 with settings of their own 38 us, 512 rows of 32,000 by mass alone 116.  What a row cannot do without is its logits, 4 bytes a token
+// (10 us of the 116); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
 #include "common.cuh"
 #include "philox.cuh"
 
@@ -33,7 +35,7 @@ constexpr int kOwnBins = kCoarseBins / kFilterThreads;
 constexpr uint32_t kWhole = 110u << 23;                // bits of 2^-17: from here up a weight times 2^40 is a whole number as it is
 constexpr int kFineBins = 1024;                        // of a step of the selection
 constexpr int kListed = 2048;                          // tokens that are set apart for the selection
-constexpr int kAlone = 512;                            // up to so many the first block goes on without the others
+constexpr int kRanked = 256;                           // up to so many the first block compares each with each, and draws without the others
 constexpr int kLimbBits = 14;                          // a mass is added in three limbs: 32-bit adds in shared memory are one instruction
 constexpr int kMostVocab = 1 << 21;                    // so that a limb's sum over a block's tokens stays within 32 bits
 
@@ -72,7 +74,7 @@ struct FilterShared {
         uint32_t own[2][kCoarseBins];                  // before that: the block's bins, see count_own
     };
     int listed;
-    uint64_t warp_sum[kFilterWarps + 1];
+    uint64_t warp_sum[kFilterWarps + 1], warp_sums[3][kFilterWarps + 1];
     uint64_t found_before, found_here;                 // what lies above the bin that was found, and in it
     int found_bin, low_bin, high_bin, cut;
     alignas(8) ArgMax best[kMostBlocks];                          // of the cluster's blocks, which write here
@@ -191,6 +193,37 @@ __device__ __noinline__ uint64_t block_scan64(uint64_t v, uint64_t* sums) {
     __syncthreads();
     return v + sums[warp];
 }
+// The same of three numbers at once.
+__device__ __forceinline__ void block_scan64(uint64_t (&v)[3], uint64_t (*sums)[kFilterWarps + 1]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            const uint64_t x = __shfl_up_sync(0xffffffffu, v[n], o);
+            if (lane >= o) v[n] += x;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 3; ++n)
+        if (lane == 31) sums[n][warp] = v[n];
+    __syncthreads();
+    if (warp < 3) {
+        const uint64_t own = lane < kFilterWarps ? sums[warp][lane] : 0;
+        uint64_t x = own;
+#pragma unroll
+        for (int o = 1; o < kFilterWarps; o <<= 1) {
+            const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncwarp();
+        if (lane < kFilterWarps) sums[warp][lane] = x - own;
+        if (lane == kFilterWarps - 1) sums[warp][kFilterWarps] = x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 3; ++n) v[n] += sums[n][warp];
+}
 __device__ __forceinline__ uint64_t block_sum64(uint64_t v, FilterShared& sm) {
     block_scan64(v, sm.warp_sum);
     return sm.warp_sum[kFilterWarps];
@@ -286,25 +319,60 @@ __device__ __noinline__ Border select(FilterShared& sm, bool mass, int listed, d
     return Border{low + prefix, above, sm.found_here};
 }
 
-// The first bin, from the largest weights down, at whose end the running sum of ``each(bin)`` reaches ``need``, and the sum before it; left alone where none does.
-template <typename Each>
-__device__ __forceinline__ void find_bin(FilterShared& sm, Each each, double need, int* bin, uint64_t* before) {
+// The bin, from the largest weights down, at whose end the number of tokens reaches ``need``: left in sm.found_bin, with the number before it.
+__device__ __forceinline__ void find_count(FilterShared& sm, double need) {
     const int top_bin = kCoarseBins - 1 - kOwnBins * threadIdx.x;
-    uint64_t sum = 0;
-#pragma unroll 1
-    for (int q = 0; q < kOwnBins; ++q) sum += each(top_bin - q);
+    uint64_t here[kOwnBins], sum = 0;
+#pragma unroll
+    for (int q = 0; q < kOwnBins; ++q) sum += here[q] = sm.coarse[top_bin - q];
     uint64_t upto = block_scan64(sum, sm.warp_sum) - sum;
-    if ((double)upto < need && (double)(upto + sum) >= need)
-#pragma unroll 1
-        for (int q = 0; q < kOwnBins; ++q) {
-            const uint64_t here = each(top_bin - q);
-            if ((double)upto < need && (double)(upto + here) >= need) {
-                *bin = top_bin - q;
-                *before = upto;
-            }
-            upto += here;
+#pragma unroll
+    for (int q = 0; q < kOwnBins; ++q) {
+        if ((double)upto < need && (double)(upto + here[q]) >= need) {
+            sm.found_bin = top_bin - q;
+            sm.found_before = upto;
         }
+        upto += here[q];
+    }
     __syncthreads();
+}
+// The bins at whose ends the masses reach ``p`` times all, by their bounds from above (sm.high_bin) and from below (sm.low_bin, with what lies before it in
+// sm.found_before): no bin between them can be ruled out.  ``within``: all, or, where the bins' masses are summed, what they do not tell exactly; returned is all.
+__device__ __forceinline__ uint64_t find_mass(FilterShared& sm, bool summed, float p, uint64_t within, int last) {
+    const int top_bin = kCoarseBins - 1 - kOwnBins * threadIdx.x;
+    uint64_t here[2][kOwnBins], v[3] = {0, 0, 0}, sum[2];
+#pragma unroll
+    for (int q = 0; q < kOwnBins; ++q) {
+        v[0] += here[0][q] = bin_mass(sm, top_bin - q, summed, true);
+        v[1] += here[1][q] = bin_mass(sm, top_bin - q, summed, false);
+        if (summed && bin_begin(top_bin - q) >= kWhole) v[2] += here[1][q];
+    }
+    sum[0] = v[0];
+    sum[1] = v[1];
+    if (threadIdx.x == 0) {
+        sm.high_bin = kCoarseBins - 1;
+        sm.low_bin = last;
+    }
+    block_scan64(v, sm.warp_sums);
+    within += sm.warp_sums[2][kFilterWarps];
+    const double need = (double)p * (double)within;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        uint64_t upto = v[n] - sum[n];
+#pragma unroll
+        for (int q = 0; q < kOwnBins; ++q) {
+            if ((double)upto < need && (double)(upto + here[n][q]) >= need) {
+                if (n == 0) sm.high_bin = top_bin - q;
+                else {
+                    sm.low_bin = top_bin - q;
+                    sm.found_before = upto;
+                }
+            }
+            upto += here[n][q];
+        }
+    }
+    __syncthreads();
+    return within;
 }
 
 // Of the tokens at a border that mass decides, how many it takes.
@@ -426,29 +494,34 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
 
     uint32_t border = 0;
     uint64_t ties = ~0ull, equal = 0;
+    // of the thread's tokens, those that were set apart (the last one in the lowest bit), and the mass above them; ``sure``: these two tell what it keeps
+    uint64_t found = 0, sure_mass = 0;
+    bool sure = false;
+    const auto each_found = [&](auto&& visit) {
+#pragma unroll 1
+        for (uint64_t left = found; left;) {
+            const int bit = 63 - __clzll(left);
+            left &= ~(1ull << bit);
+            visit(i1 - 1 - bit);
+        }
+    };
     if (by_count || by_mass) {
         if (by_mass && !by_count) put_mass(own_mass);
         add_own<STAGED>(sm, summed);
         cluster_sync();
         uint64_t within = by_mass && !by_count ? all_mass() : 0;      // mass of the tokens that top-k leaves (known to the first block alone, unless by_count)
-        if (summed && rank == 0) {
-            uint64_t sum = 0;
-#pragma unroll 1
-            for (int bin = tid; bin < kCoarseBins; bin += kFilterThreads)
-                if (bin_begin(bin) >= kWhole) sum += bin_mass(sm, bin, true, true);
-            within += block_sum64(sum, sm);
-        }
 #pragma unroll 1
         for (int round = by_count ? 0 : 1; round < (by_mass ? 2 : 1); ++round) {
             // ---- which weights the border may be among ----
-            const double need = round == 0 ? (double)k : (double)p * (double)within;
+            double need = (double)k;
+            const bool last_round = round == (by_mass ? 1 : 0);
             uint64_t above = 0;                                // what lies above them (known to the first block alone)
             uint64_t some = 0;                                 // no fewer tokens than they are (likewise)
             uint32_t low = 0, high = 0, complete = 0;
             bool known = round == 0;                           // whether ``above`` is
             if (rank == 0) {
                 if (round == 0) {
-                    find_bin(sm, [&](int bin) { return (uint64_t)sm.coarse[bin]; }, need, &sm.found_bin, &sm.found_before);
+                    find_count(sm, need);
                     above = sm.found_before;
                     low = bin_begin(sm.found_bin);
                     some = sm.coarse[sm.found_bin];
@@ -457,13 +530,8 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 } else {
                     // from where the masses reach ``need`` by their bounds from above, to where they do by those from below
                     const int last = bin_of(border);
-                    if (tid == 0) {
-                        sm.high_bin = kCoarseBins - 1;
-                        sm.low_bin = last;
-                    }
-                    __syncthreads();
-                    find_bin(sm, [&](int bin) { return bin_mass(sm, bin, summed, true); }, need, &sm.high_bin, &sm.found_before);
-                    find_bin(sm, [&](int bin) { return bin_mass(sm, bin, summed, false); }, need, &sm.low_bin, &sm.found_before);
+                    within = find_mass(sm, summed, p, within, last);
+                    need = (double)p * (double)within;
                     const int low_bin = max(sm.low_bin, last), high_bin = max(sm.high_bin, low_bin);
                     low = max(border, bin_begin(low_bin));
                     high = bin_begin(high_bin + 1);
@@ -471,9 +539,12 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                         above = sm.found_before;
                         known = true;
                     }
-                    uint64_t count = 0;
-                    for (int bin = low_bin + tid; bin <= high_bin; bin += kFilterThreads) count += sm.coarse[bin];
-                    some = block_sum64(count, sm);
+                    some = sm.coarse[low_bin];
+                    if (low_bin < high_bin) {
+                        uint64_t count = 0;
+                        for (int bin = low_bin + tid; bin <= high_bin; bin += kFilterThreads) count += sm.coarse[bin];
+                        some = block_sum64(count, sm);
+                    }
                 }
             }
             Border b{};
@@ -481,7 +552,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
 #pragma unroll 1
             while (true) {
                 if (rank == 0) {
-                    clear_fine(sm);
+                    if (some > kListed) clear_fine(sm);
                     if (tid == 0) {
                         sm.plan.low = low;
                         sm.plan.high = high;
@@ -501,16 +572,20 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 uint64_t over = 0;
                 int hits = 0;
                 if (!apart && rank > 0) clear_fine(sm);
-#pragma unroll 2
+                sure = STAGED && apart && (last_round || complete) && __float_as_uint(ratio) <= high;
+                found = 0;
+                const bool weigh = !known || sure;
+#pragma unroll 4
                 for (int i = i0; i < i1; ++i) {
                     const uint32_t bits = __float_as_uint(row.at(i));
-                    if (bits >= high) {
-                        if (!known) over += units_of(bits);
-                    } else if (bits >= low) {
-                        ++hits;
-                        if (!apart) add_fine(sm, round > 0, (bits - low) >> shift, bits);
-                    }
+                    const bool hit = bits - low < high - low;
+                    if (STAGED) found = found << 1 | hit;
+                    else hits += hit;
+                    if (hit && !apart) add_fine(sm, round > 0, (bits - low) >> shift, bits);
+                    if (weigh && bits >= high) over += units_of(bits);
                 }
+                if (STAGED) hits = __popcll(found);
+                sure_mass = over;
                 if (!known) put_mass(over);
                 if (apart) {
                     // ---- the tokens themselves to the first block: a warp asks for room once, and then goes through its tokens again ----
@@ -525,16 +600,23 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                             if (lane >= o) before += x;
                         }
                         at += before - hits;
+                        const auto put = [&](int i, uint32_t bits) {
+                            if (at < kListed) {
+                                put32(&sm.list[at], 0, bits);
+                                put32(&sm.place[at], 0, first + i);
+                            }
+                            ++at;
+                        };
+                        if constexpr (STAGED) {
+                            each_found([&](int i) { put(i, __float_as_uint(weights[i])); });
+                        } else {
 #pragma unroll 1
-                        for (int i = i0; i < i1 && hits > 0; ++i) {
-                            const uint32_t bits = __float_as_uint(row.at(i));
-                            if (bits >= low && bits < high) {
-                                if (at < kListed) {
-                                    put32(&sm.list[at], 0, bits);
-                                    put32(&sm.place[at], 0, first + i);
+                            for (int i = i0; i < i1 && hits > 0; ++i) {
+                                const uint32_t bits = __float_as_uint(row.at(i));
+                                if (bits - low < high - low) {
+                                    put(i, bits);
+                                    --hits;
                                 }
-                                ++at;
-                                --hits;
                             }
                         }
                     }
@@ -549,7 +631,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 known = true;
                 if (apart) {
                     listed = (int)peer32(&sm.listed, 0);
-                    if (rank == 0) b = select(sm, round > 0, listed, need, complete ? 0 : above, low, high);
+                    if (rank == 0 && !(complete && listed <= kRanked)) b = select(sm, round > 0, listed, need, complete ? 0 : above, low, high);
                     break;
                 }
                 // ---- too many for the list (equal weights, or a mass that flat tails make up): their masses in 1,024 bins, and on with one of these ----
@@ -567,7 +649,54 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 cluster_sync();                                // (read before the next plan is made)
             }
             if (complete) {
-                // ---- all that top-k leaves is here: the first block goes on alone ----
+                // ---- all that top-k leaves is here ----
+                if (listed <= kRanked) {
+                    // The first block goes on alone.  Some threads to a token: how many stand before it, and what mass?
+                    if (rank > 0) return;
+                    int bits_of_tokens = 5;
+                    while ((1 << bits_of_tokens) < listed) ++bits_of_tokens;
+                    const int share = kFilterThreads >> bits_of_tokens, own = tid / share, part = tid % share;
+                    uint64_t* masses = reinterpret_cast<uint64_t*>(sm.fine[0]);
+                    if (tid < listed) masses[tid] = units_of(sm.list[tid]);
+                    __syncthreads();
+                    const bool there = own < listed;
+                    const uint32_t bits = there ? sm.list[own] : 0;
+                    const int place = there ? sm.place[own] : 0;
+                    const uint64_t mass = there ? masses[own] : 0;
+                    int count = 0;
+                    uint64_t before = 0;
+#pragma unroll 4
+                    for (int i = part; i < listed; i += share) {
+                        const uint32_t other = sm.list[i];
+                        const bool ahead = other > bits || (other == bits && sm.place[i] < place);
+                        count += ahead;
+                        before += ahead ? masses[i] : 0;
+                    }
+                    for (int o = 1; o < share; o <<= 1) {
+                        count += __shfl_xor_sync(0xffffffffu, count, o);
+                        before += __shfl_xor_sync(0xffffffffu, before, o);
+                    }
+                    bool stays = there && count < k;
+                    if (by_mass) {
+                        within = block_sum64(stays && part == 0 ? mass : 0, sm);
+                        stays = stays && (double)before < (double)p * (double)within;
+                    }
+                    stays = stays && __uint_as_float(bits) >= ratio;
+                    const uint64_t total = block_sum64(stays && part == 0 ? mass : 0, sm);
+                    if (there && part == 0) masses[own] = stays ? mass : 0;
+                    __syncthreads();
+                    before = 0;
+#pragma unroll 4
+                    for (int i = part; i < listed; i += share) before += sm.place[i] < place ? masses[i] : 0;
+                    for (int o = 1; o < share; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+                    const uint64_t target = min((uint64_t)((double)u * (double)total), total - 1);
+                    if (stays && part == 0 && target >= before && target < before + mass) {
+                        a.token[r] = place;
+                        a.logprob[r] = (row.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(a.logits[(int64_t)r * a.ld + place], row.top), t))
+                                     - logf((float)((double)total * (1.0 / 1099511627776.0)));
+                    }
+                    return;
+                }
                 if (rank == 0) {
                     border = b.bits;
                     ties = (uint64_t)k - b.above;
@@ -587,36 +716,6 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                         ties = n;
                         equal = there;
                     }
-                }
-                if (listed <= kAlone) {
-                    if (rank > 0) return;
-                    // a thread's token: does it stay, and what is kept in front of it?
-                    const uint32_t bits = tid < listed ? sm.list[tid] : 0;
-                    const int place = tid < listed ? sm.place[tid] : 0;
-                    bool stays = tid < listed && bits >= border && __uint_as_float(bits) >= ratio;
-                    if (stays && bits == border && ties < equal) {
-                        uint64_t before = 0;
-#pragma unroll 1
-                        for (int i = 0; i < listed; ++i) before += sm.list[i] == border && sm.place[i] < place;
-                        stays = before < ties;
-                    }
-                    const uint64_t mine = stays ? units_of(bits) : 0;
-                    const uint64_t total = block_sum64(mine, sm);
-                    __syncthreads();
-                    uint64_t* kept = reinterpret_cast<uint64_t*>(sm.fine[0]);
-                    if (tid < listed) kept[tid] = mine;
-                    __syncthreads();
-                    if (!stays) return;
-                    uint64_t before = 0;
-#pragma unroll 4
-                    for (int i = 0; i < listed; ++i) before += sm.place[i] < place ? kept[i] : 0;
-                    const uint64_t target = min((uint64_t)((double)u * (double)total), total - 1);
-                    if (target >= before && target < before + mine) {
-                        a.token[r] = place;
-                        a.logprob[r] = (row.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(a.logits[(int64_t)r * a.ld + place], row.top), t))
-                                     - logf((float)((double)total * (1.0 / 1099511627776.0)));
-                    }
-                    return;
                 }
                 round = 2;
             } else if (rank == 0) {
@@ -687,8 +786,13 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         return bits > border || (bits == border && i <= cut) ? units_of(bits) : 0;
     };
     uint64_t mine = 0;
+    if (sure) {
+        mine = sure_mass;
+        each_found([&](int i) { mine += kept(i); });
+    } else {
 #pragma unroll 4
-    for (int i = i0; i < i1; ++i) mine += kept(i);
+        for (int i = i0; i < i1; ++i) mine += kept(i);
+    }
     const uint64_t upto = block_scan64(mine, sm.warp_sum);
     if (tid < (int)blocks) put64(&sm.mass[rank], tid, sm.warp_sum[kFilterWarps]);
     cluster_sync();
@@ -712,6 +816,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
 }
 
 constexpr int kMostStaged = (113 * 1024 - (int)sizeof(FilterShared) - 1024) / 4;      // weights that a block's half of the shared memory holds
+static_assert((kMostStaged + kFilterThreads - 1) / kFilterThreads + 1 <= 64, "a thread's tokens in a mask");
 static_assert(kMostStaged < 1 << (32 - kCountBits), "a block's tokens in a packed count");
 
 }  // namespace
