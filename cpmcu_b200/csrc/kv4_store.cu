@@ -1,7 +1,7 @@
 // Storing keys and values into the 4-bit cache, and reading them back.
 //
 // Store: q and k of a token are rotated (pairs (c, c + d/2), angle = position * inv_freq[c], cos and sin times ``magnitude``), q goes out in the
-// compute type, k and v become codes.  A warp takes one head row; a lane holds d/32 neighbouring channels, so that a pair's other half
+// compute type, k and v become codes.  Of these a warp takes one head row; a lane holds d/32 neighbouring channels, so that a pair's other half
 // and a half row's 16 lanes are one shuffle away.  The codes meet in shared memory, from where lanes write whole words (keys:
 // a token's own; values: 16 bits, for the other half of the word is the neighbouring token's, which another block may be writing).
 // What a token cannot do without: its projections, q out, d + 16 bytes per key-value head.
@@ -48,6 +48,17 @@ rope_store_kv4_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t*
     const int pos = positions[t];
     const int n_all = n_heads + (records ? 2 * n_kv : 0);
     const int begin = blockIdx.y * rows_per_block, end = min(n_all, begin + rows_per_block);
+    const T* row = qkv + (int64_t)t * (n_heads + 2 * n_kv) * D;
+    // q: half a warp to a row, a lane to E pairs of channels, the same ones in every row; the first row is on its way while the angles are formed
+    const int c0 = (lane & 15) * E, q_end = min(end, n_heads);
+    int hq = begin + 2 * warp + (lane >> 4);
+    float qa[E], qb[E];
+    const auto load_q = [&]() {
+        if (hq >= q_end) return;
+        load_row<T, E>(row + (int64_t)hq * D + c0, qa);
+        load_row<T, E>(row + (int64_t)hq * D + HALF + c0, qb);
+    };
+    load_q();
     if (inv_freq) {
         for (int c = threadIdx.x; c < HALF; c += blockDim.x) {
             float s, k;
@@ -57,11 +68,32 @@ rope_store_kv4_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t*
         }
         __syncthreads();
     }
-    uint8_t* page = nullptr;
-    if (end > n_heads)
-        page = records + (int64_t)CPM_PAGE(page_table + (int64_t)slots[token_seq[t]] * max_pages, pos / kPageTokens, max_pages) * n_kv * L::kBytes;
-    const T* row = qkv + (int64_t)t * (n_heads + 2 * n_kv) * D;
-    for (int h = begin + warp; h < end; h += kStoreWarps) {
+    if (hq < q_end) {
+        float k[E], n[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            k[i] = inv_freq ? cs[c0 + i] : 1.f;
+            n[i] = inv_freq ? sn[c0 + i] : 0.f;
+        }
+#pragma unroll 1
+        while (hq < q_end) {
+            float a[E], b[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                a[i] = inv_freq ? __fsub_rn(__fmul_rn(qa[i], k[i]), __fmul_rn(qb[i], n[i])) : qa[i];
+                b[i] = inv_freq ? __fadd_rn(__fmul_rn(qb[i], k[i]), __fmul_rn(qa[i], n[i])) : qb[i];
+            }
+            T* to = q_out + ((int64_t)t * n_heads + hq) * D + c0;
+            hq += 2 * kStoreWarps;
+            load_q();
+            store_row<T, E>(to, a);
+            store_row<T, E>(to + HALF, b);
+        }
+    }
+    if (end <= n_heads) return;
+    uint8_t* const page = records + (int64_t)CPM_PAGE(page_table + (int64_t)slots[token_seq[t]] * max_pages, pos / kPageTokens, max_pages) * n_kv * L::kBytes;
+    // k and v: a warp to a row, the last warps first, which have had the fewest rows of q
+    for (int h = max(begin, n_heads) + kStoreWarps - 1 - warp; h < end; h += kStoreWarps) {
         float x[E];
         load_row<T, E>(row + (int64_t)h * D + lane * E, x);
         if (inv_freq && h < n_heads + n_kv) {
@@ -73,10 +105,6 @@ rope_store_kv4_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t*
                 const float a = __fmul_rn(x[i], cs[c]), b = __fmul_rn(other, sn[c]);
                 x[i] = lane < 16 ? __fsub_rn(a, b) : __fadd_rn(a, b);
             }
-        }
-        if (h < n_heads) {
-            store_row<T, E>(q_out + ((int64_t)t * n_heads + h) * D + lane * E, x);
-            continue;
         }
         const bool values = h >= n_heads + n_kv;
         const int head = h - n_heads - (values ? n_kv : 0);
