@@ -61,8 +61,14 @@ struct Args {
     float scale;
 };
 
-// What unpacking a page tells the softmax: for the page, and per token where some row sees it in part.
-struct StepInfo { alignas(16) float k_token[kPageTokens]; int v_token[kPageTokens]; float k_scale; int v_power; uint32_t bad[2]; };
+// What unpacking a page tells the softmax: for each 16 tokens, and per token where some row sees the page in part.
+struct StepInfo {
+    alignas(16) float k_token[kPageTokens];
+    int v_token[kPageTokens];
+    alignas(16) float k_scale[4];
+    alignas(16) int v_power[4];
+    alignas(16) uint32_t bad[4];                        // tokens whose values are no numbers
+};
 
 enum : int { ERR_Q = 1, ERR_K_FULL, ERR_V_FULL, ERR_K_EMPTY, ERR_V_EMPTY, ERR_S_FULL, ERR_P_FULL, ERR_O_FULL };
 __device__ int g_error;
@@ -130,6 +136,7 @@ struct Slice {
     uint32_t k[D / 32][2], v[D / 32][2];                // [pair of 16-channel blocks][upper eight tokens]
     uint2 kp[2];                                        // rows g and g + 8
     uint4 vp[2];                                        // rows 2 j and 2 j + 1, and eight further
+    uint32_t k1, v1;                                    // one of the 32 parameters of the 16 rows: row lane / 2, half lane % 2
     __device__ __forceinline__ void load(const uint8_t* rec, int slice, int lane) {
         using L = Kv4<D>;
         const int g = lane >> 2, j = lane & 3;
@@ -146,6 +153,8 @@ struct Slice {
             kp[u] = *reinterpret_cast<const uint2*>(rec + L::kKeyParams + rk * 8);
             vp[u] = *reinterpret_cast<const uint4*>(rec + L::kValueParams + rv * 8);
         }
+        k1 = *reinterpret_cast<const uint32_t*>(rec + L::kKeyParams + slice * 128 + lane * 4);
+        v1 = *reinterpret_cast<const uint32_t*>(rec + L::kValueParams + slice * 128 + lane * 4);
     }
     // Behind the sequence's end, after ``tokens`` of the page: what lies there may be no number.
     __device__ __forceinline__ void trim(int slice, int lane, int tokens) {
@@ -156,6 +165,7 @@ struct Slice {
             if (rv >= tokens) vp[u].x = vp[u].y = 0u;
             if (rv + 1 >= tokens) vp[u].z = vp[u].w = 0u;
         }
+        if (16 * slice + (lane >> 1) >= tokens) k1 = v1 = 0u;
     }
 };
 __device__ __forceinline__ float bound_of(uint32_t p) { return fabsf(kv4_middle(p)) + 8.f * kv4_scale(p); }
@@ -169,8 +179,6 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ StepInfo info[kInfos];
-    __shared__ float4 bounds[2][2];                      // [step parity][keys, values], of four slices each
-    __shared__ uint32_t bads[2][4];                      // [step parity][slice]: 16 tokens each
     pdl_launch_dependents();
     pdl_wait();
 
@@ -262,47 +270,35 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             for (int e = 0; e < 2; ++e) v_off[u][e] = v_smem + (2 * g + e) * 128 + (((2 * slice + u) ^ ((2 * g + e) & 7)) << 4) + 4 * j4;
         Slice<D> now, next;
         if (n_steps > 0) load(next, 0);
-        bool alive = true;                                   // after an abort the loop goes on without waiting: the warps meet at a barrier in every step
+        bool alive = true;                                   // after an abort the loop goes on without waiting
 #pragma unroll 1
         for (int st = 0; st < n_steps; ++st) {
             now = next;
             if (st + 1 < n_steps) load(next, st + 1);
-            now.trim(slice, lane, kv_len - (page0 + st) * kPageTokens);
+            const int left = kv_len - (page0 + st) * kPageTokens;
+            if (left < kPageTokens) now.trim(slice, lane, left);
             if (__any_sync(0xffffffffu, aborted())) alive = false;
-            const int s = st % kStages, ph = (st / kStages) & 1, par = st & 1;
-            // the largest magnitudes of the page's keys and values; tokens whose values are no numbers
-            {
-                float bk = 0.f, bv = 0.f;
-                uint32_t bad = 0;
+            const int s = st % kStages, ph = (st / kStages) & 1;
+            // the largest magnitudes of the 16 tokens' keys and values; tokens whose values are no numbers
+            const float k_bound = bound_of(now.k1), v_bound = bound_of(now.v1);
+            const bool v_finite = v_bound < INFINITY;
+            const float most_k = __uint_as_float(__reduce_max_sync(0xffffffffu, k_bound < INFINITY ? __float_as_uint(k_bound) : 0u));
+            uint32_t bad = __ballot_sync(0xffffffffu, !v_finite);
+            if (bad) {
+                bad = (bad | bad >> 1) & 0x55555555u;           // bit 2 t of token t; the other half row goes too
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const float k0 = bound_of(now.kp[u].x), k1 = bound_of(now.kp[u].y);
-                    bk = fmaxf(bk, fmaxf(k0 < INFINITY ? k0 : 0.f, k1 < INFINITY ? k1 : 0.f));
-                    const float a0 = bound_of(now.vp[u].x), a1 = bound_of(now.vp[u].y), b0 = bound_of(now.vp[u].z), b1 = bound_of(now.vp[u].w);
-                    if (!(a0 + a1 < INFINITY)) { now.vp[u].x = now.vp[u].y = 0u; bad |= 1u << (2 * j4 + 8 * u); }
-                    else bv = fmaxf(bv, fmaxf(a0, a1));
-                    if (!(b0 + b1 < INFINITY)) { now.vp[u].z = now.vp[u].w = 0u; bad |= 2u << (2 * j4 + 8 * u); }
-                    else bv = fmaxf(bv, fmaxf(b0, b1));
-                }
-                const uint32_t mk = __reduce_max_sync(0xffffffffu, __float_as_uint(bk)), mv = __reduce_max_sync(0xffffffffu, __float_as_uint(bv));
-                bad = __reduce_or_sync(0xffffffffu, bad);
-                if (lane == 0) {
-                    reinterpret_cast<float*>(&bounds[par][0])[slice] = __uint_as_float(mk);
-                    reinterpret_cast<float*>(&bounds[par][1])[slice] = __uint_as_float(mv);
-                    bads[par][slice] = bad;
+                    if (bad >> (4 * j4 + 16 * u) & 1) now.vp[u].x = now.vp[u].y = 0u;
+                    if (bad >> (4 * j4 + 16 * u + 2) & 1) now.vp[u].z = now.vp[u].w = 0u;
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            const float4 k4 = bounds[par][0], v4 = bounds[par][1];
-            const int ek = power_below(fmaxf(fmaxf(k4.x, k4.y), fmaxf(k4.z, k4.w)));
-            const float most_v = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
-            const int ev = most_v > 0.f ? power_below(most_v) : -110;
+            const float most_v = __uint_as_float(__reduce_max_sync(0xffffffffu, bad >> (lane & 30) & 1 ? 0u : __float_as_uint(v_bound)));
+            const int ek = power_below(most_k), ev = most_v > 0.f ? power_below(most_v) : -110;
             StepInfo& inf = info[st % kInfos];
-            if (slice == 0 && lane == 0) {
-                inf.k_scale = power2(ek);
-                inf.v_power = ev;
-                inf.bad[0] = bads[par][0] | bads[par][1] << 16;
-                inf.bad[1] = bads[par][2] | bads[par][3] << 16;
+            if (lane == 0) {
+                inf.k_scale[slice] = power2(ek);
+                inf.v_power[slice] = ev;
+                inf.bad[slice] = bad;
             }
             float down_k[2] = {power2(-ek), power2(-ek)}, down_v[2][2] = {{power2(-ev), power2(-ev)}, {power2(-ev), power2(-ev)}};
             if (in_part(st)) {                                // every token by itself
@@ -500,7 +496,10 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                 tmem_load_32cols(s_addr, v[0]);
                 tmem_load_32cols(s_addr + 32, v[1]);
                 tmem_load_wait();
-                int highest = inf.v_power;
+                const int4 v_power = *reinterpret_cast<const int4*>(inf.v_power);
+                const float4 k_scale = *reinterpret_cast<const float4*>(inf.k_scale);
+                const float by_slice[4] = {MASKED ? sl2 : sl2 * k_scale.x, MASKED ? sl2 : sl2 * k_scale.y, MASKED ? sl2 : sl2 * k_scale.z, MASKED ? sl2 : sl2 * k_scale.w};
+                int highest = max(max(v_power.x, v_power.y), max(v_power.z, v_power.w));
                 if constexpr (MASKED) {
                     highest = -110;
 #pragma unroll
@@ -515,11 +514,12 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                 }
                 float m_new = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+                for (int c = 0; c < 4; ++c) {
+                    float most = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) m_new = max3(m_new, __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
-                const float sl = MASKED ? sl2 : sl2 * inf.k_scale;
-                m_new *= sl;
+                    for (int e = 0; e < 16; e += 2) most = max3(most, __uint_as_float(v[c / 2][16 * (c & 1) + e]), __uint_as_float(v[c / 2][16 * (c & 1) + e + 1]));
+                    m_new = fmaxf(m_new, most * by_slice[c]);
+                }
                 const bool grow = m_new > m + kBehind || (m == -INFINITY && m_new > -INFINITY);
                 const int power_new = max(power, highest);
                 if (__any_sync(0xffffffffu, grow || power_new > power)) {
@@ -543,14 +543,18 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                     if (grow) m = m_new;
                     power = power_new;
                 }
-                const float use = m == -INFINITY ? 0.f : m, factor = power2(inf.v_power - power);
-                const float2 by = make_float2(sl, sl), less = make_float2(-use, -use);
-                float2 f2 = make_float2(factor, factor), sum = make_float2(0.f, 0.f);
+                const float use = m == -INFINITY ? 0.f : m;
+                const float factor[4] = {power2(v_power.x - power), power2(v_power.y - power), power2(v_power.z - power), power2(v_power.w - power)};
+                const float2 less = make_float2(-use, -use);
+                float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int run = 0; run < 2; ++run) {
                     uint32_t packed[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
+                        const int c = 2 * run + e / 8;
+                        const float2 by = make_float2(by_slice[c], by_slice[c]);
+                        float2 f2 = make_float2(factor[c], factor[c]);
                         const float2 x = fma2(make_float2(__uint_as_float(v[run][2 * e]), __uint_as_float(v[run][2 * e + 1])), by, less);
                         const float2 w = make_float2(ex2(x.x), ex2(x.y));
                         sum = add2(sum, w);
@@ -566,11 +570,11 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             // (two copies of the code: the one for pages that every row sees whole has nothing of the other's)
             if (in_part(st)) soften(std::true_type{});
             else soften(std::false_type{});
-            if (inf.bad[0] | inf.bad[1]) {
+            if (inf.bad[0] | inf.bad[1] | inf.bad[2] | inf.bad[3]) {
                 // values that are no numbers are not in the tile: the rows that see them are no numbers
 #pragma unroll 1
                 for (int e = 0; e < kPageTokens; ++e)
-                    if ((inf.bad[e >> 5] >> (e & 31) & 1) && key0 + e <= limit && key0 + e >= from) l = NAN;
+                    if ((inf.bad[e >> 4] >> (2 * (e & 15)) & 1) && key0 + e <= limit && key0 + e >= from) l = NAN;
             }
             tmem_store_wait();
             tcgen05_fence_before();
