@@ -33,7 +33,8 @@ constexpr int kRows = 256;
 constexpr int kStages = 4;                              // tiles of keys, and of values
 constexpr int kInfos = 8;                               // steps that unpacking may be ahead of the softmax, and one
 constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4;
-constexpr int kThreads = (kSoftmaxWarps + 2 + kUnpackWarps) * 32;      // 128 registers each
+constexpr int kIssueWarps = 4;                         // scores and weighted values of both halves
+constexpr int kThreads = (kSoftmaxWarps + kIssueWarps + kUnpackWarps) * 32;      // 128 registers each
 constexpr float kBehind = 8.0f;                         // the running maximum may lie 2^8 behind
 constexpr int kQHalf = 128 * 128, kKHalf = 64 * 128;    // 128 rows of Q, 64 keys: runs of 128 bytes
 constexpr int kQExtra = 128 * 32, kKExtra = 64 * 32;    // 16 more columns, two runs of 16 bytes a row
@@ -70,7 +71,7 @@ struct StepInfo {
     alignas(16) uint32_t bad[4];                        // tokens whose values are no numbers
 };
 
-enum : int { ERR_Q = 1, ERR_K_FULL, ERR_V_FULL, ERR_K_EMPTY, ERR_V_EMPTY, ERR_S_FULL, ERR_P_FULL, ERR_O_FULL };
+enum : int { ERR_Q = 1, ERR_FULL, ERR_EMPTY, ERR_S_FULL, ERR_P_FULL, ERR_O_FULL };
 __device__ int g_error;
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 kv4_prompt_kernel(const __grid_constant__ Args a) {
     using Z = Sizes<D>;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages], s_full[2][2], p_full[2][2], o_done[2][2];      // (of two S the softmax may be two steps ahead of the products: each has its own barriers)
+    __shared__ __align__(8) uint64_t q_full[2], full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_done[2][2];      // (of two S the softmax may be two steps ahead of the products: each has its own barriers)
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ StepInfo info[kInfos];
@@ -208,10 +209,8 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     if (threadIdx.x == 0) {
 #pragma unroll 1
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(smem_u32(&k_full[s]), kUnpackWarps);
-            mbar_init(smem_u32(&v_full[s]), kUnpackWarps);
-            mbar_init(smem_u32(&k_empty[s]), 1);
-            mbar_init(smem_u32(&v_empty[s]), 1);
+            mbar_init(smem_u32(&full[s]), kUnpackWarps);
+            mbar_init(smem_u32(&empty[s]), 2);
         }
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
@@ -248,9 +247,9 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     };
     auto aborted = [&]() { return *(volatile int*)&abort_flag != 0; };
 
-    if (warp >= kSoftmaxWarps + 2) {
+    if (warp >= kSoftmaxWarps + kIssueWarps) {
         // ---- unpacking: a warp takes 16 tokens of every page, whose codes were asked for a page ahead ----
-        const int slice = warp - kSoftmaxWarps - 2, g = lane >> 2, j4 = lane & 3;
+        const int slice = warp - kSoftmaxWarps - kIssueWarps, g = lane >> 2, j4 = lane & 3;
         const int* table = a.page_table + (int64_t)a.slots[seq] * a.max_pages;
         const uint8_t* records = a.records + (int64_t)head_kv * Kv4<D>::kBytes;
         const int64_t page_stride = (int64_t)a.n_kv * Kv4<D>::kBytes;
@@ -268,13 +267,10 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int e = 0; e < 2; ++e) v_off[u][e] = v_smem + (2 * g + e) * 128 + (((2 * slice + u) ^ ((2 * g + e) & 7)) << 4) + 4 * j4;
-        Slice<D> now, next;
-        if (n_steps > 0) load(next, 0);
+        Slice<D> even, odd;
+        if (n_steps > 0) load(even, 0);
         bool alive = true;                                   // after an abort the loop goes on without waiting
-#pragma unroll 1
-        for (int st = 0; st < n_steps; ++st) {
-            now = next;
-            if (st + 1 < n_steps) load(next, st + 1);
+        const auto unpack = [&](Slice<D>& now, int st) {
             const int left = kv_len - (page0 + st) * kPageTokens;
             if (left < kPageTokens) now.trim(slice, lane, left);
             if (__any_sync(0xffffffffu, aborted())) alive = false;
@@ -320,11 +316,11 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                     }
                 }
             }
-            // ---- keys ----
-            if (alive && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&k_empty[s]), ph ^ 1))) {
-                if (lane == 0) fail(ERR_K_EMPTY);
+            if (alive && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&empty[s]), ph ^ 1))) {
+                if (lane == 0) fail(ERR_EMPTY);
                 alive = false;
             }
+            // ---- keys ----
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const float down = down_k[u];
@@ -345,14 +341,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                                      "r"(half2_bits(__hmul2(r[2 * odd], sc[h]))), "r"(half2_bits(__hmul2(r[2 * odd + 1], sc[h]))) : "memory");
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&k_full[s]));
             // ---- values ----
-            if (alive && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&v_empty[s]), ph ^ 1))) {
-                if (lane == 0) fail(ERR_V_EMPTY);
-                alive = false;
-            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint4 p4 = now.vp[u];
@@ -372,53 +361,55 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&v_full[s]));
+            if (lane == 0) mbar_arrive(smem_u32(&full[s]));
+        };
+#pragma unroll 1
+        for (int st = 0; st < n_steps; st += 2) {
+            if (st + 1 < n_steps) load(odd, st + 1);
+            unpack(even, st);
+            if (st + 1 >= n_steps) break;
+            if (st + 2 < n_steps) load(even, st + 2);
+            unpack(odd, st + 1);
         }
-    } else if (warp == kSoftmaxWarps) {
-        // ---- scores, issued by one thread as soon as a page's keys are there and an S is free ----
+    } else if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + 2) {
+        // ---- a half's scores, issued by one thread as soon as a page's keys are there and an S is free ----
+        const int i = warp - kSoftmaxWarps;
         if (lane == 0 && n_steps > 0) {
-            if (!mbar_wait_bounded(smem_u32(&q_full[0]), 0) || !mbar_wait_bounded(smem_u32(&q_full[1]), 0)) fail(ERR_Q);
+            if (!mbar_wait_bounded(smem_u32(&q_full[i]), 0)) fail(ERR_Q);
 #pragma unroll 1
             for (int st = 0; st < n_steps && !aborted(); ++st) {
                 const int s = st % kStages;
-                if (!mbar_wait_bounded(smem_u32(&k_full[s]), (st / kStages) & 1)) { fail(ERR_K_FULL); break; }
-#pragma unroll 1
-                for (int i = 0; i < 2; ++i) {
-                    if (st >= 2 && !mbar_wait_bounded(smem_u32(&o_done[i][st & 1]), ((st - 2) >> 1) & 1)) { fail(ERR_O_FULL); break; }
-                    tcgen05_fence_after();
-                    const uint32_t to = tmem + i * 128 + (st & 1) * 64;
+                if (!mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1)) { fail(ERR_FULL); break; }
+                if (st >= 2 && !mbar_wait_bounded(smem_u32(&o_done[i][st & 1]), ((st - 2) >> 1) & 1)) { fail(ERR_O_FULL); break; }
+                tcgen05_fence_after();
+                const uint32_t to = tmem + i * 128 + (st & 1) * 64;
 #pragma unroll
-                    for (int half = 0; half < Z::kHalves; ++half) {
-                        const uint64_t da = smem_desc_sw128(q_smem + i * Z::kQ + half * kQHalf), db = smem_desc_sw128(k_smem + s * Z::kKv + half * kKHalf);
+                for (int half = 0; half < Z::kHalves; ++half) {
+                    const uint64_t da = smem_desc_sw128(q_smem + i * Z::kQ + half * kQHalf), db = smem_desc_sw128(k_smem + s * Z::kKv + half * kKHalf);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) tcgen05_mma_f16(to, da + 2 * k, db + 2 * k, Z::idesc(64), (half | k) != 0);
-                    }
-                    tcgen05_mma_f16(to, smem_desc_plain(qx_smem + i * kQExtra, 128), smem_desc_plain(kx_smem + s * kKExtra, 64), Z::idesc(64), 1);
-                    tcgen05_commit(smem_u32(&s_full[i][st & 1]));
+                    for (int k = 0; k < 4; ++k) tcgen05_mma_f16(to, da + 2 * k, db + 2 * k, Z::idesc(64), (half | k) != 0);
                 }
-                tcgen05_commit(smem_u32(&k_empty[s]));
+                tcgen05_mma_f16(to, smem_desc_plain(qx_smem + i * kQExtra, 128), smem_desc_plain(kx_smem + s * kKExtra, 64), Z::idesc(64), 1);
+                tcgen05_commit(smem_u32(&s_full[i][st & 1]));
             }
         }
         __syncwarp();
-    } else if (warp == kSoftmaxWarps + 1) {
-        // ---- weighted values, issued by one thread ----
+    } else if (warp >= kSoftmaxWarps + 2) {
+        // ---- a half's weighted values, issued by one thread ----
+        const int i = warp - kSoftmaxWarps - 2;
         if (lane == 0) {
-            bool ok = true;
 #pragma unroll 1
-            for (int st = 0; ok && st < n_steps && !aborted(); ++st) {
+            for (int st = 0; st < n_steps && !aborted(); ++st) {
                 const int s = st % kStages;
-                if (!mbar_wait_bounded(smem_u32(&v_full[s]), (st / kStages) & 1)) { fail(ERR_V_FULL); break; }
+                if (!mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1)) { fail(ERR_FULL); break; }
+                if (!mbar_wait_bounded(smem_u32(&p_full[i][st & 1]), (st >> 1) & 1)) { fail(ERR_P_FULL); break; }
+                tcgen05_fence_after();
                 const uint64_t db = smem_desc_sw128(v_smem + s * Z::kKv);
-#pragma unroll 1
-                for (int i = 0; i < 2; ++i) {
-                    if (!mbar_wait_bounded(smem_u32(&p_full[i][st & 1]), (st >> 1) & 1)) { fail(ERR_P_FULL); ok = false; break; }
-                    tcgen05_fence_after();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        tcgen05_mma_f16_ts(tmem + Z::kO + i * D, tmem + i * 128 + (st & 1) * 64 + k * 8, db + 2 * k, Z::idesc(D), st > 0 || k != 0);
-                    tcgen05_commit(smem_u32(&o_done[i][st & 1]));
-                }
-                if (ok) tcgen05_commit(smem_u32(&v_empty[s]));
+                for (int k = 0; k < 4; ++k)
+                    tcgen05_mma_f16_ts(tmem + Z::kO + i * D, tmem + i * 128 + (st & 1) * 64 + k * 8, db + 2 * k, Z::idesc(D), st > 0 || k != 0);
+                tcgen05_commit(smem_u32(&o_done[i][st & 1]));
+                tcgen05_commit(smem_u32(&empty[s]));             // (the page's scores were formed before)
             }
         }
         __syncwarp();
