@@ -9,12 +9,19 @@
 // 2^-14 and 2^15 in the same way.  bf16 queries: p s_v is rounded to fp16 (11 bits; the output has 8).  fp32 queries: q and p s_v are sums of
 // two fp16 numbers (22 bits), which costs a second product each.
 //
-// One block an SM takes an equal share of all (tile, key-value head, page) units of the launch, in that order, so that a batch of unequal
-// sequences leaves no SM idle; a tile that is cut leaves its parts (weighted values, maximum, sum) to a second kernel.  Four warps take 16 tokens each
-// of a page, and the block's two to four groups of four warps every second to fourth page.  A warp brings its tokens into a ring of its own by
-// asynchronous 16-byte copies, of which a lane reads most of what it copied itself, and keeps a softmax of its own, so that nothing synchronises the
-// warps until a tile ends.  (Bulk copies of a slice's four pieces took longer than the arithmetic: each needs its addresses in uniform
-// registers.  Blocks of four warps, three an SM, leave three times as many parts to add up: 41 us where blocks of twelve took 30, for one sequence of 131,071 keys.)
+// One block an SM.  A batch's rows of pages (a tile's, of one key-value head) lie in a line, of which every block takes a piece of equal cost, so that
+// unequal sequences leave no SM idle; few rows have blocks of their own.  A row that several blocks share is put together by a second kernel.  Four
+// warps take 16 tokens each of a page, and the block's two to four groups of four warps every second to fourth page.  A warp brings its tokens into a
+// ring of its own by asynchronous 16-byte copies, of which a lane reads most of what it copied itself, and keeps a softmax of its own, so that nothing
+// synchronises the warps until a row ends.  (Bulk copies of a slice's four pieces took longer than the arithmetic: each needs its addresses in
+// uniform registers.  Blocks of four warps, three an SM, leave three times as many parts to add up: 41 us where blocks of twelve took 30, for one
+// sequence of 131,071 keys.)
+//
+// 32 heads on 2 of 128, bf16: 1,000 keys 11 us, 131,071 keys 28 us (1.35 TB/s of records); 64 sequences of 1 to 8,192 keys, 14 heads on 2 of 64,
+// 28 us (1.6 TB/s); 5 of 300 to 2,500 keys, fp32, 9 us; 200 of 1 to 4,000, 32 heads on 8 of 128, 163 us (2.9 TB/s).  Bound, where there are many keys, by
+// instructions: a slice of 16 tokens costs a warp some 500, of which unpacking the codes is a third; where there are few, by the way to the first
+// key: 2 us for lengths and shares, 1 for page numbers, 1 for queries, 2 for the first slice and 2 for the parts, whose instructions
+// come from L2, and 2.5 for the second kernel.
 #include "kv4.cuh"
 
 CPM_BOUNDS_TU(kv4_attention)

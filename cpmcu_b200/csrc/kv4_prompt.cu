@@ -3,20 +3,23 @@
 // A block takes 256 rows of queries, the query heads of one key-value head for some consecutive tokens (16 tokens at 16 heads), so that all of them share
 // every key and value.  Four warps unpack the codes, a page of 64 keys a step, into fp16 tiles in shared memory: K [keys][d] and V
 // [d][keys], 128-byte swizzle, the K-major operands of S = Q K^T and O += P V (tcgen05.mma, accumulators in tensor memory); four tiles of each.  Eight
-// warps are the softmax, a thread to a row, which writes P as fp16 over the S it read; a warp each issues the two kinds of products of both halves of 128
-// rows.  A half has two S: the next page's scores are formed while this one's are in the softmax, so that only the softmax itself is in a
-// row's way.  (2,048 tokens of 32 heads on 2 behind 4,101 keys, 172 GFLOP: one S of
-// 128 keys, whose softmax waits for its products, 347 us; two and one warp for all products, 333; as it is, 269, 640 TFLOP/s.)
+// warps are the softmax, a thread to a row, which writes P as fp16 over the S it read; four more issue the products, one each for the scores and the
+// values of a half of 128 rows (an issuing thread is busy for some 1,300 cycles a page with its waits).  A half has two S: the next page's scores are
+// formed while this one's are in the softmax, so that only the softmax itself is in a row's way.  (2,048 tokens of 32 heads on 2 behind 4,101 keys, 172
+// GFLOP: one S of 128 keys, whose softmax waits for its products, 347 us; two S and one issuing warp 333, two issuing warps 269, powers of
+// two by 16 tokens instead of by page 262, four issuing warps and one barrier for a page's keys and values 247, 700 TFLOP/s.)
 //
 // fp16 and not bf16: its 11 bits hold s (c - 8) exactly, 8 bits times 3, so that scores are as exact as their fp32 sums.  The rest of a
 // key's product, m times the sum of the query's half row, is 16 more columns of the operands: m three times and the sum as three fp16 numbers,
 // for both halves.  A value is rounded to 11 bits (2^-12 of it, where the output has 8).
-// What fp16 lacks in range is taken care of by powers of two: a query row, a page's keys and a page's values are divided by the power of two below
+// What fp16 lacks in range is taken care of by powers of two: a query row, 16 tokens' keys and 16 tokens' values are divided by the power of two below
 // their largest magnitude, scores are multiplied by the first two again, and the accumulator stands for O / 2^E with E the largest power of the
 // values so far.
 //
 // Unpacking a key and a value costs about two instructions a number, 256 rows of softmax four to five; a block of 128 rows would pay it twice.
-// Bound by the unpacking warps, about 3,000 cycles a page with their barriers, where the softmax takes 1,800 and the products 1,400.
+// Bound by the four unpacking warps, which are one to a scheduler and wait for each instruction before the next: 2,500 cycles a page, where the
+// softmax takes 1,400 to 2,000 and the products 1,400.  (Eight of them, with the softmax in runs of 32 keys or its registers given by the issuing warps, took
+// 279 to 298 us: what they hide they take from the softmax.)
 //
 // Every wait is bounded: a block that gives up records an error, stops, frees its tensor memory and returns (nothing is in flight then: tiles are
 // written by ordinary stores).
@@ -33,7 +36,7 @@ constexpr int kRows = 256;
 constexpr int kStages = 4;                              // tiles of keys, and of values
 constexpr int kInfos = 8;                               // steps that unpacking may be ahead of the softmax, and one
 constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4;
-constexpr int kIssueWarps = 4;                         // scores and weighted values of both halves
+constexpr int kIssueWarps = 4;                          // scores and weighted values of both halves
 constexpr int kThreads = (kSoftmaxWarps + kIssueWarps + kUnpackWarps) * 32;      // 128 registers each
 constexpr float kBehind = 8.0f;                         // the running maximum may lie 2^8 behind
 constexpr int kQHalf = 128 * 128, kKHalf = 64 * 128;    // 128 rows of Q, 64 keys: runs of 128 bytes

@@ -107,6 +107,9 @@ class DryOps(Ops):
     def _f32(t, what):
         return t
 
+    def _kv4(self, records, n_kv, d):
+        return records
+
     def set_page_limit(self, n_pages):
         pass
 
