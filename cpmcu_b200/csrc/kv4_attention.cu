@@ -760,9 +760,9 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
     }
 }
 
-// Adds up the parts of the rows that were cut, one block per row and column; blockIdx.y is the place of the row's head.  A warp has four of its
-// parts under way at a time.
-constexpr int kCombineWarps = 16, kCombineParts = 4;
+// Adds up the parts of the rows that were cut, one block per row and column; blockIdx.y is the place of the row's head.  A warp has five of its parts
+// under way at a time, so that the half of 148 blocks' parts are one round of loads.
+constexpr int kCombineWarps = 16, kCombineParts = 5;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kCombineWarps * 32)
 kv4_combine_kernel(const __grid_constant__ AttendArgs a, int blocks) {

@@ -1720,9 +1720,9 @@ class Ops:
 
     def kv4_prompt_ok(self, n_tokens: int, n_heads: int, n_kv: int, d: int, scale: float) -> bool:
         """Whether prompt tokens go to the tcgen05 kernel, which takes 256 query rows of a key-value head a block and shares few blocks' keys out.
-        us, token by token's kernel and this one: 32 heads on 2 of 128, 32 tokens behind 8,000 keys (4 blocks) 45 and 46, 64 tokens 73 and 41, 64
-        behind 500 27 and 24; 16 on 2 of 64, 64 behind 8,000 (4 blocks) 36 and 27, behind 500 18 and 18; 8 on 4 of 128, 128 behind 8,000 (4
-        blocks) 45 and 48, 256 72 and 45."""
+        us, the other kernel and this one: 32 heads on 2 of 128, 32 tokens behind 8,000 keys (4 blocks) 44 and 46, 64 tokens 74 and 41, 64
+        behind 500 23 and 24; 16 on 2 of 64, 64 behind 8,000 (4 blocks) 34 and 27, behind 500 16 and 18; 8 on 4 of 128, 128 behind 8,000 (4
+        blocks) 44 and 47, 256 74 and 45."""
         return (self.use_tcgen05_attention and self.code == BF16 and d in (64, 128) and scale > 0
                 and (n_tokens * (n_heads // n_kv) + 255) // 256 * n_kv >= self.KV4_PROMPT_BLOCKS)
 

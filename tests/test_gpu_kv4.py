@@ -180,6 +180,24 @@ def test_one_token_a_sequence(dtype, d, heads, kv):
         assert float(got[0].abs().max()) == 0.0           # no keys
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,n", [(8, 2, 1), (8, 2, 2), (8, 2, 18), (8, 2, 19), (24, 1, 18), (24, 1, 19), (3, 3, 12), (3, 3, 13), (8, 2, 70), (2, 1, 200)])
+def test_batches_of_unequal_sequences(dtype, heads, kv, n):
+    """Few rows of pages have blocks of their own, many are shared out by their cost: batches on both sides of the rule."""
+    ops, d = _ops(dtype), 64
+    g = torch.Generator().manual_seed(n)
+    lengths = (2500 * torch.rand(n, generator=g) ** 3).int().tolist()
+    lengths[0] = 4000 if n < 100 else 9000
+    if n > 2:
+        lengths[n // 2] = 0
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 31)
+    q = torch.randn(n, heads, d, generator=g).to(DT[dtype])
+    for window in (0, 200):
+        got = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5, window=window)
+        want = torch.cat([plain.attention(q[i:i + 1], k, v, m - 1, d ** -0.5, window) for i, (m, (k, v)) in enumerate(zip(lengths, rows))])
+        _check(got, want, rows, dtype)
+
+
 @pytest.mark.parametrize("tcgen05,shares", [(False, 0), (True, 1), (True, 3), (True, 0)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("d,heads,kv", [(32, 3, 1), (64, 8, 1), (64, 6, 2), (96, 4, 2), (128, 16, 1), (128, 2, 2), (64, 4, 2), (128, 5, 1), (64, 40, 2)])
@@ -485,6 +503,40 @@ def test_sample_filtered_large_rows(rows, vocab):
     assert torch.equal(tok.long(), (c <= target[:, None]).sum(1))
     want = (z.double().gather(1, tok.long()[:, None])[:, 0] - z.double().amax(1)) / t.double() - torch.log(c[:, -1].double() / plain.UNIT)
     assert float((lp.double() - want).abs().max()) < 2e-5
+
+
+def _defined(z, u, t, k, p, m):
+    """Token of each row by the definition in whole numbers, on the device."""
+    vocab = z.shape[1]
+    w = torch.exp((z - z.amax(1, keepdim=True)) / t[:, None])
+    units = (w.double() * plain.UNIT).long()
+    ranked, order = torch.sort(w, dim=1, descending=True, stable=True)
+    mass = units.gather(1, order).cumsum(1)
+    n = torch.where(k > 0, k, vocab).long().clamp_max(vocab)
+    within = mass.gather(1, n[:, None] - 1)
+    n = torch.where(p < 1, torch.minimum(n, (mass.double() < p.double()[:, None] * within.double()).sum(1) + 1), n)
+    n = torch.where(m > 0, torch.minimum(n, (ranked >= m[:, None]).sum(1)), n).clamp_min(1)
+    keep = torch.zeros_like(z, dtype=torch.bool).scatter(1, order, torch.arange(vocab, device="cuda") < n[:, None])
+    c = torch.where(keep, units, 0).cumsum(1)
+    return (c <= (u.double() * c[:, -1].double()).long()[:, None]).sum(1)
+
+
+@pytest.mark.parametrize("rows,vocab", [(70, 73448), (6, 73448), (300, 19000), (2, 300000)])
+@pytest.mark.parametrize("spread", ["narrow", "wide", "tail"])
+def test_sample_filtered_where_bins_are_full_or_tiny(rows, vocab, spread):
+    """Weights that all lie in one or two bins, with every bit below the bin's number in use (sums beyond 32 bits); weights over 200 octaves; and
+    a few large ones before a tail in which most of the mass lies below 2^-17 of the largest."""
+    ops, g = _ops("bfloat16"), torch.Generator().manual_seed(rows)
+    r = lambda *n: torch.rand(*n, generator=g)  # noqa: E731
+    z = {"narrow": -0.02 * r(rows, vocab), "wide": 70 * torch.randn(rows, vocab, generator=g), "tail": -11.5 - 4 * r(rows, vocab)}[spread]
+    if spread == "tail":
+        z[:, ::vocab // 3] = 0.0
+    p = torch.where(r(rows) < 0.3, torch.ones(rows), r(rows))
+    p[0] = 1 - 2.0 ** -20
+    k = torch.where(r(rows) < 0.6, torch.zeros(rows), (vocab * r(rows)).ceil()).int()
+    m = torch.where(r(rows) < 0.8, torch.zeros(rows), 1e-6 * r(rows))
+    args = [x.cuda() for x in (z, r(rows), torch.ones(rows), k, p, m)]
+    assert torch.equal(ops.sample_filtered(*args)[0].long(), _defined(*args))
 
 
 def test_sample_filtered_is_distributed_as_it_should():
