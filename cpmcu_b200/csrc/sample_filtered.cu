@@ -651,8 +651,13 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
             if (complete) {
                 // ---- all that top-k leaves is here ----
                 if (listed <= kRanked) {
-                    // The first block goes on alone.  Some threads to a token: how many stand before it, and what mass?
-                    if (rank > 0) return;
+                    // The first block goes on alone, but does not end before the others have read what lies in it.
+                    asm volatile("barrier.cluster.arrive;" ::: "memory");
+                    if (rank > 0) {
+                        asm volatile("barrier.cluster.wait;" ::: "memory");
+                        return;
+                    }
+                    // Some threads to a token: how many stand before it, and what mass?
                     int bits_of_tokens = 5;
                     while ((1 << bits_of_tokens) < listed) ++bits_of_tokens;
                     const int share = kFilterThreads >> bits_of_tokens, own = tid / share, part = tid % share;
@@ -695,6 +700,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                         a.logprob[r] = (row.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(a.logits[(int64_t)r * a.ld + place], row.top), t))
                                      - logf((float)((double)total * (1.0 / 1099511627776.0)));
                     }
+                    asm volatile("barrier.cluster.wait;" ::: "memory");
                     return;
                 }
                 if (rank == 0) {
