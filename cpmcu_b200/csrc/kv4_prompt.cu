@@ -77,6 +77,12 @@ struct StepInfo {
 enum : int { ERR_Q = 1, ERR_FULL, ERR_EMPTY, ERR_S_FULL, ERR_P_FULL, ERR_O_FULL };
 __device__ int g_error;
 
+// True in one thread of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     unsigned long long ra, rb, rc, rd;
     float2 d;
@@ -377,36 +383,41 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     } else if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + 2) {
         // ---- a half's scores, issued by one thread as soon as a page's keys are there and an S is free ----
         const int i = warp - kSoftmaxWarps;
-        if (lane == 0 && n_steps > 0) {
+        if (n_steps > 0) {
             if (!mbar_wait_bounded(smem_u32(&q_full[i]), 0)) fail(ERR_Q);
 #pragma unroll 1
-            for (int st = 0; st < n_steps && !aborted(); ++st) {
+            for (int st = 0; st < n_steps; ++st) {
                 const int s = st % kStages;
-                if (!mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1)) { fail(ERR_FULL); break; }
-                if (st >= 2 && !mbar_wait_bounded(smem_u32(&o_done[i][st & 1]), ((st - 2) >> 1) & 1)) { fail(ERR_O_FULL); break; }
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1))) { fail(ERR_FULL); break; }
+                if (st >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i][st & 1]), ((st - 2) >> 1) & 1))) { fail(ERR_O_FULL); break; }
+                if (__any_sync(0xffffffffu, aborted())) break;
                 tcgen05_fence_after();
-                const uint32_t to = tmem + i * 128 + (st & 1) * 64;
+                if (elect_one()) {
+                    const uint32_t to = tmem + i * 128 + (st & 1) * 64;
 #pragma unroll
-                for (int half = 0; half < Z::kHalves; ++half) {
-                    const uint64_t da = smem_desc_sw128(q_smem + i * Z::kQ + half * kQHalf), db = smem_desc_sw128(k_smem + s * Z::kKv + half * kKHalf);
+                    for (int half = 0; half < Z::kHalves; ++half) {
+                        const uint64_t da = smem_desc_sw128(q_smem + i * Z::kQ + half * kQHalf), db = smem_desc_sw128(k_smem + s * Z::kKv + half * kKHalf);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tcgen05_mma_f16(to, da + 2 * k, db + 2 * k, Z::idesc(64), (half | k) != 0);
+                        for (int k = 0; k < 4; ++k) tcgen05_mma_f16(to, da + 2 * k, db + 2 * k, Z::idesc(64), (half | k) != 0);
+                    }
+                    tcgen05_mma_f16(to, smem_desc_plain(qx_smem + i * kQExtra, 128), smem_desc_plain(kx_smem + s * kKExtra, 64), Z::idesc(64), 1);
+                    tcgen05_commit(smem_u32(&s_full[i][st & 1]));
                 }
-                tcgen05_mma_f16(to, smem_desc_plain(qx_smem + i * kQExtra, 128), smem_desc_plain(kx_smem + s * kKExtra, 64), Z::idesc(64), 1);
-                tcgen05_commit(smem_u32(&s_full[i][st & 1]));
+                __syncwarp();
             }
         }
         __syncwarp();
     } else if (warp >= kSoftmaxWarps + 2) {
         // ---- a half's weighted values, issued by one thread ----
         const int i = warp - kSoftmaxWarps - 2;
-        if (lane == 0) {
 #pragma unroll 1
-            for (int st = 0; st < n_steps && !aborted(); ++st) {
-                const int s = st % kStages;
-                if (!mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1)) { fail(ERR_FULL); break; }
-                if (!mbar_wait_bounded(smem_u32(&p_full[i][st & 1]), (st >> 1) & 1)) { fail(ERR_P_FULL); break; }
-                tcgen05_fence_after();
+        for (int st = 0; st < n_steps; ++st) {
+            const int s = st % kStages;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1))) { fail(ERR_FULL); break; }
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&p_full[i][st & 1]), (st >> 1) & 1))) { fail(ERR_P_FULL); break; }
+            if (__any_sync(0xffffffffu, aborted())) break;
+            tcgen05_fence_after();
+            if (elect_one()) {
                 const uint64_t db = smem_desc_sw128(v_smem + s * Z::kKv);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
@@ -414,6 +425,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                 tcgen05_commit(smem_u32(&o_done[i][st & 1]));
                 tcgen05_commit(smem_u32(&empty[s]));             // (the page's scores were formed before)
             }
+            __syncwarp();
         }
         __syncwarp();
     } else {
