@@ -4,10 +4,11 @@
 // every key and value.  Four warps unpack the codes, a page of 64 keys a step, into fp16 tiles in shared memory: K [keys][d] and V
 // [d][keys], 128-byte swizzle, the K-major operands of S = Q K^T and O += P V (tcgen05.mma, accumulators in tensor memory); four tiles of each.  Eight
 // warps are the softmax, a thread to a row, which writes P as fp16 over the S it read; four more issue the products, one each for the scores and the
-// values of a half of 128 rows (an issuing thread is busy for some 1,300 cycles a page with its waits).  A half has two S: the next page's scores are
-// formed while this one's are in the softmax, so that only the softmax itself is in a row's way.  (2,048 tokens of 32 heads on 2 behind 4,101 keys, 172
-// GFLOP: one S of 128 keys, whose softmax waits for its products, 347 us; two S and one issuing warp 333, two issuing warps 269, powers of
-// two by 16 tokens instead of by page 262, four issuing warps and one barrier for a page's keys and values 247, 700 TFLOP/s.)
+// values of a half of 128 rows.  A half has two S: the next page's scores are formed while this one's are in the softmax, so that only the softmax
+// itself is in a row's way.  (2,048 tokens of 32 heads on 2 behind 4,101 keys, 172 GFLOP: one S of 128 keys, whose softmax waits for its products, 347
+// us; two S and one issuing warp 333, two issuing warps 269, powers of two by 16 tokens instead of by page 262, four issuing warps and one barrier for a
+// page's keys and values 247, products issued by an elected thread of a converged warp instead of by lane 0 in a branch 231, no look at the abort flag
+// before a wait has failed 226, 760 TFLOP/s.)
 //
 // fp16 and not bf16: its 11 bits hold s (c - 8) exactly, 8 bits times 3, so that scores are as exact as their fp32 sums.  The rest of a
 // key's product, m times the sum of the query's half row, is 16 more columns of the operands: m three times and the sum as three fp16 numbers,
@@ -17,9 +18,9 @@
 // values so far.
 //
 // Unpacking a key and a value costs about two instructions a number, 256 rows of softmax four to five; a block of 128 rows would pay it twice.
-// Bound by the four unpacking warps, which are one to a scheduler and wait for each instruction before the next: 2,500 cycles a page, where the
-// softmax takes 1,400 to 2,000 and the products 1,400.  (Eight of them, with the softmax in runs of 32 keys or its registers given by the issuing warps, took
-// 279 to 298 us: what they hide they take from the softmax.)
+// Bound by two chains of about 2,400 cycles a page, the four unpacking warps' (one to a scheduler, which waits for each instruction before the next) and
+// the softmax's (two to a scheduler; exponentials alone are 1,024), where the products take 1,400.  (Eight unpacking warps with registers that the issuing
+// warps give up, 228 us: the softmax is as long.  Scores taken 32 at a time to need fewer registers, 250.)
 //
 // Every wait is bounded: a block that gives up records an error, stops, frees its tensor memory and returns (nothing is in flight then: tiles are
 // written by ordinary stores).
@@ -254,7 +255,17 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
         atomicCAS(&g_error, 0, code);
         atomicExch(&abort_flag, 1);
     };
-    auto aborted = [&]() { return *(volatile int*)&abort_flag != 0; };
+    // A wait that another role's failure ends too (looked at only when the barrier is not ready: it would lengthen every step).
+    auto wait = [&](const uint64_t& bar, uint32_t parity) {
+        const uint32_t at = smem_u32(&bar);
+        if (mbar_try_wait(at, parity)) return true;
+#pragma unroll 1
+        for (uint32_t i = 1; i < kSpinLimit; ++i) {
+            if (mbar_try_wait(at, parity)) return true;
+            if (*(volatile int*)&abort_flag != 0) break;
+        }
+        return false;
+    };
 
     if (warp >= kSoftmaxWarps + kIssueWarps) {
         // ---- unpacking: a warp takes 16 tokens of every page, whose codes were asked for a page ahead ----
@@ -282,7 +293,6 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
         const auto unpack = [&](Slice<D>& now, int st) {
             const int left = kv_len - (page0 + st) * kPageTokens;
             if (left < kPageTokens) now.trim(slice, lane, left);
-            if (__any_sync(0xffffffffu, aborted())) alive = false;
             const int s = st % kStages, ph = (st / kStages) & 1;
             // the largest magnitudes of the 16 tokens' keys and values; tokens whose values are no numbers
             const float k_bound = bound_of(now.k1), v_bound = bound_of(now.v1);
@@ -325,7 +335,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                     }
                 }
             }
-            if (alive && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&empty[s]), ph ^ 1))) {
+            if (alive && !__all_sync(0xffffffffu, wait(empty[s], ph ^ 1))) {
                 if (lane == 0) fail(ERR_EMPTY);
                 alive = false;
             }
@@ -384,13 +394,12 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
         // ---- a half's scores, issued by one thread as soon as a page's keys are there and an S is free ----
         const int i = warp - kSoftmaxWarps;
         if (n_steps > 0) {
-            if (!mbar_wait_bounded(smem_u32(&q_full[i]), 0)) fail(ERR_Q);
+            if (!wait(q_full[i], 0)) fail(ERR_Q);
 #pragma unroll 1
             for (int st = 0; st < n_steps; ++st) {
                 const int s = st % kStages;
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1))) { fail(ERR_FULL); break; }
-                if (st >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i][st & 1]), ((st - 2) >> 1) & 1))) { fail(ERR_O_FULL); break; }
-                if (__any_sync(0xffffffffu, aborted())) break;
+                if (!__all_sync(0xffffffffu, wait(full[s], (st / kStages) & 1))) { fail(ERR_FULL); break; }
+                if (st >= 2 && !__all_sync(0xffffffffu, wait(o_done[i][st & 1], ((st - 2) >> 1) & 1))) { fail(ERR_O_FULL); break; }
                 tcgen05_fence_after();
                 if (elect_one()) {
                     const uint32_t to = tmem + i * 128 + (st & 1) * 64;
@@ -413,9 +422,8 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
 #pragma unroll 1
         for (int st = 0; st < n_steps; ++st) {
             const int s = st % kStages;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&full[s]), (st / kStages) & 1))) { fail(ERR_FULL); break; }
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&p_full[i][st & 1]), (st >> 1) & 1))) { fail(ERR_P_FULL); break; }
-            if (__any_sync(0xffffffffu, aborted())) break;
+            if (!__all_sync(0xffffffffu, wait(full[s], (st / kStages) & 1))) { fail(ERR_FULL); break; }
+            if (!__all_sync(0xffffffffu, wait(p_full[i][st & 1], (st >> 1) & 1))) { fail(ERR_P_FULL); break; }
             tcgen05_fence_after();
             if (elect_one()) {
                 const uint64_t db = smem_desc_sw128(v_smem + s * Z::kKv);
@@ -486,8 +494,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
         bool ok = true;
 #pragma unroll 1
         for (int st = 0; st < n_steps; ++st) {
-            if (__any_sync(0xffffffffu, aborted())) { ok = false; break; }
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&s_full[i][st & 1]), (st >> 1) & 1))) {
+            if (!__all_sync(0xffffffffu, wait(s_full[i][st & 1], (st >> 1) & 1))) {
                 if (lane == 0) fail(ERR_S_FULL);
                 ok = false;
                 break;
@@ -533,7 +540,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                     l *= alpha;
                     if (st > 0) {
                         // the products of the page before have to be in O
-                        if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i][(st - 1) & 1]), ((st - 1) >> 1) & 1)) && lane == 0) fail(ERR_O_FULL);
+                        if (!__all_sync(0xffffffffu, wait(o_done[i][(st - 1) & 1], ((st - 1) >> 1) & 1)) && lane == 0) fail(ERR_O_FULL);
                         tcgen05_fence_after();
                         const float by = alpha * power2(power - power_new);
 #pragma unroll 1
@@ -588,7 +595,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             if (lane == 0) mbar_arrive(smem_u32(&p_full[i][st & 1]));
         }
         if (ok && n_steps > 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&o_done[i][(n_steps - 1) & 1]), ((n_steps - 1) >> 1) & 1))) {
+            if (!__all_sync(0xffffffffu, wait(o_done[i][(n_steps - 1) & 1], ((n_steps - 1) >> 1) & 1))) {
                 if (lane == 0) fail(ERR_O_FULL);
                 ok = false;
             }
