@@ -17,7 +17,7 @@
 // uniform registers.  Blocks of four warps, three an SM, leave three times as many parts to add up: 41 us where blocks of twelve took 30, for one
 // sequence of 131,071 keys.)
 //
-// 32 heads on 2 of 128, bf16: 1,000 keys 11 us, 131,071 keys 28 us (1.35 TB/s of records); 64 sequences of 1 to 8,192 keys, 14 heads on 2 of 64,
+// 32 heads on 2 of 128, bf16: 1,000 keys 11 us, 131,071 keys 26 us (1.45 TB/s of records); 64 sequences of 1 to 8,192 keys, 14 heads on 2 of 64,
 // 28 us (1.6 TB/s); 5 of 300 to 2,500 keys, fp32, 9 us; 200 of 1 to 4,000, 32 heads on 8 of 128, 163 us (2.9 TB/s).  Bound, where there are many keys, by
 // instructions: a slice of 16 tokens costs a warp some 500, of which unpacking the codes is a third; where there are few, by the way to the first
 // key: 2 us for lengths and shares, 1 for page numbers, 1 for queries, 2 for the first slice and 2 for the parts, whose instructions
@@ -192,7 +192,7 @@ struct Smem {
     float q_sum[kCols][2], factor[kCols];
     int last[kCols];                                   // a column's last key, -1: no such column
     int scan[kWarps];
-    int place, last_block;                             // of the head that the block writes (-1: none); of its row, where it has one only
+    int last_block;                                    // of the block's row, where it has one only, else -1
     int prefix[kMostTiles + 1];
     Tile tiles[kMostTiles];
 };
@@ -212,11 +212,13 @@ __device__ __forceinline__ int block_of(const Shares& s, int at) {
     const int longer = s.more * (s.each + 1);
     return at < longer ? at / (s.each + 1) : s.more + (at - longer) / s.each;
 }
-// Sharing by rows: a block works on one row alone, a row has a block or more by its number of pages.  Taken where there are four blocks or more
-// to a row of single tokens: a block that another row begins in takes as long again for its queries and sums as for 15 pages.
+// Sharing by rows: a block works on one row alone, a row has a block or more by its number of pages.  Possible where there is a block for every row of
+// single tokens, and taken where the longest piece of a row is no more than 5/4 of a piece of the line, in which a block may end one row and begin
+// another: us by rows and by the line, 32 heads on 2 of 128, 2,000 keys each: 5 sequences 11.9 and 15.0, 18 17.3 and 20.5, 36 24.1 and 28.6, 72 29.0 and
+// 42.7; 1 to 4,000 keys: 18 17.3 and 20.8, 36 (28 pages against 21) 28.5 and 28.1, 72 (63 against 42) 42.4 and 41.8.
 __host__ __device__ __forceinline__ int rows_of_tile(const AttendArgs& a, int columns) { return a.n_kv * ((a.group + columns - 1) / columns); }
-__host__ __device__ __forceinline__ bool shares_by_rows(const AttendArgs& a, int columns, int blocks) {
-    return !a.cu_q && (int64_t)4 * a.n_tiles * rows_of_tile(a, columns) <= blocks;
+__host__ __device__ __forceinline__ bool few_rows(const AttendArgs& a, int columns, int blocks) {
+    return !a.cu_q && (int64_t)a.n_tiles * rows_of_tile(a, columns) <= blocks;
 }
 
 // The tiles and the prefix sums of their rows' costs; every thread of the block takes part.  (A row without keys counts as one page, for the
@@ -271,8 +273,8 @@ __device__ __forceinline__ int find_tile(const int* prefix, int n, int at) {
 }
 
 // Scratch: a head of kHeadInts numbers for every block, then two parts a block.  A part holds for each column the weighted values, the
-// maximum and the sum.  A row that several blocks share has its head, for the kernel that adds up, from the block that begins it: in that block's place,
-// or, where blocks have one row each, in the row's.
+// maximum and the sum.  A row that several blocks share has its head, for the kernel that adds up, from the block that begins it: in the row's place
+// where there is a head for every row, else in that block's.
 struct CutRow { int first_block, last_block, row, part, head, columns; };
 constexpr int kHeadInts = 8;
 template <int D> constexpr int kPartStride = D + 4;
@@ -297,15 +299,31 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
     sum_tiles(a, COLS, EXTRA, sm.tiles, sm.prefix, sm.scan);
     const int cost = sm.prefix[a.n_tiles];
     int begin = 0, end = 0, start = 0;                                                    // the block's piece of the line, and its first tile
-    if (shares_by_rows(a, COLS, gridDim.x)) {
-        // a row of n pages has 1 + n / each blocks, but no more than have a page for each of their groups
-        const int per_tile = rows_of_tile(a, COLS), rows = a.n_tiles * per_tile, spare = (int)gridDim.x - rows;
-        const int each = (cost - rows * EXTRA + spare - 1) / spare;
+    const bool few = few_rows(a, COLS, gridDim.x);
+    const int per_tile = rows_of_tile(a, COLS);
+    const Shares shares = shares_of(cost, GROUPS, gridDim.x);
+    // a row of n pages has 1 + n / each blocks, but no more than have a page for each of their groups
+    int each = 0;
+    const auto blocks_of = [&](int pages) { return min(1 + pages / each, (pages + GROUPS - 1) / GROUPS); };
+    bool by_rows = false;
+    if (few) {
+        const int rows = a.n_tiles * per_tile, spare = (int)gridDim.x - rows;
+        each = spare > 0 ? (cost - rows * EXTRA + spare - 1) / spare : 0x40000000;
+        int longest = 0;
+#pragma unroll 1
+        for (int i = lane; i < a.n_tiles; i += 32) {
+            const int pages = max(1, sm.tiles[i].pages), n = blocks_of(pages);
+            longest = max(longest, (pages + n - 1) / n);
+        }
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        by_rows = 4 * (int64_t)longest <= 5 * (int64_t)(shares.each + 1);
+    }
+    if (by_rows) {
         int block = blockIdx.x;
 #pragma unroll 1
         for (int i0 = 0; i0 < a.n_tiles; i0 += 32) {
             const int pages = i0 + lane < a.n_tiles ? max(1, sm.tiles[i0 + lane].pages) : 0;
-            const int blocks = pages ? min(1 + pages / each, (pages + GROUPS - 1) / GROUPS) : 0;
+            const int blocks = pages ? blocks_of(pages) : 0;
             int v = blocks * per_tile;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -320,16 +338,12 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
                 const int row = block / n, k = block - row * n, first = sm.prefix[start] + row * (EXTRA + m);
                 begin = first + (k ? EXTRA + k * (m / n) + min(k, m % n) : 0);
                 end = first + EXTRA + (k + 1) * (m / n) + min(k + 1, m % n);
-                if (threadIdx.x == 0) {
-                    sm.last_block = (int)blockIdx.x - k + n - 1;
-                    sm.place = k ? -1 : start * per_tile + row;
-                }
+                if (threadIdx.x == 0) sm.last_block = (int)blockIdx.x - k + n - 1;
                 break;
             }
             block -= __shfl_sync(0xffffffffu, v, 31);
         }
     } else {
-        const Shares shares = shares_of(cost, GROUPS, gridDim.x);
         if ((int)blockIdx.x < shares.sharing) {
             begin = share_begin(shares, blockIdx.x);
             end = share_begin(shares, blockIdx.x + 1);
@@ -337,8 +351,7 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
         }
         if (threadIdx.x == 0) {
             sm.last_block = -1;
-            sm.place = blockIdx.x;
-            reinterpret_cast<CutRow*>(a.scratch + (int64_t)blockIdx.x * kHeadInts)->last_block = -1;
+            if (!few) reinterpret_cast<CutRow*>(a.scratch + (int64_t)blockIdx.x * kHeadInts)->last_block = -1;
         }
     }
     if (begin >= end) return;
@@ -685,10 +698,14 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
         const bool whole = first_page == 0 && stop == pages;
         // a part of a row that an earlier block began lies in the block's first place, one that goes on behind it in the second
         float* mine = part_of<D>(a, gridDim.x, blockIdx.x, first_page == 0, COLS);
-        if (first_page == 0 && threadIdx.x == 0 && (!whole || sm.last_block >= 0)) {
-            const int last = sm.prefix[index] + ((int)in_tile + 1) * (EXTRA + pages) - 1;
-            const int last_block = whole ? -1 : sm.last_block >= 0 ? sm.last_block : block_of(shares_of(sm.prefix[a.n_tiles], GROUPS, gridDim.x), last);
-            *reinterpret_cast<CutRow*>(a.scratch + (int64_t)sm.place * kHeadInts) = CutRow{(int)blockIdx.x, last_block, row, part, head, columns};
+        if (first_page == 0 && threadIdx.x == 0) {
+            const bool by_row = few_rows(a, COLS, gridDim.x);
+            if (!whole || by_row) {
+                const int last = sm.prefix[index] + ((int)in_tile + 1) * (EXTRA + pages) - 1;
+                const int last_block = whole ? -1 : sm.last_block >= 0 ? sm.last_block : block_of(shares_of(sm.prefix[a.n_tiles], GROUPS, gridDim.x), last);
+                const int place = by_row ? index * rows_of_tile(a, COLS) + (int)in_tile : (int)blockIdx.x;
+                *reinterpret_cast<CutRow*>(a.scratch + (int64_t)place * kHeadInts) = CutRow{(int)blockIdx.x, last_block, row, part, head, columns};
+            }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -836,7 +853,7 @@ int attend(const AttendArgs& a, cudaStream_t stream) {
     if (sms <= 0) return CPM_BAD_ARGUMENT;
     const int blocks = sms;
     cpm_launch(kLaunchAttention, kv4_attention_kernel<T, D, NT, TERMS>, dim3(blocks), 32 * warps_of(D, NT, TERMS), bytes, stream, a);
-    const int heads = shares_by_rows(a, 8 * NT, blocks) ? a.n_tiles * rows_of_tile(a, 8 * NT) : blocks;
+    const int heads = few_rows(a, 8 * NT, blocks) ? a.n_tiles * rows_of_tile(a, 8 * NT) : blocks;
     cpm_launch(kLaunchAttention, kv4_combine_kernel<T, D, NT>, dim3(8 * NT, heads), kCombineWarps * 32, 0, stream, a, blocks);
     return launch_status();
 }
