@@ -198,6 +198,19 @@ def test_batches_of_unequal_sequences(dtype, heads, kv, n):
         _check(got, want, rows, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,n,length", [(4, 2, 20, 700), (4, 2, 72, 300), (4, 2, 74, 300), (2, 1, 148, 130), (2, 1, 149, 130), (24, 1, 74, 65)])
+def test_batches_of_like_sequences(dtype, heads, kv, n, length):
+    """Rows of pages of like length, up to as many as a device of 148 multiprocessors has blocks and one more."""
+    ops, d = _ops(dtype), 64
+    lengths = [length + i % 3 for i in range(n)]
+    table, slots, records, rows = _filled(ops, lengths, kv, d, 37)
+    q = torch.randn(n, heads, d, generator=torch.Generator().manual_seed(n)).to(DT[dtype])
+    got = ops.kv4_attention(q.cuda(), records, _i32(lengths), _i32(slots), table, kv, d ** -0.5)
+    want = torch.cat([plain.attention(q[i:i + 1], k, v, m - 1, d ** -0.5, 0) for i, (m, (k, v)) in enumerate(zip(lengths, rows))])
+    _check(got, want, rows, dtype)
+
+
 @pytest.mark.parametrize("tcgen05,shares", [(False, 0), (True, 1), (True, 3), (True, 0)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("d,heads,kv", [(32, 3, 1), (64, 8, 1), (64, 6, 2), (96, 4, 2), (128, 16, 1), (128, 2, 2), (64, 4, 2), (128, 5, 1), (64, 40, 2)])
