@@ -22,8 +22,8 @@
 // the softmax's (two to a scheduler; exponentials alone are 1,024), where the products take 1,400.  (Eight unpacking warps with registers that the issuing
 // warps give up, 228 us: the softmax is as long.  Scores taken 32 at a time to need fewer registers, 250.)
 //
-// Every wait is bounded: a block that gives up records an error, stops, frees its tensor memory and returns (nothing is in flight then: tiles are
-// written by ordinary stores).
+// Every wait is bounded: a block that gives up records an error, stops, lets the products in flight end (tiles are written by ordinary stores, so
+// nothing else is), frees its tensor memory and returns.
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 #include <type_traits>
@@ -629,6 +629,8 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
     tcgen05_fence_before();
     __syncthreads();
     if (warp == kSoftmaxWarps) {
+        if (*(volatile int*)&abort_flag != 0)                 // a product takes less than a microsecond
+            for (int x = 0; x < 16; ++x) __nanosleep(20000);
         tcgen05_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
