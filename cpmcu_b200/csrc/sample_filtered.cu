@@ -37,7 +37,7 @@ constexpr int kFineBins = 1024;                        // of a step of the selec
 constexpr int kListed = 2048;                          // tokens that are set apart for the selection
 constexpr int kRanked = 256;                           // up to so many the first block compares each with each, and draws without the others
 constexpr int kLimbBits = 14;                          // a mass is added in three limbs: 32-bit adds in shared memory are one instruction
-constexpr int kMostVocab = 1 << 21;                    // so that a limb's sum over a block's tokens stays within 32 bits
+constexpr int kMostVocab = 1 << 21;                    // so that a limb's sum over the tokens of a block, an eighth of them, stays within 32 bits
 
 struct FilterArgs {
     const float* logits;
@@ -71,6 +71,7 @@ struct FilterShared {
             uint32_t list[kListed];                    // bits of the weights that are set apart, in the first block
             int place[kListed];                        // and their tokens
         };
+        alignas(8) uint64_t joined[kFineBins];         // where they are too many: what the other blocks have in each fine bin, in the first block
         uint32_t own[2][kCoarseBins];                  // before that: the block's bins, see count_own
     };
     int listed;
@@ -110,6 +111,9 @@ __device__ __forceinline__ void put32(const void* own, uint32_t rank, uint32_t v
 }
 __device__ __forceinline__ void put64(const void* own, uint32_t rank, uint64_t v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(cluster_address(own, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void add64(const void* own, uint32_t rank, uint64_t v) {
+    asm volatile("red.shared::cluster.add.u64 [%0], %1;" :: "r"(cluster_address(own, rank)), "l"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t add32(const void* own, uint32_t rank, uint32_t v) {
     uint32_t old;
@@ -257,20 +261,28 @@ struct Row {
 
 struct Border { uint32_t bits; uint64_t above, here; };      // a weight, and the count or mass of the tokens above it and at it
 
-// The bin of sm.fine, counts or masses in limbs, at which the running sum from the last bin down, starting with ``above``, first reaches ``need``: left in
-// sm.found_bin, with what lies above it and in it.
-__device__ __noinline__ void find_fine(FilterShared& sm, double need, uint64_t above) {
-    const int bin = kFineBins - 2 - 2 * threadIdx.x;    // two bins a thread
-    uint64_t v[2] = {0, 0};
+// What the block has in a fine bin.
+__device__ __forceinline__ uint64_t own_fine(const FilterShared& sm, int bin) {
+    uint64_t v = 0;
 #pragma unroll
-    for (int u = 0; u < 3; ++u) {
-        v[0] += (uint64_t)sm.fine[u][bin + 1] << (u * kLimbBits);
-        v[1] += (uint64_t)sm.fine[u][bin] << (u * kLimbBits);
+    for (int u = 0; u < 3; ++u) v += (uint64_t)sm.fine[u][bin] << (u * kLimbBits);
+    return v;
+}
+// The bin of sm.fine, counts or masses in limbs, at which the running sum from the last bin down, starting with ``above``, first reaches ``need``: left in
+// sm.found_bin, with what lies above it and in it.  ``joined``: with the other blocks' in sm.joined.  Exactly one bin is found, whatever the sums: the last
+// one looked at needs not reach ``need``, and the first may be reached before it.
+__device__ __noinline__ void find_fine(FilterShared& sm, double need, uint64_t above, bool joined) {
+    const int bin = kFineBins - 2 - 2 * threadIdx.x;    // two bins a thread
+    uint64_t v[2] = {own_fine(sm, bin + 1), own_fine(sm, bin)};
+    if (joined) {
+        v[0] += sm.joined[bin + 1];
+        v[1] += sm.joined[bin];
     }
     uint64_t upto = above + block_scan64(v[0] + v[1], sm.warp_sum) - v[0] - v[1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        if ((double)upto < need && (double)(upto + v[i]) >= need) {
+        const bool first = bin + 1 - i == kFineBins - 1, last = bin + 1 - i == 0;
+        if ((first || (double)upto < need) && (last || (double)(upto + v[i]) >= need)) {
             sm.found_bin = bin + 1 - i;
             sm.found_before = upto;
             sm.found_here = v[i];
@@ -311,7 +323,7 @@ __device__ __noinline__ Border select(FilterShared& sm, bool mass, int listed, d
             if (bits >= low && bits < high && (key >> done) == prefix) add_fine(sm, mass, (key >> shift) & ((1u << (done - shift)) - 1), bits);
         }
         __syncthreads();
-        find_fine(sm, need, above);
+        find_fine(sm, need, above, false);
         prefix = (prefix << (done - shift)) | sm.found_bin;
         above = sm.found_before;
         done = shift;
@@ -377,7 +389,7 @@ __device__ __forceinline__ uint64_t find_mass(FilterShared& sm, bool summed, flo
 
 // Of the tokens at a border that mass decides, how many it takes.
 __device__ __forceinline__ uint64_t ties_of(const Border& b, double need, uint64_t* equal) {
-    const uint64_t each = units_of(b.bits), there = b.here / each;
+    const uint64_t each = max((uint64_t)1, units_of(b.bits)), there = b.here / each;
     uint64_t n = (uint64_t)ceil((need - (double)b.above) / (double)each);
     n = min(max(n, (uint64_t)1), there);
     while (n > 1 && (double)(b.above + (n - 1) * each) >= need) --n;
@@ -552,7 +564,11 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
 #pragma unroll 1
             while (true) {
                 if (rank == 0) {
-                    if (some > kListed) clear_fine(sm);
+                    if (some > kListed) {
+#pragma unroll 1
+                        for (int i = tid; i < kFineBins; i += kFilterThreads) sm.joined[i] = 0;
+                        clear_fine(sm);
+                    }
                     if (tid == 0) {
                         sm.plan.low = low;
                         sm.plan.high = high;
@@ -623,21 +639,24 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 } else if (rank > 0) {
                     __syncthreads();
 #pragma unroll 1
-                    for (int i = tid; i < 3 * kFineBins; i += kFilterThreads)
-                        if (sm.fine[0][i]) add32(&sm.fine[0][i], 0, sm.fine[0][i]);
+                    for (int i = tid; i < kFineBins; i += kFilterThreads) {
+                        const uint64_t v = own_fine(sm, i);          // (the row's limbs could exceed 32 bits)
+                        if (v) add64(&sm.joined[i], 0, v);
+                    }
                 }
                 cluster_sync();
                 if (!known) above = all_mass();
                 known = true;
                 if (apart) {
-                    listed = (int)peer32(&sm.listed, 0);
+                    listed = min((int)peer32(&sm.listed, 0), kListed);
                     if (rank == 0 && !(complete && listed <= kRanked)) b = select(sm, round > 0, listed, need, complete ? 0 : above, low, high);
                     break;
                 }
                 // ---- too many for the list (equal weights, or a mass that flat tails make up): their masses in 1,024 bins, and on with one of these ----
                 if (rank == 0) {
-                    find_fine(sm, need, above);
-                    low += (uint32_t)sm.found_bin << shift;
+                    find_fine(sm, need, above, true);
+                    // (never beyond the range, so that it stays one, and ``shift`` falls until a single weight is left)
+                    low += min((uint32_t)sm.found_bin, (high - low - 1) >> shift) << shift;
                     high = min(high, low + (1u << shift));
                     above = sm.found_before;
                     some = round > 0 ? sm.found_here / max((uint64_t)1, units_of(low)) : sm.found_here;

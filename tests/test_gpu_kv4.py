@@ -552,6 +552,20 @@ def test_sample_filtered_where_bins_are_full_or_tiny(rows, vocab, spread):
     assert torch.equal(ops.sample_filtered(*args)[0].long(), _defined(*args))
 
 
+@pytest.mark.parametrize("vocab,of_one", [(1 << 20, 1.0), (1 << 21, 1.0), (1 << 19, 2.0 ** -12 * (1 - 2.0 ** -20)), (1 << 21, 2.0 ** -12 * (1 - 2.0 ** -20)),
+                                          (350000, math.exp(-1)), (300000, 2.0 ** -39)])
+def test_sample_filtered_of_flat_rows_above_2_18_tokens(vocab, of_one):
+    """One token of weight 1 and all others of one weight: the blocks of a cluster find them in a single bin, whose mass needs more than 32 bits in every limb."""
+    ops = _ops("bfloat16")
+    z = torch.full((6, vocab), math.log(of_one))
+    z[:, vocab // 3] = 0.0
+    u = torch.tensor([0.1, 0.5, 0.9, 1 - 2.0 ** -24, 0.7, 0.0])
+    p = torch.tensor([0.9, 0.3, 0.99999, 1 - 2.0 ** -20, 0.5, 0.9])
+    k = torch.tensor([0, 0, 0, 0, vocab - 7, vocab // 2], dtype=torch.int32)
+    args = [x.cuda() for x in (z, u, torch.ones(6), k, p, torch.zeros(6))]
+    assert torch.equal(ops.sample_filtered(*args)[0].long(), _defined(*args))
+
+
 def test_sample_filtered_is_distributed_as_it_should():
     """Frequencies over many given numbers against the kept probabilities: with 200,000 draws a share moves by 0.0011 (one sigma at one half)."""
     ops, vocab, n = _ops("bfloat16"), 50, 200000
