@@ -416,7 +416,8 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     int k = a.top_k ? a.top_k[r] : 0;
     float ratio = a.min_p ? a.min_p[r] : 0.f;
     if (p <= 0.f || ratio > 1.f) k = 1;
-    if (!(ratio <= 1.f)) ratio = 0.f;                          // above one: the first token alone, which it would leave out as well
+    // above one: the first token alone, which it would leave out as well; below zero, -0 (weights are compared by their bits) or no number: no limit
+    if (!(ratio > 0.f && ratio <= 1.f)) ratio = 0.f;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
     const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[r], (uint32_t)a.step_key[r]);
 

@@ -492,6 +492,16 @@ def test_sample_filtered_edges():
     _compare(_ops("bfloat16"), z, u, t, k, p, m)
 
 
+@pytest.mark.parametrize("ratio", [-0.0, -0.1, -math.inf, math.nan])
+def test_sample_filtered_takes_a_min_p_of_no_more_than_zero_as_none(ratio):
+    """Alone, with few and with many tokens left by top-k, and with top-p: the token is the one without min-p."""
+    vocab = 1500
+    z = torch.randn(5, vocab, generator=torch.Generator().manual_seed(8))
+    k = torch.tensor([0, 20, 1000, 0, 1000], dtype=torch.int32)
+    p = torch.tensor([1.0, 1.0, 1.0, 0.7, 0.7])
+    _compare(_ops("bfloat16"), z, torch.full((5,), 0.6), torch.ones(5), k, p, torch.full((5,), ratio))
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 73448), (64, 73448), (200, 40000), (1, 500000)])
 def test_sample_filtered_large_rows(rows, vocab):
     """The largest vocabularies, against the definition in whole numbers on the device; the last does not fit in shared memory."""
