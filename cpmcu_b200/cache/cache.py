@@ -148,13 +148,16 @@ class CacheGroup:
         """What the group's pages hold: [lanes, pages, ...] each."""
         return [t for t in (self.k, self.v, self.pooled, self.records) if t is not None]
 
+    def shared_pages(self, length: int) -> int:
+        """Pages that a sequence of ``length`` tokens and its forks hold together: full ones, which are never written again, but for
+        the pooled keys whose windows reach into the next one."""
+        return max(0, length - self.needs.pooled_kernel + 1 if self.needs.pooled_stride else length) // PAGE_TOKENS
+
     def fork(self, slot: int, children: Sequence[int], length: int) -> List[Tuple[int, int]]:
         """The children hold the sequence's pages with it; from the first page on that a later token still changes each takes
         pages of its own.  Returns the pages to copy, (from, to).  All or nothing."""
         pages = self.pages_of_slot.get(slot, [])[:pages_for(length)]
-        # a full page is never written again, but for the pooled keys whose windows reach into the next one
-        own = max(0, length - self.needs.pooled_kernel + 1 if self.needs.pooled_stride else length) // PAGE_TOKENS
-        own = min(own, len(pages))
+        own = min(self.shared_pages(length), len(pages))
         shared = [p for p in pages[:own] if p != RELEASED]
         fresh = self.pages.take((len(pages) - own) * len(children))
         moves: List[Tuple[int, int]] = []
@@ -170,9 +173,7 @@ class CacheGroup:
 
     def fork_needs(self, slot: int, n: int, length: int) -> int:
         """Pages that ``fork`` takes for ``n`` children."""
-        pages = pages_for(length)
-        own = max(0, length - self.needs.pooled_kernel + 1 if self.needs.pooled_stride else length) // PAGE_TOKENS
-        return max(0, pages - own) * n
+        return max(0, pages_for(length) - self.shared_pages(length)) * n
 
     def compact(self) -> List[Tuple[int, int]]:
         """Gives the held pages the lowest numbers; returns the pages to copy, (from, to)."""
@@ -393,6 +394,10 @@ class Cache:
         states = [t.unsqueeze(0) for lane in self.lanes for t in lane.state.values()]
         self._copy(states, [(slot, child) for child in children])
         return children
+
+    def shared_pages(self, length: int) -> int:
+        """Pages of every group that a sequence of ``length`` tokens and its forks hold together at least."""
+        return min((g.shared_pages(length) for g in self.groups if g.tensors()), default=length // PAGE_TOKENS)
 
     def compact(self) -> int:
         """Moves pages so that every group's held ones have the lowest numbers, behind what is queued on the current stream; the next

@@ -52,6 +52,9 @@ class EngineBackend:
     def max_sequence_pages(self) -> int:
         return self.stepper.cache.max_pages_per_seq
 
+    def shared_pages(self, length: int) -> int:
+        return self.stepper.cache.shared_pages(length)
+
     def vocab_size(self) -> int:
         return self.stepper.vocab_size
 

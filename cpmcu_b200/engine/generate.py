@@ -44,7 +44,8 @@ class Backend(Protocol):
     # Optional: ``prefill_forked(prompts, which, keys, sampling)``, as ``prefill`` for sequences that begin alike (needed for requests
     # with a ``group``).
     # Optional: ``max_sequence_pages()`` (the most pages one sequence may hold) and ``vocab_size()``; with them
-    # a request that cannot run is refused before anything is opened.
+    # a request that cannot run is refused before anything is opened.  ``shared_pages(length)``: pages that forks of a prompt of
+    # ``length`` tokens hold together with it (default: its full ones).
 
 
 @dataclass
@@ -74,9 +75,11 @@ class GenerationStats:
 
 
 def plan_batches(requests: Sequence[Request], max_batch: int, capacity_pages: int,
-                 max_sequence_pages: Optional[int] = None, vocab_size: Optional[int] = None) -> List[List[int]]:
+                 max_sequence_pages: Optional[int] = None, vocab_size: Optional[int] = None,
+                 shared_pages: Optional[Callable[[int], int]] = None) -> List[List[int]]:
     """Cuts the requests, in order, into batches that fit: at most ``max_batch`` sequences,
-    and pages for every sequence grown to its full length.  A request that can never run (longer than
+    and pages for every sequence grown to its full length (those that a group's requests share, ``shared_pages``
+    of the prompt's length or all its full ones, once).  A request that can never run (longer than
     the cache or than one sequence may be, a token id outside the vocabulary) is refused here, before
     any sequence is opened."""
     batches: List[List[int]] = []
@@ -94,8 +97,10 @@ def plan_batches(requests: Sequence[Request], max_batch: int, capacity_pages: in
             bad = next((t for t in r.prompt if not 0 <= int(t) < vocab_size), None)
             if bad is not None:
                 raise ValueError(f"request {i}: token id {bad} is outside the vocabulary [0, {vocab_size})")
-        # one more of a group holds the prompt's full pages with the first
-        shared = len(r.prompt) // PAGE_TOKENS if r.group is not None and any(requests[j].group == r.group for j in cur) else 0
+        # one more of a group holds pages of the prompt with the first
+        shared = 0
+        if r.group is not None and any(requests[j].group == r.group for j in cur):
+            shared = shared_pages(len(r.prompt)) if shared_pages else len(r.prompt) // PAGE_TOKENS
         if cur and (len(cur) >= max_batch or pages + need - shared > capacity_pages):
             batches.append(cur)
             cur, pages, shared = [], 0, 0
@@ -124,7 +129,7 @@ def run_requests(backend: Backend, requests: Sequence[Request],
     per_seq = getattr(backend, "max_sequence_pages", None)
     vocab = getattr(backend, "vocab_size", None)
     plan = plan_batches(requests, backend.max_batch(), backend.capacity_pages(),
-                        per_seq() if per_seq else None, vocab() if vocab else None)
+                        per_seq() if per_seq else None, vocab() if vocab else None, getattr(backend, "shared_pages", None))
     try:
         _run_batches(backend, requests, plan, results, stats, on_token, sync)
     except BaseException:

@@ -218,6 +218,57 @@ def test_plan_batches_counts_shared_pages_once():
     assert plan_batches([Request([0] * 130, 20) for _ in range(4)], 8, 6) == [[0, 1], [2, 3]]
 
 
+class CacheBackend(ForkingBackend):
+    """Scripted tokens over a cache whose sequences grow by a token a step."""
+
+    def __init__(self, cache):
+        super().__init__(cache.n_pages - 1, 8)
+        self.cache = cache
+        pad = cache.open_sequence()
+        cache.reserve(pad, 1)
+
+    def shared_pages(self, length):
+        return self.cache.shared_pages(length)
+
+    def _grow(self, slot, length):
+        self.cache.reserve(slot, length)
+        self.cache.set_length(slot, length)
+
+    def prefill_forked(self, prompts, which, keys, sampling):
+        firsts = self.cache.open_sequences(len(prompts))
+        slots_of = []
+        for i, (s, p) in enumerate(zip(firsts, prompts)):
+            self._grow(s, len(p))
+            slots_of.append([s] + self.cache.fork_sequence(s, which.count(i) - 1))
+        self.slots = [slots_of[w].pop(0) for w in which]
+        return super().prefill_forked(prompts, which, keys, sampling)
+
+    def decode(self, live, *args):
+        for p in live:
+            self._grow(self.slots[p], self.cache.length(self.slots[p]) + 1)
+        self.cache.check_consistent()
+        return super().decode(live, *args)
+
+    def finish(self, index):
+        super().finish(index)
+        self.cache.close_sequence(self.slots[index])
+
+
+@pytest.mark.parametrize("kernel,stride", [(0, 0), (32, 16), (128, 32)])
+@pytest.mark.parametrize("length", [1, 63, 64, 94, 95, 96, 128, 130, 159, 191, 192])
+def test_groups_that_are_planned_can_be_forked(length, kernel, stride):
+    """Every cache that holds one request alone runs a group of four, in as many batches as its pages allow: with pooled keys forks share
+    fewer pages than the prompt fills."""
+    need = pages_for(length + 20)
+    for pages in range(need, 4 * need + 1):
+        c = Cache([CacheNeeds(kv_heads=1, head_dim=16), CacheNeeds(kv_heads=1, head_dim=16, pooled_stride=stride, pooled_kernel=kernel)],
+                  max_tokens=64 * (pages + 1), dtype=torch.float32, device="cpu", n_slots=9)
+        b = CacheBackend(c)
+        out, stats = run_requests(b, [Request([1] * length, 20, key=j, group=0) for j in range(4)])
+        assert [len(f.tokens) for f in out] == [20] * 4 and c.slots.n_held == 1
+        assert stats.batches == 1 or pages < 4 * need - 3 * c.shared_pages(length)
+
+
 def test_sampling_params():
     assert not SamplingParams(0.7, 0.9).filtered and not SamplingParams(0.0, 1.0, 5, 0.1).filtered
     assert SamplingParams(0.7, 1.0, 5).filtered and SamplingParams(0.7, min_p=0.1).filtered
