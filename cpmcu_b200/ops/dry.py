@@ -90,6 +90,11 @@ class DryOps(Ops):
         arena = Arena(None, None)
         self.workspace = Workspace(arena.carve("persistent", None), [arena.carve("frame0", None), arena.carve("frame1", None)])
         self.weights = None
+        self.shared_keys = set()             # (heads, key-value heads) of prompts' attention whose keys may be shared out
+
+    def kv4_prompt_shares(self, n_tokens, n_heads, n_kv, longest):
+        self.shared_keys.add((n_heads, n_kv))
+        return super().kv4_prompt_shares(n_tokens, n_heads, n_kv, longest)
 
     # no device, no checks
     @staticmethod
@@ -237,7 +242,8 @@ def measure_workspace(spec, dtype: torch.dtype, max_step_tokens: int, max_batch:
                   max_seq_tokens=per_seq, max_step_tokens=max_step_tokens)
     recorded = model.recordable_prompt()
     notes: List[str] = []
-    for q_lens, kv, decode, captured, n_tiles in workspace_steps(max_step_tokens, max_batch, per_seq, MAX_GRAPH_PIECES if recorded else 0, sm_count):
+
+    def run(q_lens, kv, decode, captured, n_tiles):
         n_tokens = sum(q_lens)
         ops.workspace.begin_step()
         try:
@@ -249,5 +255,15 @@ def measure_workspace(spec, dtype: torch.dtype, max_step_tokens: int, max_batch:
             note = f"a part could not be measured without a device ({type(e).__name__}: {str(e)[:80]})"
             if note not in notes:
                 notes.append(note)
+
+    for step in workspace_steps(max_step_tokens, max_batch, per_seq, MAX_GRAPH_PIECES if recorded else 0, sm_count):
+        run(*step)
+    # parts of shared-out keys grow with the tokens and with the shares, of which there are fewer the more tokens there are: the last
+    # number of tokens before each step down
+    for n_heads, n_kv in sorted(ops.shared_keys):
+        shares = [ops.kv4_prompt_shares(n, n_heads, n_kv, per_seq) for n in range(1, int(max_step_tokens) + 1)]
+        for n in range(1, len(shares)):
+            if shares[n] < shares[n - 1]:
+                run([n], per_seq, False, False, None)
     persistent, frame = ops.workspace.peaks()
     return persistent, frame, notes

@@ -159,6 +159,37 @@ def test_no_step_needs_more_than_the_workspace_is_measured_for(arch_name, config
             assert need[0] <= given[0] and need[1] <= given[1], (portions[:3], max(portions), len(portions), kv)
 
 
+@pytest.mark.parametrize("chunk,heads,kv,d,intermediate", [(600, 32, 2, 128, 8192), (640, 32, 2, 128, 4096), (700, 16, 2, 64, 2048), (1300, 8, 4, 128, 1024),
+                                                          (300, 40, 40, 64, 1024)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompts_of_every_length_fit_the_workspace_of_a_4_bit_cache(chunk, heads, kv, d, intermediate, dtype):
+    """The parts of a prompt whose keys are shared out over blocks are largest just before the number of shares falls."""
+    from cpmcu_b200.cache import Cache as AnyCache
+    from cpmcu_b200.models.model import Model
+    from cpmcu_b200.ops.dry import DryOps, dry_context, measure_workspace
+    from cpmcu_b200.registry import architecture
+
+    arch = architecture("MiniCPMForCausalLM")
+    spec = arch.model_spec(arch.config_class.from_dict(dict(
+        configs.tiny_e(), cache_bits=4, hidden_size=256, num_attention_heads=heads, num_key_value_heads=kv, head_dim=d, intermediate_size=intermediate,
+        num_hidden_layers=1)))
+    _, frame, notes = measure_workspace(spec, dtype, chunk, 8, 16384)
+    assert notes == []
+    given = int(frame * 1.05) + (1 << 20)
+    ops = DryOps(dtype)
+    model = Model(spec, ops)
+    model.load_weights({name: torch.empty(w.shape, device="meta", dtype=torch.int32 if w.role == "table" else dtype)
+                        for name, w in model.weight_specs().items()})
+    cache = AnyCache(model.cache_needs(), max_tokens=16384, dtype=dtype, device="meta", n_slots=9, max_seq_tokens=16384, max_step_tokens=chunk)
+    for n in range(1, chunk + 1):
+        ops.workspace.begin_step()
+        ctx = dry_context([n], 16384, cache, n == 1)
+        rows = ops.empty(n, dtype=torch.int32)
+        ops.empty(8 * n + 4 + 64, dtype=torch.int32)
+        model.forward(ctx, rows)
+        assert ops.workspace.peaks()[1] <= given, n
+
+
 def test_cache_inside_regions():
     needs = [CacheNeeds(kv_heads=2, head_dim=16), CacheNeeds(kv_heads=1, head_dim=32, state={"s": ((8,), torch.float32)})]
     counting = Arena(None, None)
