@@ -530,19 +530,21 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
                                 if (token <= last && (a.window == 0 || token > last - a.window)) seen |= 1u << (4 * n + 2 * r + c);
                             }
                         // A row that only some columns see and that is no number would reach the others as 0 * NaN: it goes to
-                        // those that see it here, and is nobody's afterwards.
+                        // those that see it here, and is nobody's afterwards; of a value half a row alone, whose other half and whose key stay.
                         const bool kbad = !(fabsf(kv4_scale(kp[r].x)) + fabsf(kv4_middle(kp[r].x)) + fabsf(kv4_scale(kp[r].y)) + fabsf(kv4_middle(kp[r].y)) < INFINITY);
                         const bool bad0 = kbad || !(fabsf(kv4_scale(vp[r].x)) + fabsf(kv4_middle(vp[r].x)) < INFINITY);
                         const bool bad1 = kbad || !(fabsf(kv4_scale(vp[r].y)) + fabsf(kv4_middle(vp[r].y)) < INFINITY);
                         if (bad0 || bad1) {
-                            kp[r] = vp[r] = make_uint2(0u, 0u);
+                            if (bad0) vp[r].x = 0u;
+                            if (bad1) vp[r].y = 0u;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 const f32x2 poison = pair(seen >> (4 * n + 2 * r) & 1 ? NAN : 0.f, seen >> (4 * n + 2 * r + 1) & 1 ? NAN : 0.f);
                                 if (bad0) middle[n][0] = add2(middle[n][0], poison);
                                 if (bad1) middle[n][1] = add2(middle[n][1], poison);
-                                seen &= ~(3u << (4 * n + 2 * r));
+                                if (kbad) seen &= ~(3u << (4 * n + 2 * r));
                             }
+                            if (kbad) kp[r] = make_uint2(0u, 0u);
                         }
                     }
                 }

@@ -72,7 +72,7 @@ struct StepInfo {
     int v_token[kPageTokens];
     alignas(16) float k_scale[4];
     alignas(16) int v_power[4];
-    alignas(16) uint32_t bad[4];                        // tokens whose values are no numbers
+    alignas(16) uint32_t bad[4];                        // value half rows that are no numbers: bit 2 t + h of token t
 };
 
 enum : int { ERR_Q = 1, ERR_FULL, ERR_EMPTY, ERR_S_FULL, ERR_P_FULL, ERR_O_FULL };
@@ -294,20 +294,22 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             const int left = kv_len - (page0 + st) * kPageTokens;
             if (left < kPageTokens) now.trim(slice, lane, left);
             const int s = st % kStages, ph = (st / kStages) & 1;
-            // the largest magnitudes of the 16 tokens' keys and values; tokens whose values are no numbers
+            // the largest magnitudes of the 16 tokens' keys and values; value half rows that are no numbers
             const float k_bound = bound_of(now.k1), v_bound = bound_of(now.v1);
             const bool v_finite = v_bound < INFINITY;
             const float most_k = __uint_as_float(__reduce_max_sync(0xffffffffu, k_bound < INFINITY ? __float_as_uint(k_bound) : 0u));
-            uint32_t bad = __ballot_sync(0xffffffffu, !v_finite);
+            const uint32_t bad = __ballot_sync(0xffffffffu, !v_finite);
             if (bad) {
-                bad = (bad | bad >> 1) & 0x55555555u;           // bit 2 t of token t; the other half row goes too
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    if (bad >> (4 * j4 + 16 * u) & 1) now.vp[u].x = now.vp[u].y = 0u;
-                    if (bad >> (4 * j4 + 16 * u + 2) & 1) now.vp[u].z = now.vp[u].w = 0u;
+                    const uint32_t mine = bad >> (4 * j4 + 16 * u);
+                    if (mine & 1) now.vp[u].x = 0u;
+                    if (mine & 2) now.vp[u].y = 0u;
+                    if (mine & 4) now.vp[u].z = 0u;
+                    if (mine & 8) now.vp[u].w = 0u;
                 }
             }
-            const float most_v = __uint_as_float(__reduce_max_sync(0xffffffffu, bad >> (lane & 30) & 1 ? 0u : __float_as_uint(v_bound)));
+            const float most_v = __uint_as_float(__reduce_max_sync(0xffffffffu, v_finite ? __float_as_uint(v_bound) : 0u));
             const int ek = power_below(most_k), ev = most_v > 0.f ? power_below(most_v) : -110;
             StepInfo& inf = info[st % kInfos];
             if (lane == 0) {
@@ -490,6 +492,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_addr = lanes + Z::kO + i * D;
         float m = -INFINITY, l = 0.f;
+        uint32_t lost = 0;                                   // bit h: the row sees a value whose half h is no number
         int power = -1000;                                   // the accumulator stands for O / 2^power
         bool ok = true;
 #pragma unroll 1
@@ -584,10 +587,10 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             if (in_part(st)) soften(std::true_type{});
             else soften(std::false_type{});
             if (inf.bad[0] | inf.bad[1] | inf.bad[2] | inf.bad[3]) {
-                // values that are no numbers are not in the tile: the rows that see them are no numbers
+                // values that are no numbers are not in the tile: the halves of the rows that see them are no numbers
 #pragma unroll 1
                 for (int e = 0; e < kPageTokens; ++e)
-                    if ((inf.bad[e >> 4] >> (2 * (e & 15)) & 1) && key0 + e <= limit && key0 + e >= from) l = NAN;
+                    if (key0 + e <= limit && key0 + e >= from) lost |= inf.bad[e >> 4] >> (2 * (e & 15)) & 3u;
             }
             tmem_store_wait();
             tcgen05_fence_before();
@@ -607,6 +610,7 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
             const float by = shared ? (n_steps > 0 ? power2(power) : 0.f) : l == 0.f ? 0.f : power2(power) / l;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
+                const float by_half = lost >> (c >= D / 32) & 1 ? NAN : by;
                 uint32_t o[16];
                 if (n_steps > 0) {
                     tmem_load_16cols(o_addr + c * 16, o);
@@ -618,7 +622,8 @@ kv4_prompt_kernel(const __grid_constant__ Args a) {
                 if (valid)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
-                        const float4 y = make_float4(__uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by, __uint_as_float(o[e + 2]) * by, __uint_as_float(o[e + 3]) * by);
+                        const float4 y = make_float4(__uint_as_float(o[e]) * by_half, __uint_as_float(o[e + 1]) * by_half, __uint_as_float(o[e + 2]) * by_half,
+                                                     __uint_as_float(o[e + 3]) * by_half);
                         if (shared) store4(mine + c * 16 + e, y);
                         else store4(a.out + at + c * 16 + e, y);
                     }

@@ -297,6 +297,39 @@ def test_tokens_that_are_not_seen_have_no_part(dtype, poison, tcgen05):
     assert torch.equal(run(0).cpu()[:20], clean[0][:20])
 
 
+@pytest.mark.parametrize("form", ["single", "prompt", "tcgen05", "shared"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d,heads,kv", [(64, 4, 2), (128, 24, 1), (32, 2, 2)])
+@pytest.mark.parametrize("half", [0, 1])
+def test_half_a_value_that_is_no_number(half, d, heads, kv, dtype, form):
+    """A value of which half a row is no number makes that half of the output none for the queries that see it, and leaves the other half: in the last,
+    partial slice, in a whole one, and at a prompt's causal edge, whichever kernel reads it.  A key that is none makes all of the output none."""
+    ops = _ops(dtype)
+    ops.KV4_PROMPT_BLOCKS = 0 if form in ("tcgen05", "shared") else 1 << 30
+    if form == "shared":
+        ops.kv4_prompt_shares = lambda *a: 3
+    n, new = 275, 1 if form == "single" else 40
+    table, slots, total = _tables([n], 5)
+    pos, seq = _every_position([n])
+    g = torch.Generator().manual_seed(3)
+    kvs = torch.randn(n, 2 * kv, d, generator=g)
+    records = torch.zeros(total, kv, ops.kv4_page_bytes(d), dtype=torch.uint8).cuda()
+    f32 = _ops("float32")
+    q = torch.randn(new, heads, d, generator=g).to(DT[dtype])
+    prompt = {} if form == "single" else dict(cu_q=_i32([0, new]), tiles=(_i32([0]), _i32([0]), 1))
+    for what, at in (("value", 273), ("value", 260), ("value", 100), ("key", 273), ("key", 100), ("value", 250)):
+        x = kvs.clone()
+        x[at, (kv if what == "value" else 0) + kv - 1, half * (d // 2) + 5] = math.nan
+        f32.rope_store_kv4(torch.cat((torch.zeros(n, kv, d), x), 1).flatten(1).cuda(), kv, kv, d, pos, seq, _i32(slots), table, records, None, 1.0, 0)
+        k, v = (t.cpu() for t in f32.kv4_values(records, pos, seq, _i32(slots), table, kv, d))
+        for window in (0, 30):
+            got = ops.kv4_attention(q.cuda(), records, _i32([n]), _i32(slots), table, kv, d ** -0.5, window=window, **prompt).cpu().view(new, heads, d)
+            want = plain.attention(q, k, v, n - new, d ** -0.5, window)
+            assert torch.equal(got.isnan(), want.isnan()), (what, at, window)
+            whole = want.isfinite()
+            _check(torch.where(whole, got, 0).flatten(1), torch.where(whole, want, 0), [(k, v)], dtype)
+
+
 def test_shares_do_not_depend_on_neighbours():
     """However a batch is cut among the blocks, a sequence's result stays within the tolerance, and one call gives the same bits twice."""
     ops, d, heads, kv = _ops("bfloat16"), 128, 16, 1
