@@ -44,7 +44,7 @@ struct FilterArgs {
     int64_t ld;
     int vocab, per_block;
     const float *uniform, *temperature, *top_p, *min_p;
-    const int *top_k, *seq_key, *step_key;
+    const int *top_k, *seq_key, *step_key, *drawn;
     uint64_t seed;
     int* token;
     float* logprob;
@@ -407,6 +407,10 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     pdl_wait();
     const uint32_t blocks = cluster_blocks(), rank = cluster_rank();
     const int r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31;
+    if (a.drawn && !a.drawn[r]) {                               // another's row (its whole cluster leaves)
+        if (rank == 0 && tid == 0) a.logprob[r] = NAN;
+        return;
+    }
     const int first = min(a.vocab, (int)rank * a.per_block);
     Row<STAGED> row;
     row.n = min(a.vocab, first + a.per_block) - first;
@@ -849,7 +853,7 @@ static_assert(kMostStaged < 1 << (32 - kCountBits), "a block's tokens in a packe
 
 CPM_API int cpm_sample_filtered(const float* logits, int64_t ld, int n_rows, int vocab, int* token, float* logprob, const float* uniform,
                                 const float* temperature, const int* top_k, const float* top_p, const float* min_p, uint64_t seed,
-                                const int* seq_key, const int* step_key, cudaStream_t stream) {
+                                const int* seq_key, const int* step_key, const int* drawn, cudaStream_t stream) {
     if (n_rows <= 0) return CPM_OK;
     if (vocab < 1 || vocab > kMostVocab || n_rows > 0x7fffffff / 8) return CPM_BAD_ARGUMENT;
     if (!uniform && (!seq_key || !step_key)) return CPM_BAD_ARGUMENT;
@@ -858,7 +862,7 @@ CPM_API int cpm_sample_filtered(const float* logits, int64_t ld, int n_rows, int
     int blocks = 8;
     while (blocks > 1 && ((int64_t)n_rows * blocks > 2 * sms || vocab < 1024 * blocks) && (vocab + blocks / 2 - 1) / (blocks / 2) <= kMostStaged - 4) blocks /= 2;
     const int per_block = ((vocab + blocks - 1) / blocks + 3) & ~3;
-    const FilterArgs a{logits, ld, vocab, per_block, uniform, temperature, top_p, min_p, top_k, seq_key, step_key, seed, token, logprob};
+    const FilterArgs a{logits, ld, vocab, per_block, uniform, temperature, top_p, min_p, top_k, seq_key, step_key, drawn, seed, token, logprob};
     if (per_block <= kMostStaged) {
         static bool done[kMaxDevices];
         const int status = ensure_dynamic_smem(sample_filtered_kernel<true>, kMostStaged * 4, done);

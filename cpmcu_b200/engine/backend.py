@@ -39,7 +39,11 @@ class EngineBackend:
             i = torch.tensor(list(keys) + list(steps) + [p.top_k for p in sampling], dtype=torch.int32).view(3, n).to(self.ops.device)
             f = torch.tensor([p.temperature for p in sampling] + [p.top_p for p in sampling] + [p.min_p for p in sampling],
                              dtype=torch.float32).view(3, n).to(self.ops.device)
-            out, _ = self.ops.sample_filtered(logits, None, f[0], i[2], f[1], f[2], self.seed, i[0], i[1])
+            out = drawn = None
+            if any(p.unfiltered for p in sampling):          # these as they would be drawn without the others
+                drawn = torch.tensor([not p.unfiltered for p in sampling], dtype=torch.int32).to(self.ops.device)
+                out = self.ops.sample(logits, f[0] * (1 - drawn), f[1], self.seed, i[0], i[1])
+            out, _ = self.ops.sample_filtered(logits, None, f[0], i[2], f[1], f[2], self.seed, i[0], i[1], out=out, drawn=drawn)
         else:
             i = torch.tensor(list(keys) + list(steps), dtype=torch.int32).view(2, n).to(self.ops.device)
             f = torch.tensor([p.temperature for p in sampling] + [p.top_p for p in sampling],

@@ -30,17 +30,20 @@ def bucket_size(n: int) -> int:
 
 
 class _Bucket:
-    def __init__(self, size: int, device: torch.device, filtered: bool = False):
-        """``filtered``: its sequences are drawn under top-k and min-p too (a kernel of its own, so a recording of its own)."""
+    def __init__(self, size: int, device: torch.device, filtered: bool = False, mixed: bool = False):
+        """``filtered``: its sequences are drawn under top-k and min-p too (a kernel of its own, so a recording of its own).  ``mixed``: some
+        of them are, and others, which are not greedy, without (both kernels)."""
         i32 = dict(dtype=torch.int32, device=device)
         self.size = size
         # what a batch begins with lies in the rows of one tensor (each on a 16-byte boundary), so that one copy brings it
-        self.filtered = bool(filtered)
-        self.block = torch.zeros(11 if filtered else 9, (size + 3) // 4 * 4, **i32)
+        self.filtered, self.mixed = bool(filtered), bool(mixed)
+        self.block = torch.zeros(13 if mixed else 11 if filtered else 9, (size + 3) // 4 * 4, **i32)
         self.ids, self.positions, self.kv_len, self.slot, self.live, self.seq_key, self.step_key = (row[:size] for row in self.block[:7])
         self.temperature, self.top_p = (row[:size] for row in self.block[7:9].view(torch.float32))
         if filtered:
             self.min_p, self.top_k = self.block[9].view(torch.float32)[:size], self.block[10][:size]
+        if mixed:       # which are drawn with filters, and the temperatures of those that are not
+            self.drawn, self.unfiltered = self.block[11][:size], self.block[12].view(torch.float32)[:size]
         self.kv_len.fill_(1)
         self.top_p.fill_(1.0)
         self.token_seq = torch.arange(size, **i32)
@@ -61,7 +64,7 @@ class DecodeRunner:
         self.ops = stepper.ops
         self.use_graph = bool(use_graph)
         self.seed = int(seed)
-        self.buckets: Dict[object, _Bucket] = {}           # by size; with filters by (size, True)
+        self.buckets: Dict[object, _Bucket] = {}           # by size; with filters by (size, whether mixed)
         self.pad_slot = self.cache.open_sequence()       # scratch sequence the padding entries use
         self.cache.reserve(self.pad_slot, 1)
         self.cache.set_length(self.pad_slot, 1)
@@ -99,18 +102,19 @@ class DecodeRunner:
         self.ops.begin_step()
         ctx.extras["step_begun"] = True
         b.logits = self.model.forward(ctx, b.want_rows)
+        if b.mixed or not b.filtered:
+            self.ops.sample(b.logits, b.unfiltered if b.mixed else b.temperature, b.top_p, self.seed, b.seq_key, b.step_key, out=b.sampled)
         if b.filtered:
-            self.ops.sample_filtered(b.logits, None, b.temperature, b.top_k, b.top_p, b.min_p, self.seed, b.seq_key, b.step_key, out=b.sampled)
-        else:
-            self.ops.sample(b.logits, b.temperature, b.top_p, self.seed, b.seq_key, b.step_key, out=b.sampled)
+            self.ops.sample_filtered(b.logits, None, b.temperature, b.top_k, b.top_p, b.min_p, self.seed, b.seq_key, b.step_key, out=b.sampled,
+                                     drawn=b.drawn if b.mixed else None)
         self.ops.advance_decode(b.ids, b.positions, b.kv_len, b.step_key, b.sampled, b.live)
 
-    def _bucket(self, n: int, filtered: bool = False) -> _Bucket:
+    def _bucket(self, n: int, filtered: bool = False, mixed: bool = False) -> _Bucket:
         size = bucket_size(n)
-        key = (size, True) if filtered else size
+        key = (size, mixed) if filtered else size
         b = self.buckets.get(key)
         if b is None:
-            b = _Bucket(size, self.ops.device, filtered)
+            b = _Bucket(size, self.ops.device, filtered, mixed)
             b.slot.fill_(self.pad_slot)
             self.buckets[key] = b
         return b
@@ -148,7 +152,8 @@ class DecodeRunner:
         """Sets the batch: ``last_tokens`` are the tokens to feed next; every sequence's
         position is its current length in the cache."""
         n = len(slots)
-        b = self._bucket(n, any(p.filtered for p in sampling))
+        filtered = any(p.filtered for p in sampling)
+        b = self._bucket(n, filtered, filtered and any(p.unfiltered for p in sampling))
         self._prepare(b)
         lengths = [self.cache.length(s) for s in slots]
         last_tokens, seq_keys, step_keys = list(last_tokens), list(seq_keys), list(step_keys)
@@ -163,6 +168,9 @@ class DecodeRunner:
         if b.filtered:
             parts.append(torch.tensor([p.min_p for p in sampling] + [0.0] * pad, dtype=torch.float32).view(torch.int32))
             parts.append(torch.tensor([p.top_k for p in sampling] + [0] * pad, dtype=torch.int32))
+        if b.mixed:
+            parts.append(torch.tensor([int(not p.unfiltered) for p in sampling] + [1] * pad, dtype=torch.int32))
+            parts.append(torch.tensor([p.temperature if p.unfiltered else 0.0 for p in sampling] + [0.0] * pad, dtype=torch.float32).view(torch.int32))
         self.cache.staging.copy(torch.cat(parts), [b.block.view(-1)])
         self.current = b
         self.slots = list(slots)

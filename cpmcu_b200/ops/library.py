@@ -124,7 +124,7 @@ _SIGNATURES = {
     "cpm_kv4_attention": [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_float, c_int, _P],
     "cpm_kv4_prompt": [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
     "cpm_copy_pages": [_P, c_int, _P, _P, c_int, _P],
-    "cpm_sample_filtered": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P],
+    "cpm_sample_filtered": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P, _P],
     "cpm_latent_attention_mma": [_P, _P, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, _P],
 }
 

@@ -1842,13 +1842,14 @@ class Ops:
     def sample_filtered(self, logits: torch.Tensor, uniform: Optional[torch.Tensor], temperature: torch.Tensor,
                         top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
                         seed: int = 0, seq_key: Optional[torch.Tensor] = None, step_key: Optional[torch.Tensor] = None,
-                        out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                        out: Optional[torch.Tensor] = None, drawn: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """fp32 logits [rows, vocab] -> (token int32 [rows], its log-probability among the tokens that stayed, fp32 [rows]).  Per row:
         ``temperature`` (0: the largest logit, lowest index among equals), then the ``top_k`` likeliest (0: all), of these the fewest whose
         mass reaches ``top_p`` of theirs (1: all), of these the ones at least ``min_p`` times as likely as the likeliest (0: all); equal
         ones stand by index.  The token is where ``uniform`` (in [0, 1)) falls in the kept masses in index order; without it the number
         is the Philox value of (seed, seq_key, step_key), as in ``sample``.  Masses are whole multiples of 2^-40 of the likeliest, so a
-        row's token depends on nothing but the row.  A row without a number above -inf gives token 0 and -inf."""
+        row's token depends on nothing but the row.  A row without a number above -inf gives token 0 and -inf.  ``drawn`` (int32): a row
+        of 0 keeps the token that ``out`` holds, and its log-probability is no number."""
         self._f32(logits, "logits")
         if logits.dim() != 2:
             raise ValueError("logits: needs [rows, vocab]")
@@ -1857,20 +1858,23 @@ class Ops:
         for t, what in given:
             if t is not None:
                 self._f32(t, what)
-        for t, what in ((top_k, "top-k"), (seq_key, "sequence keys"), (step_key, "step keys"), (out, "tokens")):
+        whole = ((top_k, "top-k"), (seq_key, "sequence keys"), (step_key, "step keys"), (out, "tokens"), (drawn, "drawn rows"))
+        for t, what in whole:
             if t is not None:
                 self._i32(t, what)
-        for t, what in given + ((top_k, "top-k"), (seq_key, "sequence keys"), (step_key, "step keys"), (out, "tokens")):
+        for t, what in given + whole:
             if t is not None and t.numel() != rows:
                 raise ValueError(f"{what}: needs one number a row, got {t.numel()} for {rows} rows")
         if temperature is None or (uniform is None and (seq_key is None or step_key is None)):
             raise ValueError("sample_filtered needs temperatures, and random numbers or the keys to make them from")
+        if drawn is not None and out is None:
+            raise ValueError("drawn rows: the others keep the tokens that are given, but none are")
         if out is None:
             out = self.result(rows, dtype=torch.int32)
         logprob = self.result(rows, dtype=torch.float32)
         check(self.lib.cpm_sample_filtered(_ptr(logits), logits.stride(0), rows, vocab, _ptr(out), _ptr(logprob), _ptr(uniform),
                                            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
-                                           ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), self._stream()),
+                                           ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), _ptr(drawn), self._stream()),
               f"sample_filtered ({vocab} tokens)")
         return out, logprob
 

@@ -17,8 +17,9 @@ class SamplingParams:
     """temperature 0 = greedy (lowest index among equal logits); top_p < 1 keeps the
     smallest set of most likely tokens whose mass reaches top_p.  top_k > 0 keeps the
     likeliest top_k first (and top_p counts in their mass); min_p > 0 keeps of the rest
-    what is at least min_p times as likely as the likeliest.  With either of these a batch
-    is drawn by ``Ops.sample_filtered``, without by ``Ops.sample``."""
+    what is at least min_p times as likely as the likeliest.  With either of these a sequence
+    is drawn by ``Ops.sample_filtered``, without by ``Ops.sample``, whatever the others of its
+    batch are drawn by (a greedy one by either: they agree)."""
 
     temperature: float = 0.0
     top_p: float = 1.0
@@ -38,6 +39,10 @@ class SamplingParams:
     @property
     def filtered(self) -> bool:
         return self.temperature > 0 and (self.top_k > 0 or self.min_p > 0)
+
+    @property
+    def unfiltered(self) -> bool:
+        return self.temperature > 0 and not self.filtered
 
     @property
     def greedy(self) -> bool:

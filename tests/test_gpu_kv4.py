@@ -641,6 +641,22 @@ def test_sample_filtered_with_keys_draws_what_sample_draws():
     assert int((a != b).sum()) <= 1
 
 
+def test_sample_filtered_leaves_other_rows_alone():
+    ops = _ops("bfloat16")
+    rows, vocab = 9, 5000
+    z = torch.randn(rows, vocab, generator=torch.Generator().manual_seed(6)).cuda()
+    u, t, k = torch.rand(rows, generator=torch.Generator().manual_seed(7)).cuda(), torch.ones(rows).cuda(), torch.full((rows,), 900, dtype=torch.int32).cuda()
+    want, logp = ops.sample_filtered(z, u, t, k)
+    drawn = _i32([1, 0, 0, 1, 1, 0, 1, 0, 5])
+    out = torch.arange(100, 100 + rows, dtype=torch.int32).cuda()
+    got, lp = ops.sample_filtered(z, u, t, k, out=out, drawn=drawn)
+    assert got is out and torch.equal(got, torch.where(drawn > 0, want, torch.arange(100, 100 + rows, dtype=torch.int32).cuda()))
+    assert torch.equal(lp.isnan(), drawn == 0) and torch.equal(lp[drawn > 0], logp[drawn > 0])
+    for bad in (dict(drawn=drawn), dict(drawn=drawn[1:], out=out), dict(drawn=drawn.long(), out=out)):
+        with pytest.raises(ValueError):
+            ops.sample_filtered(z, u, t, k, **bad)
+
+
 def test_refusals_of_sample_filtered():
     ops = _ops("bfloat16")
     z, one = torch.zeros(2, 5).cuda(), torch.ones(2).cuda()

@@ -106,6 +106,28 @@ def test_several_answers_are_those_of_separate_requests(model_folders, settings,
     assert llm.cache.slots.n_held == 1                                                      # the decode runner's padding
 
 
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_sequence_draws_the_same_whatever_its_batch_is_drawn_by(model_folders, graph, monkeypatch):
+    """Logits of a few levels, among whose equal tokens the two kernels draw differently (``sample`` keeps all of them at top-p's border): sequences
+    with filters, with top-p or a temperature alone, and greedy ones give the same tokens together, while others leave, and alone."""
+    from cpmcu_b200.engine.generate import Request, run_requests
+    from cpmcu_b200.sampling import SamplingParams
+
+    cfgd = configs.tiny_e()
+    folder = model_folders("tiny_e_dense", cfgd, 3, "float32", std=0.08)
+    llm = _llm(folder, "float32", graph, random_seed=11, max_batch=8)
+    llm.init_storage()
+    forward = llm.model.forward
+    monkeypatch.setattr(llm.model, "forward", lambda ctx, rows: None if rows is None else torch.round(forward(ctx, rows) * 2) / 2)
+    kinds = [SamplingParams(1.0, 0.6), SamplingParams(1.0, 0.8, 30), SamplingParams(0.0), SamplingParams(0.8), SamplingParams(1.2, 0.7),
+             SamplingParams(0.9, min_p=0.1)]
+    reqs = [Request(helpers.random_ids(cfgd["vocab_size"], 9 + i, i), 6 + 3 * i, kinds[i], key=i) for i in range(6)]
+    together, _ = run_requests(llm._ready(), reqs)
+    pairs = [run_requests(llm.backend, reqs[i:i + 2])[0] for i in range(0, 6, 2)]
+    alone = [run_requests(llm.backend, [r])[0][0] for r in reqs]
+    assert [r.tokens for r in together] == [r.tokens for r in alone] == [r.tokens for p in pairs for r in p]
+
+
 def test_filters_alone_change_nothing_where_they_keep_everything(model_folders):
     """A batch drawn by the filtered kernel with limits that keep all gives the tokens that the other kernel draws from the same numbers."""
     cfgd = configs.tiny_e()
