@@ -52,11 +52,12 @@ class LLM:
             self.config = dataclasses.replace(self.config, sparse_config=None)
         if cache_bits is not None:
             import dataclasses
-            if not hasattr(self.config, "cache_bits"):
-                raise ValueError(f"{self.arch.name} has no cache in 4 bits")
             if cache_bits not in (4, 16):
                 raise ValueError(f"cache_bits is 4 or 16, got {cache_bits}")
-            self.config = dataclasses.replace(self.config, cache_bits=int(cache_bits))
+            if hasattr(self.config, "cache_bits"):
+                self.config = dataclasses.replace(self.config, cache_bits=int(cache_bits))
+            elif cache_bits == 4:
+                raise ValueError(f"{self.arch.name} has no cache in 4 bits")
         self.dtype = parse_dtype(dtype if dtype is not None else getattr(self.config, "torch_dtype", "bfloat16"))
         self.device = device
         self.memory_limit = float(memory_limit)

@@ -200,6 +200,18 @@ def test_an_architecture_without_a_4_bit_cache_says_so(tmp_path):
         LLM(folder, cache_bits=4)
 
 
+def test_an_architecture_without_a_4_bit_cache_takes_16(tmp_path):
+    from cpmcu_b200 import LLM
+    from tests import dinutar_cases as cases
+
+    cfg = cases.config_a()
+    folder = cases.write_folder(cfg, cases.random_weights(cfg, 1), str(tmp_path / "d"))
+    a, b = [LLM(folder, max_tokens=64 * 8, **kw).generate([3, 1, 4], 5)[0] for kw in ({}, dict(cache_bits=16))]
+    assert a == b and len(a) == 5
+    with pytest.raises(ValueError, match="4 or 16"):
+        LLM(folder, cache_bits=8)
+
+
 CHECKED = r'''
 import os, tempfile
 from cpmcu_b200 import LLM
