@@ -5,6 +5,7 @@ never handed out, is an error, so a leak or a double free shows at once.
 """
 from __future__ import annotations
 
+from collections import Counter
 from typing import List
 
 
@@ -64,12 +65,13 @@ class FreeList:
 
     def give_back(self, handles) -> None:
         handles = list(handles)
-        for i in handles:
-            if not (0 <= i < self.n) or not self._held[i]:
+        times = Counter(handles)
+        for i, n in times.items():
+            if not (0 <= i < self.n) or self._held[i] < n:
                 raise HandleError(f"{self.what} {i} is not held (freed twice, or never handed out)")
-        for i in handles:
-            self._held[i] -= 1
-        self._free.extend(i for i in handles if not self._held[i])
+        for i, n in times.items():
+            self._held[i] -= n
+        self._free.extend(i for i in times if not self._held[i])
         self._free.sort(reverse=True)
 
     def is_held(self, i: int) -> bool:

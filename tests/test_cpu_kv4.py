@@ -32,6 +32,19 @@ def test_free_list_shares_and_moves():
             f.move(bad)
 
 
+def test_free_list_given_back_in_one_call():
+    """A number in the list as often as it is held is free once; more often is an error, and nothing is given back."""
+    f = FreeList(4, "page")
+    f.take(3)
+    f.share([1])
+    for bad in ([0, 0], [2, 1, 1, 1], [1, 3]):
+        with pytest.raises(HandleError):
+            f.give_back(bad)
+    assert f.n_free == 1 and f.times_held(1) == 2 and f.times_held(0) == 1
+    f.give_back([1, 2, 1])
+    assert f.n_free == 3 and f.take(3) == [1, 2, 3]
+
+
 def _cache(n_pages=40, n_slots=8):
     needs = [CacheNeeds(kv_heads=2, head_dim=16), CacheNeeds(kv_heads=2, head_dim=32, bits=4), CacheNeeds(kv_heads=1, head_dim=32, window=70),
              CacheNeeds(kv_heads=1, head_dim=16, pooled_stride=16, pooled_kernel=32), CacheNeeds(state={"acc": ((8,), torch.float32)})]
