@@ -1007,7 +1007,7 @@ class Ops:
         arena = self.workspace.persistent.arena if self.workspace is not None else None
         if arena is not None and arena.guards:
             arena.check_guards()
-        if int(self.lib.cpm_kv4_prompt_error()):
+        if self.kv4_prompt_ran and int(self.lib.cpm_kv4_prompt_error()):
             raise RuntimeError("the prompts' attention over a 4-bit cache gave up waiting on a barrier; the results of this step are not valid")
         if int(self.lib.cpm_listed_tile_error()):
             raise RuntimeError("the block-list attention of a prompt chunk gave up waiting on a barrier; the results of "
@@ -1716,6 +1716,7 @@ class Ops:
                                           self.code, self._stream()), "rope_store_kv4")
         return q
 
+    kv4_prompt_ran = False               # (without a 4-bit cache no step waits for its kernel's error)
     KV4_PROMPT_BLOCKS = 5                # query rows that fill so many blocks go to the tcgen05 kernel
 
     def kv4_prompt_ok(self, n_tokens: int, n_heads: int, n_kv: int, d: int, scale: float) -> bool:
@@ -1790,6 +1791,7 @@ class Ops:
         if cu_q is not None and self.kv4_prompt_ok(n, n_heads, n_kv, d, scale):
             shares = self.kv4_prompt_shares(n, n_heads, n_kv, longest or page_table.shape[1] * PAGE_TOKENS)
             parts = self.empty(shares * n * n_heads * (d + 4), dtype=torch.float32) if shares > 1 else None
+            self.kv4_prompt_ran = True
             check(self.lib.cpm_kv4_prompt(_ptr(q), _ptr(records), _ptr(out), _ptr(kv_len), _ptr(slots), _ptr(page_table), page_table.shape[1],
                                           _ptr(cu_q), _ptr(tile_seq), _ptr(tile_row), n_tiles, _ptr(parts), shares, n, n_heads, n_kv, d,
                                           int(window), float(scale), self._stream()), "prompt attention over a 4-bit cache")

@@ -313,6 +313,31 @@ def test_the_workspace_is_measured_for_the_4_bit_cache(dtype):
     assert persistent > 0 and frame > 0 and notes == []
 
 
+def test_errors_of_the_prompt_kernel_are_asked_for_once_it_ran():
+    from cpmcu_b200.ops.dry import DryOps
+
+    class Library(type(DryOps(torch.bfloat16).lib)):
+        def __init__(self):
+            self.asked, self.code, self.checked_files = [], 0, ()
+
+        def cpm_kv4_prompt_error(self):
+            self.asked.append(self.code)
+            return self.code
+
+    ops = DryOps(torch.bfloat16)
+    ops.lib = Library()
+    ops.raise_on_kernel_error()
+    assert ops.lib.asked == []
+    meta = lambda *shape, dtype=torch.int32: torch.empty(*shape, dtype=dtype, device="meta")  # noqa: E731
+    ops.kv4_attention(meta(700, 32, 128, dtype=torch.bfloat16), meta(20, 2, ops.kv4_page_bytes(128), dtype=torch.uint8), meta(1), meta(1), meta(1, 20), 2, 0.1,
+                      cu_q=meta(2), tiles=(meta(11), meta(11), 11))
+    ops.raise_on_kernel_error()
+    ops.lib.code = 3
+    with pytest.raises(RuntimeError, match="4-bit cache"):
+        ops.raise_on_kernel_error()
+    assert ops.lib.asked == [0, 3]
+
+
 def test_cli_options():
     from cpmcu_b200.cli import create_cli_parser
     args = create_cli_parser().parse_args(["--model-path", "x", "--cache-bits", "4", "--samples", "3", "--top-k", "20", "--min-p", "0.05"])
