@@ -5,9 +5,13 @@
 //     q . k  = sum over halves of  s_k (q_h . (c - 8)) + m_k sum(q_h)
 //     o      = sum over halves of  (p s_v) (c - 8)      + p m_v
 // Keys and values are the operand with 16 rows, a tile of 8 * NT queries (query heads of one key-value head, of one or several tokens) the
-// one with 8 columns.  A query is divided by a power of two first, which makes it an fp16 number without loss; p s_v is kept between
-// 2^-14 and 2^15 in the same way.  bf16 queries: p s_v is rounded to fp16 (11 bits; the output has 8).  fp32 queries: q and p s_v are sums of
-// two fp16 numbers (22 bits), which costs a second product each.
+// one with 8 columns.  A query is divided by a power of two first, which makes it an fp16 number without loss; p s_v is kept below
+// 2^15 in the same way.  bf16 queries: p s_v is rounded to fp16 (11 bits; the output has 8), of which it keeps fewer below 2^-14 of the column's largest p
+// and scale, an error of 2^-25 of these.  fp32 queries: q and p s_v are sums of two fp16 numbers (22 bits; a third would cost a third product); p s_v
+// is taken 2^10 larger, so that the second number of a weight has all its bits down to 2^-13 of the largest and is off by 2^-35 of it below, and
+// a slice's products are added to the sums by ordinary additions, since the tensor core cuts its sums off, a bias that grows with the slices and that
+// counts where codes and middles nearly cancel.  Error against 64 bits, of the result's norm, without these two, with them, and of fp32 throughout: 40,000
+// keys 4.6e-6, 8.9e-7, 2.1e-7, values that do not average to nothing 1.8e-7, 9.2e-8, 6.4e-8, scales over some e^4 1.1e-6, 2.4e-7, 2.1e-7.
 //
 // One block an SM.  A batch's rows of pages (a tile's, of one key-value head) lie in a line, of which every block takes a piece of equal cost, so that
 // unequal sequences leave no SM idle; few rows have blocks of their own.  A row that several blocks share is put together by a second kernel.  Four
@@ -169,6 +173,12 @@ __device__ __forceinline__ int shift_of(float most) {
 }
 __device__ __forceinline__ float inverse_power2(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }      // of a power of two
 __device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// How far p s_v may lie from where it is put: the running maximum 2^kScoreLag behind, the largest scale kScaleLag above the one that has been fitted,
+// which is put at 2^kUp; together 2^15.
+template <int TERMS> constexpr float kScoreLag = TERMS == 2 ? 3.f : 8.f;
+template <int TERMS> constexpr float kScaleLag = TERMS == 2 ? 4.f : 16.f;
+template <int TERMS> constexpr int kUp = TERMS == 2 ? 10 : 0;
 
 // Warps of a block, by what the registers allow: 16 with up to 128 registers a thread, 12 with 168, 8 with 255.
 constexpr int warps_of(int d, int nt, int terms) { return nt == 1 ? 16 : terms == 2 && d > 32 ? 8 : 12; }
@@ -596,8 +606,8 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
                 }
                 const float sv[2][2] = {{kv4_scale(vp[0].x), kv4_scale(vp[0].y)}, {kv4_scale(vp[1].x), kv4_scale(vp[1].y)}};
                 const float largest = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-                // ---- the running maximum may lie up to 2^8 behind, and ``down`` fit scales up to 2^4 smaller, so that both seldom move ----
-                if (__any_sync(0xffffffffu, highest > 8.f || !(largest <= limit))) {
+                // ---- the running maximum may lie behind, and ``down`` fit smaller scales, so that both seldom move ----
+                if (__any_sync(0xffffffffu, highest > kScoreLag<TERMS> || !(largest <= limit))) {
                     limit = INFINITY;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
@@ -618,17 +628,18 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
                                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
                             }
                             // a column moves by its own keys alone, so that its neighbours' have no part in its rounding
-                            const bool first = blank >> (2 * n + c) & 1, move = first || high > 8.f;
+                            const bool first = blank >> (2 * n + c) & 1, move = first || high > kScoreLag<TERMS>;
                             const float less = c ? old.y : old.x, was = c ? was2.y : was2.x;
                             now[c] = move ? high - less : -less;
                             by[c] = first ? 0.f : move ? fast_exp2(-less - now[c]) : 1.f;
                             if (now[c] > -INFINITY) blank &= ~(1u << (2 * n + c));
                             else now[c] = 0.f;
-                            // one over the power of two below the largest scale that the column has seen (0: none above 0)
-                            const float fit = most > 0.f ? power2(-max(-120, min(120, (int)(__float_as_uint(most) >> 23) - 127))) : 0.f;
-                            next[c] = was == 0.f || most > 16.f * inverse_power2(was) ? fit : was;
+                            // 2^kUp over the power of two below the largest scale that the column has seen (0: none above 0)
+                            constexpr float room = kScaleLag<TERMS> * (1 << kUp<TERMS>);
+                            const float fit = most > 0.f ? power2(kUp<TERMS> - max(kUp<TERMS> - 120, min(120, (int)(__float_as_uint(most) >> 23) - 127))) : 0.f;
+                            next[c] = was == 0.f || most > room * inverse_power2(was) ? fit : was;
                             shrink[c] = was > 0.f ? by[c] * (next[c] * inverse_power2(was)) : by[c];
-                            limit = fminf(limit, blank >> (2 * n + c) & 1 ? -1.f : next[c] > 0.f ? 16.f * inverse_power2(next[c]) : 0.f);
+                            limit = fminf(limit, blank >> (2 * n + c) & 1 ? -1.f : next[c] > 0.f ? room * inverse_power2(next[c]) : 0.f);
 #pragma unroll
                             for (int r = 0; r < 2; ++r)
                                 if (move) x[n][2 * r + c] = x[n][2 * r + c] - less - now[c];
@@ -688,9 +699,21 @@ kv4_attention_kernel(const __grid_constant__ AttendArgs a) {
                             const int k = 2 * p + odd;
                             const uint32_t frag[4] = {lo[2 * odd], lo[2 * odd + 1], hi[2 * odd], hi[2 * odd + 1]};
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
+                            for (int n = 0; n < NT; ++n) {
+                                if constexpr (TERMS == 1) {
+                                    mma_f16(o[k][n], frag, pf[0][k * 2 / STEPS][n][0], pf[0][k * 2 / STEPS][n][1]);
+                                } else {
+                                    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                                for (int u = 0; u < TERMS; ++u) mma_f16(o[k][n], frag, pf[u][k * 2 / STEPS][n][0], pf[u][k * 2 / STEPS][n][1]);
+                                    for (int u = TERMS - 1; u >= 0; --u) mma_f16(part, frag, pf[u][k * 2 / STEPS][n][0], pf[u][k * 2 / STEPS][n][1]);
+#pragma unroll
+                                    for (int i = 0; i < 4; i += 2) {
+                                        const float2 y = both(add2(pair(o[k][n][i], o[k][n][i + 1]), pair(part[i], part[i + 1])));
+                                        o[k][n][i] = y.x;
+                                        o[k][n][i + 1] = y.y;
+                                    }
+                                }
+                            }
                         }
                     }
                 }

@@ -265,6 +265,36 @@ def test_magnitudes(dtype, q_scale, v_scale):
     _check(got, want, rows, dtype)
 
 
+@pytest.mark.parametrize("form", ["single", "prompt"])
+@pytest.mark.parametrize("keys", [100, 8000, 40000])
+@pytest.mark.parametrize("d,heads,kv", [(64, 16, 2), (128, 4, 2)])
+def test_many_keys_in_fp32(d, heads, kv, keys, form):
+    """Most of many weights are far below the largest, and each keeps its 22 bits: errors of 2^-23 of a query and of a weight, and of scores below 8 whose last
+    bit is 2^-21, are independent and move the result by about 2^-22 of its norm; twice that is tolerated."""
+    ops, new = _ops("float32"), 1 if form == "single" else 20
+    table, slots, records, rows = _filled(ops, [keys, keys // 2], kv, d, 41)
+    q = torch.randn(2 * new, heads, d, generator=torch.Generator().manual_seed(7)) * 0.8
+    prompt = {} if form == "single" else dict(cu_q=_i32([0, new, 2 * new]), tiles=(_i32([0, 1]), _i32([0, 0]), 2))
+    got = ops.kv4_attention(q.cuda(), records, _i32([keys, keys // 2]), _i32(slots), table, kv, d ** -0.5, **prompt).cpu().double().view(2 * new, heads, d)
+    want = torch.cat([plain.attention(q[i * new:(i + 1) * new], k, v, k.shape[0] - new, d ** -0.5, 0) for i, (k, v) in enumerate(rows)])
+    assert float((got - want).norm() / want.norm()) < 2.0 ** -21
+
+
+def test_many_keys_whose_values_average_to_nothing_in_fp32():
+    """Codes less 8 average to -1/2 and middles make up for it: the sums of both are some 20 times the result of 40,000 keys.  A warp adds about ten parts
+    of 2^-24 to them, which moves the result by about 2^-19 of its norm."""
+    ops, d, heads, kv, keys = _ops("float32"), 128, 32, 2, 40000
+    table, slots, records, rows = _filled(ops, [keys], kv, d, 43)
+    k, v = rows[0][0], torch.randn(keys, kv, d, generator=torch.Generator().manual_seed(9))
+    pos, seq = _every_position([keys])
+    ops.rope_store_kv4(torch.cat((torch.zeros(keys, kv, d), k, v), 1).flatten(1).cuda(), kv, kv, d, pos, seq, _i32(slots), table, records, None, 1.0, 0)
+    k, v = (t.cpu() for t in ops.kv4_values(records, pos, seq, _i32(slots), table, kv, d))
+    q = torch.randn(1, heads, d, generator=torch.Generator().manual_seed(7)) * 0.8
+    got = ops.kv4_attention(q.cuda(), records, _i32([keys]), _i32(slots), table, kv, d ** -0.5).cpu().double().view(1, heads, d)
+    want = plain.attention(q, k, v, keys - 1, d ** -0.5, 0)
+    assert float((got - want).norm() / want.norm()) < 2.0 ** -19
+
+
 @pytest.mark.parametrize("tcgen05", [False, True])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("poison", [math.nan, math.inf, 1e30])
