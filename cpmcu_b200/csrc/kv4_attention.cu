@@ -21,8 +21,9 @@
 // uniform registers.  Blocks of four warps, three an SM, leave three times as many parts to add up: 41 us where blocks of twelve took 30, for one
 // sequence of 131,071 keys.)
 //
-// 32 heads on 2 of 128, bf16: 1,000 keys 11 us, 131,071 keys 26 us (1.45 TB/s of records); 64 sequences of 1 to 8,192 keys, 14 heads on 2 of 64,
-// 28 us (1.6 TB/s); 5 of 300 to 2,500 keys, fp32, 9 us; 200 of 1 to 4,000, 32 heads on 8 of 128, 163 us (2.9 TB/s).  Bound, where there are many keys, by
+// 32 heads on 2 of 128, bf16: 1,000 keys 12 us, 131,071 keys 25 us (1.5 TB/s of records); 64 sequences of 1 to 8,192 keys, 16 heads on 2 of 64,
+// 28 us (1.6 TB/s); 5 of 300 to 2,500 keys, fp32, 9 us; 200 of 1 to 4,000, 32 heads on 8 of 128, 165 us (2.8 TB/s); prompts of 2,048 tokens behind 4,101
+// keys, 16 heads on 2: bf16 of 32 and 96 340 and 532 us, fp32 of 32, 64 and 96 456, 627 and 760, 32 heads on 2 of 128 1,659.  Bound, where there are many keys, by
 // instructions: a slice of 16 tokens costs a warp some 500, of which unpacking the codes is a third; where there are few, by the way to the first
 // key: 2 us for lengths and shares, 1 for page numbers, 1 for queries, 2 for the first slice and 2 for the parts, whose instructions
 // come from L2, and 2.5 for the second kernel.
@@ -209,7 +210,7 @@ struct Smem {
 
 // A row of pages (a tile's, of one key-value head and part) costs a block its pages and some more, for the queries that it prepares and the parts
 // that it adds up.  All rows lie one behind the other in a line of such costs, a row's extra cost first.  (Extra cost of 2, 4 and 8 pages for each group
-// of warps: 64 sequences of up to 8,192 keys, 14 heads on 2 of 64, 31.0, 27.6 and 29.5 us; 200 of up to 4,000, 32 on 8 of 128, 172, 163 and 177.)
+// of warps: 64 sequences of up to 8,192 keys, 16 heads on 2 of 64, 31.0, 27.6 and 29.5 us; 200 of up to 4,000, 32 on 8 of 128, 172, 163 and 177.)
 constexpr int extra_cost(int groups) { return 4 * groups; }
 // Sharing by cost: each of the blocks takes a piece of the line, wherever rows begin or end; fewer blocks where there is little.
 struct Shares { int sharing, each, more; };            // the first ``more`` blocks have one more than ``each``

@@ -12,7 +12,8 @@
 //
 // fp16 and not bf16: its 11 bits hold s (c - 8) exactly, 8 bits times 3, so that scores are as exact as their fp32 sums.  The rest of a
 // key's product, m times the sum of the query's half row, is 16 more columns of the operands: m three times and the sum as three fp16 numbers,
-// for both halves.  A value is rounded to 11 bits (2^-12 of it, where the output has 8).
+// for both halves.  A value is rounded to 11 bits (2^-12 of it, where the output has 8), a weight times its value's power of two to 11 as well; what is
+// below 2^-14 of the largest of its 16 tokens' values, or of the row's largest weight and power, keeps fewer, an error of 2^-25 of these.
 // What fp16 lacks in range is taken care of by powers of two: a query row, 16 tokens' keys and 16 tokens' values are divided by the power of two below
 // their largest magnitude, scores are multiplied by the first two again, and the accumulator stands for O / 2^E with E the largest power of the
 // values so far.

@@ -5,7 +5,8 @@
 // and a half row's 16 lanes are one shuffle away.  The codes meet in shared memory, from where lanes write whole words (keys:
 // a token's own; values: 16 bits, for the other half of the word is the neighbouring token's, which another block may be writing).
 // What a token cannot do without: its projections, q out, d + 16 bytes per key-value head.
-// 2,048 tokens of 32 heads on 2 of 128, with reading them back: 12.4 us, 3.1 TB/s; 64 tokens of 14 heads on 2 of 64: 4.5 us, two launches.  Bound by latency: a block's
+// 2,048 tokens of 32 heads on 2 of 128: 9.1 us (fp32 10.7) and 3.1 for reading them back, 12.4 one behind the other, 3.1 TB/s; 64 tokens of 16 heads on 2 of
+// 64: 2.8 and 1.9, 4.5 one behind the other.  Bound by latency: a block's
 // tokens are one, and its angles (sincosf) and its rows' loads lie in one chain; with all rows alike, a warp to a row, it took 15.6 us.
 #include "kv4.cuh"
 

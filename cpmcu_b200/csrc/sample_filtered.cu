@@ -18,8 +18,8 @@
 // compared with each, and it draws as well.  In the same pass a thread sums what it keeps above the bin, so that the draw looks at few tokens again.
 // (A cluster's barrier takes about 2 us, and a look into a neighbour's shared memory half of that: a selection over the whole row with
 // all blocks' histograms added up at every step took 41 us for one row of 73,448, bins of counts alone 25, and this 15.)
-// 64 rows of 73,448 with settings of their own 38 us, 512 rows of 32,000 by mass alone 116.  What a row cannot do without is its logits, 4 bytes a token
-// (10 us of the 116); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
+// 64 rows of 73,448 with settings of their own 38 us, 512 rows of 32,000 by mass alone 117.  What a row cannot do without is its logits, 4 bytes a token
+// (10 us of the 117); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
 #include "common.cuh"
 #include "philox.cuh"
 
