@@ -1755,7 +1755,8 @@ class Ops:
         """Attention over a cache in 4 bits: q [tokens, heads, d] -> [tokens, heads * d].  Without ``cu_q`` every row of q is the last token
         of a sequence of ``kv_len`` keys; with it sequence s brings the tokens cu_q[s] .. cu_q[s + 1], the last of its kv_len[s] keys, and
         ``tiles`` = (sequence, first token, count) lists them in tiles of QUERY_TILE_TOKENS, as for ``prefill_attention``.  A token at
-        position p sees the keys p - window < j <= p (``window`` 0: all j <= p); a row that sees none gives zeros.  ``longest``: a bound on the
+        position p sees the keys p - window < j <= p (``window`` 0: all j <= p); a row that sees none gives zeros.  A softmax weight enters its product
+        with 11 bits in bf16, and it and the query with 22 in fp32; maxima and sums are fp32.  ``longest``: a bound on the
         sequences' keys where the caller knows one (0: the page table's width); it only decides how a prompt's keys are shared out."""
         self._act(q, "q")
         if q.dim() != 3:
