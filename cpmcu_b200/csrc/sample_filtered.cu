@@ -20,7 +20,7 @@
 // all blocks' histograms added up at every step took 41 us for one row of 73,448, bins of counts alone 25, and this 15.)
 // 64 rows of 73,448 with settings of their own 38 us, 512 rows of 32,000 by mass alone 117.  What a row cannot do without is its logits, 4 bytes a token
 // (10 us of the 117); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
-#include "common.cuh"
+#include "filtered.cuh"
 #include "philox.cuh"
 
 namespace {
@@ -48,6 +48,11 @@ struct FilterArgs {
     uint64_t seed;
     int* token;
     float* logprob;
+    // Several rows of a sequence (null, 0 and null: a row each): a row's sequence, whose settings it takes; the places of the rows' tokens and the sequences'
+    // first rows, so that a row's random number is that of its token's place; and where what a row keeps is written, if anywhere.
+    const int *row_seq, *positions, *cu;
+    int n_seqs, n_rows;
+    KeptRow* kept;
 };
 
 // What the first block has found and the others read: the weights to set apart, or the border.
@@ -84,47 +89,6 @@ struct FilterShared {
     Plan plan;
     ArgMax scratch[33];
 };
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_blocks() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-// Reads, writes and additions in the shared memory of the cluster's block ``rank``, at the place that ``own`` is in this block's.
-__device__ __forceinline__ uint32_t peer32(const void* own, uint32_t rank) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_address(own, rank)) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint64_t peer64(const void* own, uint32_t rank) {
-    uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_address(own, rank)) : "memory");
-    return v;
-}
-__device__ __forceinline__ void put32(const void* own, uint32_t rank, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" :: "r"(cluster_address(own, rank)), "r"(v) : "memory");
-}
-__device__ __forceinline__ void put64(const void* own, uint32_t rank, uint64_t v) {
-    asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(cluster_address(own, rank)), "l"(v) : "memory");
-}
-__device__ __forceinline__ void add64(const void* own, uint32_t rank, uint64_t v) {
-    asm volatile("red.shared::cluster.add.u64 [%0], %1;" :: "r"(cluster_address(own, rank)), "l"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t add32(const void* own, uint32_t rank, uint32_t v) {
-    uint32_t old;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(cluster_address(own, rank)), "r"(v) : "memory");
-    return old;
-}
-
-// floor(w 2^40) of a weight (0 to 1) by its bits: 24 bits of significand, shifted.
-__device__ __forceinline__ uint64_t units_of(uint32_t bits) {
-    return ((uint64_t)((bits & 0x7fffffu) | 0x800000u) << 17) >> min(63u, 127u - (bits >> 23));
-}
 
 // Of a weight below 2^-17.
 __device__ __forceinline__ uint32_t small_units_of(uint32_t bits) {
@@ -235,24 +199,10 @@ __device__ __forceinline__ uint64_t block_sum64(uint64_t v, FilterShared& sm) {
 
 // STAGED: the block's weights lie in shared memory; else (a vocabulary that eight blocks' do not hold) they are formed again from the logits.
 template <bool STAGED>
-struct Row {
+struct Row : Weigher {
     const float* z;                                    // the block's first logit
     float* w;
     int n;                                             // tokens of the block
-    float top, t;
-    float inverse;                                     // 1 / t where the quotient by it is exact, else 0
-    // (x - top) / t correctly rounded.  For t within 2^60 of 1 by Markstein's method (IBM J. Res. Dev. 34, 1990): with r = 1 / t rounded, q = x r, and
-    // the remainder x - q t, which a fused multiply-add gives exactly, q + r (x - q t) rounds to the quotient.  Where it overflows the weight is 0.
-    __device__ __forceinline__ float over_t(float x) const {
-        if (inverse == 0.f) return __fdiv_rn(x, t);
-        const float q = __fmul_rn(x, inverse);
-        return __fmaf_rn(__fmaf_rn(-q, t, x), inverse, q);
-    }
-    __device__ __forceinline__ float form(float x) const {
-        if (top == INFINITY) return x == INFINITY ? 1.f : 0.f;
-        const float v = expf(over_t(__fsub_rn(x, top)));
-        return v >= 0.f ? v : 0.f;                     // a logit that is no number is never drawn
-    }
     __device__ __forceinline__ float at(int i) const {
         if constexpr (STAGED) return w[i];
         else return form(z[i]);
@@ -411,19 +361,25 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         if (rank == 0 && tid == 0) a.logprob[r] = NAN;
         return;
     }
+    int s = r, step = 0;                                        // whose settings, and how far behind the sequence's first token
+    if (a.row_seq) {
+        s = a.row_seq[r];
+        if (s < 0 || s >= a.n_seqs) return;                    // behind the last sequence
+        if (a.positions) step = a.positions[r] - a.positions[max(0, min(a.cu[s], a.n_rows - 1))];
+    }
     const int first = min(a.vocab, (int)rank * a.per_block);
     Row<STAGED> row;
     row.n = min(a.vocab, first + a.per_block) - first;
     row.z = a.logits + (int64_t)r * a.ld + first;
     row.w = weights;
-    const float t = a.temperature ? a.temperature[r] : 0.f, p = a.top_p ? a.top_p[r] : 1.f;
-    int k = a.top_k ? a.top_k[r] : 0;
-    float ratio = a.min_p ? a.min_p[r] : 0.f;
+    const float t = a.temperature ? a.temperature[s] : 0.f, p = a.top_p ? a.top_p[s] : 1.f;
+    int k = a.top_k ? a.top_k[s] : 0;
+    float ratio = a.min_p ? a.min_p[s] : 0.f;
     if (p <= 0.f || ratio > 1.f) k = 1;
     // above one: the first token alone, which it would leave out as well; below zero, -0 (weights are compared by their bits) or no number: no limit
     if (!(ratio > 0.f && ratio <= 1.f)) ratio = 0.f;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
-    const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[r], (uint32_t)a.step_key[r]);
+    const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[s], (uint32_t)(a.step_key[s] + step));
 
     asm volatile("barrier.cluster.arrive;" ::: "memory");       // (nothing is put into a block that has not begun)
 
@@ -470,12 +426,11 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         if (rank == 0 && tid == 0) {
             a.token[r] = best.v == -INFINITY ? 0 : best.i;
             a.logprob[r] = best.v == -INFINITY ? -INFINITY : 0.f;
+            if (a.kept) a.kept[r] = KeptRow{best.v, kOneToken, best.v == -INFINITY ? 0 : best.i, 0, 1ull << 40, 0};
         }
         return;
     }
-    row.top = best.v;
-    row.t = t;
-    row.inverse = t > 0x1p-60f && t < 0x1p60f ? __frcp_rn(t) : 0.f;
+    row.set(best.v, t);
 
     // weights, their histogram, and (where mass alone decides) their mass.  A thread's tokens are neighbours, an odd number of them, so that sums by
     // thread go by index and a warp's accesses to shared memory are in different banks
@@ -713,7 +668,18 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                     stays = stays && __uint_as_float(bits) >= ratio;
                     const uint64_t total = block_sum64(stays && part == 0 ? mass : 0, sm);
                     if (there && part == 0) masses[own] = stays ? mass : 0;
+                    if (a.kept && tid == 0) {                  // the last that stays, as those before it do
+                        sm.plan.border = 0xffffffffu;
+                        sm.cut = -1;
+                    }
                     __syncthreads();
+                    if (a.kept) {
+                        if (stays && part == 0) atomicMin(&sm.plan.border, bits);
+                        __syncthreads();
+                        if (stays && part == 0 && bits == sm.plan.border) atomicMax(&sm.cut, place);
+                        __syncthreads();
+                        if (tid == 0) a.kept[r] = KeptRow{row.top, sm.plan.border, sm.cut, 0, total, 0};
+                    }
                     before = 0;
 #pragma unroll 4
                     for (int i = part; i < listed; i += share) before += sm.place[i] < place ? masses[i] : 0;
@@ -801,6 +767,12 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         int64_t left = (int64_t)ties - ((int64_t)upto - mine);     // to keep of the thread's and those behind them
 #pragma unroll 1
         for (uint32_t b = 0; b < rank; ++b) left -= sm.count[b];
+        if (a.kept && left > 0 && left <= mine) {                  // the last that stays is among the thread's
+            int64_t more = left;
+#pragma unroll 1
+            for (int i = i0; i < i1; ++i)
+                if (__float_as_uint(row.at(i)) == border && --more == 0) a.kept[r].cut = first + i;
+        }
         if (left < mine) {
             cut = -1;
 #pragma unroll 1
@@ -832,6 +804,13 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         if (b < rank) run += sm.mass[b];
         total += sm.mass[b];
     }
+    if (a.kept && rank == 0 && tid == 0) {
+        KeptRow& to = a.kept[r];
+        to.top = row.top;
+        to.border = border;
+        to.total = total;
+        if (ties >= equal) to.cut = 0x7fffffff;
+    }
     const uint64_t target = min((uint64_t)((double)u * (double)total), total - 1);
     if (target < run || target >= run + mine) return;
 #pragma unroll 1
@@ -849,27 +828,45 @@ constexpr int kMostStaged = (113 * 1024 - (int)sizeof(FilterShared) - 1024) / 4;
 static_assert((kMostStaged + kFilterThreads - 1) / kFilterThreads + 1 <= 64, "a thread's tokens in a mask");
 static_assert(kMostStaged < 1 << (32 - kCountBits), "a block's tokens in a packed count");
 
+// Rows of several sequences: see FilterArgs.
+int draw_filtered(FilterArgs a, int n_rows, cudaStream_t stream) {
+    if (n_rows <= 0) return CPM_OK;
+    if (a.vocab < 1 || a.vocab > kMostVocab || n_rows > 0x7fffffff / 8) return CPM_BAD_ARGUMENT;
+    if (!a.uniform && (!a.seq_key || !a.step_key)) return CPM_BAD_ARGUMENT;
+    const int sms = device_sms(), vocab = a.vocab;
+    // as many blocks a row as run at the same time, and as the weights need; a block of few tokens is not worth its barriers
+    int blocks = 8;
+    while (blocks > 1 && ((int64_t)n_rows * blocks > 2 * sms || vocab < 1024 * blocks) && (vocab + blocks / 2 - 1) / (blocks / 2) <= kMostStaged - 4) blocks /= 2;
+    a.per_block = ((vocab + blocks - 1) / blocks + 3) & ~3;
+    a.n_rows = n_rows;
+    if (a.per_block <= kMostStaged) {
+        static bool done[kMaxDevices];
+        const int status = ensure_dynamic_smem(sample_filtered_kernel<true>, kMostStaged * 4, done);
+        if (status != CPM_OK) return status;
+        cpm_launch_cluster(kLaunchOther, sample_filtered_kernel<true>, dim3(n_rows * blocks), kFilterThreads, (size_t)a.per_block * 4, stream, blocks, a);
+    } else {
+        cpm_launch_cluster(kLaunchOther, sample_filtered_kernel<false>, dim3(n_rows * blocks), kFilterThreads, 0, stream, blocks, a);
+    }
+    return launch_status();
+}
+
 }  // namespace
 
 CPM_API int cpm_sample_filtered(const float* logits, int64_t ld, int n_rows, int vocab, int* token, float* logprob, const float* uniform,
                                 const float* temperature, const int* top_k, const float* top_p, const float* min_p, uint64_t seed,
                                 const int* seq_key, const int* step_key, const int* drawn, cudaStream_t stream) {
-    if (n_rows <= 0) return CPM_OK;
-    if (vocab < 1 || vocab > kMostVocab || n_rows > 0x7fffffff / 8) return CPM_BAD_ARGUMENT;
-    if (!uniform && (!seq_key || !step_key)) return CPM_BAD_ARGUMENT;
-    const int sms = device_sms();
-    // as many blocks a row as run at the same time, and as the weights need; a block of few tokens is not worth its barriers
-    int blocks = 8;
-    while (blocks > 1 && ((int64_t)n_rows * blocks > 2 * sms || vocab < 1024 * blocks) && (vocab + blocks / 2 - 1) / (blocks / 2) <= kMostStaged - 4) blocks /= 2;
-    const int per_block = ((vocab + blocks - 1) / blocks + 3) & ~3;
-    const FilterArgs a{logits, ld, vocab, per_block, uniform, temperature, top_p, min_p, top_k, seq_key, step_key, drawn, seed, token, logprob};
-    if (per_block <= kMostStaged) {
-        static bool done[kMaxDevices];
-        const int status = ensure_dynamic_smem(sample_filtered_kernel<true>, kMostStaged * 4, done);
-        if (status != CPM_OK) return status;
-        cpm_launch_cluster(kLaunchOther, sample_filtered_kernel<true>, dim3(n_rows * blocks), kFilterThreads, (size_t)per_block * 4, stream, blocks, a);
-    } else {
-        cpm_launch_cluster(kLaunchOther, sample_filtered_kernel<false>, dim3(n_rows * blocks), kFilterThreads, 0, stream, blocks, a);
-    }
-    return launch_status();
+    const FilterArgs a{logits, ld, vocab, 0, uniform, temperature, top_p, min_p, top_k, seq_key, step_key, drawn, seed, token, logprob,
+                       nullptr, nullptr, nullptr, 0, 0, nullptr};
+    return draw_filtered(a, n_rows, stream);
+}
+
+// The same for rows of sequences that bring several tokens each, whose settings and keys are by sequence; ``kept`` (32 bytes a row, or null) takes what a
+// row's filters leave.  A row whose sequence is none is left out.
+CPM_API int cpm_sample_drafts(const float* logits, int64_t ld, int n_rows, int vocab, int* token, float* logprob, const float* uniform,
+                              const float* temperature, const int* top_k, const float* top_p, const float* min_p, uint64_t seed, const int* seq_key,
+                              const int* step_key, const int* row_seq, const int* positions, const int* cu, int n_seqs, void* kept, cudaStream_t stream) {
+    if (!row_seq || (!uniform && (!positions || !cu)) || ((uintptr_t)kept & 15)) return CPM_BAD_ARGUMENT;
+    const FilterArgs a{logits, ld, vocab, 0, uniform, temperature, top_p, min_p, top_k, seq_key, step_key, nullptr, seed, token, logprob,
+                       row_seq, uniform ? nullptr : positions, cu, n_seqs, 0, (KeptRow*)kept};
+    return draw_filtered(a, n_rows, stream);
 }

@@ -85,7 +85,7 @@ class DryOps(Ops):
         self.element_size = 4 if dtype == torch.float32 else 2
         self.sm_count = sm_count
         self.arrivals = None
-        self.use_tcgen05 = self.use_tcgen05_attention = self.use_tcgen05_listed = self.use_tcgen05_sink = True
+        self.use_tcgen05 = self.use_tcgen05_attention = self.use_tcgen05_listed = self.use_tcgen05_sink = self.use_tcgen05_draft = True
         self.tcgen05_pair = False
         arena = Arena(None, None)
         self.workspace = Workspace(arena.carve("persistent", None), [arena.carve("frame0", None), arena.carve("frame1", None)])

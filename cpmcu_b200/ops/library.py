@@ -125,11 +125,17 @@ _SIGNATURES = {
     "cpm_kv4_prompt": [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
     "cpm_copy_pages": [_P, c_int, _P, _P, c_int, _P],
     "cpm_sample_filtered": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P, _P],
+    "cpm_sample_drafts": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P, _P, _P, c_int, _P, _P],
+    "cpm_verify_drafts": [_P, c_int64, c_int, c_int, _P, _P, c_int, c_int, _P, _P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "cpm_step_tables": [_P, _P, _P, c_int, c_int, _P, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "cpm_keep_drafts": [_P, c_int, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P],
+    "cpm_draft_attention_generic": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                    c_float, c_int, _P],
     "cpm_latent_attention_mma": [_P, _P, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, _P],
 }
 
 # source files whose kernels follow page tables; the checked build (CPMCU_CHECK_BOUNDS=1) keeps a record per file
-BOUNDS_FILES = ("attention_bf16", "attention_generic", "attention_tcgen05", "elementwise", "kv4_attention", "kv4_prompt", "kv4_store",
+BOUNDS_FILES = ("attention_bf16", "attention_generic", "attention_tcgen05", "draft_attention", "elementwise", "kv4_attention", "kv4_prompt", "kv4_store",
                 "latent_attention", "sink_attention", "sparse", "talking_attention")
 
 _lock = threading.Lock()

@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -44,6 +44,20 @@ def _current_stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+class StepTables(NamedTuple):
+    """A step's description on the device, as ``Ops.step_tables`` makes it (int32; the slot map and the ancestors int64).  What is by token is -1 (ancestors 0)
+    behind the last sequence's tokens."""
+
+    cu_q: torch.Tensor                       # [seqs + 1]: where a sequence's tokens begin
+    kv_len: torch.Tensor                     # [seqs]: keys with the step's
+    token_seq: torch.Tensor                  # [tokens]: the token's sequence
+    positions: torch.Tensor                  # [tokens]: where it stands in the text (keys held and, with parents, its depth)
+    places: torch.Tensor                     # [tokens]: where it lies in its sequence's cache
+    slot_map: torch.Tensor                   # [tokens]: page * PAGE_TOKENS + place in it; -1: none
+    ancestors: Optional[torch.Tensor]        # [tokens]: a bit for each of its sequence's new tokens that it descends from, and its own
+    taken: Optional[torch.Tensor]            # [1]: pages wanted from the free ones
+
+
 class Ops:
     def __init__(self, dtype: torch.dtype, device: "torch.device | str" = "cuda:0"):
         if dtype not in (torch.float32, torch.bfloat16):
@@ -64,6 +78,7 @@ class Ops:
         self.use_tcgen05_attention = os.environ.get("CPMCU_TCGEN05_ATTENTION", "1") != "0"
         self.use_tcgen05_sink = os.environ.get("CPMCU_TCGEN05_SINK", "1") != "0"                # sink window attention of prompts
         self.use_tcgen05_listed = os.environ.get("CPMCU_TCGEN05_LISTED", "1") != "0"      # block-list attention of prompts
+        self.use_tcgen05_draft = os.environ.get("CPMCU_TCGEN05_DRAFT", "1") != "0"        # attention of drafted tokens
         self.tcgen05_pair = os.environ.get("CPMCU_TCGEN05_PAIR", "0") == "1"      # pairs of blocks on 256-row tiles
         self.workspace = None       # cpmcu_b200.memory.Workspace: where a step's intermediates live (None: torch's allocator)
         self.weights = None         # cpmcu_b200.memory.Region that holds the weights (None: torch's allocator)
@@ -1880,6 +1895,192 @@ class Ops:
                                            ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), _ptr(drawn), self._stream()),
               f"sample_filtered ({vocab} tokens)")
         return out, logprob
+
+    # ---- drafted tokens ----
+    MOST_DRAFTS = 64                     # tokens that a sequence brings at most, the one before the drafted ones among them
+
+    def _given(self, t: torch.Tensor, dtype: torch.dtype, what: str, n: Optional[int] = None) -> torch.Tensor:
+        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.get_device() != self.device_index:
+            raise ValueError(f"{what}: needs a contiguous {dtype} tensor on cuda:{self.device_index}, got {t.dtype} on {t.device} contiguous={t.is_contiguous()}")
+        if n is not None and t.numel() != n:
+            raise ValueError(f"{what}: needs {n} numbers, got {t.numel()}")
+        return t
+
+    @property
+    def device_index(self) -> int:
+        return self.device.index if self.device.index is not None else _current_device()
+
+    def _most(self, most: int) -> int:
+        if not 1 <= int(most) <= self.MOST_DRAFTS:
+            raise ValueError(f"a sequence brings 1 to {self.MOST_DRAFTS} tokens, got {most}")
+        return int(most)
+
+    def step_tables(self, lengths: torch.Tensor, new: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor, n_tokens: int,
+                    parents: Optional[torch.Tensor] = None, free: Optional[torch.Tensor] = None) -> StepTables:
+        """A step's description from its requests' lengths, without the host: sequence s holds ``lengths[s]`` tokens in the pages of row ``slots[s]`` of the
+        page table and brings ``new[s]`` (none is allowed), ``n_tokens`` is what the token axis has room for.  ``parents`` int32 [n_tokens]: a token's parent among
+        its sequence's new ones, which comes before it (anything else: none); tokens of a tree stand at the position of their depth, and their ancestors are the
+        bits of a word, for sequences of up to MOST_DRAFTS new tokens.  ``free`` int32: pages that may be taken; those that the new tokens need are written into the
+        table in the sequences' order, and ``taken`` says how many were wanted.  A sequence whose pages are not all there gets none; pages beyond the
+        table's width are not written."""
+        n_seqs, i32 = lengths.numel(), torch.int32
+        for t, what in ((lengths, "lengths"), (new, "new tokens"), (slots, "slots")):
+            self._given(t, i32, what, n_seqs)
+        self._given(page_table, i32, "page table")
+        if page_table.dim() != 2 or page_table.numel() == 0:
+            raise ValueError("page table: needs [slots, pages]")
+        if n_tokens < 0:
+            raise ValueError(f"a step of {n_tokens} tokens")
+        if n_seqs == 0:
+            raise ValueError("a step needs a sequence")
+        if parents is not None:
+            self._given(parents, i32, "parents", n_tokens)
+        if free is not None:
+            self._given(free, i32, "free pages")
+        t = StepTables(self.empty(n_seqs + 1, dtype=i32), self.empty(n_seqs, dtype=i32), *(self.empty(n_tokens, dtype=i32) for _ in range(3)),
+                       self.empty(n_tokens, dtype=torch.int64), None if parents is None else self.empty(n_tokens, dtype=torch.int64),
+                       None if free is None else self.empty(1, dtype=i32))
+        check(self.lib.cpm_step_tables(_ptr(lengths), _ptr(new), _ptr(slots), n_seqs, n_tokens, _ptr(page_table), page_table.shape[0], page_table.shape[1],
+                                       _ptr(parents), _ptr(free), 0 if free is None else free.numel(), _ptr(t.cu_q), _ptr(t.kv_len), _ptr(t.token_seq),
+                                       _ptr(t.positions), _ptr(t.places), _ptr(t.slot_map), _ptr(t.ancestors), _ptr(t.taken), self._stream()),
+              f"step_tables ({n_seqs} sequences)")
+        return t
+
+    def draft_attention_on_tensor_cores(self, d: int, n_heads: int, n_kv: int) -> bool:
+        return False
+
+    def draft_attention_shares(self, n_seqs: int, most: int, n_heads: int, n_kv: int, longest: int) -> int:
+        """Blocks that share a sequence's pages in the 32-bit kernel: two an SM, with two pages or more each."""
+        blocks = max(1, n_seqs * n_kv * ((most * (n_heads // n_kv) + 31) // 32))
+        return max(1, min(2 * self.sm_count // blocks, (longest + 2 * PAGE_TOKENS - 1) // (2 * PAGE_TOKENS), 64))
+
+    def draft_attention(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor, slots: torch.Tensor,
+                        page_table: torch.Tensor, n_kv: int, scale: float, most: int, ancestors: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """A few tokens a sequence against its cached keys: q [tokens, heads, d] -> [tokens, heads * d].  Sequence s brings the tokens cu_q[s] .. cu_q[s + 1], at most
+        ``most`` (up to MOST_DRAFTS), which are the last of its kv_len[s] keys in k_cache [pages, kv, PAGE_TOKENS, d] and v_cache [pages, kv, d, PAGE_TOKENS].  A
+        token sees all keys before these, and of these the ones up to itself, or with ``ancestors`` (int64 [tokens]) those whose bit is set.  A row that sees none
+        gives zeros; rows of no sequence are left as they are.  What an unseen key or value holds, even if it is no number, changes nothing."""
+        self._given(q, self.dtype, "q")
+        if q.dim() != 3:
+            raise ValueError("q: needs [tokens, heads, d]")
+        n, n_heads, d = q.shape
+        if n_kv < 1 or n_heads < 1 or n_heads % n_kv:
+            raise ValueError(f"{n_heads} heads cannot be grouped over {n_kv} key-value heads")
+        most = self._most(most)
+        for t, what, shape in ((k_cache, "key cache", (n_kv, PAGE_TOKENS, d)), (v_cache, "value cache", (n_kv, d, PAGE_TOKENS))):
+            self._given(t, self.dtype, what)
+            if t.dim() != 4 or tuple(t.shape[1:]) != shape or t.shape[0] != k_cache.shape[0] or t.shape[0] == 0:
+                raise ValueError(f"{what}: needs [pages, {', '.join(str(x) for x in shape)}], got {tuple(t.shape)}")
+        n_seqs, i32 = kv_len.numel(), torch.int32
+        self._given(kv_len, i32, "key counts")
+        self._given(slots, i32, "slots", n_seqs)
+        self._given(cu_q, i32, "token offsets", n_seqs + 1)
+        self._given(page_table, i32, "page table")
+        if page_table.dim() != 2 or page_table.numel() == 0:
+            raise ValueError("page table: needs [slots, pages]")
+        if ancestors is not None:
+            self._given(ancestors, torch.int64, "ancestors", n)
+        out = self.empty(n, n_heads * d)
+        if n == 0 or n_seqs == 0:
+            return out
+        shares = self.draft_attention_shares(n_seqs, most, n_heads, n_kv, page_table.shape[1] * PAGE_TOKENS)
+        parts = self.empty(shares * n * n_heads * (d + 2), dtype=torch.float32) if shares > 1 else None
+        check(self.lib.cpm_draft_attention_generic(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
+                                                   page_table.shape[1], k_cache.shape[0], _ptr(ancestors), _ptr(parts), shares, n, n_seqs, most, n_heads, n_kv, d,
+                                                   float(scale), self.code, self._stream()), f"attention of drafted tokens (head_dim {d})")
+        if shares > 1:
+            LAUNCHES_EXTRA[0] += 1
+        return out
+
+    def verify_drafts(self, logits: torch.Tensor, ids: torch.Tensor, cu_q: torch.Tensor, token_seq: torch.Tensor, most: int, uniform: Optional[torch.Tensor],
+                      temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                      min_p: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None,
+                      accept: Optional[torch.Tensor] = None, seed: int = 0, seq_key: Optional[torch.Tensor] = None, step_key: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Checks drafted tokens: sequence s brings the tokens ids[cu_q[s]] .. ids[cu_q[s + 1]] (at most ``most``), its last one and drafted ones that follow one another or, with
+        ``parents`` (int32 [tokens], a token's parent among its sequence's, which comes before it), form a tree; row i of the fp32 logits [tokens, vocab] says what
+        follows token i, under its sequence's ``temperature``, ``top_k``, ``top_p`` and ``min_p`` (one number a sequence, as in ``sample_filtered``).  Returns (tokens int32
+        [seqs, most], count int32 [seqs], path int32 [seqs, most], log-probabilities fp32 [seqs, most]): the ``count`` tokens that the step gives, which are the accepted ones and
+        one more; the places of the tokens that stay, the first and the accepted ones; -1, -1 and 0 behind them.
+        Without ``draft_probs`` every row draws its token by its number ``uniform`` [tokens] (in [0, 1)), or by the Philox value of (seed, seq_key, step_key + how
+        far its token stands behind its sequence's first by ``positions``), as ``sample_filtered`` would one step after the other; a token that was drafted
+        there is accepted (of equal ones the first).  With ``draft_probs`` fp32 [tokens, vocab], row i the probabilities that token i + 1 was drawn from (a chain's; a
+        sequence's last row is not read), token x is accepted if accept[i] * q(x) < p(x), and a refused one is replaced by where uniform[i] falls in max(0, p - q).
+        Probabilities are whole multiples of 2^-40 of a row's likeliest token's; tokens of no sequence (``token_seq`` -1) are left out."""
+        self._given(logits, torch.float32, "logits")
+        if logits.dim() != 2:
+            raise ValueError("logits: needs [tokens, vocab]")
+        n, vocab = logits.shape
+        most, n_seqs, i32, f32 = self._most(most), temperature.numel(), torch.int32, torch.float32
+        for t, dtype, count, what in ((ids, i32, n, "tokens"), (cu_q, i32, n_seqs + 1, "token offsets"), (token_seq, i32, n, "token sequences"),
+                                      (uniform, f32, n, "random numbers"), (temperature, f32, n_seqs, "temperatures"), (top_k, i32, n_seqs, "top-k"),
+                                      (top_p, f32, n_seqs, "top-p"), (min_p, f32, n_seqs, "min-p"), (parents, i32, n, "parents"), (accept, f32, n, "numbers of acceptance"),
+                                      (seq_key, i32, n_seqs, "sequence keys"), (step_key, i32, n_seqs, "step keys"), (positions, i32, n, "positions")):
+            if t is not None:
+                self._given(t, dtype, what, count)
+        if draft_probs is not None:
+            if draft_probs.dtype != f32 or draft_probs.get_device() != self.device_index or tuple(draft_probs.shape) != (n, vocab) or (vocab > 1 and draft_probs.stride(1) != 1):
+                raise ValueError(f"drafting probabilities: need fp32 [{n}, {vocab}] with neighbouring tokens side by side")
+            if parents is not None:
+                raise ValueError("drafting probabilities go with tokens in a row, not with a tree")
+            if uniform is None or accept is None:
+                raise ValueError("drafting probabilities need random numbers and numbers of acceptance")
+        elif uniform is None and (seq_key is None or step_key is None or positions is None):
+            raise ValueError("verify_drafts needs random numbers, or keys and positions to make them from")
+        tokens, path = self.result(n_seqs, most, dtype=i32), self.result(n_seqs, most, dtype=i32)
+        count, logprob = self.result(n_seqs, dtype=i32), self.result(n_seqs, most, dtype=f32)
+        if n_seqs == 0:
+            return tokens, count, path, logprob
+        drawn, drawn_logprob = self.empty(n, dtype=i32), self.empty(n, dtype=f32)
+        kept = self.empty(n, 4, dtype=torch.int64) if draft_probs is not None else None
+        check(self.lib.cpm_sample_drafts(_ptr(logits), vocab, n, vocab, _ptr(drawn), _ptr(drawn_logprob), _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                         _ptr(min_p), ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), _ptr(token_seq), _ptr(positions),
+                                         _ptr(cu_q), n_seqs, _ptr(kept), self._stream()), f"drawing for drafted tokens ({vocab} tokens)")
+        check(self.lib.cpm_verify_drafts(_ptr(logits), vocab, n, vocab, _ptr(ids), _ptr(cu_q), n_seqs, most, _ptr(parents), _ptr(draft_probs),
+                                         0 if draft_probs is None else draft_probs.stride(0), _ptr(accept), _ptr(uniform), _ptr(temperature), _ptr(drawn),
+                                         _ptr(drawn_logprob), _ptr(kept), _ptr(tokens), _ptr(count), _ptr(path), _ptr(logprob), self._stream()), "verify_drafts")
+        return tokens, count, path, logprob
+
+    def keep_drafts(self, pairs, lengths: torch.Tensor, path: torch.Tensor, count: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor) -> None:
+        """Moves the keys and values of accepted tokens to where their sequences go on, in one launch: of sequence s, which held ``lengths[s]`` tokens before the step, the
+        token that lies at lengths[s] + path[s][j] goes to lengths[s] + j, for j below count[s], in all layers of every pair (k [layers, pages, kv, PAGE_TOKENS, d],
+        v [layers, pages, kv, dv, PAGE_TOKENS] or None).  ``path`` int32 [seqs, most] rises along a row, as ``verify_drafts`` gives it.  A place that is in no
+        page of a tensor is left out."""
+        i32 = torch.int32
+        self._given(path, i32, "path")
+        if path.dim() != 2:
+            raise ValueError("path: needs [sequences, tokens]")
+        n_seqs = path.shape[0]
+        if path.shape[1] == 0 or path.shape[1] > self.MOST_DRAFTS:
+            raise ValueError(f"a path has 1 to {self.MOST_DRAFTS} places, got {path.shape[1]}")
+        for t, what in ((lengths, "lengths"), (count, "counts"), (slots, "slots")):
+            self._given(t, i32, what, n_seqs)
+        self._given(page_table, i32, "page table")
+        if page_table.dim() != 2 or page_table.numel() == 0:
+            raise ValueError("page table: needs [slots, pages]")
+        by_size = {}
+        for k, v in pairs:
+            for t, what in ((k, "keys"), (v, "values")):
+                if t is None and what == "values":
+                    continue
+                if not t.is_cuda or not t.is_contiguous() or t.get_device() != self.device_index or t.dim() != 5 or t.element_size() not in (2, 4):
+                    raise ValueError(f"{what}: need a contiguous tensor of 2 or 4 bytes a number [layers, pages, heads, ...] on cuda:{self.device_index}, got {t.dtype} "
+                                     f"{tuple(t.shape)} on {t.device}")
+            if k.shape[3] != PAGE_TOKENS or k.shape[4] < 1 or (v is not None and (v.shape[:3] != k.shape[:3] or v.shape[4] != PAGE_TOKENS or v.dtype != k.dtype)):
+                raise ValueError(f"keys {tuple(k.shape)} and values {None if v is None else tuple(v.shape)} are not pages of {PAGE_TOKENS} tokens of the same layers")
+            if k.numel() == 0:
+                continue
+            lanes, pages, kv, _, d = k.shape
+            by_size.setdefault(k.element_size(), []).append(
+                (k.data_ptr(), 0 if v is None else v.data_ptr(), k.stride(0) * k.element_size() if lanes > 1 else 0,
+                 0 if v is None or lanes < 2 else v.stride(0) * v.element_size(), lanes, pages, kv, d * k.element_size(), 0 if v is None else v.shape[3]))
+        if n_seqs == 0:
+            return
+        for element, words in by_size.items():
+            for i in range(0, len(words), self.COPY_TENSORS):
+                part = [x for w in words[i:i + self.COPY_TENSORS] for x in w]
+                check(self.lib.cpm_keep_drafts((ctypes.c_int64 * len(part))(*part), len(part) // 9, element, _ptr(lengths), _ptr(path), _ptr(count), _ptr(slots),
+                                               _ptr(page_table), page_table.shape[0], page_table.shape[1], n_seqs, path.shape[1], self._stream()), "keep_drafts")
 
 
 LAUNCHES_EXTRA = library.LAUNCHES
