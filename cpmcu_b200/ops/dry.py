@@ -70,6 +70,13 @@ class _NoLibrary:
     def cpm_kv4_attention_most_tiles():
         return 512
 
+    @staticmethod
+    def cpm_draft_attention_scratch_floats(n_heads, n_kv, d, most):
+        group = n_heads // n_kv
+        per_half = 128 // group
+        halves = 2 if most > per_half else 1
+        return 148 * (2 if d <= 64 and halves == 1 else 1) * (4 + 2 * min(halves * per_half, most) * group * (d + 2))
+
     def __getattr__(self, name):
         return lambda *args: 0
 

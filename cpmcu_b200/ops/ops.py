@@ -1024,6 +1024,8 @@ class Ops:
             arena.check_guards()
         if self.kv4_prompt_ran and int(self.lib.cpm_kv4_prompt_error()):
             raise RuntimeError("the prompts' attention over a 4-bit cache gave up waiting on a barrier; the results of this step are not valid")
+        if self.draft_attention_ran and int(self.lib.cpm_draft_attention_error()):
+            raise RuntimeError("the attention of drafted tokens gave up waiting on a barrier; the results of this step are not valid")
         if int(self.lib.cpm_listed_tile_error()):
             raise RuntimeError("the block-list attention of a prompt chunk gave up waiting on a barrier; the results of "
                                "this step are not valid")
@@ -1946,8 +1948,10 @@ class Ops:
               f"step_tables ({n_seqs} sequences)")
         return t
 
+    draft_attention_ran = False          # (without drafted tokens no step waits for its kernel's error)
+
     def draft_attention_on_tensor_cores(self, d: int, n_heads: int, n_kv: int) -> bool:
-        return False
+        return self.code == BF16 and self.use_tcgen05_draft and d in FAST_HEAD_DIMS and n_heads // n_kv <= 128
 
     def draft_attention_shares(self, n_seqs: int, most: int, n_heads: int, n_kv: int, longest: int) -> int:
         """Blocks that share a sequence's pages in the 32-bit kernel: two an SM, with two pages or more each."""
@@ -1982,6 +1986,14 @@ class Ops:
             self._given(ancestors, torch.int64, "ancestors", n)
         out = self.empty(n, n_heads * d)
         if n == 0 or n_seqs == 0:
+            return out
+        if scale > 0 and self.draft_attention_on_tensor_cores(d, n_heads, n_kv):
+            scratch = self.empty(self.lib.cpm_draft_attention_scratch_floats(n_heads, n_kv, d, most), dtype=torch.float32)
+            self.draft_attention_ran = True
+            check(self.lib.cpm_draft_attention_tcgen05(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
+                                                       page_table.shape[1], k_cache.shape[0], _ptr(ancestors), _ptr(scratch), n, n_seqs, most, n_heads, n_kv, d,
+                                                       float(scale), self._stream()), f"tcgen05 attention of drafted tokens (head_dim {d})")
+            LAUNCHES_EXTRA[0] += 1       # the pieces, then their addition
             return out
         shares = self.draft_attention_shares(n_seqs, most, n_heads, n_kv, page_table.shape[1] * PAGE_TOKENS)
         parts = self.empty(shares * n * n_heads * (d + 2), dtype=torch.float32) if shares > 1 else None
