@@ -24,12 +24,14 @@ CPM_BOUNDS_TU(draft_attention_tcgen05)
 namespace da5 {
 using namespace tc5;
 
-constexpr int kMostSeqs = 1024;                         // of one launch
+constexpr int kMostSeqs = 512;                          // of one launch
 constexpr int kStages = 4;                              // pages under way
 constexpr int kOdd = 8;                                 // segments that half 0 may be ahead of half 1, and more
 constexpr float kBehind = 8.0f;                         // the running maximum may lie 2^8 behind
 constexpr int kExtra = 2;                               // pages that a unit's beginning and end are worth
 constexpr int kLeast = 4;                               // cost that a block is worth its part's addition
+// Of four pairs of a row's weights one is formed by ex2_poly (2,048 pages of 256 rows a key-value head, 64 tokens at 131,071 keys: none 140 us, one 127, two 152)
+constexpr int kPoly = 8;                                // a bit for each of the four
 
 template <int D, int H>
 struct Sizes {
@@ -49,13 +51,17 @@ struct Args {
     const int *kv_len, *cu, *slots, *page_table;
     const int64_t* ancestors;
     const bf16* v;
-    float* scratch;                                     // per block a Cut, then two places of rows x (D + 2) floats
+    float* scratch;                                     // Cuts, then per block two places of (D + 2) x rows floats: channels, maximum, sum
     int max_pages, n_pages, n_tokens, n_seqs, n_heads, n_kv, group, most, per_half, rows;       // per_half: tokens of a half; rows: of a place
+    int parts;                                          // tiles that a sequence has at most
     float scale_log2;
 };
 
-struct Cut { int last_block, seq, part, head; };        // of the unit that begins in a block and goes on behind it; last_block -1: none
-constexpr int kCutFloats = 4;
+// A unit that several blocks have: the one it begins in and the last.  Few units have a Cut each, (sequence, tile, head) by number; of many, a block has one of the
+// unit that goes on behind it.
+struct __align__(8) Cut { int first_block, last_block, token, rows, head, unused; };      // last_block -1: none; its first token, and rows
+constexpr int kCutFloats = sizeof(Cut) / 4;
+__host__ __device__ __forceinline__ bool by_unit(const Args& a, int grid) { return (int64_t)a.n_seqs * a.parts * a.n_kv <= grid; }
 
 enum : int { ERR_Q = 1, ERR_K_FULL, ERR_V_FULL, ERR_K_EMPTY, ERR_V_EMPTY, ERR_S_FULL, ERR_P_FULL, ERR_O_DONE, ERR_V_READY };
 __device__ int g_error;
@@ -94,6 +100,33 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long ra, rb, rd;
+    float2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x of two numbers up to 100 without the unit that ex2 runs on, which gives 16 results a cycle and multiprocessor and which a page's weights would wait for: x = n + f with
+// f in [-1/2, 1/2]; 2^f by a polynomial of degree 4 whose coefficients minimise the largest relative error, 2.6e-6 (2^-18.5; the weights enter their product with 8
+// bits); 2^n by its exponent bits, which the sum with 1.5 * 2^23 + 127 leaves in its lowest ones.  From 2^-127 down the result is 0; what is no number stays none.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    const float magic = 12582912.f + 127.f;
+    x = make_float2(max_nan(x.x, -127.f), max_nan(x.y, -127.f));
+    const float2 t = add2(x, make_float2(magic, magic)), n = add2(t, make_float2(-magic, -magic)), f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 p = fma2(f, make_float2(0.009570101276040077f, 0.009570101276040077f), make_float2(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return mul2(p, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -102,7 +135,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // ---- the line of work ----
 struct Line {                                           // in shared memory
     int begin[kMostSeqs + 1];                           // cost before a sequence
-    int keys[kMostSeqs], first[kMostSeqs + 1];          // its keys, and its first token
+    int keys[kMostSeqs], first[kMostSeqs + 1], slot[kMostSeqs];      // its keys, its first token, its row of the page table
     int warp_sum[32];
 };
 __device__ __forceinline__ int pages_of(int keys) { return (keys + kPageTokens - 1) / kPageTokens; }
@@ -115,9 +148,38 @@ __device__ __forceinline__ int units_of(const Args& a, int tokens) { return (tok
 template <int H, int THREADS>
 __device__ __forceinline__ void lay_out(const Args& a, Line& l) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (a.n_seqs <= 32) {                               // one warp's work
+        if (warp == 0) {
+            const bool there = lane < a.n_seqs;
+            const int first = there ? max(0, min(a.cu[lane], a.n_tokens)) : 0, then = there ? max(0, min(a.cu[lane + 1], a.n_tokens)) : 0;
+            const int keys = there ? max(0, min(a.kv_len[lane], a.max_pages * kPageTokens)) : 0, slot = there ? a.slots[lane] : 0;
+            const int cost = there ? units_of<H>(a, max(0, min(then - first, a.most))) * (pages_of(keys) + kExtra) : 0;
+            int upto = cost;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            if (there) {
+                l.begin[lane] = upto - cost;
+                l.first[lane] = first;
+                l.keys[lane] = keys;
+                l.slot[lane] = slot;
+                if (lane == a.n_seqs - 1) {
+                    l.begin[lane + 1] = upto;
+                    l.first[lane + 1] = then;
+                }
+            }
+        }
+        __syncthreads();
+        return;
+    }
     for (int s = tid; s <= a.n_seqs; s += THREADS) {
         l.first[s] = max(0, min(a.cu[s], a.n_tokens));
-        if (s < a.n_seqs) l.keys[s] = max(0, min(a.kv_len[s], a.max_pages * kPageTokens));
+        if (s < a.n_seqs) {
+            l.keys[s] = max(0, min(a.kv_len[s], a.max_pages * kPageTokens));
+            l.slot[s] = a.slots[s];
+        }
     }
     __syncthreads();
     const int each = (a.n_seqs + THREADS - 1) / THREADS, s0 = min(a.n_seqs, tid * each), s1 = min(a.n_seqs, s0 + each);
@@ -204,6 +266,11 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_smem = base, k_smem = q_smem + H * Z::kQBufs * Z::kQ, v_smem = k_smem + kStages * Z::kK;
     constexpr int kScoreWarp = 4 * H, kValueWarp = 5 * H, kLoadWarp = 6 * H, kCleanWarp = 6 * H + 1;
+    if (threadIdx.x == 32) {
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&map_q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&map_v) : "memory");
+    }
     if (threadIdx.x == 0) {
 #pragma unroll 1
         for (int s = 0; s < kStages; ++s) {
@@ -255,6 +322,8 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
         }
         return false;
     };
+    // Up to 64 rows keep two warps busy: of two blocks on an SM the second has its rows in the tile's upper half, which other warps, on the SM's other schedulers, read
+    const int shift = Z::kBlocks == 2 && a.rows <= 64 && blockIdx.x >= gridDim.x / 2 ? 64 : 0;
     Walk<H> walk;
     Segment g;
     walk.start(a, line, lo, hi);
@@ -265,7 +334,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
         bool ok = true;
 #pragma unroll 1
         while (ok && walk.next(a, line, g)) {
-            const int* table = a.page_table + (int64_t)a.slots[g.seq] * a.max_pages;
+            const int* table = a.page_table + (int64_t)line.slot[g.seq] * a.max_pages;
             int ids = 0;                                // 32 page numbers, one a lane
 #pragma unroll 1
             for (int i = 0; i < g.pages; ++i, ++st) {
@@ -309,24 +378,32 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
                 const int s = st % kStages, key0 = (g.page0 + i) * kPageTokens;
                 if (!__all_sync(0xffffffffu, wait(v_full[s], (st / kStages) & 1))) { fail(ERR_V_FULL); ok = false; break; }
                 if (key0 + kPageTokens > g.history) {
-                    bool found = false;
-                    const int keep = g.keys - key0, own = g.history - key0;       // keys of the page that there are, and that are not the step's
-#pragma unroll 4
-                    for (int x = lane; x < D * 8; x += 32) {
-                        const int c = x >> 3, j0 = (x & 7) * 8;
-                        const uint32_t at = v_smem + s * Z::kV + c * 128 + (uint32_t)(((x & 7) ^ (c & 7)) << 4);
-                        uint32_t w[4];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+                    // a lane has the same eight keys of every channel it looks at: those that there are, and of these the step's own, by word
+                    const int j0 = (lane & 7) * 8, keep = g.keys - key0 - j0, own = g.history - key0 - j0;
+                    uint32_t there[4], check[4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint32_t bits = w[e >> 1] >> (16 * (e & 1)) & 0x7fffu, clear = ~(0xffffu << (16 * (e & 1)));
-                            if (j0 + e >= keep) w[e >> 1] &= clear;
-                            else if (j0 + e >= own && bits >= 0x7f80u) {
-                                w[e >> 1] &= clear;
+                    for (int e = 0; e < 4; ++e) {
+                        const auto from = [&](int n) { return (2 * e >= n ? 0xffffu : 0u) | (2 * e + 1 >= n ? 0xffff0000u : 0u); };
+                        there[e] = ~from(keep);
+                        check[e] = from(own) & there[e] & 0x80008000u;
+                    }
+                    bool found = false;
+                    if (own < 8) {
+#pragma unroll 8
+                        for (int x = 0; x < D / 4; ++x) {
+                            const int c = (lane >> 3) + 4 * x;
+                            const uint32_t at = v_smem + s * Z::kV + c * 128 + (uint32_t)(((lane & 7) ^ (c & 7)) << 4);
+                            uint32_t w[4], bad[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) bad[e] = ((w[e] & 0x7fff7fffu) + 0x00800080u) & check[e];      // an exponent of ones runs over into the sign's bit
+                            if (bad[0] | bad[1] | bad[2] | bad[3]) {
                                 found = true;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) w[e] &= ~((bad[e] >> 15) * 0xffffu);
                             }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(w[0] & there[0]), "r"(w[1] & there[1]), "r"(w[2] & there[2]), "r"(w[3] & there[3]) : "memory");
                         }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                     }
                     if (found) odd[number % kOdd] = number + 1;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -343,7 +420,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
         const auto load_q = [&](const Segment& x, int n) {
             if (lane == 0) {
                 const int b = n % Z::kQBufs;
-                const uint32_t to = q_smem + (i * Z::kQBufs + b) * Z::kQ;
+                const uint32_t to = q_smem + (i * Z::kQBufs + b) * Z::kQ + shift * 128;
                 mbar_expect_tx(smem_u32(&q_full[i][b]), Z::kChunks * a.per_half * a.group * 128);
 #pragma unroll
                 for (int c = 0; c < Z::kChunks; ++c)
@@ -421,7 +498,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
         }
     } else if (warp < 4 * H) {
         // ---- softmax and output: a thread to a row ----
-        const int i = warp >> 2, r = threadIdx.x & 127;
+        const int i = warp >> 2, r = (int)(threadIdx.x & 127) - shift;       // the row of its half; below 0: none
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_addr = lanes + Z::kO + i * D;
         int st = 0, number = 0;
@@ -429,7 +506,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
 #pragma unroll 1
         for (; ok && walk.next(a, line, g); ++number) {
             const int in_half = r / a.group, token = g.row0 + i * a.per_half + in_half;
-            const bool valid = in_half < a.per_half && token < g.tokens;
+            const bool valid = r >= 0 && in_half < a.per_half && token < g.tokens;
             const bool any = __any_sync(0xffffffffu, valid);
             uint64_t word = 0;                           // the step's tokens that the row sees
             if (valid) {
@@ -503,7 +580,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const float2 x = fma2(make_float2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), by, less);
-                            const float2 w = make_float2(ex2(x.x), ex2(x.y));
+                            const float2 w = (kPoly >> (e & 3) & 1) ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
                             sum[e & 1] = add2(sum[e & 1], w);
                             packed[e] = pack_bf16(w.x, w.y);
                         }
@@ -530,18 +607,18 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
                 const bool whole = g.whole();
                 const int64_t at = ((int64_t)(line.first[g.seq] + token) * a.n_heads + g.head * a.group + r % a.group) * D;
                 // a part of a unit that an earlier block began lies in the block's first place, one that goes on behind it in the second
-                float* const to = places + (2 * (int64_t)blockIdx.x + (g.page0 == 0)) * place_floats + (int64_t)((i * a.per_half + in_half) * a.group + r % a.group) * (D + 2);
+                float* const to = places + (2 * (int64_t)blockIdx.x + (g.page0 == 0)) * place_floats + i * a.per_half * a.group + r;
                 const bool fix = g.pages > 0 && odd[number % kOdd] == number + 1;
                 const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-                for (int c = 0; c < D / 16; ++c) {
-                    uint32_t o[16];
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
                     if (g.pages > 0) {
-                        tmem_load_16cols(o_addr + c * 16, o);
+                        tmem_load_32cols(o_addr + c * 32, o);
                         tmem_load_wait();
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = 0u;
+                        for (int e = 0; e < 32; ++e) o[e] = 0u;
                     }
                     if (!valid) continue;
                     if (fix) {
@@ -550,50 +627,56 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
                         for (int j = 0; j < g.tokens; ++j) {
                             const int key = g.history + j;
                             if (!(word >> j & 1) || key < g.page0 * kPageTokens || key >= (g.page0 + g.pages) * kPageTokens) continue;
-                            const int* table = a.page_table + (int64_t)a.slots[g.seq] * a.max_pages;
+                            const int* table = a.page_table + (int64_t)line.slot[g.seq] * a.max_pages;
                             const int64_t page = max(0, min(CPM_PAGE(table, key / kPageTokens, a.max_pages), a.n_pages - 1));
-                            const bf16* from = a.v + value_offset((int)page, g.head, c * 16, key % kPageTokens, a.n_kv, D);
+                            const bf16* from = a.v + value_offset((int)page, g.head, c * 32, key % kPageTokens, a.n_kv, D);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
+                            for (int e = 0; e < 32; ++e) {
                                 const float x = __bfloat162float(from[e * kPageTokens]);
                                 if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
                             }
                         }
                     }
                     if (whole) {
-                        uint4 y[2];
+                        uint4 y[4];
                         uint32_t* w = reinterpret_cast<uint32_t*>(y);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
+                        for (int e = 0; e < 16; ++e) {
                             const float lo_ = __uint_as_float(o[2 * e]), hi_ = __uint_as_float(o[2 * e + 1]);
                             w[e] = pack_bf16(l == 0.f ? lo_ : lo_ * inv, l == 0.f ? hi_ : hi_ * inv);
                         }
-                        *reinterpret_cast<uint4*>(a.out + at + c * 16) = y[0];
-                        *reinterpret_cast<uint4*>(a.out + at + c * 16 + 8) = y[1];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(a.out + at + c * 32 + 8 * e) = y[e];
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) *reinterpret_cast<float2*>(to + c * 16 + e) = make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+                        for (int e = 0; e < 32; ++e) to[(c * 32 + e) * a.rows] = __uint_as_float(o[e]);      // (neighbouring rows side by side)
                     }
                 }
-                if (valid && !whole) *reinterpret_cast<float2*>(to + D) = make_float2(m, l);
+                if (valid && !whole) {
+                    to[D * a.rows] = m;
+                    to[(D + 1) * a.rows] = l;
+                }
             }
             tcgen05_fence_before();                      // (the next segment's products come behind this warp's next P)
         }
     }
-    // ---- the unit that begins here and goes on behind ----
-    if (threadIdx.x == 0) {
-        Cut cut{-1, 0, 0, 0};
-        if (mine) {
-            Walk<H> again;
-            Segment x;
-            again.start(a, line, lo, hi);
-            while (again.next(a, line, x))
-                if (x.page0 == 0 && !x.whole()) {
-                    const int u = x.part * a.n_kv + x.head;
-                    cut = Cut{block_of(total, blocks, line.begin[x.seq] + (u + 1) * (x.all_pages + kExtra) - 1), x.seq, x.part, x.head};
-                }
+    // ---- the units that begin here, for the kernel that adds up parts ----
+    if (warp == kCleanWarp && lane == 0) {
+        Cut* const cuts = reinterpret_cast<Cut*>(a.scratch);
+        const bool each = by_unit(a, gridDim.x);
+        Cut last{(int)blockIdx.x, -1, 0, 0, 0, 0};
+        Walk<H> again;
+        Segment x;
+        again.start(a, line, lo, hi);
+        while (again.next(a, line, x)) {
+            if (x.page0 > 0) continue;
+            const int u = x.part * a.n_kv + x.head;
+            const Cut cut{(int)blockIdx.x, x.whole() ? -1 : block_of(total, blocks, line.begin[x.seq] + (u + 1) * (x.all_pages + kExtra) - 1),
+                          line.first[x.seq] + x.row0, min(H * a.per_half, x.tokens - x.row0) * a.group, x.head, 0};
+            if (each) cuts[(x.seq * a.parts + x.part) * a.n_kv + x.head] = cut;
+            else if (cut.last_block >= 0) last = cut;
         }
-        *reinterpret_cast<Cut*>(a.scratch + (int64_t)blockIdx.x * kCutFloats) = cut;
+        if (!each) cuts[blockIdx.x] = last;
     }
     tcgen05_fence_before();
     __syncthreads();
@@ -605,40 +688,75 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
     }
 }
 
-// Adds up the parts of the units that were cut: blockIdx.y is the block that a unit begins in, a warp takes a row.
-constexpr int kJoinThreads = 256;
+// Adds up the parts of the units that were cut.  A block has 32 rows of one unit and all or (few units) an eighth of the channels; a warp has an eighth of the channels
+// and every second or sixteenth part, a lane a row.
+constexpr int kJoinWarps = 16, kEighths = 8;
 template <int D, int H>
-__global__ void __launch_bounds__(kJoinThreads)
-draft_join_tcgen05_kernel(const __grid_constant__ Args a, int grid) {
+__global__ void __launch_bounds__(32 * kJoinWarps, 2)
+draft_join_tcgen05_kernel(const __grid_constant__ Args a, int grid, int eighths) {       // eighths: of the channels a block has, 1 or 8
+    constexpr int C = D / kEighths;
+    __shared__ float tops[kJoinWarps][32], sums[kJoinWarps][32], values[kJoinWarps][C][33], weight[kJoinWarps][32];
+    __shared__ bf16* to[32];                            // where a row's channels go
     pdl_launch_dependents();
     pdl_wait();
-    const int b0 = blockIdx.y, lane = threadIdx.x & 31, row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
-    const Cut cut = *reinterpret_cast<const Cut*>(a.scratch + (int64_t)b0 * kCutFloats);
-    if (cut.last_block < 0 || row >= a.rows) return;
-    const int token = cut.part * H * a.per_half + row / a.group, begin = max(0, min(a.cu[cut.seq], a.n_tokens));
-    if (token >= min(min(a.cu[cut.seq + 1], a.n_tokens) - begin, a.most)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = kEighths / eighths, groups = kJoinWarps / eighths;
+    const int r0 = blockIdx.x / pieces * 32, first_eighth = blockIdx.x % pieces * eighths, eighth = first_eighth + warp % eighths, group = warp / eighths;
+    const Cut cut = reinterpret_cast<const Cut*>(a.scratch)[blockIdx.y];
+    if (by_unit(a, grid)) {                             // (a unit that is none has no Cut)
+        const int s = blockIdx.y / (a.parts * a.n_kv), part = blockIdx.y / a.n_kv % a.parts;
+        const int first = max(0, min(a.cu[s], a.n_tokens)), n = min(max(0, min(a.cu[s + 1], a.n_tokens) - first), a.most);
+        if (part * H * a.per_half >= n) return;
+    }
+    if (cut.last_block < 0 || r0 >= cut.rows) return;
+    const int b0 = cut.first_block, row = min(r0 + lane, cut.rows - 1);
     const float* places = a.scratch + (int64_t)grid * kCutFloats;
     const int64_t place_floats = (int64_t)a.rows * (D + 2);
-    const auto part = [&](int b) { return places + (2 * (int64_t)b + (b == b0)) * place_floats + (int64_t)row * (D + 2); };
-    float top = -INFINITY, l = 0.f, o[D / 32];
+    float top = -INFINITY, l = 0.f, o[C];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-    for (int b = b0 + lane; b <= cut.last_block; b += 32) top = fmaxf(top, part(b)[D]);
-    top = warp_max(top);
-    const float use = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-    for (int b = b0; b <= cut.last_block; ++b) {
-        const float* p = part(b);
-        const float2 ml = *reinterpret_cast<const float2*>(p + D);
-        const float by = ex2(ml.x - use);
-        l += ml.y * by;
+    for (int i = 0; i < C; ++i) o[i] = 0.f;
+#pragma unroll 2
+    for (int b = b0 + group; b <= cut.last_block; b += groups) {
+        const float* p = places + (2 * (int64_t)b + (b == b0)) * place_floats + row;
+        float v[C];
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] += p[lane + 32 * i] * by;
+        for (int i = 0; i < C; ++i) v[i] = p[(eighth * C + i) * a.rows];
+        const float m = p[D * a.rows], sum = p[(D + 1) * a.rows], now = fmaxf(top, m), use = now == -INFINITY ? 0.f : now, back = ex2(top - use), by = ex2(m - use);
+        l = l * back + sum * by;
+#pragma unroll
+        for (int i = 0; i < C; ++i) o[i] = o[i] * back + v[i] * by;
+        top = now;
     }
-    const float inv = l == 0.f ? 1.f : 1.f / l;
-    bf16* out = a.out + ((int64_t)(begin + token) * a.n_heads + cut.head * a.group + row % a.group) * D;
+    tops[warp][lane] = top;
+    sums[warp][lane] = l;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) out[lane + 32 * i] = from_f32<bf16>(o[i] * inv);
+    for (int i = 0; i < C; ++i) values[warp][i][lane] = o[i];
+    __syncthreads();
+    // the groups' weights of every row (those of the warps with the block's first eighth stand for their groups)
+    const int many = min(groups, cut.last_block - b0 + 1);
+    if (warp == 1) to[lane] = a.out + ((int64_t)(cut.token + row / a.group) * a.n_heads + cut.head * a.group + row % a.group) * D + first_eighth * C;
+    if (warp == 0) {
+        float high = -INFINITY, all = 0.f;
+        for (int g = 0; g < many; ++g) high = fmaxf(high, tops[g * eighths][lane]);
+        const float use = high == -INFINITY ? 0.f : high;
+        for (int g = 0; g < many; ++g) all += sums[g * eighths][lane] * ex2(tops[g * eighths][lane] - use);
+        const float inv = all == 0.f ? 1.f : 1.f / all;
+        for (int g = 0; g < many; ++g) weight[g][lane] = ex2(tops[g * eighths][lane] - use) * inv;
+    }
+    __syncthreads();
+    // neighbouring lanes finish neighbouring channels of a row
+    const auto finish = [&](auto all_of_them) {
+        constexpr int N = decltype(all_of_them)::value ? kEighths : 1;       // eighths, in a block of which a row has N * C neighbours
+#pragma unroll 4
+        for (int x = threadIdx.x; x < 32 * N * C; x += 32 * kJoinWarps) {
+            const int r = x / (N * C), c = x % (N * C);
+            if (r0 + r >= cut.rows) break;
+            float y = 0.f;
+            for (int g = 0; g < many; ++g) y += values[g * N + c / C][c % C][r] * weight[g][r];
+            to[r][c] = from_f32<bf16>(y);
+        }
+    };
+    if (eighths == 1) finish(std::false_type{});
+    else finish(std::true_type{});
 }
 
 template <int D, int H>
@@ -662,7 +780,8 @@ int attend(const void* q, const void* k, Args a, cudaStream_t stream) {
         a.cu = all.cu + first;
         a.slots = all.slots + first;
         cpm_launch(kLaunchAttention, draft_attention_tcgen05_kernel<D, H>, dim3(grid), Z::kThreads, Z::kSmem, stream, map_q, map_k, map_v, a);
-        cpm_launch(kLaunchAttention, draft_join_tcgen05_kernel<D, H>, dim3((a.rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32), grid), kJoinThreads, 0, stream, a, grid);
+        const int units = by_unit(a, grid) ? a.n_seqs * a.parts * a.n_kv : grid, tiles = (a.rows + 31) / 32, eighths = units * tiles * 2 <= sms ? 1 : kEighths;
+        cpm_launch(kLaunchAttention, draft_join_tcgen05_kernel<D, H>, dim3(tiles * (kEighths / eighths), units), 32 * kJoinWarps, 0, stream, a, grid, eighths);
     }
     return launch_status();
 }
@@ -670,7 +789,7 @@ int attend(const void* q, const void* k, Args a, cudaStream_t stream) {
 // Tokens of a half, halves of a tile, and rows of a place in the scratch.
 struct Shape { int per_half, halves, rows; };
 Shape shape_of(int group, int most) {
-    const int per_half = 128 / group, halves = most > per_half ? 2 : 1;
+    const int fit = 128 / group, halves = most > fit ? 2 : 1, per_half = min(fit, most);
     return Shape{per_half, halves, min(halves * per_half, most) * group};
 }
 int blocks_per_sm(int d, int halves) {
@@ -708,7 +827,8 @@ CPM_API int cpm_draft_attention_tcgen05(const void* q, const void* k, const void
         max_pages > 0x7fffffff / kPageTokens)
         return CPM_BAD_ARGUMENT;
     const da5::Args a{(bf16*)out, kv_len, cu, slots, page_table, ancestors, (const bf16*)v, scratch, max_pages, n_pages, n_tokens, n_seqs, n_heads, n_kv,
-                      n_heads / n_kv, most, s.per_half, s.rows, scale * 1.4426950408889634f};
+                      n_heads / n_kv, most, s.per_half, s.rows, (most + s.halves * s.per_half - 1) / (s.halves * s.per_half),
+                      scale * 1.4426950408889634f};
     const bool two = s.halves == 2;
     switch (d) {
         case 32: return two ? da5::attend<32, 2>(q, k, a, stream) : da5::attend<32, 1>(q, k, a, stream);

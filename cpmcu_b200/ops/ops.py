@@ -69,6 +69,7 @@ class Ops:
             raise library.KernelLibraryError("this library runs on a CUDA device only; there is no CPU path")
         if not torch.cuda.is_available():
             raise library.KernelLibraryError("no CUDA device is available; there is no CPU path")
+        self.device_index = self.device.index if self.device.index is not None else _current_device()
         self.lib = library.load()
         if int(self.lib.cpm_page_tokens()) != PAGE_TOKENS or int(self.lib.cpm_prefill_attention_tile_rows()) != PREFILL_TILE_ROWS:
             raise library.KernelLibraryError("the kernel library was built for another page or query-tile size than the package")
@@ -1902,15 +1903,11 @@ class Ops:
     MOST_DRAFTS = 64                     # tokens that a sequence brings at most, the one before the drafted ones among them
 
     def _given(self, t: torch.Tensor, dtype: torch.dtype, what: str, n: Optional[int] = None) -> torch.Tensor:
-        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.get_device() != self.device_index:
+        if t.dtype != dtype or t.get_device() != self.device_index or not t.is_contiguous():
             raise ValueError(f"{what}: needs a contiguous {dtype} tensor on cuda:{self.device_index}, got {t.dtype} on {t.device} contiguous={t.is_contiguous()}")
         if n is not None and t.numel() != n:
             raise ValueError(f"{what}: needs {n} numbers, got {t.numel()}")
         return t
-
-    @property
-    def device_index(self) -> int:
-        return self.device.index if self.device.index is not None else _current_device()
 
     def _most(self, most: int) -> int:
         if not 1 <= int(most) <= self.MOST_DRAFTS:
@@ -1939,9 +1936,13 @@ class Ops:
             self._given(parents, i32, "parents", n_tokens)
         if free is not None:
             self._given(free, i32, "free pages")
-        t = StepTables(self.empty(n_seqs + 1, dtype=i32), self.empty(n_seqs, dtype=i32), *(self.empty(n_tokens, dtype=i32) for _ in range(3)),
-                       self.empty(n_tokens, dtype=torch.int64), None if parents is None else self.empty(n_tokens, dtype=torch.int64),
-                       None if free is None else self.empty(1, dtype=i32))
+        # one tensor, cut into the tables (an allocation takes the host as long as three cuts): the words of 64 bits come first
+        wide = n_tokens * (2 if parents is None else 4)
+        room = self.empty(wide + 3 * n_tokens + 2 * n_seqs + 2, dtype=i32)
+        words, *by_token, kv_len, cu_q, taken = room.split_with_sizes((wide, n_tokens, n_tokens, n_tokens, n_seqs, n_seqs + 1, 1))
+        words = words.view(torch.int64)
+        slot_map, ancestors = (words, None) if parents is None else words.split_with_sizes((n_tokens, n_tokens))
+        t = StepTables(cu_q, kv_len, *by_token, slot_map, ancestors, None if free is None else taken)
         check(self.lib.cpm_step_tables(_ptr(lengths), _ptr(new), _ptr(slots), n_seqs, n_tokens, _ptr(page_table), page_table.shape[0], page_table.shape[1],
                                        _ptr(parents), _ptr(free), 0 if free is None else free.numel(), _ptr(t.cu_q), _ptr(t.kv_len), _ptr(t.token_seq),
                                        _ptr(t.positions), _ptr(t.places), _ptr(t.slot_map), _ptr(t.ancestors), _ptr(t.taken), self._stream()),
@@ -2039,18 +2040,20 @@ class Ops:
                 raise ValueError("drafting probabilities need random numbers and numbers of acceptance")
         elif uniform is None and (seq_key is None or step_key is None or positions is None):
             raise ValueError("verify_drafts needs random numbers, or keys and positions to make them from")
-        tokens, path = self.result(n_seqs, most, dtype=i32), self.result(n_seqs, most, dtype=i32)
-        count, logprob = self.result(n_seqs, dtype=i32), self.result(n_seqs, most, dtype=f32)
+        tokens, path, logprob = self.result(3, n_seqs, most, dtype=i32).unbind()       # (one allocation: it takes the host as long as three cuts)
+        logprob, count = logprob.view(f32), self.result(n_seqs, dtype=i32)
         if n_seqs == 0:
             return tokens, count, path, logprob
-        drawn, drawn_logprob = self.empty(n, dtype=i32), self.empty(n, dtype=f32)
-        kept = self.empty(n, 4, dtype=torch.int64) if draft_probs is not None else None
-        check(self.lib.cpm_sample_drafts(_ptr(logits), vocab, n, vocab, _ptr(drawn), _ptr(drawn_logprob), _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+        # what every row keeps (32 bytes), the token that it draws, and its log-probability
+        rows = self.empty((8 if draft_probs is not None else 0) * n + 2 * n, dtype=i32)
+        kept = rows.data_ptr() if draft_probs is not None else None
+        drawn = rows.data_ptr() + (32 * n if draft_probs is not None else 0)
+        check(self.lib.cpm_sample_drafts(_ptr(logits), vocab, n, vocab, drawn, drawn + 4 * n, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
                                          _ptr(min_p), ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), _ptr(token_seq), _ptr(positions),
-                                         _ptr(cu_q), n_seqs, _ptr(kept), self._stream()), f"drawing for drafted tokens ({vocab} tokens)")
+                                         _ptr(cu_q), n_seqs, kept, self._stream()), f"drawing for drafted tokens ({vocab} tokens)")
         check(self.lib.cpm_verify_drafts(_ptr(logits), vocab, n, vocab, _ptr(ids), _ptr(cu_q), n_seqs, most, _ptr(parents), _ptr(draft_probs),
-                                         0 if draft_probs is None else draft_probs.stride(0), _ptr(accept), _ptr(uniform), _ptr(temperature), _ptr(drawn),
-                                         _ptr(drawn_logprob), _ptr(kept), _ptr(tokens), _ptr(count), _ptr(path), _ptr(logprob), self._stream()), "verify_drafts")
+                                         0 if draft_probs is None else draft_probs.stride(0), _ptr(accept), _ptr(uniform), _ptr(temperature), drawn,
+                                         drawn + 4 * n, kept, _ptr(tokens), _ptr(count), _ptr(path), _ptr(logprob), self._stream()), "verify_drafts")
         return tokens, count, path, logprob
 
     def keep_drafts(self, pairs, lengths: torch.Tensor, path: torch.Tensor, count: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor) -> None:
