@@ -61,6 +61,13 @@ struct Weigher {
         const float q = __fmul_rn(x, inverse);
         return __fmaf_rn(__fmaf_rn(-q, t, x), inverse, q);
     }
+    // Whether ``form_quick`` gives the same: the usual case, in which a token's weight is formed without a branch.
+    __device__ __forceinline__ bool quick() const { return inverse != 0.f && top < INFINITY; }
+    __device__ __forceinline__ float form_quick(float x) const {
+        x = __fsub_rn(x, top);
+        const float q = __fmul_rn(x, inverse), v = expf(__fmaf_rn(__fmaf_rn(-q, t, x), inverse, q));
+        return v >= 0.f ? v : 0.f;
+    }
     __device__ __forceinline__ float form(float x) const {
         if (top == INFINITY) return x == INFINITY ? 1.f : 0.f;
         const float v = expf(over_t(__fsub_rn(x, top)));

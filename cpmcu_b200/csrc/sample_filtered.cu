@@ -22,6 +22,7 @@
 // (10 us of the 117); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
 #include "filtered.cuh"
 #include "philox.cuh"
+#include <type_traits>
 
 namespace {
 
@@ -437,21 +438,26 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     const int strip = (row.n + kFilterThreads - 1) / kFilterThreads | 1, i0 = min(row.n, tid * strip), i1 = min(row.n, i0 + strip);
     const bool summed = STAGED && by_mass && !by_count;        // whether the bins' masses are
     uint64_t own_mass = 0;                                     // of the thread's tokens that bins do not tell exactly
-    if (by_count || by_mass) {
-        uint32_t small = 0;
+    const auto weigh_all = [&](auto quick) {
+        const auto form = [&](float x) { return decltype(quick)::value ? row.form_quick(x) : row.form(x); };
+        if (by_count || by_mass) {
+            uint32_t small = 0;
 #pragma unroll 4
-        for (int i = i0; i < i1; ++i) {
-            const float w = STAGED ? row.form(weights[i]) : row.at(i);
-            if constexpr (STAGED) weights[i] = w;
-            count_own<STAGED>(sm, __float_as_uint(w), summed);
-            if (summed) small += small_units_of(__float_as_uint(w));
-            else if (!STAGED && !by_count) own_mass += units_of(__float_as_uint(w));
+            for (int i = i0; i < i1; ++i) {
+                const float w = form(STAGED ? weights[i] : row.z[i]);
+                if constexpr (STAGED) weights[i] = w;
+                count_own<STAGED>(sm, __float_as_uint(w), summed);
+                if (summed) small += small_units_of(__float_as_uint(w));
+                else if (!STAGED && !by_count) own_mass += units_of(__float_as_uint(w));
+            }
+            own_mass += small;
+        } else if constexpr (STAGED) {
+#pragma unroll 4
+            for (int i = i0; i < i1; ++i) weights[i] = form(weights[i]);
         }
-        own_mass += small;
-    } else if constexpr (STAGED) {
-#pragma unroll 2
-        for (int i = i0; i < i1; ++i) weights[i] = row.form(weights[i]);
-    }
+    };
+    if (row.quick()) weigh_all(std::true_type{});
+    else weigh_all(std::false_type{});
     __syncthreads();
     const auto put_mass = [&](uint64_t own) {                  // the block's sum into the first block's (or every block's) list of sums
         const uint64_t all = block_sum64(own, sm);

@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMostBlocks = 8;
+constexpr int kWarps = 16, kThreads = 32 * (kWarps + 1), kMostBlocks = 8;        // and one that writes the path
 constexpr int kMostTokens = 64;                        // of a sequence: two to a lane
 
 struct VerifyArgs {
@@ -37,13 +37,19 @@ struct VerifyArgs {
 struct Filtered {
     Weigher w;
     KeptRow k;
+    // Below this a logit less the largest has a weight that is not kept, or no units, for sure: t (log of the border, or of 2^-40, less 1/1000, which is far more than
+    // the logarithm, the exponential and these products are off).
+    __device__ __forceinline__ float floor_of() const {
+        if (k.border == kOneToken || k.top == INFINITY) return -INFINITY;
+        return w.t * (fmaxf(logf(__uint_as_float(k.border)), -27.726f) * 1.00001f - 0.001f);
+    }
     __device__ __forceinline__ uint64_t units(int v, float z) const {
         if (k.border == kOneToken) return v == k.cut ? k.total : 0;
         const uint32_t bits = __float_as_uint(w.form(z));
         return bits > k.border || (bits == k.border && v <= k.cut) ? units_of(bits) : 0;
     }
     // What the drafter's probability takes of a token's units (a number that is none: nothing).
-    __device__ __forceinline__ uint64_t taken(float q) const { return __double2ull_rz(fmin(fmax((double)q, 0.0), 1.0) * (double)k.total); }
+    __device__ __forceinline__ uint64_t taken(float q) const { return __double2ull_rz((double)fminf(fmaxf(q, 0.f), 1.f) * (double)k.total); }
     __device__ __forceinline__ float logprob(float z) const {
         if (k.border == kOneToken) return k.top == -INFINITY ? -INFINITY : 0.f;
         return (k.top == INFINITY ? 0.f : w.over_t(__fsub_rn(z, k.top))) - logf((float)((double)k.total * (1.0 / 1099511627776.0)));
@@ -61,10 +67,11 @@ struct VerifyShared {
     uint64_t warp_sum[kWarps + 1];
     alignas(8) uint64_t mass[kMostBlocks];             // of the cluster's blocks, which write here
     int drawn[kMostTokens];
-    int count, last, refused;                          // accepted tokens and the root; the last of them; whether its row is to be drawn again
+    uint64_t accepted;                                 // the root and the accepted tokens
+    int last, refused;                                 // the last of them; whether its row is to be drawn again
 };
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 1)
 verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
     __shared__ VerifyShared sm;
     pdl_wait();
@@ -94,9 +101,9 @@ verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
                 bool ok = true;                         // whether token i + 1 is accepted
                 if (i + 1 < n) {
                     const int x = a.ids[first + i + 1];
+                    const Filtered f = filtered(a, first + i, t);
                     ok = false;
                     if (x >= 0 && x < a.vocab) {
-                        const Filtered f = filtered(a, first + i, t);
                         const uint64_t w = f.units(x, a.logits[(int64_t)(first + i) * a.ld + x]), q = f.taken(a.probs[(int64_t)(first + i) * a.ldq + x]);
                         ok = (double)a.accept[first + i] * (double)q < (double)w;
                     }
@@ -123,39 +130,35 @@ verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
                 accepted |= 1ull << last;
             }
         }
-        if (rank == 0) {
-            const int count = __popcll(accepted);
-            // a token of the path stands where as many of it come before; the token behind it is the path's next one's id
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int i = lane + 32 * h;
-                if (mine[h] && accepted >> i & 1) {
-                    const int at = __popcll(accepted & ((1ull << i) - 1));
-                    a.path[(int64_t)s * a.most + at] = i;
-                    if (at > 0) {
-                        a.tokens[(int64_t)s * a.most + at - 1] = id[h];
-                        const int row = first + (a.probs ? i - 1 : parent[h]);
-                        a.logprob[(int64_t)s * a.most + at - 1] =
-                            a.probs ? filtered(a, row, t).logprob(a.logits[(int64_t)row * a.ld + id[h]]) : a.drawn_logprob[row];
-                    }
-                }
-            }
-            for (int i = lane; i < a.most; i += 32) {
-                if (i >= count) {
-                    a.tokens[(int64_t)s * a.most + i] = a.path[(int64_t)s * a.most + i] = -1;
-                    a.logprob[(int64_t)s * a.most + i] = 0.f;
-                }
-            }
-            if (lane == 0) a.count[s] = count;
-        }
         if (lane == 0) {
-            sm.count = __popcll(accepted);
+            sm.accepted = accepted;
             sm.last = last;
             sm.refused = refused;
         }
     }
     __syncthreads();
-    const int count = sm.count;
+    const uint64_t accepted = sm.accepted;
+    const int count = __popcll(accepted);
+    // ---- the path, by a warp that has nothing else to do where a row is drawn again ----
+    if (rank == 0 && warp == (int)blockDim.x / 32 - 1) {
+        // a token of the path stands where as many of it come before; the token behind it is the path's next one's id
+#pragma unroll 1
+        for (int i = lane; i < n; i += 32) {
+            if (!(accepted >> i & 1)) continue;
+            const int at = __popcll(accepted & ((1ull << i) - 1));
+            a.path[(int64_t)s * a.most + at] = i;
+            if (at == 0) continue;
+            const int id = a.ids[first + i], row = first + (a.probs || !a.parents ? i - 1 : a.parents[first + i]);
+            a.tokens[(int64_t)s * a.most + at - 1] = id;
+            a.logprob[(int64_t)s * a.most + at - 1] = a.probs ? filtered(a, row, t).logprob(a.logits[(int64_t)row * a.ld + id]) : a.drawn_logprob[row];
+        }
+#pragma unroll 1
+        for (int i = count + lane; i < a.most; i += 32) {
+            a.tokens[(int64_t)s * a.most + i] = a.path[(int64_t)s * a.most + i] = -1;
+            a.logprob[(int64_t)s * a.most + i] = 0.f;
+        }
+        if (lane == 0) a.count[s] = count;
+    }
     if (count == 0) return;                             // (the whole cluster leaves)
     const int64_t out = (int64_t)s * a.most + count - 1;
     const int row = first + sm.last;
@@ -170,39 +173,87 @@ verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
     // ---- a token in the place of the refused one ----
     const Filtered f = filtered(a, row, t);
     const int begin = min(a.vocab, rank * a.per_block), end = min(a.vocab, begin + a.per_block);
-    const int each = ((end - begin + kWarps - 1) / kWarps + 127) & ~127;             // tokens of a warp, which are neighbours
-    const int w0 = min(end, begin + warp * each), w1 = min(end, w0 + each);
+    // A warp has up to 32 runs of some times 128 neighbouring tokens, four of which are a lane's; lane g keeps the sum of run g, so that the token's run is known at the end.
+    const int per_run = 128 * max(1, ((end - begin + kWarps - 1) / kWarps + 128 * 32 - 1) / (128 * 32));
+    const int each = ((end - begin + kWarps - 1) / kWarps + per_run - 1) / per_run * per_run;
+    const int w0 = min(end, begin + warp * each), w1 = warp < kWarps ? min(end, w0 + each) : w0;       // (none of the last warp, which has the path)
     const float *z = a.logits + (int64_t)row * a.ld, *q = a.probs + (int64_t)row * a.ldq;
     const bool whole = (((uintptr_t)(z + w0) | (uintptr_t)(q + w0)) & 15) == 0;
-    // four neighbouring tokens' units beyond what the drafter's probability takes; nothing behind the warp's end
-    const auto left = [&](int v, uint64_t (&r)[4]) {
-        float zz[4], qq[4];
+    struct Four { float z[4], q[4]; };
+    const auto load = [&](int v, Four& x) {              // (nothing behind the warp's end)
         if (whole && v + 4 <= w1) {
-            *reinterpret_cast<float4*>(zz) = *reinterpret_cast<const float4*>(z + v);
-            *reinterpret_cast<float4*>(qq) = *reinterpret_cast<const float4*>(q + v);
+            *reinterpret_cast<float4*>(x.z) = __ldg(reinterpret_cast<const float4*>(z + v));
+            *reinterpret_cast<float4*>(x.q) = __ldg(reinterpret_cast<const float4*>(q + v));
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                zz[e] = v + e < w1 ? z[v + e] : -INFINITY;
-                qq[e] = v + e < w1 ? q[v + e] : 1.f;
+                x.z[e] = v + e < w1 ? z[v + e] : -INFINITY;
+                x.q[e] = v + e < w1 ? q[v + e] : 1.f;
             }
+        }
+    };
+    const float least = f.floor_of(), k_top = f.k.top;
+    // units beyond what the drafter's probability takes
+    const bool quick = f.w.quick() && f.k.border != kOneToken;
+    const auto left = [&](int v, const Four& x, uint64_t (&r)[4]) {
+        if (quick) {
+            // four tokens without a branch between them, if one of the warp's may be kept
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) any |= !(__fsub_rn(x.z[e], k_top) < least);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = 0;
+            if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float w = f.w.form_quick(x.z[e]);
+                const uint32_t bits = __float_as_uint(w);
+                const bool kept = v + e < w1 && (bits > f.k.border || (bits == f.k.border && v + e <= f.k.cut));
+                const int64_t d = (int64_t)__float2ull_rz(w * 0x1p40f) - (int64_t)f.taken(x.q[e]);      // (both below 2^62)
+                r[e] = kept && d > 0 ? d : 0;
+            }
+            return;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint64_t w = v + e < w1 ? f.units(v + e, zz[e]) : 0, taken = w ? f.taken(qq[e]) : 0;
-            r[e] = w > taken ? w - taken : 0;
+            const uint64_t w = v + e < w1 && !(__fsub_rn(x.z[e], k_top) < least) ? f.units(v + e, x.z[e]) : 0;
+            r[e] = 0;
+            if (w) {
+                const uint64_t taken = f.taken(x.q[e]);
+                r[e] = w > taken ? w - taken : 0;
+            }
         }
     };
-    uint64_t sum = 0;
-#pragma unroll 2
-    for (int v = w0 + 4 * lane; v < w1; v += 128) {
-        uint64_t r[4];
-        left(v, r);
-        sum += r[0] + r[1] + r[2] + r[3];
-    }
+    const auto warp_total = [](uint64_t v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sm.warp_sum[warp] = sum;
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    constexpr int kAhead = 4;
+    uint64_t mine = 0, run_sum = 0;                      // of the lane's run, and the lane's share of the run under way
+    int number = 0, filled = 0;
+#pragma unroll 1
+    for (int v0 = w0; v0 < w1; v0 += 128 * kAhead) {
+        Four x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) load(v0 + 128 * u + 4 * lane, x[u]);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int at = v0 + 128 * u;
+            if (at >= w1) break;
+            uint64_t r[4];
+            left(at + 4 * lane, x[u], r);
+            run_sum += r[0] + r[1] + r[2] + r[3];
+            if ((filled += 128) == per_run || at + 128 >= w1) {
+                const uint64_t all = warp_total(run_sum);
+                if (lane == number++) mine = all;
+                run_sum = 0;
+                filled = 0;
+            }
+        }
+    }
+    const uint64_t sum = warp_total(mine);
+    if (lane == 0 && warp < kWarps) sm.warp_sum[warp] = sum;
     __syncthreads();
     uint64_t before = 0, block_total = 0;
 #pragma unroll 1
@@ -232,25 +283,36 @@ verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
         return;
     }
     const uint64_t target = min((uint64_t)((double)a.uniform[row] * (double)total), total - 1);
-    if (target < before || target >= before + sum) return;
+    if (warp == kWarps || target < before || target >= before + sum) return;
+    uint64_t upto = mine;                                // the run it is in
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    const int run = __ffs(__ballot_sync(0xffffffffu, target < before + upto)) - 1;
+    before += __shfl_sync(0xffffffffu, upto - mine, run);
+    const int stop = min(w1, w0 + (run + 1) * per_run);
 #pragma unroll 1
-    for (int v0 = w0; v0 < w1; v0 += 128) {
+    for (int v0 = w0 + run * per_run; v0 < stop; v0 += 128) {
         const int v = v0 + 4 * lane;
-        uint64_t r[4] = {0, 0, 0, 0};
-        if (v < w1) left(v, r);
+        Four x;
+        uint64_t r[4];
+        load(v, x);
+        left(v, x, r);
         const uint64_t own = r[0] + r[1] + r[2] + r[3];
-        uint64_t upto = own;
+        upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
+            const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
         }
         const uint64_t all = __shfl_sync(0xffffffffu, upto, 31);
         if (target < before + all) {
-            uint64_t run = before + upto - own;
-            if (target >= run && target < run + own) {
+            uint64_t from = before + upto - own;
+            if (target >= from && target < from + own) {
                 int e = 0;
-                while (e < 3 && target >= run + r[e]) run += r[e++];
+                while (e < 3 && target >= from + r[e]) from += r[e++];
                 a.tokens[out] = v + e;
                 a.logprob[out] = f.logprob(z[v + e]);
             }
@@ -271,14 +333,14 @@ CPM_API int cpm_verify_drafts(const float* logits, int64_t ld, int n_rows, int v
     if (n_rows < 0 || vocab < 1 || most < 1 || most > kMostTokens || n_seqs > 0x7fffffff / kMostBlocks) return CPM_BAD_ARGUMENT;
     if (probs && (parents || !accept || !uniform || !kept)) return CPM_BAD_ARGUMENT;
     int blocks = 1;
-    if (probs) {                                         // as many blocks a sequence as run at the same time
+    if (probs) {                                         // as many blocks a sequence as run at the same time, one an SM
         const int sms = device_sms();
         blocks = kMostBlocks;
-        while (blocks > 1 && ((int64_t)n_seqs * blocks > 2 * sms || vocab < 2048 * blocks)) blocks /= 2;
+        while (blocks > 1 && ((int64_t)n_seqs * blocks > sms || vocab < 2048 * blocks)) blocks /= 2;
     }
     const int per_block = ((vocab + blocks - 1) / blocks + 3) & ~3;
     const VerifyArgs a{logits, ld, probs, ldq, accept, uniform, temperature, ids, cu, parents, drawn, drawn_logprob, (const KeptRow*)kept, vocab, per_block,
                        n_rows, most, tokens, count, path, logprob};
-    cpm_launch_cluster(kLaunchOther, verify_drafts_kernel, dim3(n_seqs * blocks), probs ? kThreads : 32, 0, stream, blocks, a);
+    cpm_launch_cluster(kLaunchOther, verify_drafts_kernel, dim3(n_seqs * blocks), probs ? kThreads : 64, 0, stream, blocks, a);
     return launch_status();
 }
