@@ -8,8 +8,8 @@ has them; every flag has a ``--kebab-case`` and a ``--snake_case`` spelling.
 Options the reference has and this library leaves out belong to parts that are not
 built (draft models, quantized weights, the per-flag sparse-attention knobs: those come
 from the folder's config.json here).  Added: ``--prompt-ids`` (token ids, no tokenizer
-needed), ``--top-p``, ``--top-k``, ``--min-p``, ``--samples``, ``--cache-bits``, ``--max-batch``, ``--max-tokens``, ``--plugin`` (a module that registers
-parts or an architecture of its own).
+needed), ``--top-p``, ``--top-k``, ``--min-p``, ``--samples``, ``--cache-bits``, ``--draft-tokens``, ``--max-batch``, ``--max-tokens``, ``--plugin`` (a module
+that registers parts or an architecture of its own).
 """
 from __future__ import annotations
 
@@ -82,6 +82,8 @@ def create_cli_parser() -> argparse.ArgumentParser:
                    help="Use plain text output (default: False; output is always plain here)")
     g.add_argument("--cache-bits", "--cache_bits", type=int, default=None, choices=[4, 16],
                    help="Bits of a key or value in the cache (default: the configuration's, 16)")
+    g.add_argument("--draft-tokens", "--draft_tokens", type=int, default=0,
+                   help="Tokens looked up in the text so far that a step checks per sequence (default: 0, none)")
     g.add_argument("--max-batch", "--max_batch", type=int, default=64, help="Most sequences in one batch (default: 64)")
     g.add_argument("--max-tokens", "--max_tokens", type=int, default=None,
                    help="Tokens the cache holds (default: from --memory-limit)")
@@ -148,7 +150,7 @@ def run_generation(args) -> int:
     llm = LLM(args.model_path, apply_sparse=not args.dense, memory_limit=args.memory_limit, chunk_length=args.chunk_length, dtype=args.dtype,
               cuda_graph=args.cuda_graph, temperature=args.temperature, random_seed=args.random_seed,
               top_p=args.top_p, max_batch=args.max_batch, max_tokens=args.max_tokens, top_k=args.top_k, min_p=args.min_p,
-              cache_bits=args.cache_bits)
+              cache_bits=args.cache_bits, draft_tokens=args.draft_tokens)
     llm.tokenizer = tokenizer
     prompts = make_prompts(args, tokenizer)
     terminators = [] if args.ignore_eos else list(llm.model.spec.stop_token_ids)

@@ -258,14 +258,15 @@ CPM_API int cpm_silu_mul(const void* gu, void* h, int n_tokens, int inter, int i
 // fp32 with the accurate sincosf (src/model/rotary.cuh:6-34 uses the same pairing
 // but the fast-math cos/sin).  cos and sin are multiplied by ``magnitude`` (the
 // LongRoPE attention factor).  inv_freq == nullptr: no rotation.
-// qkv row: [heads*d | kv_heads*d | kv_heads*dv]; dv, the size of a value head, may differ from d.
+// qkv row: [heads*d | kv_heads*d | kv_heads*dv]; dv, the size of a value head, may differ from d.  places: where a token lies in its sequence's
+// cache, if that is not its position (nullptr: it is).
 // ---------------------------------------------------------------------------
 constexpr int kRopeHeadsPerBlock = 4;
 
 template <typename T>
 __global__ void rope_store_kernel(const T* __restrict__ qkv, T* __restrict__ q_out,
                                   T* __restrict__ k_cache, T* __restrict__ v_cache,
-                                  const int* __restrict__ positions, const int* __restrict__ token_seq,
+                                  const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ token_seq,
                                   const int* __restrict__ slots, const int* __restrict__ page_table,
                                   int max_pages, const float* __restrict__ inv_freq, float magnitude,
                                   int n_heads, int n_kv, int d, int rot_dim, int dv) {
@@ -298,9 +299,10 @@ __global__ void rope_store_kernel(const T* __restrict__ qkv, T* __restrict__ q_o
     int64_t k_base = 0, v_base = 0;
     if (k_cache) {
         const int slot = slots[token_seq[t]];
-        const int page = CPM_PAGE(page_table + (int64_t)slot * max_pages, pos / kPageTokens, max_pages);
-        k_base = page_row_offset(page, 0, pos % kPageTokens, n_kv, d);
-        v_base = value_offset(page, 0, 0, pos % kPageTokens, n_kv, dv);
+        const int place = places ? places[t] : pos;
+        const int page = CPM_PAGE(page_table + (int64_t)slot * max_pages, place / kPageTokens, max_pages);
+        k_base = page_row_offset(page, 0, place % kPageTokens, n_kv, d);
+        v_base = value_offset(page, 0, 0, place % kPageTokens, n_kv, dv);
     }
     const int64_t head_stride_in_page = (int64_t)kPageTokens * d;
     for (int h = h_begin; h < h_end; ++h) {
@@ -331,7 +333,7 @@ __global__ void rope_store_kernel(const T* __restrict__ qkv, T* __restrict__ q_o
 // decode steps, where the tokens alone would not fill the GPU.
 __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __restrict__ q_out,
                                       bf16* __restrict__ k_cache, bf16* __restrict__ v_cache,
-                                      const int* __restrict__ positions, const int* __restrict__ token_seq,
+                                      const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ token_seq,
                                       const int* __restrict__ slots, const int* __restrict__ page_table,
                                       int max_pages, const float* __restrict__ inv_freq, float magnitude,
                                       int n_heads, int n_kv, int d, int heads_per_block) {
@@ -364,9 +366,10 @@ __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __rest
     int64_t k_base = 0, v_base = 0;
     if (k_cache && h_end > n_heads) {                            // only blocks with key or value heads look the page up
         const int slot = slots[token_seq[t]];
-        const int page = CPM_PAGE(page_table + (int64_t)slot * max_pages, pos / kPageTokens, max_pages);
-        k_base = page_row_offset(page, 0, pos % kPageTokens, n_kv, d);
-        v_base = value_offset(page, 0, 0, pos % kPageTokens, n_kv, d);
+        const int place = places ? places[t] : pos;
+        const int page = CPM_PAGE(page_table + (int64_t)slot * max_pages, place / kPageTokens, max_pages);
+        k_base = page_row_offset(page, 0, place % kPageTokens, n_kv, d);
+        v_base = value_offset(page, 0, 0, place % kPageTokens, n_kv, d);
     }
     __syncthreads();
     pdl_wait();
@@ -414,10 +417,10 @@ __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __rest
 }
 
 // ``dv``: the size of a value head (the value pages are [kv_head][dv][token]).
-CPM_API int cpm_rope_store_dv(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions,
-                              const int* token_seq, const int* slots, const int* page_table, int max_pages,
-                              const float* inv_freq, float magnitude, int n_tokens, int n_heads, int n_kv, int d,
-                              int dv, int rot_dim, int dtype, cudaStream_t stream) {
+static int rope_store(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions, const int* places,
+                      const int* token_seq, const int* slots, const int* page_table, int max_pages,
+                      const float* inv_freq, float magnitude, int n_tokens, int n_heads, int n_kv, int d,
+                      int dv, int rot_dim, int dtype, cudaStream_t stream) {
     if (n_tokens <= 0) return CPM_OK;
     if (rot_dim < 0 || rot_dim > d || (rot_dim & 1) || dv < 1) return CPM_BAD_ARGUMENT;
     if ((k_cache == nullptr) != (v_cache == nullptr)) return CPM_BAD_ARGUMENT;
@@ -430,7 +433,7 @@ CPM_API int cpm_rope_store_dv(const void* qkv, void* q_out, void* k_cache, void*
         dim3 vgrid(n_tokens, (n_all + heads_per_block - 1) / heads_per_block);
         if (vgrid.y > 65535) return CPM_BAD_ARGUMENT;
         cpm_launch(kLaunchRope, rope_store_vec_kernel, vgrid, threads, (size_t)d * sizeof(float), stream, (const bf16*)qkv, (bf16*)q_out,
-                   (bf16*)k_cache, (bf16*)v_cache, positions, token_seq, slots, page_table, max_pages, inv_freq, magnitude,
+                   (bf16*)k_cache, (bf16*)v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude,
                    n_heads, n_kv, d, heads_per_block);
         return launch_status();
     }
@@ -440,11 +443,28 @@ CPM_API int cpm_rope_store_dv(const void* qkv, void* q_out, void* k_cache, void*
     const size_t smem = (size_t)(rot_dim > 0 ? rot_dim : 2) * sizeof(float);
     if (dtype == CPM_BF16)
         cpm_launch(kLaunchRope, rope_store_kernel<bf16>, grid, threads, smem, stream, (const bf16*)qkv, (bf16*)q_out, (bf16*)k_cache,
-            (bf16*)v_cache, positions, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
+            (bf16*)v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
     else
         cpm_launch(kLaunchRope, rope_store_kernel<float>, grid, threads, smem, stream, (const float*)qkv, (float*)q_out, (float*)k_cache,
-            (float*)v_cache, positions, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
+            (float*)v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
     return launch_status();
+}
+
+CPM_API int cpm_rope_store_dv(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions,
+                              const int* token_seq, const int* slots, const int* page_table, int max_pages,
+                              const float* inv_freq, float magnitude, int n_tokens, int n_heads, int n_kv, int d,
+                              int dv, int rot_dim, int dtype, cudaStream_t stream) {
+    return rope_store(qkv, q_out, k_cache, v_cache, positions, nullptr, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_tokens, n_heads, n_kv, d,
+                      dv, rot_dim, dtype, stream);
+}
+
+// Tokens whose place in the cache is not their position (a tree of drafted tokens).
+CPM_API int cpm_rope_store_at(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions, const int* places,
+                              const int* token_seq, const int* slots, const int* page_table, int max_pages,
+                              const float* inv_freq, float magnitude, int n_tokens, int n_heads, int n_kv, int d,
+                              int rot_dim, int dtype, cudaStream_t stream) {
+    return rope_store(qkv, q_out, k_cache, v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_tokens, n_heads, n_kv, d,
+                      d, rot_dim, dtype, stream);
 }
 
 CPM_API int cpm_rope_store(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions,

@@ -8,17 +8,21 @@ import torch
 
 from ..sampling import SamplingParams
 from .decode import DecodeRunner
+from .drafts import DraftRunner, Lookup
 from .step import SequenceStep, Stepper
 
 
 class EngineBackend:
-    def __init__(self, stepper: Stepper, max_batch: int = 64, use_graph: bool = True, seed: int = 0):
+    def __init__(self, stepper: Stepper, max_batch: int = 64, use_graph: bool = True, seed: int = 0, draft_tokens: int = 0):
+        """``draft_tokens`` > 0: steps check that many looked-up tokens a sequence where they can (see ``DraftRunner``)."""
         self.stepper = stepper
         self.ops = stepper.ops
         self.seed = int(seed)
         stepper.cache.copy_pages = self.ops.copy_pages
         self.runner = DecodeRunner(stepper, use_graph=use_graph, seed=seed)
         self._max_batch = int(max_batch)
+        self.drafter = DraftRunner(self.runner, draft_tokens) if draft_tokens else None
+        self.lookups: Dict[int, Lookup] = {}        # of the current batch's sequences
         self.slots: List[int] = []
         self.open: set = set()              # slots of the current batch that are not finished yet
         self.h2d_bytes = 0
@@ -106,6 +110,7 @@ class EngineBackend:
         for s in sorted(self.open):
             self.stepper.close(s)
         self.open = set()
+        self.lookups.clear()
 
     def decode(self, live, last_tokens, keys, steps_done, sampling, changed) -> List[int]:
         if changed:
@@ -118,6 +123,30 @@ class EngineBackend:
         self.d2h_bytes += 4 * len(live)
         return self.runner.read_tokens()
 
+    def decode_drafted(self, live, texts, keys, steps_done, sampling, room):
+        """A step of drafted tokens for the live sequences; None where there are none: without a drafter, where nothing was found for any sequence, where one may
+        not get as many tokens any more, or where so many sequences leave no room in a step."""
+        if self.drafter is None:
+            return None
+        tokens = self.drafter.tokens(len(live))
+        if tokens < 2 or min(room) < tokens:
+            return None
+        drafted = []
+        for p, (prompt, so_far) in zip(live, texts):
+            slot = self.slots[p]
+            lookup = self.lookups.get(slot)
+            if lookup is None:
+                lookup = self.lookups[slot] = Lookup(prompt)
+            lookup.extend(so_far[len(lookup.tokens) - len(prompt):])
+            drafted.append(lookup.propose(tokens - 1))
+        if not any(ids for ids, _ in drafted):
+            return None
+        out = self.drafter.step([self.slots[p] for p in live], [so_far[-1] for _, so_far in texts], drafted, keys, steps_done, sampling)
+        self.h2d_bytes += 4 * len(live) * (2 * tokens + 8)
+        self.d2h_bytes += 4 * len(live) * (tokens + 1)
+        return out
+
     def finish(self, index: int) -> None:
         self.stepper.close(self.slots[index])
         self.open.discard(self.slots[index])
+        self.lookups.pop(self.slots[index], None)

@@ -43,6 +43,9 @@ class Backend(Protocol):
 
     # Optional: ``prefill_forked(prompts, which, keys, sampling)``, as ``prefill`` for sequences that begin alike (needed for requests
     # with a ``group``).
+    # Optional: ``decode_drafted(live, texts, keys, steps_done, sampling, room)``: as ``decode``, with the tokens that every live sequence has so far (the
+    # prompt's and the generated ones) and how many it may still get; returns a list of one or more tokens for each, or None where this step is to
+    # be an ordinary one.
     # Optional: ``max_sequence_pages()`` (the most pages one sequence may hold) and ``vocab_size()``; with them
     # a request that cannot run is refused before anything is opened.  ``shared_pages(length)``: pages that forks of a prompt of
     # ``length`` tokens hold together with it (default: its full ones).
@@ -189,17 +192,31 @@ def _run_batches(backend, requests, plan, results, stats, on_token, sync) -> Non
                 last[pos] = first[pos]
         changed = True
         t0 = time.perf_counter()
+        drafted = getattr(backend, "decode_drafted", None)
         while live:
-            toks = backend.decode(live, [last[p] for p in live], [keys[runnable[p]] for p in live],
-                                  [len(results[batch[runnable[p]]].tokens) for p in live],
-                                  [sampling[runnable[p]] for p in live], changed)
+            done = [len(results[batch[runnable[p]]].tokens) for p in live]
+            several = None
+            if drafted:
+                several = drafted(live, [(reqs[runnable[p]].prompt, results[batch[runnable[p]]].tokens) for p in live], [keys[runnable[p]] for p in live], done,
+                                  [sampling[runnable[p]] for p in live], [reqs[runnable[p]].max_new_tokens - n for p, n in zip(live, done)])
+            if several is None:
+                toks = backend.decode(live, [last[p] for p in live], [keys[runnable[p]] for p in live], done,
+                                      [sampling[runnable[p]] for p in live], changed)
+                several, changed = [[tok] for tok in toks], False
+            else:
+                changed = True               # (an ordinary step after this one begins with other lengths)
             stats.decode_steps += 1
             still: List[int] = []
-            for p, tok in zip(live, toks):
-                if take(runnable[p], p, tok):
-                    still.append(p)
+            for p, some in zip(live, several):
+                goes_on = True
+                for tok in some:
+                    goes_on = take(runnable[p], p, tok)
                     last[p] = tok
-            changed = len(still) != len(live)
+                    if not goes_on:
+                        break
+                if goes_on:
+                    still.append(p)
+            changed = changed or len(still) != len(live)
             live = still
         sync()
         stats.decode_time += time.perf_counter() - t0

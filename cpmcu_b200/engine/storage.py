@@ -49,12 +49,13 @@ def weight_bytes(model: Model) -> int:
 
 def make_storage(model: Model, chunk_tokens: int, max_batch: int, max_tokens: Optional[int] = None,
                  memory_limit: Optional[float] = None, max_seq_tokens: Optional[int] = None,
-                 n_slots: Optional[int] = None, reserve_bytes: int = 512 << 20) -> Storage:
+                 n_slots: Optional[int] = None, reserve_bytes: int = 512 << 20, drafts: int = 0) -> Storage:
     """One arena for ``model``: attaches the weight region and the workspace to the model's ``ops`` and returns the
     cache made inside it.  ``max_tokens``: the tokens the cache holds; without it the cache takes what
     ``memory_limit`` (a fraction of the device's memory) leaves after weights, workspace and ``reserve_bytes`` (for
     what torch allocates itself: results handed to callers, library workspaces).  Weights that are already loaded
-    stay where they are; otherwise they go into the arena when they are loaded.  Raises PoolExhausted."""
+    stay where they are; otherwise they go into the arena when they are loaded.  ``drafts``: room for steps of that many drafted tokens a
+    sequence too.  Raises PoolExhausted."""
     ops = model.ops
     spec = model.spec
     dtype, device = ops.dtype, ops.device
@@ -72,7 +73,7 @@ def make_storage(model: Model, chunk_tokens: int, max_batch: int, max_tokens: Op
               max_seq_tokens=min(tokens, per_seq_cap), max_step_tokens=chunk_tokens, state_region=st, page_region=pg)
         return round_up(st.peak) + 16 * ALIGN, round_up(pg.peak) + 16 * ALIGN
 
-    persistent, frame, notes = measure_workspace(spec, dtype, chunk_tokens, max_batch, per_seq_cap, ops.sm_count)
+    persistent, frame, notes = measure_workspace(spec, dtype, chunk_tokens, max_batch, per_seq_cap, ops.sm_count, drafts)
     persistent = round_up(int(persistent * 1.05) + (1 << 20))
     frame = round_up(int(frame * 1.05) + (1 << 20))
     w_bytes = 0 if model.loaded else weight_bytes(model)

@@ -37,12 +37,14 @@ class LLM:
                  cuda_graph: bool = False, temperature: float = 0.0, random_seed: Optional[int] = None,
                  top_p: float = 1.0, max_batch: int = 64, max_tokens: Optional[int] = None,
                  max_seq_tokens: Optional[int] = None, device: str = "cuda:0", apply_sparse: bool = True,
-                 use_arena: bool = True, top_k: int = 0, min_p: float = 0.0, cache_bits: Optional[int] = None):
+                 use_arena: bool = True, top_k: int = 0, min_p: float = 0.0, cache_bits: Optional[int] = None,
+                 draft_tokens: int = 0):
         """``apply_sparse`` False runs a model whose configuration has a ``sparse_config`` with dense attention
         (the reference's switch of the same name, cpmcu/llm.py:32, chooses the other way round).  ``use_arena``
         False leaves every tensor to torch's allocator (``max_tokens`` must then be given).  ``cache_bits`` 4 holds keys and
         values in 4 bits (None: what the configuration says, 16 without a word): the cache then takes 0.28 to 0.31 of the bytes, so
-        that more or longer sequences fit."""
+        that more or longer sequences fit.  ``draft_tokens`` > 0: a step checks up to that many tokens a sequence that followed its last ones
+        earlier in its text, and gives as many tokens more as the model would have drawn itself (dense attention over 16-bit or 32-bit keys and values)."""
         self.use_arena = bool(use_arena)
         self.storage = None
         self.path = path
@@ -68,10 +70,15 @@ class LLM:
         self.top_k, self.min_p = int(top_k), float(min_p)
         self.seed = 0 if random_seed is None else int(random_seed)
         self.max_batch = int(max_batch)
+        self.draft_tokens = int(draft_tokens)
         self.max_tokens = max_tokens
         self.max_seq_tokens = max_seq_tokens
         self.model = build_model(self.arch, self.config, self.dtype, device)
         self.ops = self.model.ops
+        if self.draft_tokens and not self.model.takes_drafts():
+            raise ValueError(f"{self.arch.name} in this configuration takes no drafted tokens")
+        if not 0 <= self.draft_tokens < self.ops.MOST_DRAFTS:
+            raise ValueError(f"draft_tokens is 0 to {self.ops.MOST_DRAFTS - 1}, got {draft_tokens}")
         self.tokenizer = None
         self.cache: Optional[Cache] = None
         self.stepper: Optional[Stepper] = None
@@ -99,7 +106,8 @@ class LLM:
         if self.use_arena:
             from .engine.storage import make_storage
             self.storage = make_storage(self.model, self.chunk_length, self.max_batch, self.max_tokens,
-                                        None if self.max_tokens is not None else self.memory_limit, self.max_seq_tokens)
+                                        None if self.max_tokens is not None else self.memory_limit, self.max_seq_tokens,
+                                        drafts=self.draft_tokens)
             self.cache = self.storage.cache
         else:
             needs = self.model.cache_needs()
@@ -133,7 +141,7 @@ class LLM:
         if not self.model.loaded:
             self.load_from_hf()
         if self.backend is None:
-            self.backend = EngineBackend(self.stepper, self.max_batch, self.cuda_graph, self.seed)
+            self.backend = EngineBackend(self.stepper, self.max_batch, self.cuda_graph, self.seed, self.draft_tokens)
         return self.backend
 
     # ---- generation ----

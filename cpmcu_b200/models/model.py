@@ -75,12 +75,19 @@ class Model:
         """Bytes of cache and state a decode step of one sequence with ``kv_len`` keys has to read."""
         return sum(self.blocks[e.layer].mixer.cache_bytes_read(kv_len) for e in self.schedule)
 
-    def recordable_prompt(self) -> bool:
-        """Whether every part can run a prompt chunk without reading the batch on the host (see Part)."""
+    def _all_parts(self):
         parts = [self.embedding, self.final_norm, self.head] + ([self.pass_entry] if self.pass_entry is not None else [])
         for b in self.blocks:
             parts += [p for p in (b, b.mixer, b.feed_forward, b.mixer_norm, b.feed_forward_norm) if p is not None]
-        return all(bool(getattr(p, "recordable_prompt", False)) for p in parts)
+        return parts
+
+    def recordable_prompt(self) -> bool:
+        """Whether every part can run a prompt chunk without reading the batch on the host (see Part)."""
+        return all(bool(getattr(p, "recordable_prompt", False)) for p in self._all_parts())
+
+    def takes_drafts(self) -> bool:
+        """Whether every part takes a step of drafted tokens (see Part)."""
+        return not self.spec.streams and all(bool(getattr(p, "takes_drafts", False)) for p in self._all_parts())
 
     # ---- cache ----
     def cache_needs(self) -> List[CacheNeeds]:

@@ -119,10 +119,17 @@ class DryOps(Ops):
     def _f32(t, what):
         return t
 
+    @staticmethod
+    def _given(t, dtype, what, n=None):
+        return t
+
     def _kv4(self, records, n_kv, d):
         return records
 
     def set_page_limit(self, n_pages):
+        pass
+
+    def keep_drafts(self, pairs, lengths, path, count, slots, page_table):
         pass
 
     def _library_bmm(self, a, w, c):          # (the fp32 form has no kernel for tensors without storage)
@@ -231,10 +238,10 @@ def workspace_steps(max_step_tokens: int, max_batch: int, max_seq_tokens: int, p
 
 
 def measure_workspace(spec, dtype: torch.dtype, max_step_tokens: int, max_batch: int, max_seq_tokens: int,
-                      sm_count: int = 148) -> Tuple[int, int, List[str]]:
+                      sm_count: int = 148, drafts: int = 0) -> Tuple[int, int, List[str]]:
     """(bytes of the persistent part, bytes of one frame, notes) that the steps of a model need at most: prompts of up to
     ``max_step_tokens`` packed tokens and decode steps of up to ``max_batch`` sequences (see ``workspace_steps``), each run once on
-    tensors without storage.  A part that cannot run that way (it reads values on the host) is left out of the
+    tensors without storage.  ``drafts`` > 0: steps of that many drafted tokens a sequence too.  A part that cannot run that way (it reads values on the host) is left out of the
     measurement; what it allocates comes from torch's allocator anyway, and the note says so."""
     from ..cache import Cache
     from ..engine.step import MAX_GRAPH_PIECES
@@ -272,5 +279,18 @@ def measure_workspace(spec, dtype: torch.dtype, max_step_tokens: int, max_batch:
         for n in range(1, len(shares)):
             if shares[n] < shares[n - 1]:
                 run([n], per_seq, False, False, None)
+    if drafts:
+        from ..engine.drafts import draft_step, tokens_of_step
+        size = 1
+        while True:
+            tokens = tokens_of_step(size, drafts, max(int(max_step_tokens), size))
+            if tokens > 1:
+                n = size * tokens
+                ops.workspace.begin_step()
+                draft_step(model, cache, tokens, _meta(n), _meta(n), _meta(size), _meta(size), _meta(size), 0, _meta(size), _meta(size),
+                           *(torch.empty(size, dtype=torch.float32, device="meta") for _ in range(3)), _meta(size), _meta(n), per_seq, False)
+            if size >= max_batch:
+                break
+            size *= 2
     persistent, frame = ops.workspace.peaks()
     return persistent, frame, notes

@@ -710,9 +710,11 @@ class Ops:
     def rope_store(self, qkv: torch.Tensor, n_heads: int, n_kv: int, d: int, positions: torch.Tensor,
                    token_seq: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor,
                    k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
-                   inv_freq: Optional[torch.Tensor], magnitude: float, rot_dim: int) -> torch.Tensor:
+                   inv_freq: Optional[torch.Tensor], magnitude: float, rot_dim: int,
+                   places: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Rotates q and k of qkv [tokens, (heads+2*kv)*d], stores k and v into the cache pages of
-        each token's sequence, and returns the rotated q [tokens, heads, d]."""
+        each token's sequence, and returns the rotated q [tokens, heads, d].  ``places`` int32 [tokens]: where a token lies in its sequence's
+        cache (None: at its position)."""
         self._act(qkv, "qkv")
         n = qkv.shape[0]
         if qkv.shape[1] != (n_heads + 2 * n_kv) * d:
@@ -725,6 +727,15 @@ class Ops:
             self._act(k_cache, "key cache")
             self._act(v_cache, "value cache")
         q = self.empty(n, n_heads, d)
+        if places is not None:
+            self._i32(places, "places")
+            if places.numel() != n:
+                raise ValueError(f"places: need one number a token, got {places.numel()} for {n}")
+            check(self.lib.cpm_rope_store_at(_ptr(qkv), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(positions), _ptr(places),
+                                             _ptr(token_seq), _ptr(slots), _ptr(page_table), page_table.shape[1],
+                                             _ptr(inv_freq), float(magnitude), n, n_heads, n_kv, d, rot_dim, self.code,
+                                             self._stream()), "rope_store_at")
+            return q
         check(self.lib.cpm_rope_store(_ptr(qkv), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(positions),
                                       _ptr(token_seq), _ptr(slots), _ptr(page_table), page_table.shape[1],
                                       _ptr(inv_freq), float(magnitude), n, n_heads, n_kv, d, rot_dim, self.code,

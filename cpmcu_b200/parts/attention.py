@@ -25,6 +25,10 @@ class GroupedQueryAttention(Mixer):
     def recordable_prompt(self) -> bool:
         return bool(self.position.recordable_prompt)
 
+    @property
+    def takes_drafts(self) -> bool:
+        return not (self.window or self.sparse or self.four_bits) and self.position.rotary() is not None and self.d % 4 == 0
+
     def __init__(self, ops, hidden_size: int, n_heads: int, n_kv_heads: int, head_dim: int,
                  position: PartSpec, window: Optional[int] = None, sparse: Optional[Mapping[str, int]] = None,
                  softmax_scale: Optional[float] = None, position_name: str = "", cache_bits: int = 16):
@@ -116,6 +120,12 @@ class GroupedQueryAttention(Mixer):
                                    lane.records if writes_cache else None, inv_freq, magnitude, rot_dim)
             prompt = {} if ctx.is_decode else dict(cu_q=ctx.cu_q, tiles=ctx.q_tiles, longest=ctx.max_kv_len)
             out = ops.kv4_attention(q, lane.records, ctx.kv_len_dev, ctx.slot_dev, lane.page_table, self.n_kv, self.scale, self.window, **prompt)
+            return ops.linear(out, self.w_o)
+        if ctx.drafts:
+            q = ops.rope_store(qkv, self.n_heads, self.n_kv, self.d, ctx.positions, ctx.token_seq, ctx.slot_dev, lane.page_table,
+                               k_cache if writes_cache else None, v_cache if writes_cache else None, inv_freq, magnitude, rot_dim, places=ctx.places)
+            out = ops.draft_attention(q, k_cache, v_cache, ctx.kv_len_dev, ctx.cu_q, ctx.slot_dev, lane.page_table, self.n_kv, self.scale, ctx.drafts,
+                                      ancestors=ctx.ancestors)
             return ops.linear(out, self.w_o)
         if rot_dim >= 0 and ops.fused_decode_ok(ctx, self.d, rot_dim, self.window, self.sparse):
             # one token per sequence: the attention kernel rotates, stores the new key and value, and attends

@@ -233,6 +233,10 @@ class Part:
     # (a part that walks ``ctx.slots`` or ``ctx.kv_lens`` on the host cannot; the default is the safe answer).
     recordable_prompt = False
 
+    # True if ``forward`` takes a step of drafted tokens (``StepContext.drafts``): a token's place in the cache is then not its position, tokens
+    # beside one another may be alternatives, and most of them are forgotten after the step (a part that keeps something per sequence cannot).
+    takes_drafts = False
+
 
 class Norm(Part):
     def forward(self, x: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -493,3 +497,8 @@ class StepContext:
     # a kernel that needs no tiles).
     q_tiles: Optional[Tuple[torch.Tensor, torch.Tensor, int]] = None
     extras: Dict[str, Any] = field(default_factory=dict)
+    # A step of drafted tokens (0: it is not): the most that a sequence brings.  ``places``: where a token lies in its sequence's cache; ``ancestors``: of the
+    # sequence's tokens of this step, the bits of those that it sees (int64; None: all up to itself).
+    drafts: int = 0
+    places: Optional[torch.Tensor] = None
+    ancestors: Optional[torch.Tensor] = None

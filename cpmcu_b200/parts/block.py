@@ -18,6 +18,7 @@ class PreNormResidualBlock(Block):
     """
 
     recordable_prompt = True
+    takes_drafts = True
 
     def __init__(self, ops, mixer, feed_forward, mixer_norm, feed_forward_norm, names,
                  residual_scale: float = 1.0):
@@ -43,6 +44,7 @@ class ParallelResidualBlock(Block):
     that layer's norms in the same pass where they are of a kind that can (layer_norm)."""
 
     recordable_prompt = True
+    takes_drafts = True
 
     def __init__(self, ops, mixer, feed_forward, mixer_norm, feed_forward_norm, names, residual_scale: float = 1.0):
         if feed_forward is None and feed_forward_norm is not None:

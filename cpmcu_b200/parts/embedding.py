@@ -20,6 +20,7 @@ HEADS: Registry[Type[Part]] = Registry("output head")
 @EMBEDDINGS.register("scaled_embedding")
 class ScaledEmbedding(Part):
     recordable_prompt = True
+    takes_drafts = True
 
     def __init__(self, ops, vocab_size: int, hidden_size: int, scale: float = 1.0, weight_name: str = "weight"):
         super().__init__(ops)
@@ -152,6 +153,7 @@ class NormedEmbedding(Part):
 @HEADS.register("scaled_lm_head")
 class ScaledHead(Part):
     recordable_prompt = True
+    takes_drafts = True
 
     def __init__(self, ops, vocab_size: int, hidden_size: int, scale: float = 1.0, tied: bool = False,
                  weight_name: str = "weight", softcap: float = 0.0):

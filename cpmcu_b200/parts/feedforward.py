@@ -23,6 +23,7 @@ def glu_clamp(limit: Optional[float], slope: float, offset: float):
 @FEED_FORWARDS.register("gated_ffn")
 class GatedFeedForward(FeedForward):
     recordable_prompt = True
+    takes_drafts = True
 
     def __init__(self, ops, hidden_size: int, intermediate_size: int, activation: str = "silu", names=None,
                  limit: Optional[float] = None, slope: float = 1.702, offset: float = 1.0):
@@ -80,6 +81,7 @@ class PlainFeedForward(FeedForward):
     and "down".  The activation (32-bit, on the product's accumulator) is applied in the product's epilogue."""
 
     recordable_prompt = True
+    takes_drafts = True
 
     def __init__(self, ops, hidden_size: int, intermediate_size: int, activation: str = "relu2", names=None):
         super().__init__(ops)

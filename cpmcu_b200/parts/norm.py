@@ -15,6 +15,7 @@ from .base import NORMS, Norm, WeightSpec
 @NORMS.register("rms_norm")
 class RMSNorm(Norm):
     recordable_prompt = True
+    takes_drafts = True
     takes_two_addends = True        # ``add_forward(..., second=)`` adds two deferred outputs in the norm's own pass
 
     def __init__(self, ops, hidden_size: int, eps: float, weight_name: str = "weight", offset: float = 0.0,
@@ -67,6 +68,7 @@ class LayerNorm(Norm):
     stream is formed in the same pass)."""
 
     recordable_prompt = True
+    takes_drafts = True
     takes_two_addends = True        # ``add_forward(..., second=)`` adds two deferred outputs in the norm's own pass
 
     def __init__(self, ops, hidden_size: int, eps: float, weight_name: str = "weight", bias_name: Optional[str] = "bias"):
@@ -124,6 +126,7 @@ class ScalarRMSNorm(Norm):
     width; ``gain`` (one 32-bit float on the device) is what a kernel that norms as part of a larger pass takes."""
 
     recordable_prompt = True
+    takes_drafts = True
 
     def __init__(self, ops, hidden_size: int, eps: float, weight_name: str = "weight"):
         super().__init__(ops)

@@ -548,3 +548,30 @@ def test_refusals_of_keep_drafts():
         with pytest.raises(ValueError):
             ops.keep_drafts(**{**args, **bad})
     ops.keep_drafts([], _i32([0]), _i32([[0, 1]]), _i32([2]), _i32([0]), _i32([[0]]))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d,rot_dim", [(64, 64), (48, 16), (20, 20)])
+def test_rope_store_at_places(dtype, d, rot_dim):
+    """A token that lies elsewhere than at its position is turned by the position and stored at the place, to the same bits."""
+    ops = _ops(dtype)
+    g = torch.Generator().manual_seed(d)
+    qkv = torch.randn(6, 8 * d, generator=g).to(DT[dtype]).cuda()
+    positions, places, seq = _i32([70, 71, 71, 72, 5, 6]), _i32([70, 71, 72, 73, 63, 64]), _i32([0, 0, 0, 0, 1, 1])
+    table, slots = _i32([[2, 5], [4, 1]]), _i32([1, 0])
+    inv_freq = (1.0 / 10000.0 ** (torch.arange(0, rot_dim, 2).float() / rot_dim)).cuda()
+    make = lambda: (torch.zeros(6, 2, PAGE, d, dtype=DT[dtype]).cuda(), torch.zeros(6, 2, d, PAGE, dtype=DT[dtype]).cuda())  # noqa: E731
+    (k, v), (k1, v1) = make(), make()
+    q = ops.rope_store(qkv, 4, 2, d, positions, seq, slots, table, k, v, inv_freq, 1.1, rot_dim, places=places)
+    for t in range(6):                                       # one at a time, so that no place is taken twice
+        one = make()
+        at = slice(t, t + 1)
+        want = ops.rope_store(qkv[at].contiguous(), 4, 2, d, positions[at].contiguous(), seq[at].contiguous(), slots, table, *one, inv_freq, 1.1, rot_dim)
+        assert torch.equal(q[at], want)
+        row = table[int(slots[int(seq[t])])]
+        x, y = int(positions[t]), int(places[t])
+        k1[row[y // PAGE], :, y % PAGE] = one[0][row[x // PAGE], :, x % PAGE]
+        v1[row[y // PAGE], :, :, y % PAGE] = one[1][row[x // PAGE], :, :, x % PAGE]
+    assert torch.equal(k, k1) and torch.equal(v, v1)
+    with pytest.raises(ValueError):
+        ops.rope_store(qkv, 4, 2, d, positions, seq, slots, table, k, v, inv_freq, 1.1, rot_dim, places=places[:3].contiguous())
