@@ -2,7 +2,7 @@
 decode steps through the decode runner, sampling by the library's kernel."""
 from __future__ import annotations
 
-from typing import Dict, List, Sequence
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -13,6 +13,9 @@ from .step import SequenceStep, Stepper
 
 
 class EngineBackend:
+    drafter: Optional[DraftRunner] = None
+    lookups: Dict[int, Lookup] = {}             # by slot, of the current batch's sequences (a backend with a drafter has its own)
+
     def __init__(self, stepper: Stepper, max_batch: int = 64, use_graph: bool = True, seed: int = 0, draft_tokens: int = 0):
         """``draft_tokens`` > 0: steps check that many looked-up tokens a sequence where they can (see ``DraftRunner``)."""
         self.stepper = stepper
@@ -22,7 +25,7 @@ class EngineBackend:
         self.runner = DecodeRunner(stepper, use_graph=use_graph, seed=seed)
         self._max_batch = int(max_batch)
         self.drafter = DraftRunner(self.runner, draft_tokens) if draft_tokens else None
-        self.lookups: Dict[int, Lookup] = {}        # of the current batch's sequences
+        self.lookups = {}
         self.slots: List[int] = []
         self.open: set = set()              # slots of the current batch that are not finished yet
         self.h2d_bytes = 0
