@@ -205,16 +205,25 @@ draft_join_kernel(const __grid_constant__ DraftArgs a, int shares) {
     const int i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
     if (i >= n * a.n_heads) return;
     const int64_t row = (int64_t)begin * a.n_heads + i, rows = (int64_t)a.n_tokens * a.n_heads;
-    const auto place = [&](int z) { return a.parts + ((int64_t)z * rows + row) * (d + 2); };
-    float top = -INFINITY;
-    for (int z = 0; z < shares; ++z) top = fmaxf(top, place(z)[d]);
-    const float use = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
-    for (int z = 0; z < shares; ++z) l += place(z)[d + 1] * expf(place(z)[d] - use);
-    for (int c = lane; c < d; c += 32) {
+    const float* part = a.parts + row * (d + 2);
+    const int64_t apart = rows * (d + 2);
+    // a lane has the maximum and the sum of two shares, and their weight in the result
+    float m[2], w[2], l = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) m[h] = lane + 32 * h < shares ? part[(lane + 32 * h) * apart + d] : -INFINITY;
+    const float top = warp_max(fmaxf(m[0], m[1])), use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w[h] = expf(m[h] - use);
+        if (lane + 32 * h < shares) l += part[(lane + 32 * h) * apart + d + 1] * w[h];
+    }
+    l = warp_sum(l);
+    for (int c0 = 0; c0 < d; c0 += 32) {
+        const int c = min(c0 + lane, d - 1);
         float o = 0.f;
-        for (int z = 0; z < shares; ++z) o = fmaf(place(z)[c], expf(place(z)[d] - use), o);
-        static_cast<T*>(a.out)[row * d + c] = from_f32<T>(l == 0.f ? o : o / l);
+#pragma unroll 8
+        for (int z = 0; z < shares; ++z) o = fmaf(part[z * apart + c], __shfl_sync(0xffffffffu, z < 32 ? w[0] : w[1], z & 31), o);
+        if (c0 + lane < d) static_cast<T*>(a.out)[row * d + c] = from_f32<T>(l == 0.f ? o : o / l);
     }
 }
 
@@ -249,7 +258,7 @@ CPM_API int cpm_draft_attention_generic(const void* q, const void* k, const void
                                         int n_seqs, int most, int n_heads, int n_kv, int d, float scale, int dtype, cudaStream_t stream) {
     if (n_tokens <= 0 || n_seqs <= 0) return CPM_OK;
     if (d < 4 || d > 256 || d % 4 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || most < 1 || most > 64 || max_pages < 1 || max_pages > 0x7fffffff / kPageTokens || n_pages < 1) return CPM_BAD_ARGUMENT;
-    if (shares < 1 || shares > 65535 || (shares > 1) != (parts != nullptr)) return CPM_BAD_ARGUMENT;
+    if (shares < 1 || shares > 64 || (shares > 1) != (parts != nullptr)) return CPM_BAD_ARGUMENT;
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) return CPM_BAD_ARGUMENT;
     const DraftArgs a{q, k, v, out, kv_len, cu, slots, page_table, ancestors, parts, max_pages, n_pages, n_tokens, n_heads, n_kv, n_heads / n_kv, d, most, scale};
     return dtype == CPM_BF16 ? by_size<bf16>(a, n_seqs, shares, stream) : by_size<float>(a, n_seqs, shares, stream);
