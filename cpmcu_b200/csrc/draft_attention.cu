@@ -8,8 +8,8 @@
 // are no finite numbers are taken out of the tile and added to the rows that see them at the end.
 //
 // All query heads of a key-value head and all tokens are rows of one matrix (row = token * group + head), so that a sequence's keys are read once for
-// 32 rows and not once a token.  A block takes 32 rows and a share of the pages: scores of 64 keys (a thread: 8 rows of one key), the softmax (a warp: four
-// rows), weighted values (a thread: some rows of one channel), all operands in shared memory.  Few rows and many keys: the pages are shared out over blocks, whose
+// 64 rows and not once a token.  A block takes 32 or 64 rows and a share of the pages: scores of 64 keys (a thread: 8 rows of one or two keys), the softmax (a warp: an
+// eighth of the rows), weighted values (a thread: some rows of one channel), all operands in shared memory.  Few rows and many keys: the pages are shared out over blocks, whose
 // parts a second kernel adds up.
 #include "common.cuh"
 
@@ -17,7 +17,7 @@ CPM_BOUNDS_TU(draft_attention)
 
 namespace {
 
-constexpr int kThreads = 256, kRows = 32;
+constexpr int kThreads = 256;
 constexpr int kLine = kPageTokens + 4;                  // floats of a row of scores, and of a channel's values
 
 struct DraftArgs {
@@ -32,13 +32,15 @@ struct DraftArgs {
 
 // floats of a key's line: an odd number of 16 bytes, so that neighbouring keys' lie in different banks
 __host__ __device__ constexpr int key_line(int d) { return (d / 4) % 2 ? d : d + 4; }
-__host__ __device__ constexpr int draft_smem_floats(int d) {
-    return kRows * d + kPageTokens * key_line(d) + d * kLine + kRows * kLine + 3 * kRows;
+__host__ __device__ constexpr int draft_smem_floats(int rows, int d) {
+    return rows * d + kPageTokens * key_line(d) + d * kLine + rows * kLine + 3 * rows;
 }
 
-template <typename T, int RPT>                          // rows that a thread adds up of one channel: 32 / RPT groups of threads have 8 RPT channels
+// J: rows of a block by 32, and keys of a thread.  RPT: rows that a thread adds up of one channel: 32 J / RPT groups of threads have 8 RPT / J channels.
+template <typename T, int RPT, int J>
 __global__ void __launch_bounds__(kThreads)
 draft_attention_kernel(const __grid_constant__ DraftArgs a) {
+    constexpr int kRows = 32 * J;
     extern __shared__ __align__(16) float draft_smem[];
     __shared__ int odd;                                 // whether a value among the step's tokens is no finite number
     const int d = a.d, line = key_line(d), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -71,7 +73,7 @@ draft_attention_kernel(const __grid_constant__ DraftArgs a) {
         sum[tid] = 0.f;
     }
     if (tid == 0) odd = 0;
-    const int channel = tid % (8 * RPT), o0 = tid / (8 * RPT) * RPT;     // of the weighted values: a channel, and rows from o0 on
+    const int channel = tid % (8 * RPT / J), o0 = tid / (8 * RPT / J) * RPT;     // of the weighted values: a channel, and rows from o0 on
     float o[RPT];
 #pragma unroll
     for (int i = 0; i < RPT; ++i) o[i] = 0.f;
@@ -106,32 +108,45 @@ draft_attention_kernel(const __grid_constant__ DraftArgs a) {
             *reinterpret_cast<float4*>(vs + c * kLine + j) = x;
         }
         __syncthreads();
-        // ---- scores: eight rows of one key ----
+        // ---- scores: eight rows of one or two keys ----
         {
-            const int j = tid % kPageTokens, first = tid / kPageTokens * 8;
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            const int j = tid % (kPageTokens / J), first = tid / (kPageTokens / J) * 8;
+            float x[J][8];
+#pragma unroll
+            for (int u = 0; u < J; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
 #pragma unroll 2
             for (int c = 0; c < d; c += 4) {
-                const float4 kk = *reinterpret_cast<const float4*>(ks + j * line + c);
+                float4 kk[J];
+#pragma unroll
+                for (int u = 0; u < J; ++u) kk[u] = *reinterpret_cast<const float4*>(ks + (j + 32 * u) * line + c);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float4 qq = *reinterpret_cast<const float4*>(qs + (first + i) * d + c);
-                    x[i] = fmaf(qq.x, kk.x, x[i]);
-                    x[i] = fmaf(qq.y, kk.y, x[i]);
-                    x[i] = fmaf(qq.z, kk.z, x[i]);
-                    x[i] = fmaf(qq.w, kk.w, x[i]);
+#pragma unroll
+                    for (int u = 0; u < J; ++u) {
+                        x[u][i] = fmaf(qq.x, kk[u].x, x[u][i]);
+                        x[u][i] = fmaf(qq.y, kk[u].y, x[u][i]);
+                        x[u][i] = fmaf(qq.z, kk[u].z, x[u][i]);
+                        x[u][i] = fmaf(qq.w, kk[u].w, x[u][i]);
+                    }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool seen = first + i < rows && key0 + j < kv_len && (key0 + j < history || sees(first + i, key0 + j));
-                ps[(first + i) * kLine + j] = seen ? x[i] * a.scale : -INFINITY;
-            }
+            for (int u = 0; u < J; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = key0 + j + 32 * u;
+                    const bool seen = first + i < rows && key < kv_len && (key < history || sees(first + i, key));
+                    ps[(first + i) * kLine + j + 32 * u] = seen ? x[u][i] * a.scale : -INFINITY;
+                }
         }
         __syncthreads();
-        // ---- softmax: four rows a warp, two keys a lane ----
+        // ---- softmax: a warp an eighth of the rows, a lane two keys ----
 #pragma unroll
         for (int i = 0; i < kRows / 8; ++i) {
+            if (warp * (kRows / 8) + i >= rows) break;
             const int r = warp * (kRows / 8) + i;
             const float x0 = ps[r * kLine + lane], x1 = ps[r * kLine + 32 + lane];
             const float was = top[r], now = fmaxf(was, warp_max(fmaxf(x0, x1))), use = now == -INFINITY ? 0.f : now;
@@ -194,60 +209,80 @@ draft_attention_kernel(const __grid_constant__ DraftArgs a) {
     }
 }
 
-// Adds up the shares of a row: a warp a row.  Rows of no sequence are left as they are.
+// Adds up the shares of a row: a block a row, a warp every eighth share.  Rows of no sequence are left as they are.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 draft_join_kernel(const __grid_constant__ DraftArgs a, int shares) {
+    constexpr int kWarps = kThreads / 32, kDims = 8;      // d <= 256
+    __shared__ float values[kWarps][32 * kDims];
     pdl_launch_dependents();
     pdl_wait();
-    const int s = blockIdx.y, lane = threadIdx.x & 31, d = a.d;
+    const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.d;
     const int begin = max(0, min(a.cu[s], a.n_tokens)), n = max(0, min(min(a.cu[s + 1], a.n_tokens) - begin, a.most));
-    const int i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    if (i >= n * a.n_heads) return;
-    const int64_t row = (int64_t)begin * a.n_heads + i, rows = (int64_t)a.n_tokens * a.n_heads;
+    if ((int)blockIdx.x >= n * a.n_heads) return;
+    const int64_t row = (int64_t)begin * a.n_heads + blockIdx.x, apart = (int64_t)a.n_tokens * a.n_heads * (d + 2);
     const float* part = a.parts + row * (d + 2);
-    const int64_t apart = rows * (d + 2);
     // a lane has the maximum and the sum of two shares, and their weight in the result
     float m[2], w[2], l = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) m[h] = lane + 32 * h < shares ? part[(lane + 32 * h) * apart + d] : -INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w[h] = lane + 32 * h < shares ? part[(lane + 32 * h) * apart + d + 1] : 0.f;
     const float top = warp_max(fmaxf(m[0], m[1])), use = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        w[h] = expf(m[h] - use);
-        if (lane + 32 * h < shares) l += part[(lane + 32 * h) * apart + d + 1] * w[h];
+        const float by = expf(m[h] - use);
+        l += w[h] * by;
+        w[h] = by;
     }
     l = warp_sum(l);
-    for (int c0 = 0; c0 < d; c0 += 32) {
-        const int c = min(c0 + lane, d - 1);
-        float o = 0.f;
-#pragma unroll 8
-        for (int z = 0; z < shares; ++z) o = fmaf(part[z * apart + c], __shfl_sync(0xffffffffu, z < 32 ? w[0] : w[1], z & 31), o);
-        if (c0 + lane < d) static_cast<T*>(a.out)[row * d + c] = from_f32<T>(l == 0.f ? o : o / l);
+    float o[kDims];
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int z = warp; z < shares; z += kWarps) {
+        const float by = __shfl_sync(0xffffffffu, z < 32 ? w[0] : w[1], z & 31);
+#pragma unroll
+        for (int i = 0; i < kDims; ++i)
+            if (lane + 32 * i < d) o[i] = fmaf(part[z * apart + lane + 32 * i], by, o[i]);
     }
+#pragma unroll
+    for (int i = 0; i < kDims; ++i)
+        if (lane + 32 * i < d) values[warp][lane + 32 * i] = o[i];
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c >= d) return;
+    float y = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) y += values[x][c];
+    static_cast<T*>(a.out)[row * d + c] = from_f32<T>(l == 0.f ? y : y / l);
 }
 
-template <typename T, int RPT>
+template <typename T, int RPT, int J>
 int launch(const DraftArgs& a, int n_seqs, int shares, cudaStream_t stream) {
     static bool done[kMaxDevices];
-    const int most_bytes = draft_smem_floats(8 * RPT) * 4, status = ensure_dynamic_smem(draft_attention_kernel<T, RPT>, most_bytes, done);
+    const int most_bytes = draft_smem_floats(32 * J, 8 * RPT / J) * 4, status = ensure_dynamic_smem(draft_attention_kernel<T, RPT, J>, most_bytes, done);
     if (status != CPM_OK) return status;
-    const int64_t tiles = (int64_t)((a.most * a.group + kRows - 1) / kRows) * a.n_kv;
+    const int64_t tiles = (int64_t)((a.most * a.group + 32 * J - 1) / (32 * J)) * a.n_kv;
     if (tiles > 0x7fffffff || n_seqs > 65535) return CPM_BAD_ARGUMENT;
-    cpm_launch(kLaunchAttention, draft_attention_kernel<T, RPT>, dim3((unsigned)tiles, n_seqs, shares), kThreads, (size_t)draft_smem_floats(a.d) * 4, stream, a);
+    cpm_launch(kLaunchAttention, draft_attention_kernel<T, RPT, J>, dim3((unsigned)tiles, n_seqs, shares), kThreads, (size_t)draft_smem_floats(32 * J, a.d) * 4, stream, a);
     if (shares > 1) {
-        const int64_t blocks = ((int64_t)a.most * a.n_heads + kThreads / 32 - 1) / (kThreads / 32);
-        cpm_launch(kLaunchAttention, draft_join_kernel<T>, dim3((unsigned)blocks, n_seqs), kThreads, 0, stream, a, shares);
+        if ((int64_t)a.most * a.n_heads > 0x7fffffff) return CPM_BAD_ARGUMENT;
+        cpm_launch(kLaunchAttention, draft_join_kernel<T>, dim3((unsigned)(a.most * a.n_heads), n_seqs), kThreads, 0, stream, a, shares);
     }
     return launch_status();
 }
 
+// Rows of a block: 64 where there are more than 32 and a thread's sums of 64 rows have room in its registers.
+__host__ constexpr bool wide_rows(int most, int group, int d) { return most * group > 32 && d <= 128; }
+
 template <typename T>
 int by_size(const DraftArgs& a, int n_seqs, int shares, cudaStream_t stream) {
-    if (a.d <= 32) return launch<T, 4>(a, n_seqs, shares, stream);
-    if (a.d <= 64) return launch<T, 8>(a, n_seqs, shares, stream);
-    if (a.d <= 128) return launch<T, 16>(a, n_seqs, shares, stream);
-    return launch<T, 32>(a, n_seqs, shares, stream);
+    const bool wide = wide_rows(a.most, a.group, a.d);
+    if (a.d <= 32) return wide ? launch<T, 8, 2>(a, n_seqs, shares, stream) : launch<T, 4, 1>(a, n_seqs, shares, stream);
+    if (a.d <= 64) return wide ? launch<T, 16, 2>(a, n_seqs, shares, stream) : launch<T, 8, 1>(a, n_seqs, shares, stream);
+    if (a.d <= 128) return wide ? launch<T, 32, 2>(a, n_seqs, shares, stream) : launch<T, 16, 1>(a, n_seqs, shares, stream);
+    return launch<T, 32, 1>(a, n_seqs, shares, stream);
 }
 
 }  // namespace

@@ -1966,9 +1966,10 @@ class Ops:
         return self.code == BF16 and self.use_tcgen05_draft and d in FAST_HEAD_DIMS and n_heads // n_kv <= 128
 
     def draft_attention_shares(self, n_seqs: int, most: int, n_heads: int, n_kv: int, longest: int) -> int:
-        """Blocks that share a sequence's pages in the 32-bit kernel: two an SM, with two pages or more each."""
-        blocks = max(1, n_seqs * n_kv * ((most * (n_heads // n_kv) + 31) // 32))
-        return max(1, min(2 * self.sm_count // blocks, (longest + 2 * PAGE_TOKENS - 1) // (2 * PAGE_TOKENS), 64))
+        """Blocks that share a sequence's pages in the 32-bit kernel, which takes 32 or 64 rows a block: two an SM, with a page or more each."""
+        rows = most * (n_heads // n_kv)
+        blocks = max(1, n_seqs * n_kv * ((rows + 63) // 64))
+        return max(1, min(2 * self.sm_count // blocks, (longest + PAGE_TOKENS - 1) // PAGE_TOKENS, 64))
 
     def draft_attention(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor, slots: torch.Tensor,
                         page_table: torch.Tensor, n_kv: int, scale: float, most: int, ancestors: Optional[torch.Tensor] = None) -> torch.Tensor:
