@@ -1957,7 +1957,7 @@ class Ops:
         check(self.lib.cpm_step_tables(_ptr(lengths), _ptr(new), _ptr(slots), n_seqs, n_tokens, _ptr(page_table), page_table.shape[0], page_table.shape[1],
                                        _ptr(parents), _ptr(free), 0 if free is None else free.numel(), _ptr(t.cu_q), _ptr(t.kv_len), _ptr(t.token_seq),
                                        _ptr(t.positions), _ptr(t.places), _ptr(t.slot_map), _ptr(t.ancestors), _ptr(t.taken), self._stream()),
-              f"step_tables ({n_seqs} sequences)")
+              "step_tables")
         return t
 
     draft_attention_ran = False          # (without drafted tokens no step waits for its kernel's error)
@@ -1977,26 +1977,30 @@ class Ops:
         ``most`` (up to MOST_DRAFTS), which are the last of its kv_len[s] keys in k_cache [pages, kv, PAGE_TOKENS, d] and v_cache [pages, kv, d, PAGE_TOKENS].  A
         token sees all keys before these, and of these the ones up to itself, or with ``ancestors`` (int64 [tokens]) those whose bit is set.  A row that sees none
         gives zeros; rows of no sequence are left as they are.  What an unseen key or value holds, even if it is no number, changes nothing."""
-        self._given(q, self.dtype, "q")
+        given, dtype, i32 = self._given, self.dtype, torch.int32
+        given(q, dtype, "q")
         if q.dim() != 3:
             raise ValueError("q: needs [tokens, heads, d]")
         n, n_heads, d = q.shape
         if n_kv < 1 or n_heads < 1 or n_heads % n_kv:
             raise ValueError(f"{n_heads} heads cannot be grouped over {n_kv} key-value heads")
         most = self._most(most)
-        for t, what, shape in ((k_cache, "key cache", (n_kv, PAGE_TOKENS, d)), (v_cache, "value cache", (n_kv, d, PAGE_TOKENS))):
-            self._given(t, self.dtype, what)
-            if t.dim() != 4 or tuple(t.shape[1:]) != shape or t.shape[0] != k_cache.shape[0] or t.shape[0] == 0:
-                raise ValueError(f"{what}: needs [pages, {', '.join(str(x) for x in shape)}], got {tuple(t.shape)}")
-        n_seqs, i32 = kv_len.numel(), torch.int32
-        self._given(kv_len, i32, "key counts")
-        self._given(slots, i32, "slots", n_seqs)
-        self._given(cu_q, i32, "token offsets", n_seqs + 1)
-        self._given(page_table, i32, "page table")
+        given(k_cache, dtype, "key cache")
+        given(v_cache, dtype, "value cache")
+        n_pages = k_cache.shape[0] if k_cache.dim() else 0
+        if n_pages == 0 or k_cache.shape != (n_pages, n_kv, PAGE_TOKENS, d) or v_cache.shape != (n_pages, n_kv, d, PAGE_TOKENS):
+            raise ValueError(f"caches: need keys [pages, {n_kv}, {PAGE_TOKENS}, {d}] and values [pages, {n_kv}, {d}, {PAGE_TOKENS}], got {tuple(k_cache.shape)} and "
+                             f"{tuple(v_cache.shape)}")
+        n_seqs = kv_len.numel()
+        given(kv_len, i32, "key counts")
+        given(slots, i32, "slots", n_seqs)
+        given(cu_q, i32, "token offsets", n_seqs + 1)
+        given(page_table, i32, "page table")
         if page_table.dim() != 2 or page_table.numel() == 0:
             raise ValueError("page table: needs [slots, pages]")
+        width = page_table.shape[1]
         if ancestors is not None:
-            self._given(ancestors, torch.int64, "ancestors", n)
+            given(ancestors, torch.int64, "ancestors", n)
         out = self.empty(n, n_heads * d)
         if n == 0 or n_seqs == 0:
             return out
@@ -2004,14 +2008,14 @@ class Ops:
             scratch = self.empty(self.lib.cpm_draft_attention_scratch_floats(n_heads, n_kv, d, most), dtype=torch.float32)
             self.draft_attention_ran = True
             check(self.lib.cpm_draft_attention_tcgen05(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
-                                                       page_table.shape[1], k_cache.shape[0], _ptr(ancestors), _ptr(scratch), n, n_seqs, most, n_heads, n_kv, d,
-                                                       float(scale), self._stream()), f"tcgen05 attention of drafted tokens (head_dim {d})")
+                                                       width, n_pages, _ptr(ancestors), _ptr(scratch), n, n_seqs, most, n_heads, n_kv, d,
+                                                       float(scale), self._stream()), "tcgen05 attention of drafted tokens")
             LAUNCHES_EXTRA[0] += 1       # the pieces, then their addition
             return out
-        shares = self.draft_attention_shares(n_seqs, most, n_heads, n_kv, page_table.shape[1] * PAGE_TOKENS)
+        shares = self.draft_attention_shares(n_seqs, most, n_heads, n_kv, width * PAGE_TOKENS)
         parts = self.empty(shares * n * n_heads * (d + 2), dtype=torch.float32) if shares > 1 else None
         check(self.lib.cpm_draft_attention_generic(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
-                                                   page_table.shape[1], k_cache.shape[0], _ptr(ancestors), _ptr(parts), shares, n, n_seqs, most, n_heads, n_kv, d,
+                                                   width, n_pages, _ptr(ancestors), _ptr(parts), shares, n, n_seqs, most, n_heads, n_kv, d,
                                                    float(scale), self.code, self._stream()), f"attention of drafted tokens (head_dim {d})")
         if shares > 1:
             LAUNCHES_EXTRA[0] += 1
@@ -2037,14 +2041,31 @@ class Ops:
             raise ValueError("logits: needs [tokens, vocab]")
         n, vocab = logits.shape
         most, n_seqs, i32, f32 = self._most(most), temperature.numel(), torch.int32, torch.float32
-        for t, dtype, count, what in ((ids, i32, n, "tokens"), (cu_q, i32, n_seqs + 1, "token offsets"), (token_seq, i32, n, "token sequences"),
-                                      (uniform, f32, n, "random numbers"), (temperature, f32, n_seqs, "temperatures"), (top_k, i32, n_seqs, "top-k"),
-                                      (top_p, f32, n_seqs, "top-p"), (min_p, f32, n_seqs, "min-p"), (parents, i32, n, "parents"), (accept, f32, n, "numbers of acceptance"),
-                                      (seq_key, i32, n_seqs, "sequence keys"), (step_key, i32, n_seqs, "step keys"), (positions, i32, n, "positions")):
-            if t is not None:
-                self._given(t, dtype, what, count)
+        given = self._given                  # (not in a loop over a list of them: the list takes the host longer than the checks)
+        given(ids, i32, "tokens", n)
+        given(cu_q, i32, "token offsets", n_seqs + 1)
+        given(token_seq, i32, "token sequences", n)
+        given(temperature, f32, "temperatures", n_seqs)
+        if uniform is not None:
+            given(uniform, f32, "random numbers", n)
+        if top_k is not None:
+            given(top_k, i32, "top-k", n_seqs)
+        if top_p is not None:
+            given(top_p, f32, "top-p", n_seqs)
+        if min_p is not None:
+            given(min_p, f32, "min-p", n_seqs)
+        if parents is not None:
+            given(parents, i32, "parents", n)
+        if accept is not None:
+            given(accept, f32, "numbers of acceptance", n)
+        if seq_key is not None:
+            given(seq_key, i32, "sequence keys", n_seqs)
+        if step_key is not None:
+            given(step_key, i32, "step keys", n_seqs)
+        if positions is not None:
+            given(positions, i32, "positions", n)
         if draft_probs is not None:
-            if draft_probs.dtype != f32 or draft_probs.get_device() != self.device_index or tuple(draft_probs.shape) != (n, vocab) or (vocab > 1 and draft_probs.stride(1) != 1):
+            if draft_probs.dtype != f32 or draft_probs.get_device() != self.device_index or draft_probs.shape != (n, vocab) or (vocab > 1 and draft_probs.stride(1) != 1):
                 raise ValueError(f"drafting probabilities: need fp32 [{n}, {vocab}] with neighbouring tokens side by side")
             if parents is not None:
                 raise ValueError("drafting probabilities go with tokens in a row, not with a tree")
@@ -2062,7 +2083,7 @@ class Ops:
         drawn = rows.data_ptr() + (32 * n if draft_probs is not None else 0)
         check(self.lib.cpm_sample_drafts(_ptr(logits), vocab, n, vocab, drawn, drawn + 4 * n, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
                                          _ptr(min_p), ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), _ptr(token_seq), _ptr(positions),
-                                         _ptr(cu_q), n_seqs, kept, self._stream()), f"drawing for drafted tokens ({vocab} tokens)")
+                                         _ptr(cu_q), n_seqs, kept, self._stream()), "drawing for drafted tokens")
         check(self.lib.cpm_verify_drafts(_ptr(logits), vocab, n, vocab, _ptr(ids), _ptr(cu_q), n_seqs, most, _ptr(parents), _ptr(draft_probs),
                                          0 if draft_probs is None else draft_probs.stride(0), _ptr(accept), _ptr(uniform), _ptr(temperature), drawn,
                                          drawn + 4 * n, kept, _ptr(tokens), _ptr(count), _ptr(path), _ptr(logprob), self._stream()), "verify_drafts")
