@@ -441,16 +441,20 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     const auto weigh_all = [&](auto quick) {
         const auto form = [&](float x) { return decltype(quick)::value ? row.form_quick(x) : row.form(x); };
         if (by_count || by_mass) {
-            uint32_t small = 0;
+            uint32_t small = 0, least = 0;
 #pragma unroll 4
             for (int i = i0; i < i1; ++i) {
                 const float w = form(STAGED ? weights[i] : row.z[i]);
                 if constexpr (STAGED) weights[i] = w;
-                count_own<STAGED>(sm, __float_as_uint(w), summed);
+                // (at a low temperature most tokens lie in the first bin, and additions to one place come one after the other: a thread counts its own)
+                if (bin_of(__float_as_uint(w)) == 0) ++least;
+                else count_own<STAGED>(sm, __float_as_uint(w), summed);
                 if (summed) small += small_units_of(__float_as_uint(w));
                 else if (!STAGED && !by_count) own_mass += units_of(__float_as_uint(w));
             }
             own_mass += small;
+            least = __reduce_add_sync(0xffffffffu, least);
+            if (lane == 0 && least) atomicAdd(&sm.own[1][0], STAGED ? least << kCountBits : least);
         } else if constexpr (STAGED) {
 #pragma unroll 4
             for (int i = i0; i < i1; ++i) weights[i] = form(weights[i]);

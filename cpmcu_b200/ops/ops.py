@@ -1950,15 +1950,16 @@ class Ops:
         # one tensor, cut into the tables (an allocation takes the host as long as three cuts): the words of 64 bits come first
         wide = n_tokens * (2 if parents is None else 4)
         room = self.empty(wide + 3 * n_tokens + 2 * n_seqs + 2, dtype=i32)
-        words, *by_token, kv_len, cu_q, taken = room.split_with_sizes((wide, n_tokens, n_tokens, n_tokens, n_seqs, n_seqs + 1, 1))
+        words, token_seq, positions, places, kv_len, cu_q, taken = room.split_with_sizes((wide, n_tokens, n_tokens, n_tokens, n_seqs, n_seqs + 1, 1))
         words = words.view(torch.int64)
         slot_map, ancestors = (words, None) if parents is None else words.split_with_sizes((n_tokens, n_tokens))
-        t = StepTables(cu_q, kv_len, *by_token, slot_map, ancestors, None if free is None else taken)
-        check(self.lib.cpm_step_tables(_ptr(lengths), _ptr(new), _ptr(slots), n_seqs, n_tokens, _ptr(page_table), page_table.shape[0], page_table.shape[1],
-                                       _ptr(parents), _ptr(free), 0 if free is None else free.numel(), _ptr(t.cu_q), _ptr(t.kv_len), _ptr(t.token_seq),
-                                       _ptr(t.positions), _ptr(t.places), _ptr(t.slot_map), _ptr(t.ancestors), _ptr(t.taken), self._stream()),
-              "step_tables")
-        return t
+        at = room.data_ptr()
+        by_token, by_seq = at + 4 * wide, at + 4 * (wide + 3 * n_tokens)
+        check(self.lib.cpm_step_tables(lengths.data_ptr(), new.data_ptr(), slots.data_ptr(), n_seqs, n_tokens, page_table.data_ptr(), page_table.shape[0],
+                                       page_table.shape[1], _ptr(parents), _ptr(free), 0 if free is None else free.numel(), by_seq + 4 * n_seqs, by_seq, by_token,
+                                       by_token + 4 * n_tokens, by_token + 8 * n_tokens, at, None if parents is None or n_tokens == 0 else at + 8 * n_tokens,
+                                       None if free is None else by_seq + 4 * (2 * n_seqs + 1), self._stream()), "step_tables")
+        return StepTables(cu_q, kv_len, token_seq, positions, places, slot_map, ancestors, None if free is None else taken)
 
     draft_attention_ran = False          # (without drafted tokens no step waits for its kernel's error)
 

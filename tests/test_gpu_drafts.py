@@ -488,6 +488,8 @@ def test_refusals_of_step_tables():
                 dict(lengths=_i32([0] * 4097), new=_i32([0] * 4097), slots=_i32([0] * 4097))):
         with pytest.raises(ValueError):
             ops.step_tables(**{**args, **bad})
+    none = ops.step_tables(_i32([3, 70]), _i32([0, 0]), _i32([0, 1]), table, 0, parents=_i32([]), free=_i32([]))
+    assert none.cu_q.tolist() == [0, 0, 0] and none.kv_len.tolist() == [3, 70] and none.ancestors.shape == (0,) and none.taken.tolist() == [0]
     # a slot that is none changes nothing and has no places
     got = ops.step_tables(_i32([3, 70]), _i32([1, 60]), _i32([5, -1]), table, 61, free=_i32([9, 9, 9]))
     assert bool((table == 0).all()) and bool((got.slot_map == -1).all())
