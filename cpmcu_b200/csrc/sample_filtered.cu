@@ -875,6 +875,7 @@ CPM_API int cpm_sample_filtered(const float* logits, int64_t ld, int n_rows, int
 CPM_API int cpm_sample_drafts(const float* logits, int64_t ld, int n_rows, int vocab, int* token, float* logprob, const float* uniform,
                               const float* temperature, const int* top_k, const float* top_p, const float* min_p, uint64_t seed, const int* seq_key,
                               const int* step_key, const int* row_seq, const int* positions, const int* cu, int n_seqs, void* kept, cudaStream_t stream) {
+    if (n_rows <= 0) return CPM_OK;
     if (!row_seq || (!uniform && (!positions || !cu)) || ((uintptr_t)kept & 15)) return CPM_BAD_ARGUMENT;
     const FilterArgs a{logits, ld, vocab, 0, uniform, temperature, top_p, min_p, top_k, seq_key, step_key, nullptr, seed, token, logprob,
                        row_seq, uniform ? nullptr : positions, cu, n_seqs, 0, (KeptRow*)kept};

@@ -1920,6 +1920,12 @@ class Ops:
             raise ValueError(f"{what}: needs {n} numbers, got {t.numel()}")
         return t
 
+    def _here(self) -> int:
+        """The stream to launch on, which has to be of the tensors' device."""
+        if _current_device() != self.device_index:
+            raise ValueError(f"the tensors are on cuda:{self.device_index}, the current device is cuda:{_current_device()}")
+        return self._stream()
+
     def _most(self, most: int) -> int:
         if not 1 <= int(most) <= self.MOST_DRAFTS:
             raise ValueError(f"a sequence brings 1 to {self.MOST_DRAFTS} tokens, got {most}")
@@ -1947,6 +1953,7 @@ class Ops:
             self._given(parents, i32, "parents", n_tokens)
         if free is not None:
             self._given(free, i32, "free pages")
+        stream = self._here()
         # one tensor, cut into the tables (an allocation takes the host as long as three cuts): the words of 64 bits come first
         wide = n_tokens * (2 if parents is None else 4)
         room = self.empty(wide + 3 * n_tokens + 2 * n_seqs + 2, dtype=i32)
@@ -1958,7 +1965,7 @@ class Ops:
         check(self.lib.cpm_step_tables(lengths.data_ptr(), new.data_ptr(), slots.data_ptr(), n_seqs, n_tokens, page_table.data_ptr(), page_table.shape[0],
                                        page_table.shape[1], _ptr(parents), _ptr(free), 0 if free is None else free.numel(), by_seq + 4 * n_seqs, by_seq, by_token,
                                        by_token + 4 * n_tokens, by_token + 8 * n_tokens, at, None if parents is None or n_tokens == 0 else at + 8 * n_tokens,
-                                       None if free is None else by_seq + 4 * (2 * n_seqs + 1), self._stream()), "step_tables")
+                                       None if free is None else by_seq + 4 * (2 * n_seqs + 1), stream), "step_tables")
         return StepTables(cu_q, kv_len, token_seq, positions, places, slot_map, ancestors, None if free is None else taken)
 
     draft_attention_ran = False          # (without drafted tokens no step waits for its kernel's error)
@@ -2002,6 +2009,7 @@ class Ops:
         width = page_table.shape[1]
         if ancestors is not None:
             given(ancestors, torch.int64, "ancestors", n)
+        stream = self._here()
         out = self.empty(n, n_heads * d)
         if n == 0 or n_seqs == 0:
             return out
@@ -2010,14 +2018,14 @@ class Ops:
             self.draft_attention_ran = True
             check(self.lib.cpm_draft_attention_tcgen05(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
                                                        width, n_pages, _ptr(ancestors), _ptr(scratch), n, n_seqs, most, n_heads, n_kv, d,
-                                                       float(scale), self._stream()), "tcgen05 attention of drafted tokens")
+                                                       float(scale), stream), "tcgen05 attention of drafted tokens")
             LAUNCHES_EXTRA[0] += 1       # the pieces, then their addition
             return out
         shares = self.draft_attention_shares(n_seqs, most, n_heads, n_kv, width * PAGE_TOKENS)
         parts = self.empty(shares * n * n_heads * (d + 2), dtype=torch.float32) if shares > 1 else None
         check(self.lib.cpm_draft_attention_generic(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
                                                    width, n_pages, _ptr(ancestors), _ptr(parts), shares, n, n_seqs, most, n_heads, n_kv, d,
-                                                   float(scale), self.code, self._stream()), f"attention of drafted tokens (head_dim {d})")
+                                                   float(scale), self.code, stream), f"attention of drafted tokens (head_dim {d})")
         if shares > 1:
             LAUNCHES_EXTRA[0] += 1
         return out
@@ -2074,6 +2082,7 @@ class Ops:
                 raise ValueError("drafting probabilities need random numbers and numbers of acceptance")
         elif uniform is None and (seq_key is None or step_key is None or positions is None):
             raise ValueError("verify_drafts needs random numbers, or keys and positions to make them from")
+        stream = self._here()
         tokens, path, logprob = self.result(3, n_seqs, most, dtype=i32).unbind()       # (one allocation: it takes the host as long as three cuts)
         logprob, count = logprob.view(f32), self.result(n_seqs, dtype=i32)
         if n_seqs == 0:
@@ -2084,10 +2093,10 @@ class Ops:
         drawn = rows.data_ptr() + (32 * n if draft_probs is not None else 0)
         check(self.lib.cpm_sample_drafts(_ptr(logits), vocab, n, vocab, drawn, drawn + 4 * n, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
                                          _ptr(min_p), ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), _ptr(token_seq), _ptr(positions),
-                                         _ptr(cu_q), n_seqs, kept, self._stream()), "drawing for drafted tokens")
+                                         _ptr(cu_q), n_seqs, kept, stream), "drawing for drafted tokens")
         check(self.lib.cpm_verify_drafts(_ptr(logits), vocab, n, vocab, _ptr(ids), _ptr(cu_q), n_seqs, most, _ptr(parents), _ptr(draft_probs),
                                          0 if draft_probs is None else draft_probs.stride(0), _ptr(accept), _ptr(uniform), _ptr(temperature), drawn,
-                                         drawn + 4 * n, kept, _ptr(tokens), _ptr(count), _ptr(path), _ptr(logprob), self._stream()), "verify_drafts")
+                                         drawn + 4 * n, kept, _ptr(tokens), _ptr(count), _ptr(path), _ptr(logprob), stream), "verify_drafts")
         return tokens, count, path, logprob
 
     def keep_drafts(self, pairs, lengths: torch.Tensor, path: torch.Tensor, count: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor) -> None:
@@ -2123,13 +2132,14 @@ class Ops:
             by_size.setdefault(k.element_size(), []).append(
                 (k.data_ptr(), 0 if v is None else v.data_ptr(), k.stride(0) * k.element_size() if lanes > 1 else 0,
                  0 if v is None or lanes < 2 else v.stride(0) * v.element_size(), lanes, pages, kv, d * k.element_size(), 0 if v is None else v.shape[3]))
+        stream = self._here()
         if n_seqs == 0:
             return
         for element, words in by_size.items():
             for i in range(0, len(words), self.COPY_TENSORS):
                 part = [x for w in words[i:i + self.COPY_TENSORS] for x in w]
                 check(self.lib.cpm_keep_drafts((ctypes.c_int64 * len(part))(*part), len(part) // 9, element, _ptr(lengths), _ptr(path), _ptr(count), _ptr(slots),
-                                               _ptr(page_table), page_table.shape[0], page_table.shape[1], n_seqs, path.shape[1], self._stream()), "keep_drafts")
+                                               _ptr(page_table), page_table.shape[0], page_table.shape[1], n_seqs, path.shape[1], stream), "keep_drafts")
 
 
 LAUNCHES_EXTRA = library.LAUNCHES

@@ -219,6 +219,57 @@ def test_attention_captured_and_on_another_stream(form):
         assert torch.equal(got, ops.draft_attention(**args))
 
 
+@pytest.mark.parametrize("form", ["tcgen05", "plain"])
+@pytest.mark.parametrize("d,heads,kv", [(64, 4, 2), (128, 20, 1)])
+def test_attention_of_more_sequences_than_a_launch_takes(form, d, heads, kv):
+    """1,100 short sequences: several launches, and units that have no place of their own for their parts."""
+    ops = _ops("bfloat16")
+    ops.use_tcgen05_draft = form == "tcgen05"
+    new = [1 + i % 3 for i in range(1100)]
+    lengths = [n + (i * 7) % 130 for i, n in enumerate(new)]
+    lengths[700] = 900
+    args, rows, cu = _attention_case("bfloat16", d, heads, kv, lengths, new, None, seed=12)
+    got = ops.draft_attention(**args)
+    for some in (slice(0, 40), slice(500, 530), slice(690, 710), slice(1080, 1100)):
+        _check_attention("bfloat16", args, rows[some], cu[some] + [cu[some.stop]], None, _weight_bits(ops, "bfloat16", d, heads, kv), got)
+
+
+def test_offsets_beyond_32_bits():
+    """Keys and values that lie behind 2^32 bytes: attention in both forms, and the moving of accepted tokens."""
+    ops = _ops("bfloat16")
+    d, kv, new, lengths = 128, 2, [5], [130]
+    args, rows, cu = _attention_case("bfloat16", d, 8, kv, lengths, new, None, seed=6)
+    pages = 2 ** 32 // (kv * PAGE * d * 2) + 40
+    k = torch.empty(pages, kv, PAGE, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.empty(pages, kv, d, PAGE, dtype=torch.bfloat16, device="cuda")
+    n = args["k_cache"].shape[0]
+    k[-n:], v[-n:] = args["k_cache"], args["v_cache"]
+    args.update(k_cache=k, v_cache=v, page_table=args["page_table"] + (pages - n))
+    for form in (True, False):
+        ops.use_tcgen05_draft = form
+        _check_attention("bfloat16", args, rows, cu, None, _weight_bits(ops, "bfloat16", d, 8, kv), ops.draft_attention(**args))
+    ops.keep_drafts([(k[None], v[None])], _i32([125]), _i32([[0, 3]]), _i32([2]), args["slots"], args["page_table"])
+    table = args["page_table"][int(args["slots"][0])]
+    a, b = int(table[1]), int(table[2])
+    assert torch.equal(k[a, :, 126 - 64], k[b, :, 0]) and torch.equal(v[a, :, :, 126 - 64], v[b, :, :, 0])
+
+
+def test_another_current_device_is_refused(monkeypatch):
+    """Tensors of one device while another is the current one."""
+    from cpmcu_b200.ops import ops as module
+
+    ops = _ops("bfloat16")
+    args, _, _ = _attention_case("bfloat16", 64, 4, 2, [70], [3], None, seed=1)
+    more, _ = _verify_case([3], 50, 2, False)
+    table = _i32([[0, 1]])
+    k = torch.zeros(1, 2, 1, PAGE, 8).bfloat16().cuda()
+    monkeypatch.setattr(module, "_current_device", lambda: 1)
+    for call in (lambda: ops.draft_attention(**args), lambda: ops.verify_drafts(**more), lambda: ops.step_tables(_i32([3]), _i32([1]), _i32([0]), table, 1),
+                 lambda: ops.keep_drafts([(k, None)], _i32([0]), _i32([[0, 1]]), _i32([2]), _i32([0]), table)):
+        with pytest.raises(ValueError, match="current device"):
+            call()
+
+
 def test_refusals_of_attention():
     ops = _ops("bfloat16")
     args, _, _ = _attention_case("bfloat16", 64, 4, 2, [70, 3], [3, 2], None, seed=1)
@@ -410,6 +461,8 @@ def test_refusals_of_verify():
     none = torch.zeros(0).cuda()
     got = ops.verify_drafts(torch.zeros(0, 50).cuda(), _i32([]), _i32([0]), _i32([]), 4, none, none)
     assert [tuple(x.shape) for x in got] == [(0, 4), (0,), (0, 4), (0, 4)]
+    got = ops.verify_drafts(torch.zeros(0, 50).cuda(), _i32([]), _i32([0, 0]), _i32([]), 4, none, torch.ones(1).cuda())          # a sequence that brings nothing
+    assert got[1].tolist() == [0] and got[0].tolist() == [[-1] * 4]
 
 
 # ---------------------------------------------------------------------------
