@@ -71,6 +71,11 @@ __device__ __forceinline__ void sum_up(const TableArgs& a, int* tokens, int* pag
     __syncthreads();
 }
 
+// Whether the free pages of a sequence are all there (and, whatever the lengths say, within the list: counts of nonsense may run over).
+__device__ __forceinline__ bool pages_there(const TableArgs& a, const int* pages, int s) {
+    return pages[s] >= 0 && pages[s] <= pages[s + 1] && pages[s + 1] <= a.n_free;
+}
+
 __device__ __forceinline__ int sequence_of(const int* cu, int n_seqs, int t) {       // the last whose first token is t or before
     int lo = 0, hi = n_seqs - 1;
     while (lo < hi) {
@@ -98,7 +103,7 @@ step_tables_kernel(const __grid_constant__ TableArgs a) {
         }
         a.kv_len[s] = length_of(a, s) + cu[s + 1] - cu[s];
         const int slot = a.slots[s], have = pages_of(length_of(a, s));
-        if (a.taken && pages[s + 1] <= a.n_free && slot >= 0 && slot < a.n_slots) {      // (a sequence whose pages are not all there gets none)
+        if (a.taken && pages_there(a, pages, s) && slot >= 0 && slot < a.n_slots) {      // (a sequence whose pages are not all there gets none)
             for (int i = 0; i < pages[s + 1] - pages[s]; ++i)
                 if (have + i < a.max_pages) a.page_table[(int64_t)slot * a.max_pages + have + i] = a.free[pages[s] + i];
         }
@@ -144,7 +149,7 @@ step_tables_kernel(const __grid_constant__ TableArgs a) {
     int64_t at = -1;
     if (place >= 0 && column < a.max_pages && slot >= 0 && slot < a.n_slots) {
         if (!a.taken || column < have) at = a.page_table[(int64_t)slot * a.max_pages + column];
-        else if (pages[s + 1] <= a.n_free) at = a.free[pages[s] + column - have];
+        else if (pages_there(a, pages, s)) at = a.free[pages[s] + column - have];
         if (at >= 0) at = at * kPageTokens + place % kPageTokens;
     }
     a.slot_map[t] = at;

@@ -3,7 +3,9 @@
 A sequence's last tokens have often been followed by something before, in the prompt or in what was generated (:class:`Lookup`): what
 followed is drafted, several continuations as a tree.  One step then gives every sequence between one token and as many as were drafted and
 one more.  A row of the logits draws its token as a step of its own would (the same random number), and a drafted token is
-accepted where it is that token, so that drafts change how many tokens a step gives and not which.
+accepted where it is that token, so that drafts change how many tokens a step gives and not which: as far as a step of several tokens computes the logits of
+single steps (in bf16 other kernels round otherwise), and but for numbers that fall on the very border of two tokens where an ordinary step
+draws with sums in fp32 (no top-k and no min-p).
 
 Every sequence brings the same number of tokens, what is not drafted being filled with tokens that nothing leads to, so that one recording per bucket size
 serves all steps.  The reference drafts with a small model of its own and verifies a tree in the same way
@@ -198,6 +200,7 @@ class DraftRunner:
             self._body(b, captured=False)
         tokens, count = b.out[0], b.out[1]
         host = torch.cat((count, tokens.reshape(-1))).cpu().tolist()        # (waits for the step)
+        self.ops.raise_on_draft_error()
         out = []
         for i in range(n):
             m = host[i]

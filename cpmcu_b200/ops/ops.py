@@ -1036,8 +1036,7 @@ class Ops:
             arena.check_guards()
         if self.kv4_prompt_ran and int(self.lib.cpm_kv4_prompt_error()):
             raise RuntimeError("the prompts' attention over a 4-bit cache gave up waiting on a barrier; the results of this step are not valid")
-        if self.draft_attention_ran and int(self.lib.cpm_draft_attention_error()):
-            raise RuntimeError("the attention of drafted tokens gave up waiting on a barrier; the results of this step are not valid")
+        self.raise_on_draft_error()
         if int(self.lib.cpm_listed_tile_error()):
             raise RuntimeError("the block-list attention of a prompt chunk gave up waiting on a barrier; the results of "
                                "this step are not valid")
@@ -1970,6 +1969,11 @@ class Ops:
 
     draft_attention_ran = False          # (without drafted tokens no step waits for its kernel's error)
 
+    def raise_on_draft_error(self) -> None:
+        """The part of ``raise_on_kernel_error`` that is the attention of drafted tokens' (12 us of the host's time; all of it takes 86)."""
+        if self.draft_attention_ran and int(self.lib.cpm_draft_attention_error()):
+            raise RuntimeError("the attention of drafted tokens gave up waiting on a barrier; the results of this step are not valid")
+
     def draft_attention_on_tensor_cores(self, d: int, n_heads: int, n_kv: int) -> bool:
         return self.code == BF16 and self.use_tcgen05_draft and d in FAST_HEAD_DIMS and n_heads // n_kv <= 128
 
@@ -1984,7 +1988,7 @@ class Ops:
         """A few tokens a sequence against its cached keys: q [tokens, heads, d] -> [tokens, heads * d].  Sequence s brings the tokens cu_q[s] .. cu_q[s + 1], at most
         ``most`` (up to MOST_DRAFTS), which are the last of its kv_len[s] keys in k_cache [pages, kv, PAGE_TOKENS, d] and v_cache [pages, kv, d, PAGE_TOKENS].  A
         token sees all keys before these, and of these the ones up to itself, or with ``ancestors`` (int64 [tokens]) those whose bit is set.  A row that sees none
-        gives zeros; rows of no sequence are left as they are.  What an unseen key or value holds, even if it is no number, changes nothing."""
+        gives zeros; rows of no sequence are not written.  What an unseen key or value holds, even if it is no number, changes nothing."""
         given, dtype, i32 = self._given, self.dtype, torch.int32
         given(q, dtype, "q")
         if q.dim() != 3:

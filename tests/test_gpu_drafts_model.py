@@ -138,6 +138,46 @@ def test_a_step_of_drafts_gives_the_logits_of_single_steps(model_folders, dtype)
     cache.check_consistent()
 
 
+@pytest.mark.parametrize("settings", [dict(temperature=0.9), dict(temperature=0.7, top_p=0.9)])
+def test_drafts_beside_steps_without_filters(model_folders, settings, monkeypatch):
+    """Steps of one token draw by sums in fp32 where there is no top-k and no min-p, steps of drafts by whole units: the same number falls on the same token unless it
+    lies within the sums' error of a border (2^-20 of the mass at 512 tokens, 4 x 40 draws: a chance of one in some thousand, and the numbers are fixed)."""
+    cfgd = configs.tiny_a()
+    folder = model_folders("tiny_a", cfgd, 3, "float32", std=0.08)
+    prompts = [_repeating(cfgd["vocab_size"], n, n) for n in (70, 33, 5, 64)]
+    want = [r.tokens for r in _llm(folder, "float32", random_seed=5).generate_batch(prompts, generation_length=40, **settings)]
+    llm = _llm(folder, "float32", random_seed=5, draft_tokens=7)
+    texts = [p + w for p, w in zip(prompts, want)]
+
+    def propose(self, n):
+        right = next(t for t in texts if t[:len(self.tokens)] == self.tokens)[len(self.tokens):][:2]
+        return right, list(range(len(right)))
+
+    monkeypatch.setattr(Lookup, "propose", propose)
+    assert [r.tokens for r in llm.generate_batch(prompts, generation_length=40, **settings)] == want
+    assert llm.backend.drafter.accepted > 80
+
+
+def test_a_kernel_that_gave_up_ends_the_generation(model_folders, monkeypatch):
+    """The step's error is read with its tokens, none of which is then given, and nothing of the batch stays held."""
+    cfgd = configs.tiny_a()
+    llm = _llm(model_folders("tiny_a", cfgd, 3, "float32", std=0.08), "float32", draft_tokens=7)
+    prompt = _repeating(cfgd["vocab_size"], 70, 1)
+    want = llm.generate_batch([prompt], generation_length=30, temperature=0.0)[0].tokens
+    assert llm.backend.drafter.steps > 0
+    with monkeypatch.context() as m:
+        m.setattr(llm.ops, "draft_attention_ran", True)
+        before, found = llm.backend.drafter.steps, []
+        real = llm.backend.drafter._bucket
+        m.setattr(llm.backend.drafter, "_bucket", lambda n: (m.setattr(llm.ops.lib, "cpm_draft_attention_error", lambda: 3), real(n))[1])
+        with pytest.raises(RuntimeError, match="drafted tokens gave up"):
+            llm.generate_batch([prompt], generation_length=30, temperature=0.0, on_token=lambda i, t, last: found.append(t))
+        assert llm.backend.drafter.steps == before and found == want[:len(found)] and len(found) < 30
+    assert llm.cache.slots.n_held == 1 and not llm.backend.lookups
+    assert llm.generate_batch([prompt], generation_length=30, temperature=0.0)[0].tokens == want
+    llm.cache.check_consistent()
+
+
 def test_refusals(model_folders):
     from cpmcu_b200 import LLM
 
