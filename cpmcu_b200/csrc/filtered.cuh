@@ -34,6 +34,9 @@ __device__ __forceinline__ void put64(const void* own, uint32_t rank, uint64_t v
 __device__ __forceinline__ void add64(const void* own, uint32_t rank, uint64_t v) {
     asm volatile("red.shared::cluster.add.u64 [%0], %1;" :: "r"(cluster_address(own, rank)), "l"(v) : "memory");
 }
+__device__ __forceinline__ void red32(const void* own, uint32_t rank, uint32_t v) {
+    asm volatile("red.shared::cluster.add.u32 [%0], %1;" :: "r"(cluster_address(own, rank)), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint32_t add32(const void* own, uint32_t rank, uint32_t v) {
     uint32_t old;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(cluster_address(own, rank)), "r"(v) : "memory");

@@ -15,11 +15,11 @@
 // histogram of the weights' upper bits (32 bins to an octave) holds each bin's number of tokens and, where mass decides, the sum of their lower bits: so the
 // bin in which the k-th token lies, or at which the mass is reached, is known exactly.  The tokens in that bin, a few hundred, go to the cluster's first
 // block, which finds the border by radix selection; where no more than kRanked tokens are in or above the bin of top-k, all of them go there, each is
-// compared with each, and it draws as well.  In the same pass a thread sums what it keeps above the bin, so that the draw looks at few tokens again.
+// compared with each, and it draws as well (a small top-k needs no weights and bins of the whole row for that: draw_few).  In the same pass a thread sums what it keeps above the bin, so that the draw looks at few tokens again.
 // (A cluster's barrier takes about 2 us, and a look into a neighbour's shared memory half of that: a selection over the whole row with
-// all blocks' histograms added up at every step took 41 us for one row of 73,448, bins of counts alone 25, and this 15.)
-// 64 rows of 73,448 with settings of their own 38 us, 512 rows of 32,000 by mass alone 117.  What a row cannot do without is its logits, 4 bytes a token
-// (10 us of the 117); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
+// all blocks' histograms added up at every step took 41 us for one row of 73,448, bins of counts alone 25, and this 14.)
+// 64 rows of 73,448 with settings of their own 37 us, 512 rows of 32,000 by mass alone 122.  What a row cannot do without is its logits, 4 bytes a token
+// (10 us of the 122); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
 #include "filtered.cuh"
 #include "philox.cuh"
 #include <type_traits>
@@ -349,7 +349,134 @@ __device__ __forceinline__ uint64_t ties_of(const Border& b, double need, uint64
     return n;
 }
 
-template <bool STAGED>
+// A row's settings, for what is done out of line (the other rows' code keeps its registers).
+struct Drawn {
+    int r, k;
+    float t, p, ratio, u, top;
+    bool by_mass;
+};
+
+// All that top-k may leave is listed in the first block, no more than kRanked tokens: each is compared with each, and one is drawn.
+__device__ __noinline__ void draw_ranked(FilterShared& sm, const FilterArgs& a, Drawn g, int listed) {
+    const int tid = threadIdx.x;
+    // Some threads to a token: how many stand before it, and what mass?
+    int bits_of_tokens = 5;
+    while ((1 << bits_of_tokens) < listed) ++bits_of_tokens;
+    const int share = kFilterThreads >> bits_of_tokens, own = tid / share, part = tid % share;
+    uint64_t* masses = reinterpret_cast<uint64_t*>(sm.fine[0]);
+    if (tid < listed) masses[tid] = units_of(sm.list[tid]);
+    __syncthreads();
+    const bool there = own < listed;
+    const uint32_t bits = there ? sm.list[own] : 0;
+    const int place = there ? sm.place[own] : 0;
+    const uint64_t mass = there ? masses[own] : 0;
+    int count = 0;
+    uint64_t before = 0;
+#pragma unroll 4
+    for (int i = part; i < listed; i += share) {
+        const uint32_t other = sm.list[i];
+        const bool ahead = other > bits || (other == bits && sm.place[i] < place);
+        count += ahead;
+        before += ahead ? masses[i] : 0;
+    }
+    for (int o = 1; o < share; o <<= 1) {
+        count += __shfl_xor_sync(0xffffffffu, count, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    bool stays = there && count < g.k;
+    if (g.by_mass) {
+        const uint64_t within = block_sum64(stays && part == 0 ? mass : 0, sm);
+        stays = stays && (double)before < (double)g.p * (double)within;
+    }
+    stays = stays && __uint_as_float(bits) >= g.ratio;
+    const uint64_t total = block_sum64(stays && part == 0 ? mass : 0, sm);
+    if (there && part == 0) masses[own] = stays ? mass : 0;
+    if (a.kept && tid == 0) {                  // the last that stays, as those before it do
+        sm.plan.border = 0xffffffffu;
+        sm.cut = -1;
+    }
+    __syncthreads();
+    if (a.kept) {
+        if (stays && part == 0) atomicMin(&sm.plan.border, bits);
+        __syncthreads();
+        if (stays && part == 0 && bits == sm.plan.border) atomicMax(&sm.cut, place);
+        __syncthreads();
+        if (tid == 0) a.kept[g.r] = KeptRow{g.top, sm.plan.border, sm.cut, 0, total, 0};
+    }
+    before = 0;
+#pragma unroll 4
+    for (int i = part; i < listed; i += share) before += sm.place[i] < place ? masses[i] : 0;
+    for (int o = 1; o < share; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    const uint64_t target = min((uint64_t)((double)g.u * (double)total), total - 1);
+    if (stays && part == 0 && target >= before && target < before + mass) {
+        a.token[g.r] = place;
+        a.logprob[g.r] = (g.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(a.logits[(int64_t)g.r * a.ld + place], g.top), g.t))
+                     - logf((float)((double)total * (1.0 / 1099511627776.0)));
+    }
+}
+
+// Few tokens by their number: the threads' largest ones alone go into bins.  The bin in which the k-th of them lies begins no higher than the row's k-th token, so all
+// that top-k may leave is found by comparing logits with it, and only these tokens' weights are formed.  False: they are more than kRanked, or the threads' largest
+// tokens mostly without weight; nothing has been drawn then.
+__device__ __noinline__ bool draw_few(FilterShared& sm, const FilterArgs& a, Drawn g, Weigher row, const float* logits, int n, int first, float thread_top) {
+    const int blocks = (int)cluster_blocks(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31;
+    const uint32_t top_bits = __float_as_uint(row.form_quick(thread_top));
+    if (bin_of(top_bits) > 0) atomicAdd(&sm.own[1][bin_of(top_bits)], 1u);
+    __syncthreads();
+#pragma unroll 1
+    for (int bin = tid; bin < kCoarseBins; bin += kFilterThreads) {      // (every block finds the bin for itself)
+        const uint32_t here = sm.own[1][bin];
+        for (int b = 0; here && b < blocks; ++b) red32(&sm.coarse[bin], b, here);
+    }
+    cluster_sync();
+    find_count(sm, (double)g.k);
+    const uint32_t low = bin_begin(sm.found_bin);
+    // what lies below this has a smaller weight for sure (1/1000 is far more than the logarithm, the exponential and the products are off)
+    const float least = low > 0 ? g.t * (logf(__uint_as_float(low)) * 1.00001f - 0.001f) : INFINITY;
+    // a lane's tokens that may be among them, the first one in the lowest bit
+    uint64_t found = 0;
+    int turn = 0;
+#pragma unroll 8
+    for (int i = tid; i < n; i += kFilterThreads, ++turn) found |= (uint64_t)!(__fsub_rn(logits[i], row.top) < least) << turn;
+    int hits = 0;
+#pragma unroll 1
+    for (uint64_t left = found; left; left &= left - 1) {
+        const int bit = __ffsll(left) - 1;
+        if (__float_as_uint(row.form_quick(logits[tid + bit * kFilterThreads])) >= low) ++hits;
+        else found &= ~(1ull << bit);
+    }
+    const int all = __reduce_add_sync(0xffffffffu, hits);
+    if (all) {                                                 // a warp asks for room once
+        uint32_t at = lane == 0 ? add32(&sm.listed, 0, all) : 0;
+        at = __shfl_sync(0xffffffffu, at, 0);
+        int upto = hits;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        at += upto - hits;
+#pragma unroll 1
+        for (uint64_t left = found; left; left &= left - 1, ++at) {
+            const int i = tid + (__ffsll(left) - 1) * kFilterThreads;
+            if (at < kRanked) {
+                put32(&sm.list[at], 0, __float_as_uint(row.form_quick(logits[i])));
+                put32(&sm.place[at], 0, first + i);
+            }
+        }
+    }
+    cluster_sync();
+    const int listed = (int)peer32(&sm.listed, 0);
+    // The first block goes on alone, but does not end (or, without a draw, forget the count) before the others have read it.
+    asm volatile("barrier.cluster.arrive;" ::: "memory");
+    const bool ok = low > 0 && listed >= g.k && listed <= kRanked;
+    if (ok && rank == 0) draw_ranked(sm, a, g, listed);
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+    return ok;
+}
+
+// COUNT: rows may have a top-k (without it the code is half as long, and keeps more of its numbers in registers).
+template <bool STAGED, bool COUNT>
 __global__ void __launch_bounds__(kFilterThreads, 2)
 sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     extern __shared__ float weights[];
@@ -379,7 +506,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     if (p <= 0.f || ratio > 1.f) k = 1;
     // above one: the first token alone, which it would leave out as well; below zero, -0 (weights are compared by their bits) or no number: no limit
     if (!(ratio > 0.f && ratio <= 1.f)) ratio = 0.f;
-    const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
+    const bool by_count = COUNT && k > 0 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
     const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[s], (uint32_t)(a.step_key[s] + step));
 
     asm volatile("barrier.cluster.arrive;" ::: "memory");       // (nothing is put into a block that has not begun)
@@ -412,10 +539,13 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         if constexpr (STAGED) weights[i] = v;
         if (v > best.v) best = ArgMax{v, first + i};
     }
-    if (by_count || by_mass)
+    const auto clear_bins = [&]() {
 #pragma unroll 1
         for (int i = tid; i < kCoarseBins; i += kFilterThreads) sm.coarse[i] = sm.low[0][i] = sm.low[1][i] = sm.own[0][i] = sm.own[1][i] = 0;
-    if (tid == 0) sm.listed = 0;
+    };
+    if (by_count || by_mass) clear_bins();
+    if (tid == 0) sm.listed = sm.found_bin = 0;
+    const float thread_top = best.v;
     best = block_argmax(best, sm.scratch);
     asm volatile("barrier.cluster.wait;" ::: "memory");
     if (tid < (int)blocks) put64(&sm.best[rank], tid, (uint64_t)__float_as_uint(best.v) | (uint64_t)(uint32_t)best.i << 32);
@@ -423,7 +553,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     best = ArgMax{-INFINITY, 0x7fffffff};
 #pragma unroll 1
     for (uint32_t b = 0; b < blocks; ++b) best = better(best, sm.best[b]);
-    if (best.v == -INFINITY || !(t > 0.f)) {                   // nothing that can be drawn: token 0; a greedy row: the largest
+    if (best.v == -INFINITY || !(t > 0.f) || k == 1) {         // nothing that can be drawn: token 0; a greedy row, or one token: the largest
         if (rank == 0 && tid == 0) {
             a.token[r] = best.v == -INFINITY ? 0 : best.i;
             a.logprob[r] = best.v == -INFINITY ? -INFINITY : 0.f;
@@ -433,28 +563,66 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     }
     row.set(best.v, t);
 
+    if constexpr (STAGED && COUNT) {
+        // (Two of the k may be one thread's, and the k-th of the threads' largest then lies below the row's: with k up to a quarter of the threads some k / 8 tokens more, and
+        // these have room among kRanked.  64 conversations of 5 rows of 73,448, half of them with a top-k of 200: 129 us, 142 with all weights formed; one of 50: 24 and 25.)
+        if (by_count && row.quick() && k <= kRanked - kRanked / 8 && 4 * k <= (int)blocks * kFilterThreads) {
+            if (draw_few(sm, a, Drawn{r, k, t, p, ratio, u, row.top, by_mass}, row, weights, row.n, first, thread_top)) return;
+            if (tid == 0) sm.listed = 0;
+            clear_bins();
+            cluster_sync();
+        }
+    }
+
     // weights, their histogram, and (where mass alone decides) their mass.  A thread's tokens are neighbours, an odd number of them, so that sums by
     // thread go by index and a warp's accesses to shared memory are in different banks
     const int strip = (row.n + kFilterThreads - 1) / kFilterThreads | 1, i0 = min(row.n, tid * strip), i1 = min(row.n, i0 + strip);
     const bool summed = STAGED && by_mass && !by_count;        // whether the bins' masses are
+    // Where mass alone decides: tokens lighter than (1 - p) / vocab hold less than 1 - p of the mass together, so that the border lies above them, and bins need not
+    // know them.  (Below 2^-17, so that such a token's mass is counted as the other small ones' are; 0.99: more than the roundings.)
+    const uint32_t light = by_mass && !by_count ? min(bin_begin(bin_of(__float_as_uint(0.99f * (1.f - p) / (float)a.vocab))), kWhole) : 0u;
     uint64_t own_mass = 0;                                     // of the thread's tokens that bins do not tell exactly
+    // Where few of the block's tokens are in bins (a tenth by a look at one of each thread's) a thread gathers its own in ``heavy``, the last one in the lowest bit, and
+    // goes through them one by one: else of 32 neighbours one is in a bin nearly always, and what is done for one lane takes as long as for all.  (512 rows of 32,000, 0.8
+    // of the mass, temperatures of 0.35 to 0.95: 76 us, 86 without; from a quarter of the tokens on the separate loop loses: at 1.3 138 us and 122.)
+    uint64_t heavy = 0;
+    bool sparse = false;
     const auto weigh_all = [&](auto quick) {
         const auto form = [&](float x) { return decltype(quick)::value ? row.form_quick(x) : row.form(x); };
         if (by_count || by_mass) {
-            uint32_t small = 0, least = 0;
+            uint32_t small = 0;
+            int least = 0;                                     // tokens in the first bin: a thread counts its own, as additions to one place come one after the other
+            if constexpr (STAGED)
+                if (light > 0) sparse = __syncthreads_count(i0 < i1 && __float_as_uint(form(weights[i0])) >= light) <= kFilterThreads / 10;
+            if (STAGED && sparse) {
+                heavy = 0;
 #pragma unroll 4
-            for (int i = i0; i < i1; ++i) {
-                const float w = form(STAGED ? weights[i] : row.z[i]);
-                if constexpr (STAGED) weights[i] = w;
-                // (at a low temperature most tokens lie in the first bin, and additions to one place come one after the other: a thread counts its own)
-                if (bin_of(__float_as_uint(w)) == 0) ++least;
-                else count_own<STAGED>(sm, __float_as_uint(w), summed);
-                if (summed) small += small_units_of(__float_as_uint(w));
-                else if (!STAGED && !by_count) own_mass += units_of(__float_as_uint(w));
+                for (int i = i0; i < i1; ++i) {
+                    const float w = form(weights[i]);
+                    weights[i] = w;
+                    heavy = heavy << 1 | (__float_as_uint(w) >= light);
+                    small += small_units_of(__float_as_uint(w));
+                }
+#pragma unroll 1
+                for (uint64_t left = heavy; left;) {
+                    const int bit = __ffsll(left) - 1;
+                    left &= left - 1;
+                    count_own<STAGED>(sm, __float_as_uint(weights[i1 - 1 - bit]), true);
+                }
+            } else {
+#pragma unroll 4
+                for (int i = i0; i < i1; ++i) {
+                    const float w = form(STAGED ? weights[i] : row.z[i]);
+                    if constexpr (STAGED) weights[i] = w;
+                    if (bin_of(__float_as_uint(w)) == 0) ++least;
+                    else count_own<STAGED>(sm, __float_as_uint(w), summed);
+                    if (summed) small += small_units_of(__float_as_uint(w));
+                    else if (!STAGED && !by_count) own_mass += units_of(__float_as_uint(w));
+                }
             }
             own_mass += small;
             least = __reduce_add_sync(0xffffffffu, least);
-            if (lane == 0 && least) atomicAdd(&sm.own[1][0], STAGED ? least << kCountBits : least);
+            if (lane == 0 && least) atomicAdd(&sm.own[1][0], STAGED ? (uint32_t)least << kCountBits : (uint32_t)least);
         } else if constexpr (STAGED) {
 #pragma unroll 4
             for (int i = i0; i < i1; ++i) weights[i] = form(weights[i]);
@@ -511,7 +679,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                     high = complete ? 0x3f800001u : bin_begin(sm.found_bin + 1);
                 } else {
                     // from where the masses reach ``need`` by their bounds from above, to where they do by those from below
-                    const int last = bin_of(border);
+                    const int last = bin_of(max(border, light));
                     within = find_mass(sm, summed, p, within, last);
                     need = (double)p * (double)within;
                     const int low_bin = max(sm.low_bin, last), high_bin = max(sm.high_bin, low_bin);
@@ -539,21 +707,21 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                         for (int i = tid; i < kFineBins; i += kFilterThreads) sm.joined[i] = 0;
                         clear_fine(sm);
                     }
-                    if (tid == 0) {
-                        sm.plan.low = low;
-                        sm.plan.high = high;
-                        sm.plan.complete = complete;
-                        sm.plan.known = known;
-                        sm.plan.apart = some <= kListed;
-                        sm.listed = 0;
+                    if (tid < (int)blocks) {                   // (into every block: a look at the first one's takes a microsecond)
+                        put32(&sm.plan.low, tid, low);
+                        put32(&sm.plan.high, tid, high);
+                        put32(&sm.plan.complete, tid, complete);
+                        put32(&sm.plan.known, tid, known);
+                        put32(&sm.plan.apart, tid, some <= kListed);
+                        if (tid == 0) sm.listed = 0;
                     }
                 }
                 cluster_sync();
-                low = peer32(&sm.plan.low, 0);
-                high = peer32(&sm.plan.high, 0);
-                complete = peer32(&sm.plan.complete, 0);
-                known = peer32(&sm.plan.known, 0);
-                const bool apart = peer32(&sm.plan.apart, 0);
+                low = sm.plan.low;
+                high = sm.plan.high;
+                complete = sm.plan.complete;
+                known = sm.plan.known;
+                const bool apart = sm.plan.apart;
                 const int range = bits_of_range(low, high), shift = max(0, range - 10);
                 uint64_t over = 0;
                 int hits = 0;
@@ -561,6 +729,18 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 sure = STAGED && apart && (last_round || complete) && __float_as_uint(ratio) <= high;
                 found = 0;
                 const bool weigh = !known || sure;
+                if (STAGED && sparse) {
+#pragma unroll 1
+                    for (uint64_t left = heavy; left;) {
+                        const int bit = __ffsll(left) - 1;
+                        left &= left - 1;
+                        const uint32_t bits = __float_as_uint(weights[i1 - 1 - bit]);
+                        const bool hit = bits - low < high - low;
+                        if (hit) found |= 1ull << bit;
+                        if (hit && !apart) add_fine(sm, true, (bits - low) >> shift, bits);
+                        if (weigh && bits >= high) over += units_of(bits);
+                    }
+                } else
 #pragma unroll 4
                 for (int i = i0; i < i1; ++i) {
                     const uint32_t bits = __float_as_uint(row.at(i));
@@ -630,11 +810,11 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                     high = min(high, low + (1u << shift));
                     above = sm.found_before;
                     some = round > 0 ? sm.found_here / max((uint64_t)1, units_of(low)) : sm.found_here;
-                    if (tid == 0) sm.plan.apart = shift > 0;
+                    if (tid < (int)blocks) put32(&sm.plan.apart, tid, shift > 0);
                     b = Border{low, above, sm.found_here};
                 }
                 cluster_sync();
-                if (peer32(&sm.plan.apart, 0) == 0) break;      // a single weight is left
+                if (sm.plan.apart == 0) break;                  // a single weight is left
                 cluster_sync();                                // (read before the next plan is made)
             }
             if (complete) {
@@ -646,60 +826,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                         asm volatile("barrier.cluster.wait;" ::: "memory");
                         return;
                     }
-                    // Some threads to a token: how many stand before it, and what mass?
-                    int bits_of_tokens = 5;
-                    while ((1 << bits_of_tokens) < listed) ++bits_of_tokens;
-                    const int share = kFilterThreads >> bits_of_tokens, own = tid / share, part = tid % share;
-                    uint64_t* masses = reinterpret_cast<uint64_t*>(sm.fine[0]);
-                    if (tid < listed) masses[tid] = units_of(sm.list[tid]);
-                    __syncthreads();
-                    const bool there = own < listed;
-                    const uint32_t bits = there ? sm.list[own] : 0;
-                    const int place = there ? sm.place[own] : 0;
-                    const uint64_t mass = there ? masses[own] : 0;
-                    int count = 0;
-                    uint64_t before = 0;
-#pragma unroll 4
-                    for (int i = part; i < listed; i += share) {
-                        const uint32_t other = sm.list[i];
-                        const bool ahead = other > bits || (other == bits && sm.place[i] < place);
-                        count += ahead;
-                        before += ahead ? masses[i] : 0;
-                    }
-                    for (int o = 1; o < share; o <<= 1) {
-                        count += __shfl_xor_sync(0xffffffffu, count, o);
-                        before += __shfl_xor_sync(0xffffffffu, before, o);
-                    }
-                    bool stays = there && count < k;
-                    if (by_mass) {
-                        within = block_sum64(stays && part == 0 ? mass : 0, sm);
-                        stays = stays && (double)before < (double)p * (double)within;
-                    }
-                    stays = stays && __uint_as_float(bits) >= ratio;
-                    const uint64_t total = block_sum64(stays && part == 0 ? mass : 0, sm);
-                    if (there && part == 0) masses[own] = stays ? mass : 0;
-                    if (a.kept && tid == 0) {                  // the last that stays, as those before it do
-                        sm.plan.border = 0xffffffffu;
-                        sm.cut = -1;
-                    }
-                    __syncthreads();
-                    if (a.kept) {
-                        if (stays && part == 0) atomicMin(&sm.plan.border, bits);
-                        __syncthreads();
-                        if (stays && part == 0 && bits == sm.plan.border) atomicMax(&sm.cut, place);
-                        __syncthreads();
-                        if (tid == 0) a.kept[r] = KeptRow{row.top, sm.plan.border, sm.cut, 0, total, 0};
-                    }
-                    before = 0;
-#pragma unroll 4
-                    for (int i = part; i < listed; i += share) before += sm.place[i] < place ? masses[i] : 0;
-                    for (int o = 1; o < share; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-                    const uint64_t target = min((uint64_t)((double)u * (double)total), total - 1);
-                    if (stays && part == 0 && target >= before && target < before + mass) {
-                        a.token[r] = place;
-                        a.logprob[r] = (row.top == INFINITY ? 0.f : __fdiv_rn(__fsub_rn(a.logits[(int64_t)r * a.ld + place], row.top), t))
-                                     - logf((float)((double)total * (1.0 / 1099511627776.0)));
-                    }
+                    draw_ranked(sm, a, Drawn{r, k, t, p, ratio, u, row.top, by_mass}, listed);
                     asm volatile("barrier.cluster.wait;" ::: "memory");
                     return;
                 }
@@ -739,15 +866,15 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
                 }
             }
             // ---- known to all ----
-            if (rank == 0 && tid == 0) {
-                sm.plan.border = border;
-                sm.plan.ties = ties;
-                sm.plan.equal = equal;
+            if (rank == 0 && tid < (int)blocks) {
+                put32(&sm.plan.border, tid, border);
+                put64(&sm.plan.ties, tid, ties);
+                put64(&sm.plan.equal, tid, equal);
             }
             cluster_sync();
-            border = peer32(&sm.plan.border, 0);
-            ties = peer64(&sm.plan.ties, 0);
-            equal = peer64(&sm.plan.equal, 0);
+            border = sm.plan.border;
+            ties = sm.plan.ties;
+            equal = sm.plan.equal;
             if (round == 0 && by_mass) {
                 uint64_t sum = 0;                              // (the second round looks at the row's masses anyway)
 #pragma unroll 1
@@ -850,12 +977,14 @@ int draw_filtered(FilterArgs a, int n_rows, cudaStream_t stream) {
     a.per_block = ((vocab + blocks - 1) / blocks + 3) & ~3;
     a.n_rows = n_rows;
     if (a.per_block <= kMostStaged) {
-        static bool done[kMaxDevices];
-        const int status = ensure_dynamic_smem(sample_filtered_kernel<true>, kMostStaged * 4, done);
+        static bool done[2][kMaxDevices];
+        const auto kernel = a.top_k ? sample_filtered_kernel<true, true> : sample_filtered_kernel<true, false>;
+        const int status = ensure_dynamic_smem(kernel, kMostStaged * 4, done[a.top_k != nullptr]);
         if (status != CPM_OK) return status;
-        cpm_launch_cluster(kLaunchOther, sample_filtered_kernel<true>, dim3(n_rows * blocks), kFilterThreads, (size_t)a.per_block * 4, stream, blocks, a);
+        cpm_launch_cluster(kLaunchOther, kernel, dim3(n_rows * blocks), kFilterThreads, (size_t)a.per_block * 4, stream, blocks, a);
     } else {
-        cpm_launch_cluster(kLaunchOther, sample_filtered_kernel<false>, dim3(n_rows * blocks), kFilterThreads, 0, stream, blocks, a);
+        cpm_launch_cluster(kLaunchOther, a.top_k ? sample_filtered_kernel<false, true> : sample_filtered_kernel<false, false>, dim3(n_rows * blocks), kFilterThreads, 0,
+                           stream, blocks, a);
     }
     return launch_status();
 }
