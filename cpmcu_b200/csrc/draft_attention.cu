@@ -11,6 +11,9 @@
 // 64 rows and not once a token.  A block takes 32 or 64 rows and a share of the pages: scores of 64 keys (a thread: 8 rows of one or two keys), the softmax (a warp: an
 // eighth of the rows), weighted values (a thread: some rows of one channel), all operands in shared memory.  Few rows and many keys: the pages are shared out over blocks, whose
 // parts a second kernel adds up.
+//
+// Bound by FMA and shared memory, and with few rows by the chain of one page: 3 sequences of 300 to 2,500 keys, 7 tokens of 16 heads on 2 of 64 in fp32 take 27 us, of which
+// a page is 10 to 11 (scores 4.7, softmax 2.1, values 3 to 4); the keys and values alone would be a microsecond.  Blocks of 32 rows took 33 us there, of 64 27.
 #include "common.cuh"
 
 CPM_BOUNDS_TU(draft_attention)

@@ -9,8 +9,11 @@
 // The work is a line: every (sequence, tile, key-value head) is a unit of its pages and a few more for its beginning and end, and every block takes a piece of
 // equal cost of that line, so that unequal sequences leave no SM idle.  A unit that several blocks have is put together by a second kernel.
 //
-// Bound by the keys' way from memory (32 KB a page at head size 128) as long as a block's rows are no more than 256: the tensor cores take 512 cycles a page for
-// 128 rows, the softmax some 800, memory 1,390.
+// What bounds it: with 256 rows a block the softmax's chains (a row a thread: 64 scores scaled, raised, added and packed a page; 64 drafted tokens of 32 heads on 2 of 128
+// behind 131,071 keys take 127 to 142 us by the card's clock, 1,020 to 1,140 TFLOP/s; tensor pipe 61 % of the active time, issue slots 52 %, exponentials' unit 46 %).
+// With few rows what surrounds the pages: 64 sequences of 6 to 8,192 keys, 5 tokens, 16 heads on 2 of 64 take 44 us, of which the keys' way from memory is 21, the line and
+// the first page 5, blocks that end at 27 to 38 us, and the parts' addition the rest; 16 trees of 16 tokens behind 500 to 6,000 keys 37 us, 12 pages of 1.08 us a block
+// and 8 us for the parts; one sequence of 1,000 keys 12.5 us, all of it launch, first page and parts.
 //
 // Of the pages that hold the step's own tokens a warp looks at the values before they are multiplied: what lies behind the keys becomes 0, and so does what is no
 // finite number, which is added at the end to the rows that see it (0 times such a value would reach the others).
@@ -28,6 +31,7 @@ constexpr int kMostSeqs = 512;                          // of one launch
 constexpr int kStages = 4;                              // pages under way
 constexpr int kOdd = 8;                                 // segments that half 0 may be ahead of half 1, and more
 constexpr float kBehind = 8.0f;                         // the running maximum may lie 2^8 behind
+// (kExtra of 1 to 4 and kLeast of 1 to 8 differ by less than two boxes do.)
 constexpr int kExtra = 2;                               // pages that a unit's beginning and end are worth
 constexpr int kLeast = 4;                               // cost that a block is worth its part's addition
 // Of four pairs of a row's weights one is formed by ex2_poly (2,048 pages of 256 rows a key-value head, 64 tokens at 131,071 keys: none 140 us, one 127, two 152)

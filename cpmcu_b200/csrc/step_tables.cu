@@ -5,6 +5,7 @@
 // the new tokens need, ceil((l + n) / 64) - ceil(l / 64), come from a list of free ones in the sequences' order.
 // Every block forms both running sums for itself (a few bytes a sequence, out of L2), so that one launch without a barrier between blocks does; a token's
 // depth is a walk over at most 64 parents in shared memory.
+// Bound by the launch and the two passes over the sequences: 64 sequences of 5 tokens 3.1 us, 512 trees of 64 tokens with their pages handed out 5.0 (1 MB written: 0.14 us).
 #include "common.cuh"
 
 namespace {
@@ -158,7 +159,8 @@ step_tables_kernel(const __grid_constant__ TableArgs a) {
 // ---------------------------------------------------------------------------
 // Keys and values of an accepted path.  Token j of it lies at l + path[j] and goes to l + j.  Paths rise, so that path[j] >= j and what a token is written over has
 // been read by a token before it: a block takes one key-value head of one layer and sequence and moves the tokens in groups, read whole before they are written.
-// There is nothing to compute; the floor is every moved byte in and out, of which values, stored transposed, lie two or four bytes in a row.
+// There is nothing to compute; the floor is every moved byte in and out, of which values, stored transposed, lie two or four bytes in a row: each moves 32 bytes both ways.
+// 32 layers of one sequence, 4 tokens of 2 heads of 128: 4.3 us, a launch and the chain of three loads; 24 layers of 64 sequences, 5 tokens of 2 of 64: 12.7 us, 3,072 blocks.
 // ---------------------------------------------------------------------------
 constexpr int kKeepThreads = 128, kKeepLoads = 4, kKeepTensors = 8;
 
