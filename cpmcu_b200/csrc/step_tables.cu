@@ -268,14 +268,19 @@ keep_drafts_kernel(const __grid_constant__ KeptTensors t, const __grid_constant_
 
 }  // namespace
 
-// All tables of one step; ``parents`` and ``ancestors`` together or null; with ``taken`` pages are handed out of ``free``.  Pages beyond the table's width are not written.
+// All tables of one step in ``room``, one behind the other: slot map int64 [tokens], with ``parents`` ancestors int64 [tokens], sequences, positions and places int32
+// [tokens], key counts [seqs], offsets [seqs + 1], and the number of pages wanted from ``free`` [1] (written if there is such a list).  Pages beyond the table's width are not
+// written.
 CPM_API int cpm_step_tables(const int* lengths, const int* fresh, const int* slots, int n_seqs, int n_tokens, int* page_table, int n_slots, int max_pages,
-                            const int* parents, const int* free, int n_free, int* cu, int* kv_len, int* token_seq, int* positions, int* places,
-                            int64_t* slot_map, int64_t* ancestors, int* taken, cudaStream_t stream) {
-    if (n_seqs < 1 || n_seqs > kMostSeqs || n_tokens < 0 || max_pages < 1 || n_free < 0) return CPM_BAD_ARGUMENT;
-    if ((parents == nullptr) != (ancestors == nullptr) || (!free && n_free > 0) || (free && !taken)) return CPM_BAD_ARGUMENT;
-    const TableArgs a{lengths, fresh, slots, parents, free, n_free, n_seqs, n_tokens, n_slots, max_pages, page_table, cu, kv_len, token_seq, positions, places, taken,
-                      slot_map, ancestors};
+                            const int* parents, const int* free, int n_free, int hand_out, void* room, cudaStream_t stream) {
+    if (n_seqs < 1 || n_seqs > kMostSeqs || n_tokens < 0 || max_pages < 1 || n_free < 0 || !room || ((uintptr_t)room & 7)) return CPM_BAD_ARGUMENT;
+    if (!free && n_free > 0) return CPM_BAD_ARGUMENT;
+    int64_t* const slot_map = (int64_t*)room;
+    int64_t* const ancestors = parents ? slot_map + n_tokens : nullptr;
+    int* const token_seq = (int*)(slot_map + (parents ? 2 : 1) * (int64_t)n_tokens);
+    int *const positions = token_seq + n_tokens, *const places = positions + n_tokens, *const kv_len = places + n_tokens, *const cu = kv_len + n_seqs;
+    const TableArgs a{lengths, fresh, slots, parents, free, n_free, n_seqs, n_tokens, n_slots, max_pages, page_table, cu, kv_len, token_seq, positions, places,
+                      hand_out ? cu + n_seqs + 1 : nullptr, slot_map, ancestors};
     const int blocks = (max(n_tokens, n_seqs + 1) + kTableThreads - 1) / kTableThreads;
     cpm_launch(kLaunchOther, step_tables_kernel, dim3(blocks), kTableThreads, (size_t)(n_seqs + 1) * 8, stream, a);
     return launch_status();

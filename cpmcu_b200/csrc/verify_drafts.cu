@@ -17,6 +17,11 @@
 // again); one sequence: 24 us, 15 and 9.  32 trees of 16 tokens, vocabulary 32,000, without probabilities: 76 us, 3 of them this launch.
 #include "filtered.cuh"
 
+// Every row's draw (sample_filtered.cu).
+CPM_API int cpm_sample_drafts(const float* logits, int64_t ld, int n_rows, int vocab, int* token, float* logprob, const float* uniform, const float* temperature,
+                              const int* top_k, const float* top_p, const float* min_p, uint64_t seed, const int* seq_key, const int* step_key,
+                              const int* row_seq, const int* positions, const int* cu, int n_seqs, void* kept, cudaStream_t stream);
+
 namespace {
 
 constexpr int kWarps = 16, kThreads = 32 * (kWarps + 1), kMostBlocks = 8;        // and one that writes the path
@@ -327,14 +332,24 @@ verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
 
 }  // namespace
 
-// ``kept`` and the draws are what cpm_sample_drafts left for the same rows.  tokens, path int32 and logprob fp32 [seqs, most]: the tokens that a step gives, the
-// places of the tokens that stay (the root and the accepted ones), and what is behind ``count`` of them -1, -1 and 0.
-CPM_API int cpm_verify_drafts(const float* logits, int64_t ld, int n_rows, int vocab, const int* ids, const int* cu, int n_seqs, int most, const int* parents,
-                              const float* probs, int64_t ldq, const float* accept, const float* uniform, const float* temperature, const int* drawn,
-                              const float* drawn_logprob, const void* kept, int* tokens, int* count, int* path, float* logprob, cudaStream_t stream) {
+// rows: 8 bytes a row of the logits (its draw and that one's log-probability), with ``probs`` behind 32 (what its filters keep).  out [3][seqs][most]: the tokens that a
+// step gives (int32), the places of the tokens that stay, the root and the accepted ones (int32), and log-probabilities (fp32); what is behind ``count`` of them: -1, -1 and 0.
+CPM_API int cpm_verify_drafts(const float* logits, int64_t ld, int n_rows, int vocab, void* rows, const int* ids, const int* row_seq, const int* cu, int n_seqs, int most,
+                              const int* parents, const float* probs, int64_t ldq, const float* accept, const float* uniform, const float* temperature,
+                              const int* top_k, const float* top_p, const float* min_p, uint64_t seed, const int* seq_key, const int* step_key,
+                              const int* positions, int* out, int* count, cudaStream_t stream) {
     if (n_seqs <= 0) return CPM_OK;
     if (n_rows < 0 || vocab < 1 || most < 1 || most > kMostTokens || n_seqs > 0x7fffffff / kMostBlocks) return CPM_BAD_ARGUMENT;
-    if (probs && (parents || !accept || !uniform || !kept)) return CPM_BAD_ARGUMENT;
+    if ((probs && (parents || !accept || !uniform)) || (!rows && n_rows > 0)) return CPM_BAD_ARGUMENT;
+    KeptRow* const kept = probs ? (KeptRow*)rows : nullptr;
+    int* const drawn = (int*)((char*)rows + (probs ? sizeof(KeptRow) * n_rows : 0));
+    const float* const drawn_logprob = (const float*)(drawn + n_rows);
+    const int status = cpm_sample_drafts(logits, ld, n_rows, vocab, drawn, (float*)(drawn + n_rows), uniform, temperature, top_k, top_p, min_p, seed, seq_key, step_key,
+                                         row_seq, positions, cu, n_seqs, kept, stream);
+    if (status != CPM_OK) return status;
+    int* const tokens = out;
+    int* const path = out + (int64_t)n_seqs * most;
+    float* const logprob = (float*)(out + 2 * (int64_t)n_seqs * most);
     int blocks = 1;
     if (probs) {                                         // as many blocks a sequence as run at the same time, one an SM
         const int sms = device_sms();
@@ -342,7 +357,7 @@ CPM_API int cpm_verify_drafts(const float* logits, int64_t ld, int n_rows, int v
         while (blocks > 1 && ((int64_t)n_seqs * blocks > sms || vocab < 2048 * blocks)) blocks /= 2;
     }
     const int per_block = ((vocab + blocks - 1) / blocks + 3) & ~3;
-    const VerifyArgs a{logits, ld, probs, ldq, accept, uniform, temperature, ids, cu, parents, drawn, drawn_logprob, (const KeptRow*)kept, vocab, per_block,
+    const VerifyArgs a{logits, ld, probs, ldq, accept, uniform, temperature, ids, cu, parents, drawn, drawn_logprob, kept, vocab, per_block,
                        n_rows, most, tokens, count, path, logprob};
     cpm_launch_cluster(kLaunchOther, verify_drafts_kernel, dim3(n_seqs * blocks), probs ? kThreads : 64, 0, stream, blocks, a);
     return launch_status();

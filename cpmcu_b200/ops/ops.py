@@ -1959,12 +1959,9 @@ class Ops:
         words, token_seq, positions, places, kv_len, cu_q, taken = room.split_with_sizes((wide, n_tokens, n_tokens, n_tokens, n_seqs, n_seqs + 1, 1))
         words = words.view(torch.int64)
         slot_map, ancestors = (words, None) if parents is None else words.split_with_sizes((n_tokens, n_tokens))
-        at = room.data_ptr()
-        by_token, by_seq = at + 4 * wide, at + 4 * (wide + 3 * n_tokens)
         check(self.lib.cpm_step_tables(lengths.data_ptr(), new.data_ptr(), slots.data_ptr(), n_seqs, n_tokens, page_table.data_ptr(), page_table.shape[0],
-                                       page_table.shape[1], _ptr(parents), _ptr(free), 0 if free is None else free.numel(), by_seq + 4 * n_seqs, by_seq, by_token,
-                                       by_token + 4 * n_tokens, by_token + 8 * n_tokens, at, None if parents is None or n_tokens == 0 else at + 8 * n_tokens,
-                                       None if free is None else by_seq + 4 * (2 * n_seqs + 1), stream), "step_tables")
+                                       page_table.shape[1], _ptr(parents), _ptr(free), 0 if free is None else free.numel(), free is not None, room.data_ptr(), stream),
+              "step_tables")
         return StepTables(cu_q, kv_len, token_seq, positions, places, slot_map, ancestors, None if free is None else taken)
 
     draft_attention_ran = False          # (without drafted tokens no step waits for its kernel's error)
@@ -2020,8 +2017,8 @@ class Ops:
         if scale > 0 and self.draft_attention_on_tensor_cores(d, n_heads, n_kv):
             scratch = self.empty(self.lib.cpm_draft_attention_scratch_floats(n_heads, n_kv, d, most), dtype=torch.float32)
             self.draft_attention_ran = True
-            check(self.lib.cpm_draft_attention_tcgen05(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
-                                                       width, n_pages, _ptr(ancestors), _ptr(scratch), n, n_seqs, most, n_heads, n_kv, d,
+            check(self.lib.cpm_draft_attention_tcgen05(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), slots.data_ptr(),
+                                                       page_table.data_ptr(), width, n_pages, _ptr(ancestors), scratch.data_ptr(), n, n_seqs, most, n_heads, n_kv, d,
                                                        float(scale), stream), "tcgen05 attention of drafted tokens")
             LAUNCHES_EXTRA[0] += 1       # the pieces, then their addition
             return out
@@ -2093,14 +2090,11 @@ class Ops:
             return tokens, count, path, logprob
         # what every row keeps (32 bytes), the token that it draws, and its log-probability
         rows = self.empty((8 if draft_probs is not None else 0) * n + 2 * n, dtype=i32)
-        kept = rows.data_ptr() if draft_probs is not None else None
-        drawn = rows.data_ptr() + (32 * n if draft_probs is not None else 0)
-        check(self.lib.cpm_sample_drafts(_ptr(logits), vocab, n, vocab, drawn, drawn + 4 * n, _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                                         _ptr(min_p), ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key), _ptr(step_key), _ptr(token_seq), _ptr(positions),
-                                         _ptr(cu_q), n_seqs, kept, stream), "drawing for drafted tokens")
-        check(self.lib.cpm_verify_drafts(_ptr(logits), vocab, n, vocab, _ptr(ids), _ptr(cu_q), n_seqs, most, _ptr(parents), _ptr(draft_probs),
-                                         0 if draft_probs is None else draft_probs.stride(0), _ptr(accept), _ptr(uniform), _ptr(temperature), drawn,
-                                         drawn + 4 * n, kept, _ptr(tokens), _ptr(count), _ptr(path), _ptr(logprob), stream), "verify_drafts")
+        check(self.lib.cpm_verify_drafts(logits.data_ptr(), vocab, n, vocab, rows.data_ptr(), ids.data_ptr(), token_seq.data_ptr(), cu_q.data_ptr(), n_seqs, most,
+                                         _ptr(parents), _ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0), _ptr(accept), _ptr(uniform),
+                                         temperature.data_ptr(), _ptr(top_k), _ptr(top_p), _ptr(min_p), ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(seq_key),
+                                         _ptr(step_key), _ptr(positions), tokens.data_ptr(), count.data_ptr(), stream), f"verify_drafts ({vocab} tokens)")
+        LAUNCHES_EXTRA[0] += 1           # the rows' draws, then the check
         return tokens, count, path, logprob
 
     def keep_drafts(self, pairs, lengths: torch.Tensor, path: torch.Tensor, count: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor) -> None:
