@@ -221,25 +221,38 @@ skinny_gemm_kernel(const bf16* __restrict__ W, const bf16* __restrict__ X, void*
     }
 }
 
+// Loads under way need room in L1, of which an SM has little left after a kernel that took nearly all of its memory as shared memory, and it stays divided so
+// until a kernel asks for something else: a step of 8 tokens through 8 layers of 8B sizes, whose attention of drafted tokens is such a kernel, took 1,387 us, and
+// 946 with this; steps of one token, 837, are as before.  A tenth, 23 KB, is rounded up to 32: an SM's blocks have up to 30 KB of shared memory.  (A quarter: 960 and 842.)
+static void prefer_cache(const void* kernel, bool* done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices || done[dev]) return;
+    done[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 10) == cudaSuccess;
+}
+
 template <int NT, int EPI>
 static int launch_skinny_epi(const void* W, const void* X, void* out, int M, int N, int K, float alpha,
                              const GluClamp& clamp, cudaStream_t stream) {
     const unsigned blocks = (unsigned)((N + 15) / 16), sms = (unsigned)device_sms();
     // per_sm: blocks an SM holds by their registers (128 a thread beyond K 1,024, 64 and 80 with four steps)
-    auto start = [&](auto kern, int warps, unsigned per_sm) {
+    static bool preferred[6][kMaxDevices];
+    auto start = [&](int variant, auto kern, int warps, unsigned per_sm) {
+        prefer_cache((const void*)kern, preferred[variant]);
         cpm_launch(kLaunchProduct, kern, blocks, warps * 32, 0, stream, (const bf16*)W, (const bf16*)X, out, M, N, K, alpha,
                    g_skinny_prefetch_lines, (int)(blocks <= per_sm * sms), clamp);
     };
     if (K >= kManyWarpsK && 2 * blocks <= sms)
-        start(skinny_gemm_kernel<NT, EPI, 16, 8, NT == 1>, 16, 1u);
+        start(0, skinny_gemm_kernel<NT, EPI, 16, 8, NT == 1>, 16, 1u);
     else if (K <= kShortK / 4)
-        start(skinny_gemm_kernel<NT, EPI, 8, 1, true>, 8, NT == 1 ? 4u : 3u);
+        start(1, skinny_gemm_kernel<NT, EPI, 8, 1, true>, 8, NT == 1 ? 4u : 3u);
     else if (K <= kShortK / 2)
-        start(skinny_gemm_kernel<NT, EPI, 8, 2, true>, 8, NT == 1 ? 4u : 3u);
+        start(2, skinny_gemm_kernel<NT, EPI, 8, 2, true>, 8, NT == 1 ? 4u : 3u);
     else if (K <= kShortK)
-        start(skinny_gemm_kernel<NT, EPI, 8, 4, true>, 8, NT == 1 ? 4u : 3u);
+        start(3, skinny_gemm_kernel<NT, EPI, 8, 4, true>, 8, NT == 1 ? 4u : 3u);
+    else if (NT == 1 || K < 2 * kShortK)
+        start(4, skinny_gemm_kernel<NT, EPI, 8, 8, true>, 8, 2u);
     else
-        start(NT == 1 || K < 2 * kShortK ? skinny_gemm_kernel<NT, EPI, 8, 8, true> : skinny_gemm_kernel<NT, EPI, 8, 8, NT == 1>, 8, 2u);
+        start(5, skinny_gemm_kernel<NT, EPI, 8, 8, NT == 1>, 8, 2u);
     return launch_status();
 }
 
