@@ -150,6 +150,7 @@ def build(force: bool = False, verbose: bool = True, check_bounds: bool = False)
         if p.returncode != 0:
             raise BuildError(f"link failed:\n{' '.join(cmd)}\n{p.stdout}\n{p.stderr}")
         os.replace(tmp_lib, os.path.join(out_dir, LIB_NAME))
+        shutil.rmtree(obj_dir, ignore_errors=True)       # (as large as the library, and never used again: a stale library is compiled as a whole)
         with open(os.path.join(out_dir, "fingerprint"), "w") as f:
             f.write(_fingerprint(check_bounds))
     finally:
