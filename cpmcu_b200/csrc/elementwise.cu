@@ -258,15 +258,32 @@ CPM_API int cpm_silu_mul(const void* gu, void* h, int n_tokens, int inter, int i
 // fp32 with the accurate sincosf (src/model/rotary.cuh:6-34 uses the same pairing
 // but the fast-math cos/sin).  cos and sin are multiplied by ``magnitude`` (the
 // LongRoPE attention factor).  inv_freq == nullptr: no rotation.
-// qkv row: [heads*d | kv_heads*d | kv_heads*dv]; dv, the size of a value head, may differ from d.  places: where a token lies in its sequence's
-// cache, if that is not its position (nullptr: it is).
+// qkv row: [heads*d | kv_heads*d | kv_heads*dv]; dv, the size of a value head, may differ from d.
+// AT: a token's place in the cache is not its position (drafted tokens), see StoreAt.
 // ---------------------------------------------------------------------------
 constexpr int kRopeHeadsPerBlock = 4;
 
-template <typename T>
+// Where tokens are stored: ``rows`` are page * kPageTokens + the place in it, or ``places`` lie in the pages of the token's sequence.  A token that has no
+// such row (no sequence, slot, place or page; a row below 0) is not stored, so that room left on the token axis and pages that ran out touch nobody's keys.
+struct StoreAt {
+    const int* places;
+    const int64_t* rows;
+    int n_seqs, n_slots, n_pages;
+};
+__device__ __forceinline__ int64_t row_to_store(const StoreAt& at, int t, const int* token_seq, const int* slots, const int* page_table, int max_pages) {
+    if (at.rows) return at.rows[t] < (int64_t)at.n_pages * kPageTokens ? at.rows[t] : -1;
+    const int seq = token_seq[t], place = at.places[t];
+    if (seq < 0 || seq >= at.n_seqs || place < 0 || place / kPageTokens >= max_pages) return -1;
+    const int slot = slots[seq];
+    if (slot < 0 || slot >= at.n_slots) return -1;
+    const int page = page_table[(int64_t)slot * max_pages + place / kPageTokens];
+    return page >= 0 && page < at.n_pages ? (int64_t)page * kPageTokens + place % kPageTokens : -1;
+}
+
+template <typename T, bool AT>
 __global__ void rope_store_kernel(const T* __restrict__ qkv, T* __restrict__ q_out,
                                   T* __restrict__ k_cache, T* __restrict__ v_cache,
-                                  const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ token_seq,
+                                  const int* __restrict__ positions, const StoreAt at, const int* __restrict__ token_seq,
                                   const int* __restrict__ slots, const int* __restrict__ page_table,
                                   int max_pages, const float* __restrict__ inv_freq, float magnitude,
                                   int n_heads, int n_kv, int d, int rot_dim, int dv) {
@@ -297,16 +314,24 @@ __global__ void rope_store_kernel(const T* __restrict__ qkv, T* __restrict__ q_o
     __syncthreads();
 
     int64_t k_base = 0, v_base = 0;
+    bool stored = true;
     if (k_cache) {
-        const int slot = slots[token_seq[t]];
-        const int place = places ? places[t] : pos;
-        const int page = CPM_PAGE(page_table + (int64_t)slot * max_pages, place / kPageTokens, max_pages);
-        k_base = page_row_offset(page, 0, place % kPageTokens, n_kv, d);
-        v_base = value_offset(page, 0, 0, place % kPageTokens, n_kv, dv);
+        int page, in_page = pos % kPageTokens;
+        if constexpr (AT) {
+            const int64_t to = row_to_store(at, t, token_seq, slots, page_table, max_pages);
+            stored = to >= 0;
+            page = stored ? (int)(to / kPageTokens) : 0;
+            in_page = stored ? (int)(to % kPageTokens) : 0;
+        } else {
+            page = CPM_PAGE(page_table + (int64_t)slots[token_seq[t]] * max_pages, pos / kPageTokens, max_pages);
+        }
+        k_base = page_row_offset(page, 0, in_page, n_kv, d);
+        v_base = value_offset(page, 0, 0, in_page, n_kv, dv);
     }
     const int64_t head_stride_in_page = (int64_t)kPageTokens * d;
     for (int h = h_begin; h < h_end; ++h) {
         const T* src = row + (int64_t)h * d;
+        if (AT && !stored && h >= n_heads) break;
         if (h >= n_heads + n_kv) {                               // a value head: transposed store
             const int kvh = h - n_heads - n_kv;
             src = row + (int64_t)(n_heads + n_kv) * d + (int64_t)kvh * dv;
@@ -331,9 +356,10 @@ __global__ void rope_store_kernel(const T* __restrict__ qkv, T* __restrict__ q_o
 // two 16-byte loads and two 16-byte stores; value heads are copied 16 elements per thread (their store is
 // transposed, one element per 128 bytes).  heads_per_block: all heads of a token for prompts, a few for
 // decode steps, where the tokens alone would not fill the GPU.
+template <bool AT>
 __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __restrict__ q_out,
                                       bf16* __restrict__ k_cache, bf16* __restrict__ v_cache,
-                                      const int* __restrict__ positions, const int* __restrict__ places, const int* __restrict__ token_seq,
+                                      const int* __restrict__ positions, const StoreAt at, const int* __restrict__ token_seq,
                                       const int* __restrict__ slots, const int* __restrict__ page_table,
                                       int max_pages, const float* __restrict__ inv_freq, float magnitude,
                                       int n_heads, int n_kv, int d, int heads_per_block) {
@@ -364,12 +390,19 @@ __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __rest
     }
 
     int64_t k_base = 0, v_base = 0;
+    bool stored = true;
     if (k_cache && h_end > n_heads) {                            // only blocks with key or value heads look the page up
-        const int slot = slots[token_seq[t]];
-        const int place = places ? places[t] : pos;
-        const int page = CPM_PAGE(page_table + (int64_t)slot * max_pages, place / kPageTokens, max_pages);
-        k_base = page_row_offset(page, 0, place % kPageTokens, n_kv, d);
-        v_base = value_offset(page, 0, 0, place % kPageTokens, n_kv, d);
+        int page, in_page = pos % kPageTokens;
+        if constexpr (AT) {
+            const int64_t to = row_to_store(at, t, token_seq, slots, page_table, max_pages);
+            stored = to >= 0;
+            page = stored ? (int)(to / kPageTokens) : 0;
+            in_page = stored ? (int)(to % kPageTokens) : 0;
+        } else {
+            page = CPM_PAGE(page_table + (int64_t)slots[token_seq[t]] * max_pages, pos / kPageTokens, max_pages);
+        }
+        k_base = page_row_offset(page, 0, in_page, n_kv, d);
+        v_base = value_offset(page, 0, 0, in_page, n_kv, d);
     }
     __syncthreads();
     pdl_wait();
@@ -378,6 +411,7 @@ __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __rest
     for (int item = threadIdx.x; item < items; item += blockDim.x) {
         const int h = h_begin + item / per_head, part = item % per_head;
         const bf16* src = row + (int64_t)h * d;
+        if (AT && !stored && h >= n_heads) break;                // (a thread's items come by head)
         if (h >= n_heads + n_kv) {                               // a value head: transposed store
             const int kvh = h - n_heads - n_kv;
             const uint4 a = *reinterpret_cast<const uint4*>(src + 16 * part);
@@ -417,7 +451,8 @@ __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __rest
 }
 
 // ``dv``: the size of a value head (the value pages are [kv_head][dv][token]).
-static int rope_store(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions, const int* places,
+template <bool AT>
+static int rope_store(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions, const StoreAt& at,
                       const int* token_seq, const int* slots, const int* page_table, int max_pages,
                       const float* inv_freq, float magnitude, int n_tokens, int n_heads, int n_kv, int d,
                       int dv, int rot_dim, int dtype, cudaStream_t stream) {
@@ -432,8 +467,8 @@ static int rope_store(const void* qkv, void* q_out, void* k_cache, void* v_cache
         const int threads = items >= 256 ? 256 : ((items + 31) / 32) * 32;
         dim3 vgrid(n_tokens, (n_all + heads_per_block - 1) / heads_per_block);
         if (vgrid.y > 65535) return CPM_BAD_ARGUMENT;
-        cpm_launch(kLaunchRope, rope_store_vec_kernel, vgrid, threads, (size_t)d * sizeof(float), stream, (const bf16*)qkv, (bf16*)q_out,
-                   (bf16*)k_cache, (bf16*)v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude,
+        cpm_launch(kLaunchRope, rope_store_vec_kernel<AT>, vgrid, threads, (size_t)d * sizeof(float), stream, (const bf16*)qkv, (bf16*)q_out,
+                   (bf16*)k_cache, (bf16*)v_cache, positions, at, token_seq, slots, page_table, max_pages, inv_freq, magnitude,
                    n_heads, n_kv, d, heads_per_block);
         return launch_status();
     }
@@ -442,11 +477,11 @@ static int rope_store(const void* qkv, void* q_out, void* k_cache, void* v_cache
     const int threads = d >= 128 ? 64 : 32;
     const size_t smem = (size_t)(rot_dim > 0 ? rot_dim : 2) * sizeof(float);
     if (dtype == CPM_BF16)
-        cpm_launch(kLaunchRope, rope_store_kernel<bf16>, grid, threads, smem, stream, (const bf16*)qkv, (bf16*)q_out, (bf16*)k_cache,
-            (bf16*)v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
+        cpm_launch(kLaunchRope, rope_store_kernel<bf16, AT>, grid, threads, smem, stream, (const bf16*)qkv, (bf16*)q_out, (bf16*)k_cache,
+            (bf16*)v_cache, positions, at, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
     else
-        cpm_launch(kLaunchRope, rope_store_kernel<float>, grid, threads, smem, stream, (const float*)qkv, (float*)q_out, (float*)k_cache,
-            (float*)v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
+        cpm_launch(kLaunchRope, rope_store_kernel<float, AT>, grid, threads, smem, stream, (const float*)qkv, (float*)q_out, (float*)k_cache,
+            (float*)v_cache, positions, at, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_heads, n_kv, d, rot_dim, dv);
     return launch_status();
 }
 
@@ -454,17 +489,19 @@ CPM_API int cpm_rope_store_dv(const void* qkv, void* q_out, void* k_cache, void*
                               const int* token_seq, const int* slots, const int* page_table, int max_pages,
                               const float* inv_freq, float magnitude, int n_tokens, int n_heads, int n_kv, int d,
                               int dv, int rot_dim, int dtype, cudaStream_t stream) {
-    return rope_store(qkv, q_out, k_cache, v_cache, positions, nullptr, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_tokens, n_heads, n_kv, d,
-                      dv, rot_dim, dtype, stream);
+    return rope_store<false>(qkv, q_out, k_cache, v_cache, positions, StoreAt{}, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_tokens, n_heads,
+                             n_kv, d, dv, rot_dim, dtype, stream);
 }
 
-// Tokens whose place in the cache is not their position (a tree of drafted tokens).
-CPM_API int cpm_rope_store_at(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions, const int* places,
-                              const int* token_seq, const int* slots, const int* page_table, int max_pages,
+// Tokens whose place in the cache is not their position (a tree of drafted tokens): ``places`` in the pages of n_seqs sequences in n_slots rows of the page
+// table, or ``rows`` of the cache of n_pages pages.
+CPM_API int cpm_rope_store_at(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions, const int* places, const int64_t* rows,
+                              const int* token_seq, const int* slots, const int* page_table, int n_seqs, int n_slots, int max_pages, int n_pages,
                               const float* inv_freq, float magnitude, int n_tokens, int n_heads, int n_kv, int d,
                               int rot_dim, int dtype, cudaStream_t stream) {
-    return rope_store(qkv, q_out, k_cache, v_cache, positions, places, token_seq, slots, page_table, max_pages, inv_freq, magnitude, n_tokens, n_heads, n_kv, d,
-                      d, rot_dim, dtype, stream);
+    if (!places && !rows) return CPM_BAD_ARGUMENT;
+    return rope_store<true>(qkv, q_out, k_cache, v_cache, positions, StoreAt{places, rows, n_seqs, n_slots, n_pages}, token_seq, slots, page_table, max_pages, inv_freq,
+                            magnitude, n_tokens, n_heads, n_kv, d, d, rot_dim, dtype, stream);
 }
 
 CPM_API int cpm_rope_store(const void* qkv, void* q_out, void* k_cache, void* v_cache, const int* positions,

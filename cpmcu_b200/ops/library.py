@@ -30,8 +30,8 @@ _SIGNATURES = {
     "cpm_gemm_skinny_bf16": [_P, _P, _P, c_int, c_int, c_int, c_float, c_int, c_float, c_float, c_float, _P],
     "cpm_rope_store": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, _P, c_float, c_int, c_int, c_int, c_int, c_int,
                        c_int, _P],
-    "cpm_rope_store_at": [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, _P, c_float, c_int, c_int, c_int, c_int, c_int,
-                          c_int, _P],
+    "cpm_rope_store_at": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, c_float, c_int, c_int, c_int, c_int,
+                          c_int, c_int, _P],
     "cpm_attention_generic": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_int,
                               c_int, c_int, c_float, c_int, _P],
     "cpm_gemm_f32": [_P, _P, _P, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_float, _P],

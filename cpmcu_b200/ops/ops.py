@@ -711,10 +711,12 @@ class Ops:
                    token_seq: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor,
                    k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
                    inv_freq: Optional[torch.Tensor], magnitude: float, rot_dim: int,
-                   places: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   places: Optional[torch.Tensor] = None, slot_map: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Rotates q and k of qkv [tokens, (heads+2*kv)*d], stores k and v into the cache pages of
         each token's sequence, and returns the rotated q [tokens, heads, d].  ``places`` int32 [tokens]: where a token lies in its sequence's
-        cache (None: at its position)."""
+        cache (None: at its position).  ``slot_map`` int64 [tokens] instead: the rows of the cache that tokens are stored at, page * PAGE_TOKENS + place in it,
+        as ``step_tables`` gives them.  With either a token that has no row (no sequence, slot or place, or a page that is none; a row of -1) is not stored.
+        ``places`` find their pages in the table, which still has earlier pages where ``step_tables`` had too few to hand out; its slot map has -1 there."""
         self._act(qkv, "qkv")
         n = qkv.shape[0]
         if qkv.shape[1] != (n_heads + 2 * n_kv) * d:
@@ -727,12 +729,20 @@ class Ops:
             self._act(k_cache, "key cache")
             self._act(v_cache, "value cache")
         q = self.empty(n, n_heads, d)
-        if places is not None:
-            self._i32(places, "places")
-            if places.numel() != n:
-                raise ValueError(f"places: need one number a token, got {places.numel()} for {n}")
-            check(self.lib.cpm_rope_store_at(_ptr(qkv), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(positions), _ptr(places),
-                                             _ptr(token_seq), _ptr(slots), _ptr(page_table), page_table.shape[1],
+        if places is not None or slot_map is not None:
+            if places is not None and slot_map is not None:
+                raise ValueError("tokens are stored at places of their sequences or at rows of the cache, not both")
+            for t, what in ((positions, "positions"), (token_seq, "token sequences"), (places, "places")):
+                if t is not None and self._i32(t, what).numel() != n:
+                    raise ValueError(f"{what}: need one number a token, got {t.numel()} for {n}")
+            if slot_map is not None:
+                self._given(slot_map, torch.int64, "slot map", n)
+            n_pages = 0 if k_cache is None else k_cache.shape[0]
+            if k_cache is not None and (k_cache.shape != (n_pages, n_kv, PAGE_TOKENS, d) or v_cache.shape != (n_pages, n_kv, d, PAGE_TOKENS)):
+                raise ValueError(f"caches: need keys [pages, {n_kv}, {PAGE_TOKENS}, {d}] and values [pages, {n_kv}, {d}, {PAGE_TOKENS}], got {tuple(k_cache.shape)} "
+                                 f"and {tuple(v_cache.shape)}")
+            check(self.lib.cpm_rope_store_at(_ptr(qkv), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(positions), _ptr(places), _ptr(slot_map),
+                                             _ptr(token_seq), _ptr(slots), _ptr(page_table), slots.numel(), page_table.shape[0], page_table.shape[1], n_pages,
                                              _ptr(inv_freq), float(magnitude), n, n_heads, n_kv, d, rot_dim, self.code,
                                              self._stream()), "rope_store_at")
             return q

@@ -1,0 +1,90 @@
+"""Operators of drafted tokens put together as their documentation allows: room left on the token axis, too few pages, sequences without keys."""
+import pytest
+import torch
+
+from tests.test_gpu_drafts import DT, PAGE, _i32, _ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _short_step(ops, dtype, d, room=5):
+    """Three sequences of which the free list has pages for the first alone, the second having some of its tokens' places and the third none, and ``room`` more tokens
+    than they bring.  The table's columns behind what a sequence holds name pages of others.  Returns the tables, the rows of the tokens that are to be stored
+    (token, page, place), and what ``rope_store`` takes."""
+    lengths, new = [64, 100, 128], [3, 70, 4]
+    table = torch.tensor([[5, 0, 1], [2, 3, 5], [7, 8, 2]], dtype=torch.int32)          # (sequence 2's slot is 0)
+    slots = [1, 2, 0]
+    n = sum(new) + room
+    on_device = table.cuda()
+    free = _i32([9])
+    tables = ops.step_tables(_i32(lengths), _i32(new), _i32(slots), on_device, n, free=free)
+    rows, t = [], 0
+    for s, (held, count) in enumerate(zip(lengths, new)):
+        for i in range(count):
+            place = held + i
+            if s == 0:
+                rows.append((t, 9, place % PAGE))
+            elif place // PAGE < (held + PAGE - 1) // PAGE:
+                rows.append((t, int(table[slots[s], place // PAGE]), place % PAGE))
+            t += 1
+    g = torch.Generator().manual_seed(d)
+    qkv = torch.randn(n, 8 * d, generator=g).to(DT[dtype]).cuda()
+    k = torch.randn(10, 2, PAGE, d, generator=g).to(DT[dtype]).cuda()
+    v = torch.randn(10, 2, d, PAGE, generator=g).to(DT[dtype]).cuda()
+    return tables, rows, dict(qkv=qkv, n_heads=4, n_kv=2, d=d, positions=tables.positions, token_seq=tables.token_seq, slots=_i32(slots), page_table=on_device, k_cache=k,
+                              v_cache=v, inv_freq=None, magnitude=1.0, rot_dim=d)
+
+
+def _stored(k, v, qkv, rows, d):
+    """The caches with the tokens' own keys and values (which are not turned) at their rows."""
+    k, v = k.clone(), v.clone()
+    for t, page, place in rows:
+        k[page, :, place] = qkv[t, 4 * d:6 * d].view(2, d)
+        v[page, :, :, place] = qkv[t, 6 * d:].view(2, d)
+    return k, v
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 20])
+def test_what_has_no_page_is_not_stored(dtype, d):
+    """By the slot map, tokens of no sequence and of sequences that got no pages leave every other row of the cache as it was."""
+    ops = _ops(dtype)
+    tables, rows, args = _short_step(ops, dtype, d)
+    assert tables.taken.tolist() == [3] and len(rows) == 3 + 28 and tables.slot_map.tolist().count(-1) == 82 - len(rows)
+    want = _stored(args["k_cache"], args["v_cache"], args["qkv"], rows, d)
+    q = ops.rope_store(**args, slot_map=tables.slot_map)
+    assert torch.equal(args["k_cache"], want[0]) and torch.equal(args["v_cache"], want[1])
+    assert torch.equal(q[:77], args["qkv"][:77, :4 * d].view(77, 4, d))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 20])
+def test_tokens_of_no_sequence_are_not_stored_at_places(dtype, d):
+    """Room behind the last sequence, as ``step_tables`` describes it, and places, slots and pages that are none."""
+    ops = _ops(dtype)
+    table = _i32([[5, 0], [2, 3], [-1, 40]])
+    got = ops.step_tables(_i32([64, 10]), _i32([3, 2]), _i32([1, 0]), table, 9)
+    g = torch.Generator().manual_seed(d)
+    qkv = torch.randn(9, 8 * d, generator=g).to(DT[dtype]).cuda()
+    k = torch.randn(10, 2, PAGE, d, generator=g).to(DT[dtype]).cuda()
+    v = torch.randn(10, 2, d, PAGE, generator=g).to(DT[dtype]).cuda()
+    args = dict(n_heads=4, n_kv=2, d=d, page_table=table, inv_freq=None, magnitude=1.0, rot_dim=d)
+    want = _stored(k, v, qkv, [(0, 3, 0), (1, 3, 1), (2, 3, 2), (3, 5, 10), (4, 5, 11)], d)
+    ops.rope_store(qkv=qkv, positions=got.positions, token_seq=got.token_seq, slots=_i32([1, 0]), k_cache=k, v_cache=v, places=got.places, **args)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    # sequences, slots, places and pages that are none
+    seq, places = _i32([0, 0, 1, 2, 3, 4, 5, -7, 0]), _i32([128, -1, 3, 3, 70, 3, 3, 3, 2 ** 31 - 1])
+    ops.rope_store(qkv=qkv, positions=_i32([0] * 9), token_seq=seq, slots=_i32([0, -1, 3, 2, 2]), k_cache=k, v_cache=v, places=places, **args)
+    ops.rope_store(qkv=qkv, positions=_i32([0] * 9), token_seq=_i32([0] * 9), slots=_i32([0]), k_cache=k, v_cache=v,
+                   slot_map=torch.tensor([-1, 640, 2 ** 40, -2 ** 62, -64, 641, 1000, -1, -1]).cuda(), **args)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_refusals_of_storing_at_rows():
+    ops = _ops("bfloat16")
+    tables, _, args = _short_step(ops, "bfloat16", 64)
+    for bad in (dict(slot_map=tables.slot_map[:5]), dict(slot_map=tables.places), dict(slot_map=tables.slot_map.cpu()), dict(slot_map=tables.slot_map, places=tables.places),
+                dict(slot_map=tables.slot_map, positions=tables.positions[:7].contiguous()), dict(places=tables.places, token_seq=tables.token_seq.long()),
+                dict(slot_map=tables.slot_map, k_cache=args["k_cache"][:, :, :32].contiguous()), dict(places=tables.places, v_cache=args["v_cache"][:9])):
+        with pytest.raises(ValueError):
+            ops.rope_store(**{**args, **bad})
