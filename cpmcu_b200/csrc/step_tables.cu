@@ -176,6 +176,9 @@ struct KeptTensors {
 struct KeepArgs {
     const int *lengths, *path, *count, *slots, *page_table;
     int n_slots, max_pages, most;
+    const int64_t* rows;                                 // where the step's tokens lie, by token (below 0: nowhere); null: where the page table says
+    const int* cu;
+    int n_tokens;
 };
 
 template <typename K, typename V>
@@ -196,7 +199,16 @@ keep_drafts_kernel(const __grid_constant__ KeptTensors t, const __grid_constant_
         int64_t src = -1, dst = -1;
         const int x = j < n ? a.path[(int64_t)s * a.most + j] : j;
         const int slot = a.slots[s];
-        if (j < n && x > j && slot >= 0 && slot < a.n_slots) {
+        if (a.rows) {
+            const int first = max(0, a.cu[s]), end = min(a.cu[s + 1], a.n_tokens);
+            if (j < n && x > j && x < end - first) {         // (and so j)
+                const int64_t b = a.rows[first + x], c = a.rows[first + j], rows = (int64_t)p.pages * kPageTokens;
+                if (b >= 0 && b < rows && c >= 0 && c < rows) {
+                    src = b;
+                    dst = c;
+                }
+            }
+        } else if (j < n && x > j && slot >= 0 && slot < a.n_slots) {
             const int* table = a.page_table + (int64_t)slot * a.max_pages;
             const int64_t b = (int64_t)a.lengths[s] + x, c = (int64_t)a.lengths[s] + j;
             if (b / kPageTokens < a.max_pages && c >= 0) {
@@ -287,9 +299,9 @@ CPM_API int cpm_step_tables(const int* lengths, const int* fresh, const int* slo
 }
 
 // pairs: n times {keys, values or 0, bytes of a layer's keys, of its values, layers, pages, key-value heads, bytes of a key, value channels}, each a 64-bit number.
-// ``element``: bytes of a number.
+// ``element``: bytes of a number.  ``rows`` with ``cu`` and n_tokens, or null: see KeepArgs.
 CPM_API int cpm_keep_drafts(const int64_t* pairs, int n_pairs, int element, const int* lengths, const int* path, const int* count, const int* slots,
-                            const int* page_table, int n_slots, int max_pages, int n_seqs, int most, cudaStream_t stream) {
+                            const int* page_table, int n_slots, int max_pages, int n_seqs, int most, const int64_t* rows, const int* cu, int n_tokens, cudaStream_t stream) {
     if (n_pairs < 0 || n_pairs > kKeepTensors || n_seqs < 0 || n_seqs > 65535 || most < 1 || most > kTreeTokens || max_pages < 1) return CPM_BAD_ARGUMENT;
     if (element != 2 && element != 4) return CPM_BAD_ARGUMENT;
     if (n_seqs == 0 || most == 1) return CPM_OK;
@@ -306,7 +318,8 @@ CPM_API int cpm_keep_drafts(const int64_t* pairs, int n_pairs, int element, cons
     }
     if (units == 0) return CPM_OK;
     t.n = n_pairs;
-    const KeepArgs a{lengths, path, count, slots, page_table, n_slots, max_pages, most};
+    if (rows && !cu) return CPM_BAD_ARGUMENT;
+    const KeepArgs a{lengths, path, count, slots, page_table, n_slots, max_pages, most, rows, cu, n_tokens};
     const dim3 grid((unsigned)units, n_seqs);
     const bool whole = (bits & 15) == 0;                 // keys that begin and end on 16 bytes
     if (element == 2) {

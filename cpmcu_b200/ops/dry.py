@@ -133,7 +133,7 @@ class DryOps(Ops):
     def set_page_limit(self, n_pages):
         pass
 
-    def keep_drafts(self, pairs, lengths, path, count, slots, page_table):
+    def keep_drafts(self, pairs, lengths, path, count, slots, page_table, slot_map=None, cu_q=None):
         pass
 
     def _library_bmm(self, a, w, c):          # (the fp32 form has no kernel for tensors without storage)

@@ -129,7 +129,7 @@ _SIGNATURES = {
     "cpm_sample_filtered": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P, _P],
     "cpm_verify_drafts": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int64, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P, _P, _P, _P],
     "cpm_step_tables": [_P, _P, _P, c_int, c_int, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P],
-    "cpm_keep_drafts": [_P, c_int, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P],
+    "cpm_keep_drafts": [_P, c_int, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _P],
     "cpm_draft_attention_generic": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_float, c_int, _P],
     "cpm_draft_attention_tcgen05": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],

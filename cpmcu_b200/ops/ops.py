@@ -1946,8 +1946,9 @@ class Ops:
         page table and brings ``new[s]`` (none is allowed), ``n_tokens`` is what the token axis has room for.  ``parents`` int32 [n_tokens]: a token's parent among
         its sequence's new ones, which comes before it (anything else: none); tokens of a tree stand at the position of their depth, and their ancestors are the
         bits of a word, for sequences of up to MOST_DRAFTS new tokens.  ``free`` int32: pages that may be taken; those that the new tokens need are written into the
-        table in the sequences' order, and ``taken`` says how many were wanted.  A sequence whose pages are not all there gets none; pages beyond the
-        table's width are not written."""
+        table in the sequences' order, and ``taken`` says how many were wanted.  A sequence whose pages are not all there gets none, and the
+        table stays as it was: give the slot map to ``rope_store`` and ``keep_drafts``, which then leave its tokens out (the results of its own rows mean nothing).  Pages
+        beyond the table's width are not written."""
         n_seqs, i32 = lengths.numel(), torch.int32
         for t, what in ((lengths, "lengths"), (new, "new tokens"), (slots, "slots")):
             self._given(t, i32, what, n_seqs)
@@ -2107,11 +2108,13 @@ class Ops:
         LAUNCHES_EXTRA[0] += 1           # the rows' draws, then the check
         return tokens, count, path, logprob
 
-    def keep_drafts(self, pairs, lengths: torch.Tensor, path: torch.Tensor, count: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor) -> None:
+    def keep_drafts(self, pairs, lengths: torch.Tensor, path: torch.Tensor, count: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor,
+                    slot_map: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None) -> None:
         """Moves the keys and values of accepted tokens to where their sequences go on, in one launch: of sequence s, which held ``lengths[s]`` tokens before the step, the
         token that lies at lengths[s] + path[s][j] goes to lengths[s] + j, for j below count[s], in all layers of every pair (k [layers, pages, kv, PAGE_TOKENS, d],
         v [layers, pages, kv, dv, PAGE_TOKENS] or None).  ``path`` int32 [seqs, most] rises along a row, as ``verify_drafts`` gives it.  A place that is in no
-        page of a tensor is left out."""
+        page of a tensor is left out.  The page table says where places lie, or with ``slot_map`` and ``cu_q`` (both as ``step_tables`` gives them) the rows of the step's
+        tokens: what to give after a step whose ``free`` pages may have been too few, since the table still has earlier pages in the place of those."""
         i32 = torch.int32
         self._given(path, i32, "path")
         if path.dim() != 2:
@@ -2124,6 +2127,11 @@ class Ops:
         self._given(page_table, i32, "page table")
         if page_table.dim() != 2 or page_table.numel() == 0:
             raise ValueError("page table: needs [slots, pages]")
+        if (slot_map is None) != (cu_q is None):
+            raise ValueError("a slot map goes with the tokens' offsets")
+        if slot_map is not None:
+            self._given(slot_map, torch.int64, "slot map")
+            self._given(cu_q, i32, "token offsets", n_seqs + 1)
         by_size = {}
         for k, v in pairs:
             for t, what in ((k, "keys"), (v, "values")):
@@ -2147,7 +2155,8 @@ class Ops:
             for i in range(0, len(words), self.COPY_TENSORS):
                 part = [x for w in words[i:i + self.COPY_TENSORS] for x in w]
                 check(self.lib.cpm_keep_drafts((ctypes.c_int64 * len(part))(*part), len(part) // 9, element, _ptr(lengths), _ptr(path), _ptr(count), _ptr(slots),
-                                               _ptr(page_table), page_table.shape[0], page_table.shape[1], n_seqs, path.shape[1], stream), "keep_drafts")
+                                               _ptr(page_table), page_table.shape[0], page_table.shape[1], n_seqs, path.shape[1], _ptr(slot_map), _ptr(cu_q),
+                                               0 if slot_map is None else slot_map.numel(), stream), "keep_drafts")
 
 
 LAUNCHES_EXTRA = library.LAUNCHES

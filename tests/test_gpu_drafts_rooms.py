@@ -88,3 +88,53 @@ def test_refusals_of_storing_at_rows():
                 dict(slot_map=tables.slot_map, k_cache=args["k_cache"][:, :, :32].contiguous()), dict(places=tables.places, v_cache=args["v_cache"][:9])):
         with pytest.raises(ValueError):
             ops.rope_store(**{**args, **bad})
+
+
+def test_accepted_tokens_without_pages_move_nothing():
+    """After a step with too few pages: the table's columns behind what a sequence holds name others' pages, which accepted tokens must not be moved in."""
+    ops = _ops("bfloat16")
+    tables, rows, args = _short_step(ops, "bfloat16", 64)
+    k, v = args["k_cache"][None].contiguous(), args["v_cache"][None].contiguous()
+    want_k, want_v = k.clone(), v.clone()
+    # the second's accepted tokens lie in its own page and behind it, the third's all behind it
+    path, count = [[0, 2, -1, -1], [0, 3, 27, 60], [0, 1, 3, -1]], [2, 4, 3]
+    where = {t: (page, place) for t, page, place in rows}
+    for first, accepted, n in zip((0, 3, 73), path, count):
+        for j in range(n):
+            if first + accepted[j] in where and first + j in where:
+                (a, x), (b, y) = where[first + accepted[j]], where[first + j]
+                want_k[0, b, :, y] = want_k[0, a, :, x].clone()
+                want_v[0, b, :, :, y] = want_v[0, a, :, :, x].clone()
+    assert not torch.equal(k, want_k)
+    ops.keep_drafts([(k, v)], _i32([64, 100, 128]), _i32(path), _i32(count), args["slots"], args["page_table"], slot_map=tables.slot_map, cu_q=tables.cu_q)
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+    # places behind a sequence's own tokens, and offsets behind the slot map
+    ops.keep_drafts([(k, v)], _i32([64, 100, 128]), _i32([[0, 3], [0, 75], [0, 63]]), _i32([2, 2, 2]), args["slots"], args["page_table"], slot_map=tables.slot_map[:74].contiguous(),
+                    cu_q=tables.cu_q)
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+    more = dict(pairs=[(k, v)], lengths=_i32([64]), path=_i32([[0, 1]]), count=_i32([2]), slots=_i32([0]), page_table=args["page_table"])
+    for bad in (dict(slot_map=tables.slot_map), dict(cu_q=_i32([0, 3])), dict(slot_map=tables.slot_map.int(), cu_q=_i32([0, 3])), dict(slot_map=tables.slot_map, cu_q=_i32([0]))):
+        with pytest.raises(ValueError):
+            ops.keep_drafts(**more, **bad)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_accepted_tokens_move_by_the_slot_map_as_by_the_table(dtype):
+    ops = _ops(dtype)
+    g = torch.Generator().manual_seed(3)
+    held, new = [0, 60, 127, 500], [64, 30, 20, 7]
+    pages = torch.randperm(24, generator=g).int()
+    table = torch.cat((pages[:20].view(4, 5), pages[20:].expand(4, 4)), 1)               # (one sequence alone has more than five)
+    slots = [2, 0, 3, 1]
+    path, counts = torch.full((4, 64), -1, dtype=torch.int32), [40, 30, 3, 5]
+    for s, c in enumerate(counts):
+        path[s, 1:c] = (torch.randperm(new[s] - 1, generator=g)[:c - 1] + 1).sort().values.int()
+        path[s, 0] = 0
+    on_device = table.contiguous().cuda()
+    tables = ops.step_tables(_i32(held), _i32(new), _i32(slots), on_device, sum(new) + 2)
+    make = lambda *shape: torch.randn(2, 24, 2, *shape, generator=torch.Generator().manual_seed(8)).to(DT[dtype]).cuda()  # noqa: E731
+    (k, v), (k1, v1) = (make(PAGE, 32), make(32, PAGE)), (make(PAGE, 32), make(32, PAGE))
+    args = (_i32(held), path.cuda(), _i32(counts), _i32(slots), on_device)
+    ops.keep_drafts([(k, v)], *args)
+    ops.keep_drafts([(k1, v1)], *args, slot_map=tables.slot_map, cu_q=tables.cu_q)
+    assert torch.equal(k, k1) and torch.equal(v, v1) and not torch.equal(k, make(PAGE, 32))
