@@ -186,7 +186,8 @@ __device__ __forceinline__ float2 turn_pair(float x, float y, float cs, float sn
 // this one begin its own launch.  Both are no-ops for a kernel launched the ordinary way.
 // Since a kernel may start as soon as the one ahead has been let go, and that one as soon as the one before it, what is read before
 // pdl_wait() has to be older than the step: weights; the step's description (positions, lengths, offsets, slots, page tables); pages and states
-// that earlier steps wrote.  (The one exception, an expert product that reads the choice of experts, says why.)  What keeps
+// that earlier steps wrote.  (The one exception, an expert product that reads the choice of experts, says why.)  The description of a step of drafted tokens is not:
+// step_tables_kernel writes it within the step, and what takes it (rope_store at places, the attention of drafted tokens, their check) waits first.  What keeps
 // this true at the border of two steps is advance_decode_kernel, the last of a decode step: it lets nothing go before it has
 // waited and written the next step's description, whatever the mask below.  Steps from the host begin with copies, which nothing overtakes.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -366,7 +366,9 @@ __global__ void rope_store_vec_kernel(const bf16* __restrict__ qkv, bf16* __rest
     extern __shared__ float cs_table[];       // cos[half], sin[half] of this token
     pdl_launch_dependents();
     // Positions, slots and page tables were written before this step's kernels began; the angles and the page are
-    // worked out from them while the product ahead of this kernel is still finishing.  Only qkv needs the wait.
+    // worked out from them while the product ahead of this kernel is still finishing.  Only qkv needs the wait.  A step of drafted tokens
+    // writes its description itself (step_tables_kernel), so there everything does.
+    if constexpr (AT) pdl_wait();
     const int t = blockIdx.x;
     const int pos = positions[t];
     const int half = d >> 1;

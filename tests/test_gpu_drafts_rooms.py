@@ -138,3 +138,40 @@ def test_accepted_tokens_move_by_the_slot_map_as_by_the_table(dtype):
     ops.keep_drafts([(k, v)], *args)
     ops.keep_drafts([(k1, v1)], *args, slot_map=tables.slot_map, cu_q=tables.cu_q)
     assert torch.equal(k, k1) and torch.equal(v, v1) and not torch.equal(k, make(PAGE, 32))
+
+
+@pytest.mark.parametrize("mask", [None, 63])
+@pytest.mark.parametrize("d", [64, 128, 48])
+def test_tables_and_storing_launched_one_behind_the_other(mask, d):
+    """The description that a step makes itself is there when its tokens are turned and stored, whichever kernels may start early; another description each time, in the
+    same tensors."""
+    ops = _ops("bfloat16")
+    g = torch.Generator().manual_seed(d)
+    n_seqs, most, heads = 512, 8, 2
+    n, pages = n_seqs * most, n_seqs * 4
+    table = torch.randperm(pages, generator=g).view(n_seqs, 4).int().cuda()
+    slots, new = _i32(list(range(n_seqs))), _i32([most] * n_seqs)
+    qkv = torch.randn(n, 3 * heads * d, generator=g).bfloat16().cuda()
+    room = torch.zeros(wide := 4 * n + 3 * n + 2 * n_seqs + 2, dtype=torch.int32).cuda()
+    ops.empty, make = (lambda *shape, **kw: room if shape == (wide,) else make(*shape, **kw)), ops.empty
+    inv_freq = (1.0 / 10000.0 ** (torch.arange(0, d, 2).float() / d)).cuda()
+    shape = (pages, heads, PAGE, d), (pages, heads, d, PAGE)
+    parents = _i32([-1, 0, 0, 1, 1, 2, 3, 4] * n_seqs)
+    try:
+        if mask is not None:
+            ops.lib.cpm_set_pdl(mask)
+        for turn in range(12):
+            lengths = torch.randint(0, 240, (n_seqs,), generator=g).int().cuda()
+            k, v = torch.zeros(shape[0], dtype=torch.bfloat16, device="cuda"), torch.zeros(shape[1], dtype=torch.bfloat16, device="cuda")
+            room.fill_(0)
+            t = ops.step_tables(lengths, new, slots, table, n, parents=parents)
+            q = ops.rope_store(qkv, heads, heads, d, t.positions, t.token_seq, slots, table, k, v, inv_freq, 1.0, d, places=t.places)
+            torch.cuda.synchronize()
+            # the same with everything of the description in place
+            k1, v1 = torch.zeros_like(k), torch.zeros_like(v)
+            positions, seq, places = t.positions.clone(), t.token_seq.clone(), t.places.clone()
+            torch.cuda.synchronize()
+            q1 = ops.rope_store(qkv, heads, heads, d, positions, seq, slots, table, k1, v1, inv_freq, 1.0, d, places=places)
+            assert torch.equal(places.view(n_seqs, most)[:, 0], lengths) and torch.equal(q, q1) and torch.equal(k, k1) and torch.equal(v, v1), turn
+    finally:
+        ops.lib.cpm_set_pdl(-1)
