@@ -3,7 +3,7 @@
 //     o_t = sum_j p_j v_j,  p = softmax over the keys j that token t sees of  q_t . k_j * scale
 //
 // A sequence of kv_len keys brings its last n tokens at once.  A token sees every key before them, and of the n either those up to itself or those whose bit is
-// set in its word of 64 (its ancestors in a tree of drafted tokens, and itself).  A row that sees nothing gives zeros.  What a key holds that a row does not see
+// set in its word of 64 (its ancestors in a tree of drafted tokens, and itself).  A sequence whose slot is none has no keys.  A row that sees nothing gives zeros.  What a key holds that a row does not see
 // never reaches it, whatever it is: scores are replaced, and of the tokens' own values (and what lies behind them in their page), which rows see or not, those that
 // are no finite numbers are taken out of the tile and added to the rows that see them at the end.
 //
@@ -29,7 +29,7 @@ struct DraftArgs {
     const int *kv_len, *cu, *slots, *page_table;
     const int64_t* ancestors;                           // null: every token sees those up to itself
     float* parts;                                       // [share][token][head][d + 2]: values, maximum, sum; null: one share
-    int max_pages, n_pages, n_tokens, n_heads, n_kv, group, d, most;
+    int n_slots, max_pages, n_pages, n_tokens, n_heads, n_kv, group, d, most;
     float scale;
 };
 
@@ -54,11 +54,12 @@ draft_attention_kernel(const __grid_constant__ DraftArgs a) {
     const int begin = max(0, min(a.cu[s], a.n_tokens)), n = max(0, min(min(a.cu[s + 1], a.n_tokens) - begin, a.most));
     const int rows = min(kRows, n * a.group - r0);
     if (rows <= 0) return;
-    const int kv_len = max(0, min(a.kv_len[s], a.max_pages * kPageTokens)), history = kv_len - n;       // (negative: the first tokens are none of the keys)
+    const int slot = a.slots[s];
+    const int kv_len = slot >= 0 && slot < a.n_slots ? max(0, min(a.kv_len[s], a.max_pages * kPageTokens)) : 0, history = kv_len - n;       // (negative: the first tokens are none of the keys)
     const int n_keys = a.ancestors ? kv_len : min(kv_len, history + (r0 + rows - 1) / a.group + 1);
     const int all = (n_keys + kPageTokens - 1) / kPageTokens, share = (all + gridDim.z - 1) / gridDim.z;
     const int page0 = min(all, (int)blockIdx.z * share), page1 = min(all, page0 + share);
-    const int* table = a.page_table + (int64_t)a.slots[s] * a.max_pages;
+    const int* table = a.page_table + (int64_t)slot * a.max_pages;           // (followed where there are keys)
     const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
 
     // whether row r sees key j of the step's tokens
@@ -292,12 +293,12 @@ int by_size(const DraftArgs& a, int n_seqs, int shares, cudaStream_t stream) {
 
 // q, out [tokens, heads, d]; k [pages, kv, 64, d], v [pages, kv, d, 64]; ``parts``: shares * tokens * heads * (d + 2) floats where there is more than one share.
 CPM_API int cpm_draft_attention_generic(const void* q, const void* k, const void* v, void* out, const int* kv_len, const int* cu, const int* slots,
-                                        const int* page_table, int max_pages, int n_pages, const int64_t* ancestors, float* parts, int shares, int n_tokens,
+                                        const int* page_table, int n_slots, int max_pages, int n_pages, const int64_t* ancestors, float* parts, int shares, int n_tokens,
                                         int n_seqs, int most, int n_heads, int n_kv, int d, float scale, int dtype, cudaStream_t stream) {
     if (n_tokens <= 0 || n_seqs <= 0) return CPM_OK;
     if (d < 4 || d > 256 || d % 4 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || most < 1 || most > 64 || max_pages < 1 || max_pages > 0x7fffffff / kPageTokens || n_pages < 1) return CPM_BAD_ARGUMENT;
     if (shares < 1 || shares > 64 || (shares > 1) != (parts != nullptr)) return CPM_BAD_ARGUMENT;
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) return CPM_BAD_ARGUMENT;
-    const DraftArgs a{q, k, v, out, kv_len, cu, slots, page_table, ancestors, parts, max_pages, n_pages, n_tokens, n_heads, n_kv, n_heads / n_kv, d, most, scale};
+    const DraftArgs a{q, k, v, out, kv_len, cu, slots, page_table, ancestors, parts, n_slots, max_pages, n_pages, n_tokens, n_heads, n_kv, n_heads / n_kv, d, most, scale};
     return dtype == CPM_BF16 ? by_size<bf16>(a, n_seqs, shares, stream) : by_size<float>(a, n_seqs, shares, stream);
 }

@@ -56,7 +56,7 @@ struct Args {
     const int64_t* ancestors;
     const bf16* v;
     float* scratch;                                     // Cuts, then per block two places of (D + 2) x rows floats: channels, maximum, sum
-    int max_pages, n_pages, n_tokens, n_seqs, n_heads, n_kv, group, most, per_half, rows;       // per_half: tokens of a half; rows: of a place
+    int n_slots, max_pages, n_pages, n_tokens, n_seqs, n_heads, n_kv, group, most, per_half, rows;       // per_half: tokens of a half; rows: of a place
     int parts;                                          // tiles that a sequence has at most
     float scale_log2;
 };
@@ -143,6 +143,12 @@ struct Line {                                           // in shared memory
     int warp_sum[32];
 };
 __device__ __forceinline__ int pages_of(int keys) { return (keys + kPageTokens - 1) / kPageTokens; }
+// A sequence's row of the page table, and its keys: none where the row is none.
+__device__ __forceinline__ int slot_of(const Args& a, int s) {
+    const int slot = a.slots[s];
+    return slot >= 0 && slot < a.n_slots ? slot : -1;
+}
+__device__ __forceinline__ int keys_of(const Args& a, int s, int slot) { return slot < 0 ? 0 : max(0, min(a.kv_len[s], a.max_pages * kPageTokens)); }
 __device__ __forceinline__ int tokens_of(const Args& a, const Line& l, int s) { return max(0, min(l.first[s + 1] - l.first[s], a.most)); }
 
 template <int H>
@@ -156,7 +162,7 @@ __device__ __forceinline__ void lay_out(const Args& a, Line& l) {
         if (warp == 0) {
             const bool there = lane < a.n_seqs;
             const int first = there ? max(0, min(a.cu[lane], a.n_tokens)) : 0, then = there ? max(0, min(a.cu[lane + 1], a.n_tokens)) : 0;
-            const int keys = there ? max(0, min(a.kv_len[lane], a.max_pages * kPageTokens)) : 0, slot = there ? a.slots[lane] : 0;
+            const int slot = there ? slot_of(a, lane) : -1, keys = there ? keys_of(a, lane, slot) : 0;
             const int cost = there ? units_of<H>(a, max(0, min(then - first, a.most))) * (pages_of(keys) + kExtra) : 0;
             int upto = cost;
 #pragma unroll
@@ -181,8 +187,8 @@ __device__ __forceinline__ void lay_out(const Args& a, Line& l) {
     for (int s = tid; s <= a.n_seqs; s += THREADS) {
         l.first[s] = max(0, min(a.cu[s], a.n_tokens));
         if (s < a.n_seqs) {
-            l.keys[s] = max(0, min(a.kv_len[s], a.max_pages * kPageTokens));
-            l.slot[s] = a.slots[s];
+            l.slot[s] = slot_of(a, s);
+            l.keys[s] = keys_of(a, s, l.slot[s]);
         }
     }
     __syncthreads();
@@ -819,7 +825,7 @@ CPM_API int64_t cpm_draft_attention_scratch_floats(int n_heads, int n_kv, int d,
 }
 
 CPM_API int cpm_draft_attention_tcgen05(const void* q, const void* k, const void* v, void* out, const int* kv_len, const int* cu, const int* slots,
-                                        const int* page_table, int max_pages, int n_pages, const int64_t* ancestors, float* scratch, int n_tokens, int n_seqs,
+                                        const int* page_table, int n_slots, int max_pages, int n_pages, const int64_t* ancestors, float* scratch, int n_tokens, int n_seqs,
                                         int most, int n_heads, int n_kv, int d, float scale, cudaStream_t stream) {
     if (n_tokens <= 0 || n_seqs <= 0) return CPM_OK;
     if (n_kv < 1 || n_heads < 1 || n_heads % n_kv || n_heads / n_kv > 128 || most < 1 || most > 64 || max_pages < 1 || n_pages < 1 || !(scale > 0.f) || !scratch) return CPM_BAD_ARGUMENT;
@@ -830,7 +836,7 @@ CPM_API int cpm_draft_attention_tcgen05(const void* q, const void* k, const void
     if (units * (max_pages + da5::kExtra) * min(n_seqs, da5::kMostSeqs) > 0x7fffffff || (int64_t)n_pages * n_kv * max(d, kPageTokens) > 0x7fffffff ||
         max_pages > 0x7fffffff / kPageTokens)
         return CPM_BAD_ARGUMENT;
-    const da5::Args a{(bf16*)out, kv_len, cu, slots, page_table, ancestors, (const bf16*)v, scratch, max_pages, n_pages, n_tokens, n_seqs, n_heads, n_kv,
+    const da5::Args a{(bf16*)out, kv_len, cu, slots, page_table, ancestors, (const bf16*)v, scratch, n_slots, max_pages, n_pages, n_tokens, n_seqs, n_heads, n_kv,
                       n_heads / n_kv, most, s.per_half, s.rows, (most + s.halves * s.per_half - 1) / (s.halves * s.per_half),
                       scale * 1.4426950408889634f};
     const bool two = s.halves == 2;

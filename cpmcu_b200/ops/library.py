@@ -130,9 +130,9 @@ _SIGNATURES = {
     "cpm_verify_drafts": [_P, c_int64, c_int, c_int, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int64, _P, _P, _P, _P, _P, _P, c_uint64, _P, _P, _P, _P, _P, _P],
     "cpm_step_tables": [_P, _P, _P, c_int, c_int, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P],
     "cpm_keep_drafts": [_P, c_int, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _P],
-    "cpm_draft_attention_generic": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+    "cpm_draft_attention_generic": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_float, c_int, _P],
-    "cpm_draft_attention_tcgen05": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
+    "cpm_draft_attention_tcgen05": [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
     "cpm_latent_attention_mma": [_P, _P, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, _P],
 }
 

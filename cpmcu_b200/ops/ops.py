@@ -1996,7 +1996,7 @@ class Ops:
         """A few tokens a sequence against its cached keys: q [tokens, heads, d] -> [tokens, heads * d].  Sequence s brings the tokens cu_q[s] .. cu_q[s + 1], at most
         ``most`` (up to MOST_DRAFTS), which are the last of its kv_len[s] keys in k_cache [pages, kv, PAGE_TOKENS, d] and v_cache [pages, kv, d, PAGE_TOKENS].  A
         token sees all keys before these, and of these the ones up to itself, or with ``ancestors`` (int64 [tokens]) those whose bit is set.  A row that sees none
-        gives zeros; rows of no sequence are not written.  What an unseen key or value holds, even if it is no number, changes nothing."""
+        gives zeros, as all of a sequence's do whose slot is none; rows of no sequence are not written.  What an unseen key or value holds, even if it is no number, changes nothing."""
         given, dtype, i32 = self._given, self.dtype, torch.int32
         given(q, dtype, "q")
         if q.dim() != 3:
@@ -2018,7 +2018,7 @@ class Ops:
         given(page_table, i32, "page table")
         if page_table.dim() != 2 or page_table.numel() == 0:
             raise ValueError("page table: needs [slots, pages]")
-        width = page_table.shape[1]
+        n_slots, width = page_table.shape
         if ancestors is not None:
             given(ancestors, torch.int64, "ancestors", n)
         stream = self._here()
@@ -2029,14 +2029,14 @@ class Ops:
             scratch = self.empty(self.lib.cpm_draft_attention_scratch_floats(n_heads, n_kv, d, most), dtype=torch.float32)
             self.draft_attention_ran = True
             check(self.lib.cpm_draft_attention_tcgen05(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), slots.data_ptr(),
-                                                       page_table.data_ptr(), width, n_pages, _ptr(ancestors), scratch.data_ptr(), n, n_seqs, most, n_heads, n_kv, d,
+                                                       page_table.data_ptr(), n_slots, width, n_pages, _ptr(ancestors), scratch.data_ptr(), n, n_seqs, most, n_heads, n_kv, d,
                                                        float(scale), stream), "tcgen05 attention of drafted tokens")
             LAUNCHES_EXTRA[0] += 1       # the pieces, then their addition
             return out
         shares = self.draft_attention_shares(n_seqs, most, n_heads, n_kv, width * PAGE_TOKENS)
         parts = self.empty(shares * n * n_heads * (d + 2), dtype=torch.float32) if shares > 1 else None
         check(self.lib.cpm_draft_attention_generic(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(kv_len), _ptr(cu_q), _ptr(slots), _ptr(page_table),
-                                                   width, n_pages, _ptr(ancestors), _ptr(parts), shares, n, n_seqs, most, n_heads, n_kv, d,
+                                                   n_slots, width, n_pages, _ptr(ancestors), _ptr(parts), shares, n, n_seqs, most, n_heads, n_kv, d,
                                                    float(scale), self.code, stream), f"attention of drafted tokens (head_dim {d})")
         if shares > 1:
             LAUNCHES_EXTRA[0] += 1

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_gpu_drafts import DT, PAGE, _i32, _ops
+from tests.test_gpu_drafts import DT, PAGE, _attention_case, _check_attention, _i32, _ops, _weight_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -175,3 +175,21 @@ def test_tables_and_storing_launched_one_behind_the_other(mask, d):
             assert torch.equal(places.view(n_seqs, most)[:, 0], lengths) and torch.equal(q, q1) and torch.equal(k, k1) and torch.equal(v, v1), turn
     finally:
         ops.lib.cpm_set_pdl(-1)
+
+
+@pytest.mark.parametrize("form", ["tcgen05", "plain"])
+@pytest.mark.parametrize("sequences", [5, 40])
+def test_attention_of_sequences_whose_slot_is_none(form, sequences):
+    """A sequence without a row of the page table has no keys: its rows are zero, and the others' are what they are without it."""
+    ops = _ops("bfloat16")
+    ops.use_tcgen05_draft = form == "tcgen05"
+    new, lengths = [2 + i % 3 for i in range(sequences)], [20 + 61 * i for i in range(sequences)]
+    args, rows, cu = _attention_case("bfloat16", 64, 4, 2, lengths, new, None, seed=7)
+    slots = args["slots"].clone()
+    slots[1], slots[3], slots[4] = -1, args["page_table"].shape[0], 2 ** 31 - 1
+    got = ops.draft_attention(**{**args, "slots": slots})
+    none = [1, 3, 4]
+    for s in none:
+        assert bool((got[cu[s]:cu[s + 1]] == 0).all())
+    for s in [s for s in range(sequences) if s not in none]:
+        _check_attention("bfloat16", args, rows[s:s + 1], cu[s:s + 2], None, _weight_bits(ops, "bfloat16", 64, 4, 2), got)
