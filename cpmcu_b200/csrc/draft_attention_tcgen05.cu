@@ -29,7 +29,8 @@ using namespace tc5;
 
 constexpr int kMostSeqs = 512;                          // of one launch
 constexpr int kStages = 4;                              // pages under way
-constexpr int kOdd = 8;                                 // segments that half 0 may be ahead of half 1, and more
+constexpr int kOdd = 8;                                 // places for marks of segments with pages: the cleaning warp is at most kStages pages, and so segments, ahead
+static_assert(kOdd > kStages + 1, "a mark is read before its place is taken again");
 constexpr float kBehind = 8.0f;                         // the running maximum may lie 2^8 behind
 // (kExtra of 1 to 4 and kLeast of 1 to 8 differ by less than two boxes do.)
 constexpr int kExtra = 2;                               // pages that a unit's beginning and end are worth
@@ -270,7 +271,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
     __shared__ __align__(8) uint64_t q_full[H][Z::kQBufs], k_full[kStages], v_full[kStages], v_ready[kStages], k_empty[kStages], v_empty[kStages], s_full[H][2], p_full[H][2],
         o_done[H][2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag, odd[kOdd];               // odd: a segment's number and one, where its own tokens' values hold what is no finite number
+    __shared__ int abort_flag, odd[kOdd];               // odd: a segment's number and one (of those with pages), where its own tokens' values hold what is no finite number
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -382,7 +383,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
         int st = 0, number = 0;
         bool ok = true;
 #pragma unroll 1
-        for (; ok && walk.next(a, line, g); ++number) {
+        for (; ok && walk.next(a, line, g); number += g.pages > 0) {       // (segments without pages are not waited for)
 #pragma unroll 1
             for (int i = 0; i < g.pages; ++i, ++st) {
                 const int s = st % kStages, key0 = (g.page0 + i) * kPageTokens;
@@ -514,7 +515,7 @@ draft_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const 
         int st = 0, number = 0;
         bool ok = true;
 #pragma unroll 1
-        for (; ok && walk.next(a, line, g); ++number) {
+        for (; ok && walk.next(a, line, g); number += g.pages > 0) {
             const int in_half = r / a.group, token = g.row0 + i * a.per_half + in_half;
             const bool valid = r >= 0 && in_half < a.per_half && token < g.tokens;
             const bool any = __any_sync(0xffffffffu, valid);

@@ -193,3 +193,27 @@ def test_attention_of_sequences_whose_slot_is_none(form, sequences):
         assert bool((got[cu[s]:cu[s + 1]] == 0).all())
     for s in [s for s in range(sequences) if s not in none]:
         _check_attention("bfloat16", args, rows[s:s + 1], cu[s:s + 2], None, _weight_bits(ops, "bfloat16", 64, 4, 2), got)
+
+
+@pytest.mark.parametrize("form", ["tcgen05", "plain"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_no_numbers_between_sequences_without_keys(form, bad):
+    """Every eighth piece of work of a block has such a value among its own tokens' and those between have no keys at all: each reaches the rows that see it."""
+    ops = _ops("bfloat16")
+    ops.use_tcgen05_draft = form == "tcgen05"
+    new, lengths = [4, 48] * 256, [30, 0] * 256                   # 2 pieces with a page, and 6 without, of 16 tokens and a key-value head each
+    args, rows, cu = _attention_case("bfloat16", 64, 32, 2, lengths, new, None, seed=5)
+    clean = ops.draft_attention(**args).view(-1, 32, 64).clone()
+    table, slots = args["page_table"].cpu(), args["slots"].cpu()
+    for s in range(0, 512, 2):
+        page = int(table[int(slots[s]), 0])
+        for head in range(2):
+            args["v_cache"][page, head, (s // 2 + 7 * head) % 64, 27] = bad            # of the second of four tokens
+    got = ops.draft_attention(**args).view(-1, 32, 64)
+    want = clean.clone()
+    for s in range(0, 512, 2):
+        for head in range(2):
+            want[cu[s] + 1:cu[s + 1], 16 * head:16 * head + 16, (s // 2 + 7 * head) % 64] = bad
+    assert bool(torch.isfinite(clean).all())
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), finite) and torch.equal(got.isnan(), want.isnan()) and torch.equal(got[finite], want[finite])
