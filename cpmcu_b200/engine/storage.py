@@ -17,7 +17,7 @@ import torch
 from ..cache import Cache, PAGE_TOKENS
 from ..memory import ALIGN, Arena, PoolExhausted, Workspace, plan_storage, round_up
 from ..models.model import Model
-from ..ops.dry import measure_weights, measure_workspace
+from ..ops.dry import measure_weights, measure_workspace, most_step_tokens
 from .decode import bucket_size
 
 
@@ -94,7 +94,7 @@ def make_storage(model: Model, chunk_tokens: int, max_batch: int, max_tokens: Op
     if w_bytes:
         ops.weights = arena.carve("weights", w_bytes)
     workspace = Workspace(arena.carve("workspace", persistent), [arena.carve("frame0", frame), arena.carve("frame1", frame)],
-                          sized_tokens=max(chunk_tokens, bucket), sized_seqs=max(bucket, 1))
+                          sized_tokens=most_step_tokens(chunk_tokens, max_batch), sized_seqs=max(bucket, 1))
     cache = Cache(needs, max_tokens=tokens, dtype=dtype, device=device, n_slots=slots_for(tokens),
                   max_seq_tokens=min(tokens, per_seq_cap), max_step_tokens=chunk_tokens,
                   state_region=arena.carve("state", st_bytes), page_region=arena.carve("cache", pg_bytes))

@@ -205,6 +205,14 @@ def _half_full_tiles(n_tokens: int, most_seqs: int) -> List[int]:
     return [1] * ones + [n_tokens - ones]
 
 
+def most_step_tokens(max_step_tokens: int, max_batch: int) -> int:
+    """Tokens of the largest step that a workspace lets through: a prompt's, or a decode step's of as many sequences as a bucket has."""
+    b = 1
+    while b < max_batch:
+        b *= 2
+    return max(int(max_step_tokens), b)
+
+
 def workspace_steps(max_step_tokens: int, max_batch: int, max_seq_tokens: int, packed_pieces: int = 0, sm_count: int = 148):
     """The steps a workspace is measured with: (portions, keys of the longest sequence, decode, captured, query tiles or None).
 
@@ -287,7 +295,7 @@ def measure_workspace(spec, dtype: torch.dtype, max_step_tokens: int, max_batch:
         from ..engine.drafts import draft_step, tokens_of_step
         size = 1
         while True:
-            tokens = tokens_of_step(size, drafts, max(int(max_step_tokens), size))
+            tokens = tokens_of_step(size, drafts, most_step_tokens(max_step_tokens, max_batch))
             if tokens > 1:
                 n = size * tokens
                 ops.workspace.begin_step()

@@ -133,3 +133,38 @@ def test_cli_option():
     parse = create_cli_parser().parse_args
     assert parse(["--model-path", "x"]).draft_tokens == 0
     assert parse(["--model-path", "x", "--draft-tokens", "7"]).draft_tokens == 7 == parse(["--model-path", "x", "--draft_tokens", "7"]).draft_tokens
+
+
+@pytest.mark.parametrize("chunk,max_batch", [(16, 64), (64, 4), (1, 9), (100, 33)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_steps_of_drafts_fit_the_workspace_that_is_measured(chunk, max_batch, dtype):
+    """As many tokens as the runner brings at every bucket size, with prompts' chunks smaller than a batch too."""
+    from cpmcu_b200.cache import Cache
+    from cpmcu_b200.engine.decode import bucket_size
+    from cpmcu_b200.engine.drafts import DraftRunner, draft_step
+    from cpmcu_b200.engine.storage import make_storage
+
+    spec = _spec(configs.tiny_e())
+    persistent, frame, _ = measure_workspace(spec, dtype, chunk, max_batch, 512, drafts=63)
+    model = Model(spec, DryOps(dtype))
+    model.loaded, model.ops.device = True, torch.device("cpu")
+    make_storage(model, chunk, max_batch, max_tokens=512, max_seq_tokens=512, drafts=63)
+    runner = DraftRunner.__new__(DraftRunner)
+    runner.drafts, runner.ops = 63, model.ops                    # (with the storage's workspace)
+    assert runner.ops.workspace.sized_tokens > 0
+    meta = lambda n, **kw: torch.empty(n, device="meta", **{"dtype": torch.int32, **kw})  # noqa: E731
+    size = 1
+    while size <= bucket_size(max_batch):
+        tokens = runner.tokens(size)
+        if tokens > 1:
+            ops = DryOps(dtype)
+            model = Model(spec, ops)
+            model.load_weights({name: torch.empty(w.shape, device="meta", dtype=torch.int32 if w.role == "table" else dtype) for name, w in model.weight_specs().items()})
+            cache = Cache(model.cache_needs(), max_tokens=512, dtype=dtype, device="meta", n_slots=max_batch + 1, max_seq_tokens=512)
+            n = size * tokens
+            ops.workspace.begin_step()
+            draft_step(model, cache, tokens, meta(n), meta(n), meta(size), meta(size), meta(size), 0, meta(size), meta(size), *(meta(size, dtype=torch.float32) for _ in range(3)),
+                       meta(size), meta(n), 512, False)
+            needs = ops.workspace.peaks()
+            assert needs[0] <= persistent and needs[1] <= frame, (size, tokens, needs, frame)
+        size *= 2
