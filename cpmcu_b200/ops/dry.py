@@ -22,6 +22,9 @@ from .ops import BF16, F32, Ops, PREFILL_TILE_ROWS
 class _NoLibrary:
     """Stands in for the compiled library: every entry point "launches" successfully."""
 
+    def __init__(self, sm_count: int = 148):
+        self.sm_count = sm_count
+
     @staticmethod
     def cpm_decode_attention_scratch_floats(n_seqs, n_heads, n_kv, d, n_splits):
         return n_seqs * n_kv * ((n_heads // n_kv + 15) // 16) * n_splits * (16 * d + 32)
@@ -62,20 +65,20 @@ class _NoLibrary:
     def cpm_listed_attention_tcgen05_max_pages():
         return 11808
 
-    @staticmethod
-    def cpm_kv4_attention_scratch_floats(d):
-        return 148 * (8 + 2 * 16 * (d + 4))
+    def cpm_kv4_attention_scratch_floats(self, d):
+        return self.sm_count * (8 + 2 * 16 * (d + 4))
 
     @staticmethod
     def cpm_kv4_attention_most_tiles():
         return 512
 
-    @staticmethod
-    def cpm_draft_attention_scratch_floats(n_heads, n_kv, d, most):
+    def cpm_draft_attention_scratch_floats(self, n_heads, n_kv, d, most):
         group = n_heads // n_kv
+        if group > 128:
+            return 0
         per_half = 128 // group
         halves = 2 if most > per_half else 1
-        return 148 * (2 if d <= 64 and halves == 1 else 1) * (4 + 2 * min(halves * per_half, most) * group * (d + 2))
+        return self.sm_count * (2 if d <= 64 and halves == 1 else 1) * (6 + 2 * min(halves * per_half, most) * group * (d + 2))
 
     def __getattr__(self, name):
         return lambda *args: 0
@@ -88,7 +91,7 @@ class DryOps(Ops):
         self.dtype = dtype
         self.code = F32 if dtype == torch.float32 else BF16
         self.device = torch.device("meta")
-        self.lib = _NoLibrary()
+        self.lib = _NoLibrary(sm_count)
         self.element_size = 4 if dtype == torch.float32 else 2
         self.sm_count = sm_count
         self.arrivals = None

@@ -168,3 +168,12 @@ def test_steps_of_drafts_fit_the_workspace_that_is_measured(chunk, max_batch, dt
             needs = ops.workspace.peaks()
             assert needs[0] <= persistent and needs[1] <= frame, (size, tokens, needs, frame)
         size *= 2
+
+
+@pytest.mark.parametrize("sms", [20, 148, 160])
+def test_rooms_for_parts_go_by_the_devices_multiprocessors(sms):
+    ops = DryOps(torch.bfloat16, sms)
+    # a block's entry of 6 numbers, and two places of 5 rows times 16 heads: two blocks a multiprocessor at 64 channels, one at 128
+    assert ops.lib.cpm_draft_attention_scratch_floats(32, 2, 64, 5) == sms * 2 * (6 + 2 * 5 * 16 * 66)
+    assert ops.lib.cpm_draft_attention_scratch_floats(32, 2, 128, 5) == sms * (6 + 2 * 5 * 16 * 130)
+    assert ops.lib.cpm_kv4_attention_scratch_floats(128) == sms * (8 + 32 * 132)

@@ -217,3 +217,14 @@ def test_values_that_are_no_numbers_between_sequences_without_keys(form, bad):
     assert bool(torch.isfinite(clean).all())
     finite = torch.isfinite(want)
     assert torch.equal(torch.isfinite(got), finite) and torch.equal(got.isnan(), want.isnan()) and torch.equal(got[finite], want[finite])
+
+
+def test_the_dry_run_counts_as_much_room_for_parts_as_the_library():
+    from cpmcu_b200.ops.dry import DryOps
+
+    ops = _ops("bfloat16")
+    dry = DryOps(torch.bfloat16, ops.sm_count)
+    for heads, kv in ((1, 1), (4, 2), (32, 2), (32, 8), (21, 1), (40, 1), (128, 1), (129, 1), (256, 1)):
+        for d in (32, 64, 96, 128):
+            for most in range(1, 65):
+                assert ops.lib.cpm_draft_attention_scratch_floats(heads, kv, d, most) == dry.lib.cpm_draft_attention_scratch_floats(heads, kv, d, most), (heads, kv, d, most)
