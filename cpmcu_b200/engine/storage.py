@@ -47,6 +47,17 @@ def weight_bytes(model: Model) -> int:
     return max(total, measure_weights(model.spec, model.ops.dtype)) + 64 * ALIGN
 
 
+def draft_logit_bytes(vocab_size: int, chunk_tokens: int, max_batch: int, drafts: int) -> int:
+    """Bytes of the logits of drafted tokens' steps, which torch's allocator gives: every recorded bucket size keeps its own (fp32, a row for each token), and the largest
+    was made once more before it was recorded."""
+    from .drafts import tokens_of_step
+    sizes, room = [1], most_step_tokens(chunk_tokens, max_batch)
+    while sizes[-1] < max_batch:
+        sizes.append(2 * sizes[-1])
+    tokens = [size * n for size in sizes for n in (tokens_of_step(size, drafts, room),) if n > 1]
+    return (sum(tokens) + max(tokens, default=0)) * int(vocab_size) * 4 if drafts else 0
+
+
 def make_storage(model: Model, chunk_tokens: int, max_batch: int, max_tokens: Optional[int] = None,
                  memory_limit: Optional[float] = None, max_seq_tokens: Optional[int] = None,
                  n_slots: Optional[int] = None, reserve_bytes: int = 512 << 20, drafts: int = 0) -> Storage:
@@ -55,7 +66,7 @@ def make_storage(model: Model, chunk_tokens: int, max_batch: int, max_tokens: Op
     ``memory_limit`` (a fraction of the device's memory) leaves after weights, workspace and ``reserve_bytes`` (for
     what torch allocates itself: results handed to callers, library workspaces).  Weights that are already loaded
     stay where they are; otherwise they go into the arena when they are loaded.  ``drafts``: room for steps of that many drafted tokens a
-    sequence too.  Raises PoolExhausted."""
+    sequence too, in the workspace and for their logits, which come on top of ``reserve_bytes``.  Raises PoolExhausted."""
     ops = model.ops
     spec = model.spec
     dtype, device = ops.dtype, ops.device
@@ -79,6 +90,7 @@ def make_storage(model: Model, chunk_tokens: int, max_batch: int, max_tokens: Op
     w_bytes = 0 if model.loaded else weight_bytes(model)
     budget = None
     if max_tokens is None:
+        reserve_bytes = int(reserve_bytes) + draft_logit_bytes(spec.vocab_size, chunk_tokens, max_batch, drafts)
         if memory_limit is None:
             raise ValueError("make_storage needs max_tokens or memory_limit")
         free, total = torch.cuda.mem_get_info(device)

@@ -177,3 +177,23 @@ def test_rooms_for_parts_go_by_the_devices_multiprocessors(sms):
     assert ops.lib.cpm_draft_attention_scratch_floats(32, 2, 64, 5) == sms * 2 * (6 + 2 * 5 * 16 * 66)
     assert ops.lib.cpm_draft_attention_scratch_floats(32, 2, 128, 5) == sms * (6 + 2 * 5 * 16 * 130)
     assert ops.lib.cpm_kv4_attention_scratch_floats(128) == sms * (8 + 32 * 132)
+
+
+def test_a_cache_leaves_room_for_the_logits_of_drafts(monkeypatch):
+    """What a memory limit leaves for the cache is less by the logits of every bucket's recorded step, 1 to 8 sequences of 16 tokens (and of 8, where a step has no more room),
+    and of the largest once more."""
+    from cpmcu_b200.engine.storage import draft_logit_bytes, make_storage
+
+    assert draft_logit_bytes(900, 64, 8, 15) == (16 + 32 + 64 + 64 + 64) * 900 * 4
+    assert draft_logit_bytes(900, 64, 5, 63) == (64 * 4 + 64) * 900 * 4 and draft_logit_bytes(900, 16, 64, 1) == (2 + 4 + 8 + 16 + 32 + 64 + 64) * 900 * 4
+    assert draft_logit_bytes(900, 64, 8, 0) == draft_logit_bytes(900, 1, 1, 15) == 0
+    free = 96 << 20
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device=None: (free, free))
+    spec = _spec(configs.tiny_e())
+    left = {}
+    for drafts in (0, 15):
+        model = Model(spec, DryOps(torch.bfloat16))
+        model.loaded, model.ops.device = True, torch.device("cpu")
+        storage = make_storage(model, 64, 8, memory_limit=1.0, reserve_bytes=1 << 20, max_seq_tokens=4096, drafts=drafts)
+        left[drafts] = free - (1 << 20) - storage.arena.total
+    assert left[0] >= 0 and left[15] >= 240 * 900 * 4
