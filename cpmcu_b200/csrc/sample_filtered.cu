@@ -506,7 +506,7 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     if (p <= 0.f || ratio > 1.f) k = 1;
     // above one: the first token alone, which it would leave out as well; below zero, -0 (weights are compared by their bits) or no number: no limit
     if (!(ratio > 0.f && ratio <= 1.f)) ratio = 0.f;
-    const bool by_count = COUNT && k > 0 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
+    const bool by_count = COUNT && k > 1 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
     const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[s], (uint32_t)(a.step_key[s] + step));
 
     asm volatile("barrier.cluster.arrive;" ::: "memory");       // (nothing is put into a block that has not begun)
@@ -553,7 +553,10 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     best = ArgMax{-INFINITY, 0x7fffffff};
 #pragma unroll 1
     for (uint32_t b = 0; b < blocks; ++b) best = better(best, sm.best[b]);
-    if (best.v == -INFINITY || !(t > 0.f) || k == 1) {         // nothing that can be drawn: token 0; a greedy row, or one token: the largest
+    row.set(best.v, t);
+    // One token: the first whose weight is 1.  That is the largest logit's, unless the next smaller number has that weight too (temperatures above the largest logit).
+    const bool one = k == 1 && t > 0.f, largest = one && !(row.form(nextafterf(best.v, -INFINITY)) >= 1.f);
+    if (best.v == -INFINITY || !(t > 0.f) || largest) {        // nothing that can be drawn: token 0; a greedy row, or one token: the largest
         if (rank == 0 && tid == 0) {
             a.token[r] = best.v == -INFINITY ? 0 : best.i;
             a.logprob[r] = best.v == -INFINITY ? -INFINITY : 0.f;
@@ -561,7 +564,6 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         }
         return;
     }
-    row.set(best.v, t);
 
     if constexpr (STAGED && COUNT) {
         // (Two of the k may be one thread's, and the k-th of the threads' largest then lies below the row's: with k up to a quarter of the threads some k / 8 tokens more, and
@@ -642,8 +644,8 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
         return all;
     };
 
-    uint32_t border = 0;
-    uint64_t ties = ~0ull, equal = 0;
+    uint32_t border = one ? 0x3f800000u : 0u;                  // (one token: of those of weight 1, one or more, the first)
+    uint64_t ties = one ? 1 : ~0ull, equal = one ? 2 : 0;
     // of the thread's tokens, those that were set apart (the last one in the lowest bit), and the mass above them; ``sure``: these two tell what it keeps
     uint64_t found = 0, sure_mass = 0;
     bool sure = false;

@@ -93,3 +93,71 @@ def test_tokens_at_the_border_of_the_light_ones(of_light):
         z[i, 1:] = math.log(of_light * (1 - float(p[i])) / vocab)
     z[:, 1:] += 1e-3 * torch.rand(4, vocab - 1, generator=torch.Generator().manual_seed(1))
     _compare(z, torch.zeros(4), p=p)
+
+
+def _one_of_equal_weights(vocab, g):
+    """Rows whose largest logit is not the only token of weight 1, and not the first: differences that a temperature or the exponential rounds away."""
+    z = torch.randn(8, vocab, generator=g)
+    t = torch.tensor([1.0, 3000.0, 1e9, 1.0, 2e4, 1e30, 1.0, math.inf])
+    z[0] *= 1e-9
+    z[1] *= 1e-4
+    z[3] = -1.0
+    z[3, vocab // 3:] = -1e-12 * torch.rand(vocab - vocab // 3, generator=g)
+    z[4] *= 1e-3
+    z[4, ::2] = math.nan
+    z[6] = -torch.finfo(torch.float32).tiny * torch.arange(vocab, 0, -1).float()
+    return z, t
+
+
+@pytest.fixture
+def weights_of_the_device(monkeypatch):
+    """The definition's weights with the device's exponential.  exp(x) lies half a step of fp32 below 1 at x = -2^-25, and between there and -2^-23 an exponential that is
+    off by up to a step may or may not give 1: which tokens of a row weigh 1 is then for the function to say, and the host's is another one."""
+    exp = torch.exp
+    monkeypatch.setattr(torch, "exp", lambda x: exp(x.cuda()).cpu())
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 40, 1100, 20000, 73448, 250001])
+@pytest.mark.parametrize("setting", ["k", "p", "m"])
+@pytest.mark.parametrize("counts", [True, False])
+def test_one_token_is_the_first_of_those_of_weight_one(vocab, setting, counts, weights_of_the_device):
+    """By a top-k of one, by no mass at all, and by a min-p above one; in calls with and without counts; and where the next number's weight is less after all."""
+    from cpmcu_b200.ops.ops import Ops
+    ops = Ops(torch.bfloat16)
+    z, t = _one_of_equal_weights(vocab, torch.Generator().manual_seed(vocab))
+    z = torch.cat((z, torch.randn(4, vocab, generator=torch.Generator().manual_seed(1)) * 3))
+    t = torch.cat((t, torch.tensor([0.7, 1.0, 2.0, 5.0])))
+    rows = z.shape[0]
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(2))
+    if setting == "k" and not counts:
+        pytest.skip("a count")
+    k = torch.full((rows,), 1 if setting == "k" else 0)
+    p = torch.full((rows,), 0.0 if setting == "p" else 1.0)
+    m = torch.full((rows,), 1.5 if setting == "m" else 0.0)
+    tok, lp = ops.sample_filtered(z.cuda(), u.cuda(), t.cuda(), k.int().cuda() if counts else None, p.cuda(), m.cuda())
+    for i in range(rows):
+        want, logp = plain.sampled(z[i], float(u[i]), float(t[i]), int(k[i]), float(p[i]), float(m[i]))
+        assert int(tok[i]) == want and (float(lp[i]) == logp or abs(float(lp[i]) - logp) < 2e-5), (i, int(tok[i]), want)
+
+
+@pytest.mark.parametrize("vocab", [40, 20000])
+def test_verification_of_rows_of_one_token(vocab, weights_of_the_device):
+    """The same rows as a model's, with drafting probabilities and without: what a row keeps is that token."""
+    from cpmcu_b200.ops.ops import Ops
+    from tests.test_gpu_drafts import _check_verify, _i32
+    ops = Ops(torch.bfloat16)
+    g = torch.Generator().manual_seed(vocab)
+    z, t = _one_of_equal_weights(vocab, g)
+    z, t = z[:7].repeat_interleave(2, 0), t[:7]                   # seven sequences of two tokens
+    cu, seq = [2 * i for i in range(8)], [i // 2 for i in range(14)]
+    u, accept = torch.rand(14, generator=g), torch.rand(14, generator=g)
+    q = torch.softmax(torch.randn(14, vocab, generator=g), 1)
+    ids = [0, 0] * 7
+    for s in range(7):                                            # what is drafted: the token itself, the largest logit's, or another
+        ids[2 * s + 1] = [plain.sampled(z[2 * s], 0.5, float(t[s]), 1, 1.0, 0.0)[0], int(torch.nan_to_num(z[2 * s], -9.0).argmax()), vocab // 2][s % 3]
+    settings = (t, torch.ones(7, dtype=torch.int32), torch.ones(7), torch.zeros(7))
+    args = dict(logits=z.cuda(), ids=_i32(ids), cu_q=_i32(cu), token_seq=_i32(seq), most=2, uniform=u.cuda(), temperature=t.cuda(), top_k=settings[1].cuda(), top_p=settings[2].cuda(),
+                min_p=settings[3].cuda())
+    want = dict(z=z, ids=ids, cu=cu, u=u, settings=settings)
+    _check_verify(ops.verify_drafts(**args), **want)
+    _check_verify(ops.verify_drafts(**args, draft_probs=q.cuda(), accept=accept.cuda()), **want, probs=q, accept=accept)
