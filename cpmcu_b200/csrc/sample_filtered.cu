@@ -18,8 +18,8 @@
 // compared with each, and it draws as well (a small top-k needs no weights and bins of the whole row for that: draw_few).  In the same pass a thread sums what it keeps above the bin, so that the draw looks at few tokens again.
 // (A cluster's barrier takes about 2 us, and a look into a neighbour's shared memory half of that: a selection over the whole row with
 // all blocks' histograms added up at every step took 41 us for one row of 73,448, bins of counts alone 25, and this 14.)
-// 64 rows of 73,448 with settings of their own 37 us, 512 rows of 32,000 by mass alone 122.  What a row cannot do without is its logits, 4 bytes a token
-// (10 us of the 122); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
+// 64 rows of 73,448 with settings of their own 38 us, 512 rows of 32,000 by mass alone 116.  What a row cannot do without is its logits, 4 bytes a token
+// (10 us of the 116); the instructions bound it, some hundred a token, and the phases in which a cluster's blocks wait for the first.
 #include "filtered.cuh"
 #include "philox.cuh"
 #include <type_traits>
@@ -475,39 +475,26 @@ __device__ __noinline__ bool draw_few(FilterShared& sm, const FilterArgs& a, Dra
     return ok;
 }
 
-// COUNT: rows may have a top-k (without it the code is half as long, and keeps more of its numbers in registers).
+// What a row is drawn with.
+struct Settings {
+    int k;
+    float t, p, ratio, u;
+};
+
+// COUNT: the row has a top-k (without it the code is half as long, and keeps more of its numbers in registers).
 template <bool STAGED, bool COUNT>
-__global__ void __launch_bounds__(kFilterThreads, 2)
-sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
+__device__ __forceinline__ void sample_row(FilterShared& sm, const FilterArgs& a, const Settings& set) {
     extern __shared__ float weights[];
-    __shared__ FilterShared sm;
-    pdl_launch_dependents();
-    pdl_wait();
     const uint32_t blocks = cluster_blocks(), rank = cluster_rank();
-    const int r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31;
-    if (a.drawn && !a.drawn[r]) {                               // another's row (its whole cluster leaves)
-        if (rank == 0 && tid == 0) a.logprob[r] = NAN;
-        return;
-    }
-    int s = r, step = 0;                                        // whose settings, and how far behind the sequence's first token
-    if (a.row_seq) {
-        s = a.row_seq[r];
-        if (s < 0 || s >= a.n_seqs) return;                    // behind the last sequence
-        if (a.positions) step = a.positions[r] - a.positions[max(0, min(a.cu[s], a.n_rows - 1))];
-    }
+    const int r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, k = set.k;
+    const float t = set.t, p = set.p, ratio = set.ratio, u = set.u;
     const int first = min(a.vocab, (int)rank * a.per_block);
     Row<STAGED> row;
     row.n = min(a.vocab, first + a.per_block) - first;
     row.z = a.logits + (int64_t)r * a.ld + first;
     row.w = weights;
-    const float t = a.temperature ? a.temperature[s] : 0.f, p = a.top_p ? a.top_p[s] : 1.f;
-    int k = a.top_k ? a.top_k[s] : 0;
-    float ratio = a.min_p ? a.min_p[s] : 0.f;
-    if (p <= 0.f || ratio > 1.f) k = 1;
-    // above one: the first token alone, which it would leave out as well; below zero, -0 (weights are compared by their bits) or no number: no limit
-    if (!(ratio > 0.f && ratio <= 1.f)) ratio = 0.f;
-    const bool by_count = COUNT && k > 1 && k < a.vocab, by_mass = p < 1.f && p > 0.f && k != 1;
-    const float u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[s], (uint32_t)(a.step_key[s] + step));
+    constexpr bool by_count = COUNT;
+    const bool by_mass = p < 1.f && p > 0.f && k != 1;
 
     asm volatile("barrier.cluster.arrive;" ::: "memory");       // (nothing is put into a block that has not begun)
 
@@ -585,8 +572,8 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
     const uint32_t light = by_mass && !by_count ? min(bin_begin(bin_of(__float_as_uint(0.99f * (1.f - p) / (float)a.vocab))), kWhole) : 0u;
     uint64_t own_mass = 0;                                     // of the thread's tokens that bins do not tell exactly
     // Where few of the block's tokens are in bins (a tenth by a look at one of each thread's) a thread gathers its own in ``heavy``, the last one in the lowest bit, and
-    // goes through them one by one: else of 32 neighbours one is in a bin nearly always, and what is done for one lane takes as long as for all.  (512 rows of 32,000, 0.8
-    // of the mass, temperatures of 0.35 to 0.95: 76 us, 86 without; from a quarter of the tokens on the separate loop loses: at 1.3 138 us and 122.)
+    // goes through them one by one: else of 32 neighbours one is in a bin nearly always, and what is done for one lane takes as long as for all.  (512 rows of 32,000 of spread 3,
+    // 0.8 of the mass, temperatures of 0.35 to 0.95: 110 us, 112 without; where most tokens are in bins the separate loop loses: at 1.3 141 us and 116.)
     uint64_t heavy = 0;
     bool sparse = false;
     const auto weigh_all = [&](auto quick) {
@@ -961,6 +948,43 @@ sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
             return;
         }
     }
+}
+
+// COUNT: rows may have a top-k.  Those that have none run the code without: 512 rows of 32,000 by mass alone 116 us, and 123
+// where they share the other's registers (111 in a call without counts); 64 of 73,448, half of them with a count, 37.7 and 39.6.
+template <bool STAGED, bool COUNT>
+__global__ void __launch_bounds__(kFilterThreads, 2)
+sample_filtered_kernel(const __grid_constant__ FilterArgs a) {
+    __shared__ FilterShared sm;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int r = blockIdx.x / cluster_blocks();
+    if (a.drawn && !a.drawn[r]) {                               // another's row (its whole cluster leaves)
+        if (cluster_rank() == 0 && threadIdx.x == 0) a.logprob[r] = NAN;
+        return;
+    }
+    int s = r, step = 0;                                        // whose settings, and how far behind the sequence's first token
+    if (a.row_seq) {
+        s = a.row_seq[r];
+        if (s < 0 || s >= a.n_seqs) return;                    // behind the last sequence
+        if (a.positions) step = a.positions[r] - a.positions[max(0, min(a.cu[s], a.n_rows - 1))];
+    }
+    Settings set;
+    set.t = a.temperature ? a.temperature[s] : 0.f;
+    set.p = a.top_p ? a.top_p[s] : 1.f;
+    set.k = a.top_k ? a.top_k[s] : 0;
+    set.ratio = a.min_p ? a.min_p[s] : 0.f;
+    set.u = a.uniform ? a.uniform[r] : philox_uniform(a.seed, (uint32_t)a.seq_key[s], (uint32_t)(a.step_key[s] + step));
+    if (set.p <= 0.f || set.ratio > 1.f) set.k = 1;
+    // above one: the first token alone, which it would leave out as well; below zero, -0 (weights are compared by their bits) or no number: no limit
+    if (!(set.ratio > 0.f && set.ratio <= 1.f)) set.ratio = 0.f;
+    if constexpr (COUNT) {
+        if (set.k > 1 && set.k < a.vocab) {
+            sample_row<STAGED, true>(sm, a, set);
+            return;
+        }
+    }
+    sample_row<STAGED, false>(sm, a, set);
 }
 
 constexpr int kMostStaged = (113 * 1024 - (int)sizeof(FilterShared) - 1024) / 4;      // weights that a block's half of the shared memory holds

@@ -161,3 +161,22 @@ def test_verification_of_rows_of_one_token(vocab, weights_of_the_device):
     want = dict(z=z, ids=ids, cu=cu, u=u, settings=settings)
     _check_verify(ops.verify_drafts(**args), **want)
     _check_verify(ops.verify_drafts(**args, draft_probs=q.cuda(), accept=accept.cuda()), **want, probs=q, accept=accept)
+
+
+@pytest.mark.parametrize("vocab", [300, 32000, 73448])
+def test_rows_without_a_count_among_others(vocab):
+    """Rows of a call that has counts: those whose count is none (0, below, or the vocabulary's size and more) draw what they draw in a call without counts, to the last bit."""
+    from cpmcu_b200.ops.ops import Ops
+    ops = Ops(torch.bfloat16)
+    g = torch.Generator().manual_seed(vocab)
+    z, u = (torch.randn(24, vocab, generator=g) * 3).cuda(), torch.rand(24, generator=g).cuda()
+    t, p = (0.3 + 1.5 * torch.rand(24, generator=g)).cuda(), torch.where(torch.rand(24, generator=g) < 0.3, torch.ones(24), torch.rand(24, generator=g)).cuda()
+    m = torch.where(torch.rand(24, generator=g) < 0.5, torch.zeros(24), 0.1 * torch.rand(24, generator=g)).cuda()
+    k = torch.tensor([0, 5, -1, vocab, 60, vocab + 1, 1, 2 ** 31 - 1] * 3).int()
+    tokens, logs = ops.sample_filtered(z, u, t, k.cuda(), p, m)
+    without, without_logs = ops.sample_filtered(z, u, t, None, p, m)
+    none = ((k <= 0) | (k >= vocab)).cuda()
+    assert torch.equal(tokens[none], without[none]) and torch.equal(logs[none], without_logs[none])
+    for i in range(24):
+        want, logp = plain.sampled(z[i].cpu(), float(u[i]), float(t[i]), int(k[i]), float(p[i]), float(m[i]))
+        assert int(tokens[i]) == want and abs(float(logs[i]) - logp) < 2e-5
