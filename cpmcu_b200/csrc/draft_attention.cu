@@ -54,8 +54,8 @@ draft_attention_kernel(const __grid_constant__ DraftArgs a) {
     const int begin = max(0, min(a.cu[s], a.n_tokens)), n = max(0, min(min(a.cu[s + 1], a.n_tokens) - begin, a.most));
     const int rows = min(kRows, n * a.group - r0);
     if (rows <= 0) return;
-    const int slot = a.slots[s];
-    const int kv_len = slot >= 0 && slot < a.n_slots ? max(0, min(a.kv_len[s], a.max_pages * kPageTokens)) : 0, history = kv_len - n;       // (negative: the first tokens are none of the keys)
+    const int slot = a.slots[s], held = a.kv_len[s];
+    const int kv_len = slot >= 0 && slot < a.n_slots ? max(0, min(held, a.max_pages * kPageTokens)) : 0, history = kv_len - n;       // (negative: the first tokens are none of the keys)
     const int n_keys = a.ancestors ? kv_len : min(kv_len, history + (r0 + rows - 1) / a.group + 1);
     const int all = (n_keys + kPageTokens - 1) / kPageTokens, share = (all + gridDim.z - 1) / gridDim.z;
     const int page0 = min(all, (int)blockIdx.z * share), page1 = min(all, page0 + share);

@@ -149,7 +149,10 @@ __device__ __forceinline__ int slot_of(const Args& a, int s) {
     const int slot = a.slots[s];
     return slot >= 0 && slot < a.n_slots ? slot : -1;
 }
-__device__ __forceinline__ int keys_of(const Args& a, int s, int slot) { return slot < 0 ? 0 : max(0, min(a.kv_len[s], a.max_pages * kPageTokens)); }
+__device__ __forceinline__ int keys_of(const Args& a, int s, int slot) {
+    const int keys = max(0, min(a.kv_len[s], a.max_pages * kPageTokens));       // (read beside the slot, not behind it)
+    return slot < 0 ? 0 : keys;
+}
 __device__ __forceinline__ int tokens_of(const Args& a, const Line& l, int s) { return max(0, min(l.first[s + 1] - l.first[s], a.most)); }
 
 template <int H>
