@@ -12,9 +12,9 @@
 //
 // Two launches: one reads every row once, draws its token and notes what its filters keep (cpm_sample_drafts); this one, a cluster of blocks a sequence, looks at
 // n logits and probabilities, and reads one row of each again where a token was refused.
-// What bounds it: the first launch, whose phases wait for one another (sample_filtered.cu).  64 sequences of 5 tokens, vocabulary 73,448, with probabilities: 130 us, 108 of
+// What bounds it: the first launch, whose phases wait for one another (sample_filtered.cu).  64 sequences of 5 tokens, vocabulary 73,448, with probabilities: 128 us, 106 of
 // them the first launch and 22 this one (37 MB of the refused rows: 6 us from memory, the rest the path before it, two barriers of the cluster and the run that is read
-// again); one sequence: 24 us, 15 and 9.  32 trees of 16 tokens, vocabulary 32,000, without probabilities: 76 us, 3 of them this launch.
+// again); one sequence: 24 us, 15 and 9.  32 trees of 16 tokens, vocabulary 32,000, without probabilities: 74 us, 3 of them this launch.
 #include "filtered.cuh"
 
 // Every row's draw (sample_filtered.cu).

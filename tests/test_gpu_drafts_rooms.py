@@ -85,7 +85,9 @@ def test_refusals_of_storing_at_rows():
     tables, _, args = _short_step(ops, "bfloat16", 64)
     for bad in (dict(slot_map=tables.slot_map[:5]), dict(slot_map=tables.places), dict(slot_map=tables.slot_map.cpu()), dict(slot_map=tables.slot_map, places=tables.places),
                 dict(slot_map=tables.slot_map, positions=tables.positions[:7].contiguous()), dict(places=tables.places, token_seq=tables.token_seq.long()),
-                dict(slot_map=tables.slot_map, k_cache=args["k_cache"][:, :, :32].contiguous()), dict(places=tables.places, v_cache=args["v_cache"][:9])):
+                dict(slot_map=tables.slot_map, k_cache=args["k_cache"][:, :, :32].contiguous()), dict(places=tables.places, v_cache=args["v_cache"][:9]),
+                dict(places=tables.places, slots=args["slots"].long()), dict(places=tables.places, page_table=args["page_table"][0].contiguous()),
+                dict(places=tables.places, page_table=args["page_table"][:, :2])):
         with pytest.raises(ValueError):
             ops.rope_store(**{**args, **bad})
 
