@@ -100,14 +100,15 @@ def draft_step(model, cache, tokens: int, ids, parents, lengths, new, slots, see
     ctx = StepContext(
         n_tokens=n, n_seqs=size, is_decode=False, captured=captured, q_lens=[tokens] * size, kv_lens=[], slots=[], max_q_len=tokens, max_kv_len=longest,
         token_ids=ids, positions=t.positions, token_seq=t.token_seq, cu_q=t.cu_q, kv_len_dev=t.kv_len, slot_dev=slots, cache=cache,
-        drafts=tokens, places=t.places, ancestors=t.ancestors)
+        drafts=tokens, places=t.places, slot_map=t.slot_map, slot_table=group.page_table, ancestors=t.ancestors)
     ctx.extras["step_begun"] = True
     logits = model.forward(ctx, want_rows)
     got = ops.verify_drafts(logits, ids, t.cu_q, t.token_seq, tokens, None, temperature, top_k, top_p, min_p, parents=parents, seed=seed, seq_key=seq_key,
                             step_key=step_key, positions=t.positions)
     for g in cache.groups:
         if g.k is not None:
-            ops.keep_drafts([(g.k, g.v)], lengths, got[2], got[1], slots, g.page_table)
+            known = dict(slot_map=t.slot_map, cu_q=t.cu_q) if g is group else {}
+            ops.keep_drafts([(g.k, g.v)], lengths, got[2], got[1], slots, g.page_table, **known)
     return got
 
 

@@ -122,8 +122,10 @@ class GroupedQueryAttention(Mixer):
             out = ops.kv4_attention(q, lane.records, ctx.kv_len_dev, ctx.slot_dev, lane.page_table, self.n_kv, self.scale, self.window, **prompt)
             return ops.linear(out, self.w_o)
         if ctx.drafts:
+            known = ctx.slot_map is not None and lane.page_table is ctx.slot_table        # (one look instead of three in a row)
             q = ops.rope_store(qkv, self.n_heads, self.n_kv, self.d, ctx.positions, ctx.token_seq, ctx.slot_dev, lane.page_table,
-                               k_cache if writes_cache else None, v_cache if writes_cache else None, inv_freq, magnitude, rot_dim, places=ctx.places)
+                               k_cache if writes_cache else None, v_cache if writes_cache else None, inv_freq, magnitude, rot_dim,
+                               **(dict(slot_map=ctx.slot_map) if known else dict(places=ctx.places)))
             out = ops.draft_attention(q, k_cache, v_cache, ctx.kv_len_dev, ctx.cu_q, ctx.slot_dev, lane.page_table, self.n_kv, self.scale, ctx.drafts,
                                       ancestors=ctx.ancestors)
             return ops.linear(out, self.w_o)

@@ -497,8 +497,10 @@ class StepContext:
     # a kernel that needs no tiles).
     q_tiles: Optional[Tuple[torch.Tensor, torch.Tensor, int]] = None
     extras: Dict[str, Any] = field(default_factory=dict)
-    # A step of drafted tokens (0: it is not): the most that a sequence brings.  ``places``: where a token lies in its sequence's cache; ``ancestors``: of the
-    # sequence's tokens of this step, the bits of those that it sees (int64; None: all up to itself).
+    # A step of drafted tokens (0: it is not): the most that a sequence brings.  ``places``: where a token lies in its sequence's cache; ``slot_map``: the rows that this
+    # is in lanes whose page table is ``slot_table``; ``ancestors``: of the sequence's tokens of this step, the bits of those that it sees (int64; None: all up to itself).
     drafts: int = 0
     places: Optional[torch.Tensor] = None
+    slot_map: Optional[torch.Tensor] = None
+    slot_table: Optional[torch.Tensor] = None
     ancestors: Optional[torch.Tensor] = None
